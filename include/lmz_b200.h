@@ -9,7 +9,7 @@
  *
  * Section 1 is the interface the reference's Python layer binds
  * (lmz/gpu/__init__.py:130-148) and is call-compatible with the reference
- * library (lmz/gpu/lmzgpu.cu).  Section 2 is additive.
+ * library (lmz/gpu/lmzgpu.cu).  Sections 2 and 3 are additive.
  */
 #ifndef LMZ_B200_H
 #define LMZ_B200_H
@@ -343,6 +343,62 @@ typedef struct lmz_decode_plan {
 int lmz_gpu_decode_chunks_dev(const lmz_decode_plan *plan, void *cuda_stream);
 /* How many kernels this thread's last lmz_gpu_decode_chunks_dev launched. */
 unsigned lmz_gpu_plan_launches(void);
+
+/* ------------------------------------------------------------------ section 3 */
+
+/* Operators on a checkpoint's tensors.  No counterpart in the reference.  All are asynchronous on
+ * cuda_stream, allocate nothing and may be captured into a graph; results do not depend on the order in
+ * which blocks run.  Sums are held in 32 bits and rounded to the tensors' type once. */
+#define LMZ_GPU_BF16 0
+#define LMZ_GPU_F16 1
+#define LMZ_GPU_F32 2
+
+/* Rows of an embedding table: out[t] = scale * table[ids[t]], for n ids of id_bytes (4 or 8) each; an id outside
+ * [0, rows) gives a row of zeros.  row_stride: elements from one row of the table to the next; the rows of d_out
+ * follow each other. */
+int lmz_gpu_rows_dev(const void *d_table, uint64_t rows, uint64_t dim, uint64_t row_stride, int dtype,
+                     const void *d_ids, int id_bytes, uint64_t n, float scale, void *d_out, void *cuda_stream);
+
+/* The table's gradient: dtable[v] = scale * the sum of dy[t] over the tokens t with ids[t] = v, all rows of it
+ * written.  d_work: lmz_gpu_rows_grad_work_bytes(n, rows, dim) bytes, 256-byte aligned. */
+size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t rows, uint64_t dim);
+int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dtype, const void *d_ids, int id_bytes,
+                          uint64_t rows, float scale, void *d_dtable, void *d_work, void *cuda_stream);
+
+/* A projection with low-rank adapters of many requests beside the shared weight:
+ *   y[t] = x[t] W^T + h[t] B_i^T,  h[t] = s_i x[t] A_i^T,  i = index[t]
+ * where tokens whose index is outside [0, adapters) have no adapter.  All tensors are of one type, BF16 or F16; the
+ * factors, y, dy, dx, da and db are contiguous. */
+#define LMZ_GPU_MAX_RANK 256
+typedef struct lmz_projection {
+    const void *x;              /* tokens x in, rows x_stride elements apart */
+    const void *weight;         /* out x in, rows weight_stride elements apart */
+    const void *a;              /* adapters x rank x in */
+    const void *b;              /* adapters x out x rank */
+    const void *index;          /* tokens int32 or int64 (index_bytes 4 or 8), or NULL: adapter 0 for every token */
+    const void *scales;         /* adapters float32, times `scale`; or NULL */
+    void *y;                    /* tokens x out */
+    void *hidden;               /* lmz_gpu_project_hidden_bytes(), 256-byte aligned: what the gradients need of the
+                                 * forward pass */
+    const void *dy;             /* tokens x out */
+    void *dx, *da, *db;         /* like x (contiguous), a and b; NULL: not wanted */
+    void *work;                 /* lmz_gpu_project_work_bytes(), 256-byte aligned */
+    uint64_t tokens, in, out, x_stride, weight_stride;
+    uint32_t adapters, rank, dtype, index_bytes;
+    float scale;
+} lmz_projection;
+/* Both read the sizes, strides and types alone, and the addresses' last bits; `grad`: for the gradients' call. */
+size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p);
+size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad);
+int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream);
+/* g[t] = s_i dy[t] B_i;  dx[t] = dy[t] W + g[t] A_i;  da_i = the sum of g[t]^T x[t], db_i = the sum of dy[t]^T h[t] over
+ * the tokens of adapter i (zeros for an adapter without any). */
+int lmz_gpu_project_grad_dev(const lmz_projection *p, void *cuda_stream);
+
+/* out = W + scale * B A for an out x in weight (rows weight_stride elements apart), BF16 or F16; d_out is contiguous, and
+ * may be the weight itself where that is. */
+int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a,
+                      const void *d_b, unsigned rank, float scale, int dtype, void *d_out, void *cuda_stream);
 
 #ifdef __cplusplus
 }

@@ -15,11 +15,11 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "liblmz_b200.so")
-SOURCES = ["lmz_b200.cu"]
+SOURCES = ["lmz_b200.cu", "model_ops.cu"]
 last_error = ""
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "--extended-lambda", "-shared", "-Xcompiler", "-fPIC"]
+              "--extended-lambda", "-shared", "-Xcompiler", "-fPIC", "-t", "0"]
 
 
 def find_nvcc() -> str | None:

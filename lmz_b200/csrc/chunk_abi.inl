@@ -66,19 +66,6 @@ static int launch_cond_finish(const FinishArgs &fa, int sms, cudaStream_t cs)
     return LMZ_GPU_OK;
 }
 
-static int sm_count(int *out)
-{
-    static int cached[64];
-    int dev = 0;
-    CK("cudaGetDevice", cudaGetDevice(&dev));
-    if (dev >= 0 && dev < 64 && cached[dev]) { *out = cached[dev]; return LMZ_GPU_OK; }
-    int n = 0;
-    CK("cudaDeviceGetAttribute", cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    if (dev >= 0 && dev < 64) cached[dev] = n;
-    *out = n;
-    return LMZ_GPU_OK;
-}
-
 // A second stream per device, so the fused kernel (most of the work) overlaps the
 // few latency-bound streams and pieces that cannot be fused.  Created on first use.
 struct SideStream {

@@ -1,10 +1,10 @@
-// How an entry point says what went wrong (included by lmz_b200.cu).
+// How an entry point says what went wrong (included by every source file of the library).
 #include <cstdarg>
 #include <cstdio>
 #include <exception>
 
-// Why the last call on this thread failed (lmz_gpu_last_error).
-static thread_local char g_err[256];
+// Why the last call on this thread failed (lmz_gpu_last_error); one for all source files.
+__attribute__((visibility("hidden"))) inline thread_local char g_err[256];
 
 // Record a reason and hand back the code to return.
 static int report(int code, const char *fmt, ...)

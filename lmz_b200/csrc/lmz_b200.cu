@@ -28,31 +28,7 @@ using namespace lmz;
 
 #include "host_error.inl"
 
-static int device_ready()
-{
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        return fail_msg(LMZ_GPU_ENODEV, "no CUDA device");
-    }
-    return LMZ_GPU_OK;
-}
-
-// Kernels ask for more dynamic shared memory than the default 48 KiB; the
-// opt-in is per device and is made once.
-template <class K>
-static int opt_in_smem(K kernel, uint32_t bytes, bool *done /* [64] by device */)
-{
-    int dev = 0;
-    CK("cudaGetDevice", cudaGetDevice(&dev));
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev >= 0 && dev < 64 && done[dev]) return LMZ_GPU_OK;
-    CK("cudaFuncSetAttribute",
-       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev >= 0 && dev < 64) done[dev] = true;
-    return LMZ_GPU_OK;
-}
+#include "host_device.inl"
 
 // k_stream takes all the shared memory one CTA may have and lays its tables out from
 // both ends, counting on the window starting F_SMEM_BASE bytes in (what the
@@ -73,8 +49,6 @@ static int stream_smem_ok()
         return fail_msg(LMZ_GPU_EUNSUPPORTED, "this GPU's shared memory per CTA is not the 1 KiB + 227 KiB k_stream is laid out for");
     return LMZ_GPU_OK;
 }
-
-static int sm_count(int *out);
 
 // Kernels this thread has launched for the plan it was last given (lmz_gpu_plan_launches).
 static thread_local unsigned g_launches;

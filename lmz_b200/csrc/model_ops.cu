@@ -1,0 +1,304 @@
+// C-ABI entry points of the operators on a checkpoint's tensors: rows of an embedding table, projections with low-rank
+// adapters, merges.  Declarations and the per-function contract live in include/lmz_b200.h.
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/lmz_b200.h"
+#include "adapter_kernels.cuh"
+#include "rows_kernels.cuh"
+
+using namespace lmz;
+
+#define API extern "C" __attribute__((visibility("default")))
+
+#include "host_error.inl"
+#include "host_device.inl"
+
+static int launched(const char *what)
+{
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LMZ_GPU_OK : fail_cuda(what, e);
+}
+
+static uint32_t element_bytes(int dtype) { return dtype == LMZ_GPU_F32 ? 4 : dtype == LMZ_GPU_BF16 || dtype == LMZ_GPU_F16 ? 2 : 0; }
+
+// The widest vector, of at most 16 bytes, that rows of `row_bytes` at the given addresses and strides are made of.
+static uint32_t vector_bytes(uint64_t row_bytes, std::initializer_list<uint64_t> at)
+{
+    uint64_t bits = row_bytes | 16;
+    for (uint64_t v : at) bits |= v;
+    return static_cast<uint32_t>(bits & (~bits + 1));
+}
+
+static uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
+
+// f(type tag, vector width tag) for a type and width; EUNSUPPORTED for a width below the type's.
+template <class T, class F>
+static int by_width(uint32_t vb, F f)
+{
+    switch (vb) {
+    case 16: return f(Vec<T, 16>{});
+    case 8: return f(Vec<T, 8>{});
+    case 4: return f(Vec<T, 4>{});
+    case 2:
+        if constexpr (sizeof(T) == 2) return f(Vec<T, 2>{});
+        break;
+    }
+    return fail_msg(LMZ_GPU_EUNSUPPORTED, "a tensor does not start on a boundary of its elements");
+}
+
+template <class F>
+static int by_type(int dtype, uint32_t vb, F f)
+{
+    if (dtype == LMZ_GPU_BF16) return by_width<__nv_bfloat16>(vb, [&](auto v) { return f(__nv_bfloat16{}, v); });
+    if (dtype == LMZ_GPU_F16) return by_width<__half>(vb, [&](auto v) { return f(__half{}, v); });
+    if (dtype == LMZ_GPU_F32) return by_width<float>(vb, [&](auto v) { return f(float{}, v); });
+    return fail_msg(LMZ_GPU_EUNSUPPORTED, "an element type other than BF16, F16 and F32");
+}
+
+static uint32_t lanes_log(uint32_t vectors)
+{
+    uint32_t log = 0;
+    while ((1u << log) < vectors && (1u << log) < ROW_THREADS) log++;
+    return log;
+}
+
+static int check_rows(uint64_t rows, uint64_t dim, int dtype, int id_bytes, uint64_t n)
+{
+    const uint32_t e = element_bytes(dtype);
+    if (!e) return fail_msg(LMZ_GPU_EUNSUPPORTED, "an element type other than BF16, F16 and F32");
+    if (id_bytes != 4 && id_bytes != 8) return fail_msg(LMZ_GPU_EUNSUPPORTED, "ids are int32 or int64");
+    if (rows >= 1ull << 31 || n >= 1ull << 31) return fail_msg(LMZ_GPU_EUNSUPPORTED, "2^31 rows or tokens and more");
+    if (dim == 0 || dim >= 1ull << 24) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a row has between 1 and 2^24 - 1 elements");
+    return LMZ_GPU_OK;
+}
+
+API int lmz_gpu_rows_dev(const void *d_table, uint64_t rows, uint64_t dim, uint64_t row_stride, int dtype, const void *d_ids,
+                         int id_bytes, uint64_t n, float scale, void *d_out, void *cuda_stream)
+{
+    int rc = check_rows(rows, dim, dtype, id_bytes, n);
+    if (rc) return rc;
+    if (n == 0) return LMZ_GPU_OK;
+    rc = device_ready();
+    if (rc) return rc;
+    const uint64_t e = element_bytes(dtype), bytes = dim * e;
+    const uint32_t vb = vector_bytes(bytes, {address(d_table), address(d_out), row_stride * e});
+    return by_type(dtype, vb, [&](auto type, auto vec) {
+        using T = decltype(type);
+        constexpr int VB = sizeof(vec.raw);
+        RowsArgs a{};
+        a.table = static_cast<const uint8_t *>(d_table), a.ids = d_ids, a.out = static_cast<uint8_t *>(d_out);
+        a.rows = rows, a.n = n, a.row_bytes = bytes, a.stride_bytes = row_stride * e;
+        a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = lanes_log(a.vectors);
+        a.scale = scale, a.wide = id_bytes == 8;
+        constexpr int U = 4;
+        const uint32_t per = (ROW_THREADS >> a.lane_log) * U;
+        k_rows<T, VB, U><<<static_cast<unsigned>((n + per - 1) / per), ROW_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
+        return launched("launch k_rows");
+    });
+}
+
+// Tokens of a window of the rows' gradient: windows of 32, but not more than 4096 of them.
+static uint32_t rows_window(uint64_t n) { return static_cast<uint32_t>(std::max<uint64_t>(32, (n + 4095) / 4096)); }
+
+struct RowsGradLayout {
+    uint64_t keys[2], pos[2], start, partial, end;
+    RowsGradLayout(uint64_t n, uint64_t rows, uint64_t dim)
+    {
+        uint64_t at = 0;
+        auto take = [&](uint64_t bytes) { const uint64_t r = at; at += (bytes + 255) & ~255ull; return r; };
+        for (int i = 0; i < 2; i++) keys[i] = take(n * 4), pos[i] = take(n * 4);
+        start = take((rows + 1) * 4);
+        const uint64_t w = rows_window(n);
+        partial = take(n > w ? (n + w - 1) / w * 2 * dim * 4 : 0);
+        end = at;
+    }
+};
+
+// Sort ids; on return *side is where the result lies.
+static int launch_sort(SortArgs &s, cudaStream_t cs, int *side)
+{
+    static bool done[64];
+    int rc = opt_in_smem(k_sort, SORT_SMEM, done);
+    if (rc) return rc;
+    uint32_t bits = 1;
+    while (bits < 32 && s.nkeys >> bits) bits++;
+    s.passes = (bits + 7) / 8;
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    const uint32_t ctas = s.n <= 2 * SORT_THREADS ? 1 : SORT_CTAS;
+    attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    c.gridDim = dim3(ctas), c.blockDim = dim3(SORT_THREADS), c.dynamicSmemBytes = SORT_SMEM, c.stream = cs;
+    c.attrs = &attr, c.numAttrs = 1;
+    CK("launch k_sort", cudaLaunchKernelEx(&c, k_sort, s));
+    *side = (s.passes - 1) & 1;
+    return LMZ_GPU_OK;
+}
+
+API size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t rows, uint64_t dim) { return RowsGradLayout(n, rows, dim).end; }
+
+API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dtype, const void *d_ids, int id_bytes, uint64_t rows,
+                              float scale, void *d_dtable, void *d_work, void *cuda_stream)
+{
+    int rc = check_rows(rows, dim, dtype, id_bytes, n);
+    if (rc) return rc;
+    if (rows == 0) return LMZ_GPU_OK;
+    rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    const uint64_t bytes = dim * element_bytes(dtype);
+    if (n == 0) {
+        CK("cudaMemsetAsync", cudaMemsetAsync(d_dtable, 0, rows * bytes, cs));
+        return LMZ_GPU_OK;
+    }
+    const RowsGradLayout l(n, rows, dim);
+    uint8_t *work = static_cast<uint8_t *>(d_work);
+    auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(work + off); };
+    SortArgs s{};
+    s.ids = d_ids, s.n = n, s.nkeys = rows, s.wide = id_bytes == 8;
+    for (int i = 0; i < 2; i++) s.keys[i] = words(l.keys[i]), s.pos[i] = words(l.pos[i]);
+    int side = 0;
+    rc = launch_sort(s, cs, &side);
+    if (rc) return rc;
+    k_key_starts<<<static_cast<unsigned>(rows / 256 + 1), 256, 0, cs>>>(s.keys[side], static_cast<uint32_t>(n), static_cast<uint32_t>(rows), words(l.start));
+    rc = launched("launch k_key_starts");
+    if (rc) return rc;
+    return by_type(dtype, vector_bytes(bytes, {address(d_dy), address(d_dtable)}), [&](auto type, auto vec) {
+        using T = decltype(type);
+        constexpr int VB = sizeof(vec.raw), U = 4;
+        RowsGradArgs a{};
+        a.dy = static_cast<const uint8_t *>(d_dy), a.keys = s.keys[side], a.pos = s.pos[side], a.start = words(l.start);
+        a.partial = reinterpret_cast<float *>(work + l.partial), a.out = static_cast<uint8_t *>(d_dtable);
+        a.rows = rows, a.row_bytes = bytes, a.dim = dim, a.n = static_cast<uint32_t>(n), a.window = rows_window(n), a.scale = scale;
+        a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = lanes_log(a.vectors);
+        const uint32_t slices = (a.vectors + ROW_THREADS - 1) / ROW_THREADS, per = (ROW_THREADS >> a.lane_log) * U;
+        if (a.n > a.window) {
+            k_rows_grad_windows<T, VB><<<dim3((a.n + a.window - 1) / a.window, slices), ROW_THREADS, 0, cs>>>(a);
+            const int failed = launched("launch k_rows_grad_windows");
+            if (failed) return failed;
+        }
+        k_rows_grad<T, VB, U><<<dim3(static_cast<unsigned>((rows + per - 1) / per), slices), ROW_THREADS, 0, cs>>>(a);
+        return launched("launch k_rows_grad");
+    });
+}
+
+// ------------------------------------------------------------------ adapters
+
+static int check_projection(const lmz_projection *p)
+{
+    if (p->dtype != LMZ_GPU_BF16 && p->dtype != LMZ_GPU_F16) return fail_msg(LMZ_GPU_EUNSUPPORTED, "projections are of BF16 or F16");
+    if (p->index && p->index_bytes != 4 && p->index_bytes != 8) return fail_msg(LMZ_GPU_EUNSUPPORTED, "an index is of int32 or int64");
+    if (p->rank == 0 || p->rank > LMZ_GPU_MAX_RANK) return report(LMZ_GPU_EUNSUPPORTED, "ranks are between 1 and %d", LMZ_GPU_MAX_RANK);
+    if (p->adapters == 0 || p->adapters > 65535) return fail_msg(LMZ_GPU_EUNSUPPORTED, "between 1 and 65535 adapters");
+    if (p->in == 0 || p->out == 0 || p->in >= 1u << 21 || p->out >= 1u << 21)
+        return fail_msg(LMZ_GPU_EUNSUPPORTED, "a weight has between 1 and 2^21 - 1 rows and columns");
+    if (p->tokens >= 1ull << 31) return fail_msg(LMZ_GPU_EUNSUPPORTED, "2^31 tokens and more");
+    return LMZ_GPU_OK;
+}
+
+static TokenIndex token_index(const lmz_projection *p)
+{
+    return {p->index, static_cast<const float *>(p->scales), p->scale, p->adapters, p->index_bytes == 8};
+}
+
+API size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p) { return p->tokens * p->rank * 4; }
+API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { return grad ? p->tokens * p->rank * 4 : 0; }
+
+template <class T>
+static int project_as(const lmz_projection *p, cudaStream_t cs)
+{
+    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight);
+    float *h = static_cast<float *>(p->hidden);
+    const uint64_t r = p->rank;
+    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in}, b{static_cast<const T *>(p->b), r * p->out, r, 1};
+    k_hidden<T><<<static_cast<unsigned>((p->tokens * r + 7) / 8), 256, 0, cs>>>(x, p->x_stride, p->in, a, token_index(p), p->tokens, p->rank, h);
+    int rc = launched("launch k_hidden");
+    if (rc) return rc;
+    k_project<T><<<dim3(static_cast<unsigned>((p->tokens + 63) / 64), static_cast<unsigned>((p->out + 63) / 64)), 256, 0, cs>>>(
+        x, p->x_stride, p->in, w, p->weight_stride, 1, b, token_index(p), h, p->rank, p->tokens, p->out, static_cast<T *>(p->y));
+    return launched("launch k_project");
+}
+
+template <class T>
+static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
+{
+    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *dy = static_cast<const T *>(p->dy);
+    const float *h = static_cast<const float *>(p->hidden);
+    float *g = static_cast<float *>(p->work);
+    const uint64_t r = p->rank;
+    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in}, b{static_cast<const T *>(p->b), r * p->out, r, 1};
+    int rc = LMZ_GPU_OK;
+    if (p->tokens && (p->dx || p->da)) {
+        k_hidden<T><<<static_cast<unsigned>((p->tokens * r + 7) / 8), 256, 0, cs>>>(dy, p->out, p->out, b, token_index(p), p->tokens, p->rank, g);
+        rc = launched("launch k_hidden");
+        if (rc) return rc;
+    }
+    if (p->tokens && p->dx) {
+        k_project<T><<<dim3(static_cast<unsigned>((p->tokens + 63) / 64), static_cast<unsigned>((p->in + 63) / 64)), 256, 0, cs>>>(
+            dy, p->out, p->out, w, 1, p->weight_stride, a, token_index(p), g, p->rank, p->tokens, p->in, static_cast<T *>(p->dx));
+        rc = launched("launch k_project");
+        if (rc) return rc;
+    }
+    if (p->da) {
+        k_factor_grad<T><<<dim3(static_cast<unsigned>((p->in + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
+            g, x, p->x_stride, token_index(p), p->tokens, p->rank, p->in, static_cast<T *>(p->da), r * p->in, 1, p->in);
+        rc = launched("launch k_factor_grad");
+        if (rc) return rc;
+    }
+    if (p->db) {
+        k_factor_grad<T><<<dim3(static_cast<unsigned>((p->out + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
+            h, dy, p->out, token_index(p), p->tokens, p->rank, p->out, static_cast<T *>(p->db), r * p->out, r, 1);
+        rc = launched("launch k_factor_grad");
+    }
+    return rc;
+}
+
+API int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream)
+{
+    int rc = check_projection(p);
+    if (rc || p->tokens == 0) return rc;
+    rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    return p->dtype == LMZ_GPU_BF16 ? project_as<__nv_bfloat16>(p, cs) : project_as<__half>(p, cs);
+}
+
+API int lmz_gpu_project_grad_dev(const lmz_projection *p, void *cuda_stream)
+{
+    int rc = check_projection(p);
+    if (rc) return rc;
+    rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    return p->dtype == LMZ_GPU_BF16 ? project_grad_as<__nv_bfloat16>(p, cs) : project_grad_as<__half>(p, cs);
+}
+
+template <class T>
+static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, const void *a, const void *b, unsigned rank, float scale, void *to,
+                    cudaStream_t cs)
+{
+    for (uint64_t r0 = 0; r0 < out; r0 += 65535) {               // (a grid's second dimension ends there)
+        const uint64_t rows = std::min<uint64_t>(65535, out - r0);
+        k_merge<T><<<dim3(static_cast<unsigned>((in + 255) / 256), static_cast<unsigned>(rows)), 256, 0, cs>>>(
+            static_cast<const T *>(w) + r0 * stride, stride, static_cast<const T *>(a), static_cast<const T *>(b) + r0 * rank, rank, scale, in,
+            static_cast<T *>(to) + r0 * in);
+        const int rc = launched("launch k_merge");
+        if (rc) return rc;
+    }
+    return LMZ_GPU_OK;
+}
+
+API int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a, const void *d_b, unsigned rank,
+                          float scale, int dtype, void *d_out, void *cuda_stream)
+{
+    lmz_projection p{};
+    p.dtype = dtype, p.rank = rank, p.adapters = 1, p.in = in, p.out = out;
+    int rc = check_projection(&p);
+    if (rc) return rc;
+    rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    return dtype == LMZ_GPU_BF16 ? merge_as<__nv_bfloat16>(d_weight, out, in, weight_stride, d_a, d_b, rank, scale, d_out, cs)
+                                 : merge_as<__half>(d_weight, out, in, weight_stride, d_a, d_b, rank, scale, d_out, cs);
+}

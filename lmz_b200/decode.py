@@ -568,17 +568,8 @@ def _range_groups(ar, cuts, nslices):
     return out
 
 
-def decode_tensors(ar, names, device=None, checksum: bool = True):
-    """Decode only what the named tensors need.  `names`: (member path, tensor name)
-    keys of `Archive.tensor_index()`, or bare tensor names when they are unambiguous.
-    Uploads the payload bytes of the chunks that overlap those tensors (and of the
-    sources of any ref or delta among them), decodes them into a buffer that spans
-    just their part of the output space, verifies, and returns {key: device tensor}."""
-    import torch
-    from . import multi
-
-    ar = ar if isinstance(ar, fmt.Archive) else fmt.Archive(ar)
-    index = ar.tensor_index()
+def _resolve(index, names):
+    """Keys of a tensor index for (member path, tensor name) keys or bare names that are unambiguous."""
     by_name = {}
     for key in index:
         by_name.setdefault(key[1], []).append(key)
@@ -593,9 +584,106 @@ def decode_tensors(ar, names, device=None, checksum: bool = True):
             if len(hits) != 1:
                 raise KeyError(f"{n!r} names {len(hits)} tensors; give (member path, name)")
             keys.append(hits[0])
+    return keys
+
+
+def decode_tensors(ar, names, device=None, checksum: bool = True, adapter=None, scale: float = 1.0):
+    """Decode only what the named tensors need.  `names`: (member path, tensor name)
+    keys of `Archive.tensor_index()`, or bare tensor names when they are unambiguous.
+    Uploads the payload bytes of the chunks that overlap those tensors (and of the
+    sources of any ref or delta among them), decodes them into a buffer that spans
+    just their part of the output space, verifies, and returns {key: device tensor}.
+
+    `adapter`: an archive (or path, or bytes) that holds a fine-tune of this one as low-rank factors (`adapters.load` says
+    how they are named).  The named tensors that it has factors for come out as the fine-tune's own, merged with
+    `scale` (alpha / rank); the others as they are."""
+    ar = ar if isinstance(ar, fmt.Archive) else fmt.Archive(ar)
+    index = ar.tensor_index()
+    keys = _resolve(index, names)
     if not keys:
         return {}
-    select = multi.cover(ar, [(index[k][2], index[k][3]) for k in keys])
+    dec, out_lo = _decode_ranges(ar, [(index[k][2], index[k][3]) for k in keys], device, checksum)
+    out = {}
+    for k in keys:
+        dt, shape, s, e = index[k]
+        raw = dec.d_out[s - out_lo:e - out_lo]
+        name = _TORCH_DTYPES.get(dt)
+        if name is not None and (s - out_lo) % 2 == 0:
+            try:
+                raw = raw.view(_torch_type(name)).reshape(shape)
+            except RuntimeError:
+                pass
+        out[k] = raw
+    if adapter is not None:
+        _merge_adapter(out, adapter, scale)
+    return out
+
+
+def _torch_type(name):
+    import torch
+    return getattr(torch, name)
+
+
+def _merge_adapter(tensors, adapter, scale):
+    """Put merged weights in the place of the tensors that an adapter archive has factors for."""
+    from . import adapters
+    adapter = adapter if isinstance(adapter, fmt.Archive) else fmt.Archive(adapter)
+    for key, weight in tensors.items():
+        pair = adapters._factors(adapter, key[1], weight.device)
+        if pair is not None:
+            a, b = (t.to(weight.dtype) for t in pair)
+            tensors[key] = adapters.merge(weight, a, b, scale=scale)
+
+
+def decode_rows(ar, name, rows, scale: float = 1.0, device=None, checksum: bool = True):
+    """`scale * table[rows]` of a table in an archive, decoding only the chunks that hold those rows.  `name`: the
+    table's key or unambiguous name, a tensor [rows, dim] of BF16, F16 or F32.  `rows`: row numbers of any shape on the
+    host (a sequence, numpy array or CPU tensor), each in [0, rows).  Returns a device tensor of shape `rows.shape + (dim,)`;
+    `embed.lookup` is the same for a table that is resident."""
+    import torch
+    from . import embed
+
+    ar = ar if isinstance(ar, fmt.Archive) else fmt.Archive(ar)
+    index = ar.tensor_index()
+    (key,) = _resolve(index, [name])
+    dt, shape, start, end = index[key]
+    if dt not in ("BF16", "F16", "F32") or len(shape) != 2:
+        raise ValueError(f"{key[1]!r} is {dt} {list(shape)}, not a table of BF16, F16 or F32 rows")
+    ids = np.asarray(rows)
+    if ids.size == 0:
+        ids = ids.astype(np.int64)
+    if ids.dtype.kind not in "iu":
+        raise TypeError(f"rows are whole numbers, not {ids.dtype}")
+    count, dim = shape
+    if ids.size and (int(ids.min()) < 0 or int(ids.max()) >= count):
+        raise IndexError(f"a row outside [0, {count})")
+    dtype = _torch_type(_TORCH_DTYPES[dt])
+    dev = torch.device(device if device is not None else f"cuda:{torch.cuda.current_device()}")
+    if not ids.size or not dim:
+        return torch.empty((*ids.shape, dim), dtype=dtype, device=dev)
+    row = dim * dtype.itemsize
+    used = np.unique(ids).astype(np.int64)
+    # consecutive rows are one range
+    first = np.concatenate(([True], np.diff(used) > 1))
+    lo, hi = used[first], used[np.concatenate((first[1:], [True]))] + 1
+    dec, out_lo = _decode_ranges(ar, [(start + a * row, start + b * row) for a, b in zip(lo.tolist(), hi.tolist())], dev, checksum)
+    base = int(used[0])                                    # the table from its first row used: the rows before it may not be there
+    raw = dec.d_out[start + base * row - out_lo:start + (int(used[-1]) + 1) * row - out_lo]
+    try:
+        table = raw.view(dtype)
+    except RuntimeError:                                   # not on a boundary of its elements
+        table = raw.clone().view(dtype)
+    with torch.cuda.device(dev):
+        return embed.lookup(table.view(-1, dim), torch.from_numpy(ids.astype(np.int64) - base).to(dev), scale=scale)
+
+
+def _decode_ranges(ar, ranges, device, checksum):
+    """(an ArchiveDecoder that has run and been checked, where its output starts): the chunks that the byte ranges of the
+    output space need, decoded into a buffer that spans just their part of it."""
+    import torch
+    from . import multi
+
+    select = multi.cover(ar, ranges)
     r = ar.records[select]
     out_lo = int(r["dst"].min()) & ~15                     # keep the output's 16-byte phase
     out_hi = int((r["dst"].astype(np.int64) + r["rlen"]).max())
@@ -623,18 +711,7 @@ def decode_tensors(ar, names, device=None, checksum: bool = True):
         finally:
             up.close()
     dec.check()
-    out = {}
-    for k in keys:
-        dt, shape, s, e = index[k]
-        raw = dec.d_out[s - out_lo:e - out_lo]
-        name = _TORCH_DTYPES.get(dt)
-        if name is not None and (s - out_lo) % 2 == 0:
-            try:
-                raw = raw.view(getattr(torch, name)).reshape(shape)
-            except RuntimeError:
-                pass
-        out[k] = raw
-    return out
+    return dec, out_lo
 
 
 def decode_archive(ar, device=None, checksum: bool = True):

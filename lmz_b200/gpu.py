@@ -111,8 +111,9 @@ class _Loader:
         for name, (res, args) in _SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-        from . import _chunks
+        from . import _chunks, _ops
         _chunks.bind(lib)
+        _ops.bind(lib)
         if not _known_answer(lib):
             return self._give_up("unavailable", f"the CUDA decoder did not reproduce the known "
                                                 f"plaintext on {device}; refusing to use it")
