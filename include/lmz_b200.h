@@ -395,6 +395,10 @@ int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream);
  * the tokens of adapter i (zeros for an adapter without any). */
 int lmz_gpu_project_grad_dev(const lmz_projection *p, void *cuda_stream);
 
+/* Every wait inside the kernels above has a limit.  1 if one has run out on the current device since the library was
+ * loaded (the results of that launch are not to be used), 0 if none has, negative on failure; waits for the device. */
+int lmz_gpu_ops_gave_up(void);
+
 /* out = W + scale * B A for an out x in weight (rows weight_stride elements apart), BF16 or F16; d_out is contiguous, and
  * may be the weight itself where that is. */
 int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a,

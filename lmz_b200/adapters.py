@@ -180,6 +180,16 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
     return out
 
 
+def check(device=None) -> None:
+    """Synchronise, and raise if a kernel has given up waiting for one of its own copies on this device (every wait in
+    them has a limit; none runs out unless the hardware fails)."""
+    import torch
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        rc = gpu.library().lmz_gpu_ops_gave_up()
+    if rc:
+        raise RuntimeError("a projection's kernel gave up waiting: its results are not to be used" if rc > 0 else gpu.last_error())
+
+
 def _span(t):
     """The bytes from a tensor's first element to the end of its last."""
     lo = t.data_ptr()

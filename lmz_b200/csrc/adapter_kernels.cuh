@@ -32,64 +32,44 @@ struct Factor {
     __device__ __forceinline__ T at(int i, uint64_t f, uint32_t j) const { return p[i * each + f * wide + j * place]; }
 };
 
+// Thin products are kept as two halves of 16 bits, [token][2][rp] with rp the rank up to a multiple of 8: a value to the
+// nearest T, and what that lacks.  One T alone would cost as much as the result's own rounding.
+template <class T>
+__device__ __forceinline__ void split_halves(float v, T &hi, T &lo)
+{
+    hi = narrow<T>(v);
+    lo = narrow<T>(isfinite(widen(hi)) ? v - widen(hi) : 0.0f);
+}
+
 // h[t][j] = s_i * sum over k of x[t][k] F_i(k, j): a warp each.
 template <class T>
 __global__ void __launch_bounds__(256) k_hidden(const T *x, uint64_t stride, uint64_t k, Factor<T> f, TokenIndex index, uint64_t tokens,
-                                                uint32_t rank, float *h)
+                                                uint32_t rank, uint32_t rp, T *h)
 {
-    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), t = at / rank;
-    const uint32_t j = static_cast<uint32_t>(at % rank), lane = threadIdx.x & 31;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), t = at / rp;
+    const uint32_t j = static_cast<uint32_t>(at % rp), lane = threadIdx.x & 31;
     if (t >= tokens) return;
     const int i = index.of(t);
     float sum = 0;
-    if (i >= 0)
+    if (i >= 0 && j < rank)
         for (uint64_t c = lane; c < k; c += 32) sum += widen(x[t * stride + c]) * widen(f.at(i, c, j));
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) h[at] = i >= 0 ? sum * index.scale_of(i) : 0.0f;
+    if (lane == 0) split_halves(i >= 0 && j < rank ? sum * index.scale_of(i) : 0.0f, h[t * 2 * rp + j], h[t * 2 * rp + rp + j]);
 }
 
-// y[t][f] = sum over k of x[t][k] W(f, k) + sum over j of h[t][j] F_i(f, j): tiles of 64 by 64.
+// A copy whose rows start on a boundary of 16 bytes and end in zeros: out[o][r][c] = in(o, r, c) for r < rows, c < cols, else 0.
 template <class T>
-__global__ void __launch_bounds__(256) k_project(const T *x, uint64_t stride, uint64_t k, const T *w, uint64_t wf, uint64_t wk, Factor<T> fac,
-                                                 TokenIndex index, const float *h, uint32_t rank, uint64_t tokens, uint64_t feats, T *y)
+__global__ void __launch_bounds__(256) k_pack(const T *in, uint64_t so, uint64_t sr, uint64_t sc, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t total, T *out)
 {
-    __shared__ float xs[16][65], ws[16][65];
-    const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * 64, f0 = static_cast<uint64_t>(blockIdx.y) * 64;
-    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (uint64_t k0 = 0; k0 < k; k0 += 16) {
-        for (uint32_t e = threadIdx.x; e < 64 * 16; e += 256) {
-            const uint32_t r = e >> 4, c = e & 15;
-            xs[c][r] = t0 + r < tokens && k0 + c < k ? widen(x[(t0 + r) * stride + k0 + c]) : 0.0f;
-            ws[c][r] = f0 + r < feats && k0 + c < k ? widen(w[(f0 + r) * wf + (k0 + c) * wk]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t c = 0; c < 16; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += xs[c][ty + 16 * i] * ws[c][tx + 16 * j];
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; i++) {
-        const uint64_t t = t0 + ty + 16 * i;
-        if (t >= tokens) continue;
-        const int ad = index.of(t);
-        for (int j = 0; j < 4; j++) {
-            const uint64_t f = f0 + tx + 16 * j;
-            if (f >= feats) continue;
-            float sum = acc[i][j];
-            if (ad >= 0)
-                for (uint32_t c = 0; c < rank; c++) sum += h[t * rank + c] * widen(fac.at(ad, f, c));
-            y[t * feats + f] = narrow<T>(sum);
-        }
+    for (uint64_t e = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; e < total; e += static_cast<uint64_t>(gridDim.x) * 256) {
+        const uint64_t c = e % pitch, q = e / pitch, r = q % rows, o = q / rows;
+        out[e] = c < cols ? in[o * so + r * sr + c * sc] : narrow<T>(0.0f);
     }
 }
 
 // dF_i(f, j) = sum over i's tokens of g[t][j] z[t][f].
 template <class T>
-__global__ void __launch_bounds__(256) k_factor_grad(const float *g, const T *z, uint64_t stride, TokenIndex index, uint64_t tokens, uint32_t rank,
+__global__ void __launch_bounds__(256) k_factor_grad(const T *g, uint32_t rp, const T *z, uint64_t stride, TokenIndex index, uint64_t tokens, uint32_t rank,
                                                      uint64_t feats, T *out, uint64_t each, uint64_t wide, uint64_t place)
 {
     const uint64_t f = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -97,7 +77,7 @@ __global__ void __launch_bounds__(256) k_factor_grad(const float *g, const T *z,
     if (f >= feats) return;
     float sum = 0;
     for (uint64_t t = 0; t < tokens; t++)
-        if (index.of(t) == static_cast<int>(i)) sum += g[t * rank + j] * widen(z[t * stride + f]);
+        if (index.of(t) == static_cast<int>(i)) sum += (widen(g[t * 2 * rp + j]) + widen(g[t * 2 * rp + rp + j])) * widen(z[t * stride + f]);
     out[i * each + f * wide + j * place] = narrow<T>(sum);
 }
 

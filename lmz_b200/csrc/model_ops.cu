@@ -2,9 +2,12 @@
 // adapters, merges.  Declarations and the per-function contract live in include/lmz_b200.h.
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/lmz_b200.h"
 #include "adapter_kernels.cuh"
+#include "project_kernel.cuh"
 #include "rows_kernels.cuh"
 
 using namespace lmz;
@@ -202,56 +205,195 @@ static TokenIndex token_index(const lmz_projection *p)
     return {p->index, static_cast<const float *>(p->scales), p->scale, p->adapters, p->index_bytes == 8};
 }
 
-API size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p) { return p->tokens * p->rank * 4; }
-API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { return grad ? p->tokens * p->rank * 4 : 0; }
+static uint64_t up8(uint64_t n) { return (n + 7) & ~7ull; }
+static uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
+
+// Rows of 16-bit elements that TMA and 16-byte copies take as they lie.
+static bool on_boundary(const void *p, uint64_t cols, uint64_t stride) { return address(p) % 16 == 0 && stride % 8 == 0 && stride >= cols; }
+
+// A tensor map of [planes] x rows x cols 16-bit elements, tiles of 64 columns with the 128-byte swizzle.
+static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows)
+{
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (!encode) return fail_msg(LMZ_GPU_EUNSUPPORTED, "the driver makes no tensor maps");
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
+    const cuuint32_t box[2] = {STEP_K, tile_rows}, steps[2] = {1, 1};
+    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(p), dims, strides, box,
+                              steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? LMZ_GPU_OK : report(LMZ_GPU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+// What a projection's kernels read in place of tensors that do not lie on boundaries, and between each other.
+struct ProjectLayout {
+    uint64_t x = 0, w = 0, a = 0, b = 0, dy = 0, g = 0, end = 0;
+    bool pack_x, pack_w, pack_a, pack_b, pack_dy;
+    ProjectLayout(const lmz_projection *p, bool grad)
+    {
+        auto take = [&](bool on, uint64_t elements) {
+            const uint64_t r = end;
+            if (on) end += up256(elements * 2);
+            return r;
+        };
+        pack_x = !grad && !on_boundary(p->x, p->in, p->x_stride);
+        pack_w = !on_boundary(p->weight, p->in, p->weight_stride);
+        pack_a = grad && !on_boundary(p->a, p->in, p->in);
+        pack_b = !grad && !on_boundary(p->b, p->rank, p->rank);
+        pack_dy = grad && !on_boundary(p->dy, p->out, p->out);
+        x = take(pack_x, p->tokens * up8(p->in));
+        w = take(pack_w, p->out * up8(p->in));
+        a = take(pack_a, p->adapters * p->rank * up8(p->in));
+        b = take(pack_b, p->adapters * p->out * up8(p->rank));
+        dy = take(pack_dy, p->tokens * up8(p->out));
+        g = take(grad, p->tokens * 2 * up8(p->rank));
+    }
+};
+
+API size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p) { return p->tokens * 4 * up8(p->rank); }
+API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { return ProjectLayout(p, grad).end; }
+
+// out[o][r][0 .. up8(cols)) of a tensor with any strides.
+template <class T>
+static int launch_pack(const T *in, uint64_t outer, uint64_t so, uint64_t rows, uint64_t sr, uint64_t cols, uint64_t sc, T *out, cudaStream_t cs)
+{
+    const uint64_t total = outer * rows * up8(cols);
+    if (!total) return LMZ_GPU_OK;
+    k_pack<T><<<static_cast<unsigned>(std::min<uint64_t>((total + 255) / 256, 148 * 16)), 256, 0, cs>>>(in, so, sr, sc, rows, cols, up8(cols), total, out);
+    return launched("launch k_pack");
+}
+
+// y[t][f] = sum of x[t][k] W(f, k) + sum of h[t][j] F_i(f, j) (MN: W and F with their f next to each other).
+template <class T, bool MN>
+static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride, uint64_t k, const T *w, uint64_t w_stride, uint64_t feats, const T *factor,
+                          uint64_t factor_rows, uint64_t factor_row, const T *hidden, T *y, cudaStream_t cs)
+{
+    static bool done[64];
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    ProjectArgs<T> a{};
+    a.index = token_index(p), a.hidden = hidden, a.factor = factor, a.factor_each = factor_rows * factor_row, a.factor_row = factor_row;
+    a.y = y, a.tokens = p->tokens, a.feats = feats, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
+    a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K);
+    a.nt = P_GROUP;
+    while (a.nt < P_TOKENS && a.nt < p->tokens) a.nt *= 2;
+    a.feat_tiles = static_cast<uint32_t>((feats + P_FEATS - 1) / P_FEATS);
+    const uint64_t token_tiles = (p->tokens + a.nt - 1) / a.nt, tiles = a.feat_tiles * token_tiles;
+    if (tiles >= 1u << 31) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many tokens for a weight of this size");
+    a.token_tiles = static_cast<uint32_t>(token_tiles);
+    a.stage_bytes = project_stage_bytes(a.nt);
+    const uint32_t per_sm = a.nt <= 64 ? 2 : 1;
+    a.stages = std::min<uint32_t>(P_MAX_STAGES, (per_sm == 2 ? 100u << 10 : 200u << 10) / a.stage_bytes);
+    a.split = 1;
+    while (a.split < 8 && tiles * a.split * 2 <= (uint64_t)sms * per_sm && a.steps >= 8 * a.split) a.split *= 2;
+    a.tmem_columns = std::max(32u, a.split > 1 ? a.nt : 2 * a.nt);
+    rc = tensor_map(&a.x, x, std::is_same_v<T, __nv_bfloat16>, k, p->tokens, x_stride, a.nt);
+    if (!rc) rc = MN ? tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, feats, k, w_stride, STEP_K)
+                     : tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, k, feats, w_stride, P_FEATS);
+    if (rc) return rc;
+    rc = opt_in_smem(k_project<T, MN>, 201u << 10, done);
+    if (rc) return rc;
+    cudaLaunchConfig_t c{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = a.split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    c.gridDim = dim3(a.split > 1 ? static_cast<unsigned>(tiles * a.split) : static_cast<unsigned>(std::min<uint64_t>(tiles, (uint64_t)sms * per_sm)));
+    c.blockDim = dim3(P_THREADS), c.dynamicSmemBytes = a.stages * a.stage_bytes + ATOM_BYTES, c.stream = cs, c.attrs = &attr, c.numAttrs = 1;
+    CK("launch k_project", cudaLaunchKernelEx(&c, k_project<T, MN>, a));
+    return LMZ_GPU_OK;
+}
 
 template <class T>
 static int project_as(const lmz_projection *p, cudaStream_t cs)
 {
-    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight);
-    float *h = static_cast<float *>(p->hidden);
-    const uint64_t r = p->rank;
-    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in}, b{static_cast<const T *>(p->b), r * p->out, r, 1};
-    k_hidden<T><<<static_cast<unsigned>((p->tokens * r + 7) / 8), 256, 0, cs>>>(x, p->x_stride, p->in, a, token_index(p), p->tokens, p->rank, h);
-    int rc = launched("launch k_hidden");
+    const ProjectLayout l(p, false);
+    uint8_t *work = static_cast<uint8_t *>(p->work);
+    auto at = [&](uint64_t off) { return reinterpret_cast<T *>(work + off); };
+    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *fb = static_cast<const T *>(p->b);
+    uint64_t x_stride = p->x_stride, w_stride = p->weight_stride;
+    T *h = static_cast<T *>(p->hidden);
+    const uint64_t r = p->rank, rp = up8(r);
+    int rc = LMZ_GPU_OK;
+    if (l.pack_x) {
+        rc = launch_pack(x, 1, 0, p->tokens, x_stride, p->in, 1, at(l.x), cs);
+        x = at(l.x), x_stride = up8(p->in);
+    }
+    if (!rc && l.pack_w) {
+        rc = launch_pack(w, 1, 0, p->out, w_stride, p->in, 1, at(l.w), cs);
+        w = at(l.w), w_stride = up8(p->in);
+    }
+    if (!rc && l.pack_b) {
+        rc = launch_pack(fb, p->adapters, p->out * r, p->out, r, r, 1, at(l.b), cs);
+        fb = at(l.b);
+    }
     if (rc) return rc;
-    k_project<T><<<dim3(static_cast<unsigned>((p->tokens + 63) / 64), static_cast<unsigned>((p->out + 63) / 64)), 256, 0, cs>>>(
-        x, p->x_stride, p->in, w, p->weight_stride, 1, b, token_index(p), h, p->rank, p->tokens, p->out, static_cast<T *>(p->y));
-    return launched("launch k_project");
+    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in};
+    k_hidden<T><<<static_cast<unsigned>((p->tokens * rp + 7) / 8), 256, 0, cs>>>(x, x_stride, p->in, a, token_index(p), p->tokens, p->rank, (uint32_t)rp, h);
+    rc = launched("launch k_hidden");
+    if (rc) return rc;
+    return launch_project<T, false>(p, x, x_stride, p->in, w, w_stride, p->out, fb, p->out, rp, h, static_cast<T *>(p->y), cs);
 }
 
 template <class T>
 static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
 {
-    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *dy = static_cast<const T *>(p->dy);
-    const float *h = static_cast<const float *>(p->hidden);
-    float *g = static_cast<float *>(p->work);
-    const uint64_t r = p->rank;
-    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in}, b{static_cast<const T *>(p->b), r * p->out, r, 1};
+    const ProjectLayout l(p, true);
+    uint8_t *work = static_cast<uint8_t *>(p->work);
+    auto at = [&](uint64_t off) { return reinterpret_cast<T *>(work + off); };
+    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *dy = static_cast<const T *>(p->dy), *fa = static_cast<const T *>(p->a);
+    uint64_t w_stride = p->weight_stride, dy_stride = p->out, a_row = p->in;
+    const T *h = static_cast<const T *>(p->hidden);
+    T *g = at(l.g);
+    const uint64_t r = p->rank, rp = up8(r);
+    const Factor<T> b{static_cast<const T *>(p->b), r * p->out, r, 1};
     int rc = LMZ_GPU_OK;
     if (p->tokens && (p->dx || p->da)) {
-        k_hidden<T><<<static_cast<unsigned>((p->tokens * r + 7) / 8), 256, 0, cs>>>(dy, p->out, p->out, b, token_index(p), p->tokens, p->rank, g);
+        k_hidden<T><<<static_cast<unsigned>((p->tokens * rp + 7) / 8), 256, 0, cs>>>(dy, p->out, p->out, b, token_index(p), p->tokens, p->rank, (uint32_t)rp, g);
         rc = launched("launch k_hidden");
         if (rc) return rc;
     }
     if (p->tokens && p->dx) {
-        k_project<T><<<dim3(static_cast<unsigned>((p->tokens + 63) / 64), static_cast<unsigned>((p->in + 63) / 64)), 256, 0, cs>>>(
-            dy, p->out, p->out, w, 1, p->weight_stride, a, token_index(p), g, p->rank, p->tokens, p->in, static_cast<T *>(p->dx));
-        rc = launched("launch k_project");
+        const T *d = dy;
+        if (l.pack_dy) {
+            rc = launch_pack(dy, 1, 0, p->tokens, p->out, p->out, 1, at(l.dy), cs);
+            d = at(l.dy), dy_stride = up8(p->out);
+        }
+        if (!rc && l.pack_w) {
+            rc = launch_pack(w, 1, 0, p->out, w_stride, p->in, 1, at(l.w), cs);
+            w = at(l.w), w_stride = up8(p->in);
+        }
+        if (!rc && l.pack_a) {
+            rc = launch_pack(fa, p->adapters, r * p->in, r, p->in, p->in, 1, at(l.a), cs);
+            fa = at(l.a), a_row = up8(p->in);
+        }
+        if (!rc) rc = launch_project<T, true>(p, d, dy_stride, p->out, w, w_stride, p->in, fa, r, a_row, g, static_cast<T *>(p->dx), cs);
         if (rc) return rc;
     }
     if (p->da) {
         k_factor_grad<T><<<dim3(static_cast<unsigned>((p->in + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
-            g, x, p->x_stride, token_index(p), p->tokens, p->rank, p->in, static_cast<T *>(p->da), r * p->in, 1, p->in);
+            g, (uint32_t)rp, x, p->x_stride, token_index(p), p->tokens, p->rank, p->in, static_cast<T *>(p->da), r * p->in, 1, p->in);
         rc = launched("launch k_factor_grad");
         if (rc) return rc;
     }
     if (p->db) {
         k_factor_grad<T><<<dim3(static_cast<unsigned>((p->out + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
-            h, dy, p->out, token_index(p), p->tokens, p->rank, p->out, static_cast<T *>(p->db), r * p->out, r, 1);
+            h, (uint32_t)rp, dy, p->out, token_index(p), p->tokens, p->rank, p->out, static_cast<T *>(p->db), r * p->out, r, 1);
         rc = launched("launch k_factor_grad");
     }
     return rc;
+}
+
+API int lmz_gpu_ops_gave_up(void)
+{
+    uint32_t word = 0;
+    CK("cudaMemcpyFromSymbol", cudaMemcpyFromSymbol(&word, g_gave_up, sizeof word));
+    return word != 0;
 }
 
 API int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream)

@@ -1,0 +1,383 @@
+// The projection through a shared weight with low-rank adapters beside it, and by the same kernel the gradient of its input.
+#pragma once
+#include "adapter_kernels.cuh"
+#include "tcgen.cuh"
+
+namespace lmz {
+
+constexpr uint32_t P_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
+constexpr uint32_t P_TOKENS = 256;             // most tokens of a tile: its N, a TMEM column each
+constexpr uint32_t P_GROUP = 16;               // tokens that are looked at together: N counts in sixteens
+constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 8;
+constexpr uint32_t P_EPILOGUE = 128, P_FEED = 128, P_THREADS = P_EPILOGUE + P_FEED + 64;
+
+// What a tile's tokens have for adapters.
+struct TileInfo {
+    int32_t adapter[P_TOKENS];                 // per token, -1: none
+    uint32_t mixed;                            // bit per group: its tokens have different adapters
+    uint32_t runs;
+    struct { int32_t adapter; uint32_t column, tokens; } run[P_TOKENS / P_GROUP];
+};
+
+struct ProjectShared {
+    uint64_t full[P_MAX_STAGES], empty[P_MAX_STAGES];
+    uint64_t info_full[P_INFOS], info_empty[P_INFOS];
+    uint64_t loaded[P_INFOS], fed[P_INFOS];    // a tile's steps of the weight, and of the adapters, have all got their stages
+    uint64_t sums_full[2], sums_empty[2];
+    uint32_t tmem, over;
+    uint32_t same[P_TOKENS / 32];              // bit 0, 1: the tokens of these two groups have one adapter
+    TileInfo info[P_INFOS];
+};
+
+template <class T>
+struct ProjectArgs {
+    CUtensorMap x, w;
+    TokenIndex index;
+    const T *hidden;                           // [token][2][rp]: the thin product, its upper and its lower half
+    const T *factor;                           // of adapter i from i * factor_each; rows of factor_row elements, multiples of 8
+    uint64_t factor_each, factor_row;
+    T *y;
+    uint64_t tokens, feats;
+    uint32_t rank, rp;                         // rp: rank up to a multiple of 8
+    uint32_t steps;                            // of 64 along K
+    uint32_t nt;                               // tokens of a tile
+    uint32_t split;                            // CTAs of a cluster that share K
+    uint32_t feat_tiles, token_tiles;
+    uint32_t stages, stage_bytes, tmem_columns;
+};
+
+__host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt) { return P_FEATS * ROW_BYTES + nt * ROW_BYTES; }
+
+// Eight elements of a factor times eight of h (upper and lower halves).
+template <class T>
+__device__ __forceinline__ float dot8(const Vec<T, 16> &f, const Vec<T, 16> &hi, const Vec<T, 16> &lo, float sum)
+{
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum += (widen(hi.e[e]) + widen(lo.e[e])) * widen(f.e[e]);
+    return sum;
+}
+
+// What the adapters add to one feature of sixteen tokens that have different ones.  Not on the tensor core: a factor
+// multiplied by the zeros of tokens it does not belong to would still hand them its infinities and NaN.
+template <class T, bool MN>
+__device__ __forceinline__ void add_mixed(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f, float *v)
+{
+    constexpr int BATCH = 4;
+#pragma unroll
+    for (int c0 = 0; c0 < static_cast<int>(P_GROUP); c0 += BATCH) {
+        float sum[BATCH] = {};
+        for (uint32_t j = 0; j < a.rp; j += 8) {
+            Vec<T, 16> fac[BATCH], hi[BATCH], lo[BATCH];
+#pragma unroll
+            for (int c = 0; c < BATCH; c++) {
+                const int i = adapter[c0 + c];
+                fac[c].raw = hi[c].raw = lo[c].raw = {};
+                if (i < 0) continue;
+                const T *h = a.hidden + (t0 + c0 + c) * 2 * a.rp + j;
+                hi[c].raw = *reinterpret_cast<const uint4 *>(h);
+                lo[c].raw = *reinterpret_cast<const uint4 *>(h + a.rp);
+                const T *p = a.factor + i * a.factor_each;
+                if constexpr (MN) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++)
+                        if (j + e < a.rank) fac[c].e[e] = p[(j + e) * a.factor_row + f];
+                } else {
+                    fac[c].raw = *reinterpret_cast<const uint4 *>(p + f * a.factor_row + j);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < BATCH; c++) sum[c] = dot8(fac[c], hi[c], lo[c], sum[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < BATCH; c++)
+            if (adapter[c0 + c] >= 0) v[c0 + c] += sum[c];
+    }
+}
+
+// Sixteen tokens' sums of a lane's feature, to y: two lanes exchange halves, so that a store has two features.
+template <class T>
+__device__ __forceinline__ void store_group(const ProjectArgs<T> &a, uint64_t t0, uint64_t f, bool pairs, const float *v)
+{
+    const uint32_t odd = threadIdx.x & 1;
+#pragma unroll
+    for (int c = 0; c < static_cast<int>(P_GROUP); c += 2) {
+        if (pairs) {
+            const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
+            union { T e[2]; uint32_t raw; } both;
+            both.e[0] = narrow<T>(odd ? got : v[c]);
+            both.e[1] = narrow<T>(odd ? v[c + 1] : got);
+            const uint64_t t = t0 + c + odd;
+            if (t < a.tokens && f < a.feats) *reinterpret_cast<uint32_t *>(a.y + t * a.feats + (f & ~1ull)) = both.raw;
+        } else if (f < a.feats) {
+            if (t0 + c < a.tokens) a.y[(t0 + c) * a.feats + f] = narrow<T>(v[c]);
+            if (t0 + c + 1 < a.tokens) a.y[(t0 + c + 1) * a.feats + f] = narrow<T>(v[c + 1]);
+        }
+    }
+}
+
+// y[t][f] = sum over k of x[t][k] W(f, k) + sum over j of h[t][j] F_i(f, j), i = index[t].
+// MN false: W is [f][k], F_i [f][j] (the projection).  MN true: W is [k][f], F_i [j][f] (the gradient of its input: x is
+// dy, k runs over the output's features, h is g).
+//
+// Features are the tensor core's M and tokens its N, whatever their number: a single token streams the weight past 16 columns,
+// a prompt past 256, and what an adapter adds to a run of its own tokens is one more product into just their columns.
+//
+// Roles: a TMA warp loads tiles of W and x (64 along K) into a ring of stages; four warps feed the ring with what adapters
+// need (h and a factor's tile: 2 rp wide, the factor beside both halves of h); one thread issues the MMAs; four warps take
+// the sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.
+// Few tiles: the CTAs of a cluster share K, and their sums meet in distributed shared memory.
+template <class T, bool MN>
+__global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant__ ProjectArgs<T> a)
+{
+    extern __shared__ uint8_t p_smem[];
+    __shared__ ProjectShared s;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
+    const uint32_t first = blockIdx.x / a.split, stride = gridDim.x / a.split, tiles = a.feat_tiles * a.token_tiles;
+    const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split);
+    const uint32_t k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
+    const uint32_t ring = (smem_addr(p_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
+    const uint32_t wide = (2 * a.rp + STEP_K - 1) / STEP_K;      // steps of a run
+    volatile uint32_t *over = &s.over;
+
+    if (tid == 0) {
+        s.over = 0;
+        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
+        for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], 2 + P_EPILOGUE / 32), bar_init(&s.loaded[i], 1), bar_init(&s.fed[i], 1);
+        for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], P_EPILOGUE / 32);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(&s.tmem, a.tmem_columns);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s.tmem;
+
+    // Eight token tiles side by side, features outside: what a wave reads of x and W stays in L2.
+    auto place = [&](uint32_t tile, uint32_t &ft, uint32_t &tt) {
+        const uint32_t band = 8 * a.feat_tiles, b = tile / band, in = tile - b * band;
+        const uint32_t w = a.token_tiles - 8 * b < 8 ? a.token_tiles - 8 * b : 8;
+        ft = in / w, tt = 8 * b + in % w;
+    };
+    auto mine = [&](uint32_t run) { return run % a.split == rank; };
+
+    if (warp == 8) {
+        if (lane == 0) {
+            uint32_t at = 0, n = 0, filled = 0;
+            for (uint32_t tile = first; tile < tiles && !*over; tile += stride, n++) {
+                uint32_t ft, tt;
+                place(tile, ft, tt);
+                for (uint32_t k = k0; k < k1; k++, at++) {
+                    const uint32_t st = at % a.stages;
+                    if (at >= a.stages && !bar_wait(&s.empty[st], (at / a.stages - 1) & 1, over)) break;
+                    const uint32_t dst = ring + st * a.stage_bytes;
+                    bar_expect(&s.full[st], a.stage_bytes);
+                    if constexpr (MN) {
+                        tma_load_2d(&a.w, &s.full[st], dst, ft * P_FEATS, k * STEP_K);
+                        tma_load_2d(&a.w, &s.full[st], dst + STEP_K * ROW_BYTES, ft * P_FEATS + 64, k * STEP_K);
+                    } else {
+                        tma_load_2d(&a.w, &s.full[st], dst, k * STEP_K, ft * P_FEATS);
+                    }
+                    tma_load_2d(&a.x, &s.full[st], dst + P_FEATS * ROW_BYTES, k * STEP_K, tt * a.nt);
+                    filled = at + 1;
+                }
+                if (*over) break;
+                bar_arrive(&s.loaded[n % P_INFOS]);
+                if (!bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+                const TileInfo &info = s.info[n % P_INFOS];
+                uint32_t steps = 0;
+                for (uint32_t r = 0; r < info.runs; r++) steps += mine(r) ? wide : 0;
+                at += steps;
+                bar_arrive(&s.info_empty[n % P_INFOS]);
+                // A parity tells two phases apart, no more: whoever has skipped a whole turn of the ring first waits for the
+                // others' last stage in it.
+                if (steps >= a.stages && !bar_wait(&s.fed[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+            }
+            if (*over)                                           // nothing may still be on its way into this block's memory
+                for (uint32_t i = filled > a.stages ? filled - a.stages : 0; i < filled; i++)
+                    for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.full[i % a.stages], (i / a.stages) & 1); tries++) {}
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            const uint32_t a_step = MN ? 16 * ROW_BYTES : 32, a_block = MN ? STEP_K * ROW_BYTES : 16;
+            const bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+            uint32_t at = 0, n = 0;
+            for (uint32_t tile = first; tile < tiles && !*over; tile += stride, n++) {
+                const uint32_t buf = n & 1, sums = tmem + buf * a.nt;
+                if (n >= 2 && !bar_wait(&s.sums_empty[buf], (n / 2 - 1) & 1, over)) break;
+                tc_after();
+                const uint32_t desc = mma_desc(bf16, MN, false, P_FEATS, a.nt);
+                for (uint32_t k = k0; k < k1; k++, at++) {
+                    const uint32_t st = at % a.stages, src = ring + st * a.stage_bytes;
+                    if (!bar_wait(&s.full[st], (at / a.stages) & 1, over)) break;
+                    tc_after();
+#pragma unroll
+                    for (uint32_t c = 0; c < STEP_K / 16; c++)
+                        mma16(sums, tile_desc(src + c * a_step, a_block), tile_desc(src + P_FEATS * ROW_BYTES + c * 32, 16), desc, k != k0 || c);
+                    mma_commit(&s.empty[st]);
+                }
+                if (*over || !bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+                const TileInfo &info = s.info[n % P_INFOS];
+                for (uint32_t r = 0; r < info.runs && !*over; r++) {
+                    if (!mine(r)) continue;
+                    const uint32_t column = info.run[r].column, rdesc = mma_desc(bf16, MN, false, P_FEATS, info.run[r].tokens);
+                    for (uint32_t v = 0; v < 2 * a.rp; v += STEP_K, at++) {
+                        const uint32_t st = at % a.stages, src = ring + st * a.stage_bytes;
+                        if (!bar_wait(&s.full[st], (at / a.stages) & 1, over)) break;
+                        tc_after();
+                        for (uint32_t c = 0; c < STEP_K / 16 && v + c * 16 < 2 * a.rp; c++)
+                            mma16(sums + column, tile_desc(src + c * a_step, a_block),
+                                  tile_desc(src + P_FEATS * ROW_BYTES + column * ROW_BYTES + c * 32, 16), rdesc, true);
+                        mma_commit(&s.empty[st]);
+                    }
+                }
+                bar_arrive(&s.info_empty[n % P_INFOS]);
+                mma_commit(&s.sums_full[buf]);
+            }
+            if (*over) {                                         // the products under way end before their memory goes
+                mma_commit(&s.sums_full[n & 1]);
+                for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums_full[n & 1], (n / 2) & 1); tries++) {}
+            }
+        }
+    } else if (warp >= 4) {
+        const uint32_t id = tid - P_EPILOGUE;
+        auto look = [&](uint32_t tile, uint32_t n) {             // the tile's tokens and their adapters
+            uint32_t ft, tt;
+            place(tile, ft, tt);
+            TileInfo &info = s.info[n % P_INFOS];
+            if (!sync_all(1, P_FEED, n < P_INFOS || bar_wait(&s.info_empty[n % P_INFOS], (n / P_INFOS - 1) & 1, over))) return false;
+            const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt;
+            for (uint32_t c = id; c < P_TOKENS; c += P_FEED) {
+                const bool in = c < a.nt && t0 + c < a.tokens;
+                const int i = in ? a.index.of(t0 + c) : -1;
+                info.adapter[c] = i;
+                const int head = __shfl_sync(~0u, i, lane & 16);
+                const uint32_t agree = __ballot_sync(~0u, !in || i == head);
+                if (lane == 0) s.same[c / 32] = ((agree & 0xFFFF) == 0xFFFF) | ((agree >> 16) == 0xFFFF) << 1;
+            }
+            sync_threads(1, P_FEED);
+            if (id == 0) {
+                uint32_t runs = 0, mixed = 0, end = ~0u;
+                for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
+                    const int i = info.adapter[g * P_GROUP];
+                    if (!(s.same[g / 2] >> (g & 1) & 1)) {
+                        mixed |= 1u << g;
+                    } else if (i >= 0) {
+                        if (end == g && info.run[runs - 1].adapter == i) info.run[runs - 1].tokens += P_GROUP;
+                        else info.run[runs].adapter = i, info.run[runs].column = g * P_GROUP, info.run[runs].tokens = P_GROUP, runs++;
+                        end = g + 1;
+                    }
+                }
+                info.mixed = mixed, info.runs = runs;
+                bar_arrive(&s.info_full[n % P_INFOS]);
+            }
+            sync_threads(1, P_FEED);
+            return true;
+        };
+        uint32_t at = 0, n = 0;
+        bool go = first < tiles && look(first, 0);
+        for (uint32_t tile = first; go && tile < tiles; tile += stride, n++) {
+            if (tile + stride < tiles) go = look(tile + stride, n + 1);
+            uint32_t ft, tt;
+            place(tile, ft, tt);
+            const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = static_cast<uint64_t>(ft) * P_FEATS;
+            const TileInfo &info = s.info[n % P_INFOS];
+            at += k1 - k0;
+            if (!sync_all(1, P_FEED, go && bar_wait(&s.loaded[n % P_INFOS], (n / P_INFOS) & 1, over))) break;
+            for (uint32_t r = 0; go && r < info.runs; r++) {
+                if (!mine(r)) continue;
+                const T *factor = a.factor + info.run[r].adapter * a.factor_each;
+                for (uint32_t v0 = 0; v0 < 2 * a.rp; v0 += STEP_K, at++) {
+                    const uint32_t st = at % a.stages, fdst = ring + st * a.stage_bytes, hdst = fdst + P_FEATS * ROW_BYTES;
+                    if (!sync_all(1, P_FEED, at < a.stages || bar_wait(&s.empty[st], (at / a.stages - 1) & 1, over))) { go = false; break; }
+                    const uint32_t parts = (2 * a.rp - v0 < STEP_K ? 2 * a.rp - v0 : STEP_K) / 8;
+                    if constexpr (MN) {                          // a row per j of the rank, 64 features a block
+                        for (uint32_t e = id; e < parts * 8 * 16; e += P_FEED) {
+                            const uint32_t row = e >> 4, c = e & 15, v = v0 + row, j = v < a.rp ? v : v - a.rp;
+                            const uint64_t f = f0 + c * 8;
+                            const bool on = j < a.rank && f < a.feats;
+                            copy16(fdst + (c >> 3) * STEP_K * ROW_BYTES + swizzled(row, c & 7), on ? factor + j * a.factor_row + f : factor, on);
+                        }
+                    } else {                                     // a row per feature
+                        for (uint32_t e = id; e < P_FEATS * 8; e += P_FEED) {
+                            const uint32_t row = e >> 3, c = e & 7, v = v0 + c * 8, j = v < a.rp ? v : v - a.rp;
+                            const uint64_t f = f0 + row;
+                            const bool on = c < parts && f < a.feats;
+                            if (c < parts) copy16(fdst + swizzled(row, c), on ? factor + f * a.factor_row + j : factor, on);
+                        }
+                    }
+                    for (uint32_t e = id; e < info.run[r].tokens * 8; e += P_FEED) {
+                        const uint32_t row = info.run[r].column + (e >> 3), c = e & 7;
+                        const uint64_t t = t0 + row;
+                        const bool on = t < a.tokens;
+                        if (c < parts) copy16(hdst + swizzled(row, c), on ? a.hidden + t * 2 * a.rp + v0 + c * 8 : a.hidden, on);
+                    }
+                    copies_commit();
+                    copies_wait<0>();
+                    publish_smem();
+                    sync_threads(1, P_FEED);
+                    if (id == 0) bar_arrive(&s.full[st]);
+                }
+            }
+            if (id == 0) bar_arrive(&s.fed[n % P_INFOS]);
+        }
+    } else {
+        const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
+        uint32_t n = 0;
+        for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
+            uint32_t ft, tt;
+            place(tile, ft, tt);
+            const uint32_t buf = n & 1;
+            if (!__all_sync(~0u, bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over) && bar_wait(&s.sums_full[buf], (n / 2) & 1, over))) break;
+            tc_after();
+            const TileInfo &info = s.info[n % P_INFOS];
+            const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
+                if (a.split == 1 && t0 + g * P_GROUP >= a.tokens) break;
+                float v[P_GROUP];
+                tmem_load16(tmem + (warp << 21) + buf * a.nt + g * P_GROUP, v);
+                if (a.split > 1) {                               // (the stages are free: all products have ended)
+                    float *sums = reinterpret_cast<float *>(p_smem + (ring - smem_addr(p_smem)));
+#pragma unroll
+                    for (uint32_t c = 0; c < P_GROUP; c++) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
+                } else {
+                    if (info.mixed >> g & 1 && f < a.feats) add_mixed<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f, v);
+                    __syncwarp();
+                    store_group(a, t0 + g * P_GROUP, f, pairs, v);
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&s.sums_empty[buf]), bar_arrive(&s.info_empty[n % P_INFOS]);
+        }
+    }
+    __syncwarp();
+    if (a.split > 1) {                                           // one tile per cluster: its CTAs take its groups in turn
+        cluster_barrier();
+        if (warp < 4 && !*over && first < tiles) {
+            uint32_t ft, tt;
+            place(first, ft, tt);
+            const TileInfo &info = s.info[0];
+            const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
+            const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            for (uint32_t g = rank; g * P_GROUP < a.nt && t0 + g * P_GROUP < a.tokens; g += a.split) {
+                float v[P_GROUP] = {};
+                for (uint32_t q = 0; q < a.split; q++)
+#pragma unroll
+                    for (uint32_t c = 0; c < P_GROUP; c++) v[c] += peer_float(ring + ((g * P_GROUP + c) * P_FEATS + tid) * 4, q);
+                if (info.mixed >> g & 1 && f < a.feats) add_mixed<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f, v);
+                __syncwarp();
+                store_group(a, t0 + g * P_GROUP, f, pairs, v);
+            }
+        }
+        cluster_barrier();
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_after();
+        tmem_free(tmem, a.tmem_columns);
+    }
+}
+
+}  // namespace lmz

@@ -1,0 +1,161 @@
+// Fifth-generation tensor cores, TMA and mbarriers of sm_100a, as the projection kernels use them.
+//
+// Operand tiles lie in shared memory in 128-byte rows whose 16-byte parts are swizzled by the row's number (what TMA's 128-byte
+// swizzle writes): either a row per M or N index with 64 consecutive K elements (K-major), or a row per K index with 64
+// consecutive M or N elements, further 64 of them in a block of their own (MN-major).  Tiles start on 1024 bytes.
+#pragma once
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+namespace lmz {
+
+constexpr uint32_t ROW_BYTES = 128, ATOM_BYTES = 1024, STEP_K = 64;
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// ---- mbarriers
+
+__device__ __forceinline__ void bar_init(uint64_t *b, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *b)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t *b, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(smem_addr(b)), "r"(parity) : "memory");
+    return done;
+}
+
+// Set once a wait has run out (no wait does unless the hardware loses a copy): lmz_gpu_ops_gave_up() tells the host.
+static __device__ uint32_t g_gave_up;
+
+// Wait for a phase, but not for ever: after WAIT_TRIES (each a few microseconds at most) the block's waits are all over,
+// and with them its work; `over` is the block's flag.
+constexpr uint32_t WAIT_TRIES = 1u << 20;
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile uint32_t *over)
+{
+    for (uint32_t i = 0; i < WAIT_TRIES; i++) {
+        if (bar_try(b, parity)) return true;
+        if ((i & 63) == 63 && *over) return false;
+    }
+    *over = 1;
+    g_gave_up = 1;
+    return false;
+}
+
+// ---- asynchronous copies
+
+__device__ __forceinline__ void tma_load_2d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// 16 bytes from global to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// What this thread has written to shared memory becomes visible to the tensor core.
+__device__ __forceinline__ void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Where 16-byte part c of row r of a tile lies.
+__device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * ROW_BYTES + ((c ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ void sync_threads(uint32_t barrier, uint32_t threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+
+// Whether `ok` holds for all threads that come to a barrier.
+__device__ __forceinline__ bool sync_all(uint32_t barrier, uint32_t threads, bool ok)
+{
+    uint32_t all;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbarrier.cta.red.and.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(all) : "r"(barrier), "r"(threads), "r"(static_cast<uint32_t>(ok)) : "memory");
+    return all;
+}
+
+// ---- tensor cores
+
+__device__ __forceinline__ void tmem_alloc(uint32_t *at, uint32_t columns)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// A tile's descriptor.  K-major: eight rows of 128 bytes, 1024 bytes to the next eight.  MN-major: eight K indices, 1024 bytes to
+// the next eight; `block` bytes to the next 64 M or N elements.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block)
+{
+    return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(block >> 4) << 16 | static_cast<uint64_t>(ATOM_BYTES >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+// 16-bit operands of one type, sums in 32 bits.
+__device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, uint32_t m, uint32_t n)
+{
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (m >> 4) << 24;
+}
+// D (+)= A B^T over 16 K elements.
+__device__ __forceinline__ void mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add)
+{
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add)) : "memory");
+}
+// The barrier gets an arrival when all MMAs issued so far have ended.
+__device__ __forceinline__ void mma_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Sixteen columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_load16(uint32_t at, float *v)
+{
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// ---- clusters
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of another CTA's shared memory, by this CTA's address of it.
+__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank)
+{
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+}  // namespace lmz

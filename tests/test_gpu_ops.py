@@ -181,6 +181,8 @@ def _index(kind, tokens, n, seed=20):
         return None
     if kind == "mixed":
         v = rng.integers(-1, n, tokens)
+    elif kind == "short":                                  # many runs in every tile
+        v = np.repeat(rng.integers(0, n, tokens // 32 + 1), 32)[:tokens]
     elif kind == "off":
         v = np.full(tokens, -1)
     elif kind == "far":                                    # outside on both sides
@@ -261,6 +263,9 @@ SHAPES = [
     (17, 72, 200, 64, 5, "mixed"), (33, 1024, 384, 24, 6, "runs"), (64, 320, 640, 16, 48, "mixed"), (100, 128, 96, 128, 3, "mixed"),
     (129, 200, 264, 256, 2, "runs"), (255, 192, 520, 32, 9, "runs"), (300, 448, 128, 16, 1, "none"), (513, 256, 512, 40, 4, "runs"),
     (640, 128, 1032, 16, 70, "mixed"), (1000, 512, 256, 64, 2, "runs"), (257, 128, 256, 16, 3, "off"), (40, 128, 256, 16, 3, "far"), (1500, 64, 136, 8, 7, "far"),
+    # more tiles than multiprocessors, more steps than a ring has stages, more runs than that too
+    (2600, 64, 2200, 16, 5, "runs"), (2600, 648, 2056, 40, 30, "short"), (4700, 1400, 1288, 8, 3, "runs"), (900, 1032, 5000, 100, 12, "short"),
+    (2300, 776, 2200, 16, 40, "mixed"), (200, 2048, 264, 64, 6, "short"),
     # sizes where rows do not start on a boundary
     (5, 1, 1, 1, 1, "none"), (9, 33, 65, 3, 2, "mixed"), (333, 777, 501, 5, 5, "runs"), (70, 250, 1001, 7, 4, "mixed"), (600, 100, 77, 12, 3, "runs"),
 ]
