@@ -1,0 +1,165 @@
+// The thin products h = s x A^T and g = s dy B.
+#pragma once
+#include "adapter_kernels.cuh"
+#include "tcgen.cuh"
+
+namespace lmz {
+
+constexpr uint32_t H_TOKENS = 128;             // tokens of a tile: the tensor core's M, a TMEM lane each
+constexpr uint32_t H_COLUMNS = 256;            // most columns of a tile: its N
+constexpr uint32_t H_THREADS = H_TOKENS + 64, H_MAX_STAGES = 8;
+constexpr uint32_t H_PITCH = H_TOKENS + 1;     // of the partial sums in shared memory: neighbouring columns in neighbouring banks
+
+struct HiddenShared {
+    uint64_t full[H_MAX_STAGES], empty[H_MAX_STAGES], sums;
+    uint32_t tmem, over, present;
+    int32_t adapter[H_TOKENS];                 // per token
+    int32_t list[H_TOKENS];                    // the tile's adapters in the order of their first tokens
+    int32_t slot[H_TOKENS];                    // per token: where its adapter stands in that list, -1: none
+    uint32_t firsts[H_TOKENS / 32];
+};
+
+template <class T>
+struct HiddenArgs {
+    CUtensorMap x, f;                          // f: adapters x rank x K
+    TokenIndex index;
+    T *h;                                      // [token][2][rp]
+    uint64_t tokens;
+    uint32_t rank, rp, steps, split;
+    uint32_t each;                             // adapters of a block: as many as have room in H_COLUMNS columns
+    uint32_t stages, stage_bytes, tmem_columns;
+};
+
+// h[t][j] = s_i * sum over k of x[t][k] F_i[j][k], for tokens with an adapter, as two halves.
+//
+// A block multiplies 128 tokens by up to 256 / rp of the adapters they have side by side, and each token keeps the columns of
+// its own: nothing of another adapter or token comes into a sum.  Reads x once per 256 columns of present adapters (for one
+// adapter, and for most batches of prompts: once) and is bound by that; for few tokens by latency, so K is shared by the CTAs
+// of a cluster and their sums meet in distributed shared memory.
+template <class T>
+__global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ HiddenArgs<T> a)
+{
+    extern __shared__ uint8_t h_smem[];
+    __shared__ HiddenShared s;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
+    const uint32_t tile = blockIdx.x / a.split;
+    const uint64_t t0 = static_cast<uint64_t>(tile) * H_TOKENS;
+    const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split);
+    const uint32_t k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
+    const uint32_t ring = (smem_addr(h_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
+    volatile uint32_t *over = &s.over;
+
+    // Which adapters the tile has: a token is its adapter's first if none before it has it.
+    if (tid == 0) {
+        s.over = 0;
+        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
+        bar_init(&s.sums, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    int mine = -1;
+    if (tid < H_TOKENS) {
+        if (t0 + tid < a.tokens) mine = a.index.of(t0 + tid);
+        s.adapter[tid] = mine;
+    }
+    __syncthreads();
+    uint32_t first = 0;
+    if (tid < H_TOKENS) {
+        if (a.index.ids) while (s.adapter[first] != mine) first++;
+        const uint32_t firsts = __ballot_sync(~0u, first == tid && mine >= 0);
+        if (lane == 0) s.firsts[warp] = firsts;
+    }
+    __syncthreads();
+    if (tid < H_TOKENS) {
+        uint32_t at = __popc(s.firsts[first >> 5] & ((1u << (first & 31)) - 1));
+        for (uint32_t w = 0; w < first >> 5; w++) at += __popc(s.firsts[w]);
+        s.slot[tid] = mine >= 0 ? static_cast<int>(at) : -1;
+        if (first == tid && mine >= 0) s.list[at] = mine;
+    }
+    const uint32_t present = __popc(s.firsts[0]) + __popc(s.firsts[1]) + __popc(s.firsts[2]) + __popc(s.firsts[3]);
+    const uint32_t from = blockIdx.y * a.each;
+    if (from >= present) return;                                 // (all CTAs of the cluster)
+    const uint32_t count = present - from < a.each ? present - from : a.each;
+    if (warp == 5) tmem_alloc(&s.tmem, a.tmem_columns);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            uint32_t n = 0;
+            for (uint32_t k = k0; k < k1; k++, n++) {
+                const uint32_t st = n % a.stages, dst = ring + st * a.stage_bytes;
+                if (n >= a.stages && !bar_wait(&s.empty[st], (n / a.stages - 1) & 1, over)) break;
+                bar_expect(&s.full[st], H_TOKENS * ROW_BYTES + count * a.rank * ROW_BYTES);
+                tma_load_2d(&a.x, &s.full[st], dst, k * STEP_K, tile * H_TOKENS);
+                for (uint32_t i = 0; i < count; i++)
+                    tma_load_3d(&a.f, &s.full[st], dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
+            }
+            if (*over)                                           // nothing may still be on its way into this block's memory
+                for (uint32_t i = n > a.stages ? n - a.stages : 0; i < n; i++)
+                    for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.full[i % a.stages], (i / a.stages) & 1); tries++) {}
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), false, false, H_TOKENS, (count * a.rp + 15) & ~15u);
+            uint32_t n = 0;
+            for (uint32_t k = k0; k < k1; k++, n++) {
+                const uint32_t st = n % a.stages, src = ring + st * a.stage_bytes;
+                if (!bar_wait(&s.full[st], (n / a.stages) & 1, over)) break;
+                tc_after();
+#pragma unroll
+                for (uint32_t c = 0; c < STEP_K / 16; c++)
+                    mma16(tmem, tile_desc(src + c * 32, 16), tile_desc(src + H_TOKENS * ROW_BYTES + c * 32, 16), desc, n || c);
+                mma_commit(&s.empty[st]);
+            }
+            mma_commit(&s.sums);
+            if (*over)
+                for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums, 0); tries++) {}
+        }
+    } else if (__all_sync(~0u, bar_wait(&s.sums, 0, over))) {
+        // every token's own columns, over the stages (all products have ended)
+        tc_after();
+        float *part = reinterpret_cast<float *>(h_smem + (ring - smem_addr(h_smem)));
+        const int slot = s.slot[tid] - static_cast<int>(from);
+        for (uint32_t i = 0; i < count; i++) {
+            if (!__any_sync(~0u, slot == static_cast<int>(i))) continue;
+            for (uint32_t c = 0; c < a.rp; c += 8) {
+                float v[8];
+                tmem_load8(tmem + (warp << 21) + i * a.rp + c, v);
+                if (slot == static_cast<int>(i)) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) part[(c + e) * H_PITCH + tid] = v[e];
+                }
+            }
+        }
+        tc_before();
+    }
+    __syncwarp();
+    if (a.split > 1) cluster_barrier();
+    else __syncthreads();
+    if (!*over) {                                                // a CTA's share of the tokens: the sums of all, in order
+        const uint32_t each = H_TOKENS / a.split, lo = rank * each;
+        for (uint32_t e = tid; e < each * a.rp; e += H_THREADS) {
+            const uint32_t row = lo + e / a.rp, c = e % a.rp;
+            const int slot = s.slot[row] - static_cast<int>(from);
+            if (slot < 0 || slot >= static_cast<int>(count)) continue;
+            float sum = 0;
+            for (uint32_t q = 0; q < a.split; q++) sum += peer_float(ring + (c * H_PITCH + row) * 4, q);
+            T hi, lo_half;
+            split_halves(c < a.rank ? sum * a.index.scale_of(s.adapter[row]) : 0.0f, hi, lo_half);
+            T *to = a.h + (t0 + row) * 2 * a.rp + c;
+            to[0] = hi, to[a.rp] = lo_half;
+        }
+    }
+    if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums
+    tc_before();
+    __syncthreads();
+    if (warp == 5) {
+        tc_after();
+        tmem_free(tmem, a.tmem_columns);
+    }
+}
+
+}  // namespace lmz

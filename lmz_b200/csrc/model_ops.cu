@@ -7,6 +7,9 @@
 
 #include "../../include/lmz_b200.h"
 #include "adapter_kernels.cuh"
+#include "factor_grad_kernel.cuh"
+#include "hidden_kernel.cuh"
+#include "merge_kernel.cuh"
 #include "project_kernel.cuh"
 #include "rows_kernels.cuh"
 
@@ -211,8 +214,9 @@ static uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
 // Rows of 16-bit elements that TMA and 16-byte copies take as they lie.
 static bool on_boundary(const void *p, uint64_t cols, uint64_t stride) { return address(p) % 16 == 0 && stride % 8 == 0 && stride >= cols; }
 
-// A tensor map of [planes] x rows x cols 16-bit elements, tiles of 64 columns with the 128-byte swizzle.
-static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows)
+// A tensor map of planes x rows x cols 16-bit elements, a plane's rows behind those of the plane before: tiles of 64 columns
+// with the 128-byte swizzle.
+static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0)
 {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -223,36 +227,39 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
         return reinterpret_cast<Encode>(f);
     }();
     if (!encode) return fail_msg(LMZ_GPU_EUNSUPPORTED, "the driver makes no tensor maps");
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
-    const cuuint32_t box[2] = {STEP_K, tile_rows}, steps[2] = {1, 1};
-    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(p), dims, strides, box,
-                              steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {stride * 2, stride * rows * 2};
+    const cuuint32_t box[3] = {STEP_K, tile_rows, 1}, steps[3] = {1, 1, 1};
+    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes ? 3 : 2, const_cast<void *>(p), dims,
+                              strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? LMZ_GPU_OK : report(LMZ_GPU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
 // What a projection's kernels read in place of tensors that do not lie on boundaries, and between each other.
 struct ProjectLayout {
-    uint64_t x = 0, w = 0, a = 0, b = 0, dy = 0, g = 0, end = 0;
+    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, end = 0;
     bool pack_x, pack_w, pack_a, pack_b, pack_dy;
     ProjectLayout(const lmz_projection *p, bool grad)
     {
-        auto take = [&](bool on, uint64_t elements) {
+        auto take = [&](bool on, uint64_t bytes) {
             const uint64_t r = end;
-            if (on) end += up256(elements * 2);
+            if (on) end += up256(bytes);
             return r;
         };
-        pack_x = !grad && !on_boundary(p->x, p->in, p->x_stride);
+        pack_x = !on_boundary(p->x, p->in, p->x_stride);
         pack_w = !on_boundary(p->weight, p->in, p->weight_stride);
-        pack_a = grad && !on_boundary(p->a, p->in, p->in);
-        pack_b = !grad && !on_boundary(p->b, p->rank, p->rank);
+        pack_a = !on_boundary(p->a, p->in, p->in);
+        pack_b = grad || !on_boundary(p->b, p->rank, p->rank);   // (the gradients' transposed: [adapter][rank][out])
         pack_dy = grad && !on_boundary(p->dy, p->out, p->out);
-        x = take(pack_x, p->tokens * up8(p->in));
-        w = take(pack_w, p->out * up8(p->in));
-        a = take(pack_a, p->adapters * p->rank * up8(p->in));
-        b = take(pack_b, p->adapters * p->out * up8(p->rank));
-        dy = take(pack_dy, p->tokens * up8(p->out));
-        g = take(grad, p->tokens * 2 * up8(p->rank));
+        x = take(pack_x, p->tokens * up8(p->in) * 2);
+        w = take(pack_w, p->out * up8(p->in) * 2);
+        a = take(pack_a, p->adapters * p->rank * up8(p->in) * 2);
+        b = take(pack_b, 2 * p->adapters * (grad ? p->rank * up8(p->out) : p->out * up8(p->rank)));
+        dy = take(pack_dy, p->tokens * up8(p->out) * 2);
+        g = take(grad, p->tokens * 4 * up8(p->rank));
+        const bool sorted = grad && p->index;
+        for (int i = 0; i < 2; i++) keys[i] = take(sorted, p->tokens * 4), pos[i] = take(sorted, p->tokens * 4);
+        start = take(sorted, (p->adapters + 1ull) * 4);
     }
 };
 
@@ -268,6 +275,24 @@ static int launch_pack(const T *in, uint64_t outer, uint64_t so, uint64_t rows, 
     k_pack<T><<<static_cast<unsigned>(std::min<uint64_t>((total + 255) / 256, 148 * 16)), 256, 0, cs>>>(in, so, sr, sc, rows, cols, up8(cols), total, out);
     return launched("launch k_pack");
 }
+
+static uint32_t tmem_columns(uint32_t n)
+{
+    uint32_t c = 32;
+    while (c < n) c *= 2;
+    return c;
+}
+
+static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute *attr)
+{
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster, attr->val.clusterDim.y = 1, attr->val.clusterDim.z = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attr, c.numAttrs = 1;
+    return c;
+}
+
+constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
 
 // y[t][f] = sum of x[t][k] W(f, k) + sum of h[t][j] F_i(f, j) (MN: W and F with their f next to each other).
 template <class T, bool MN>
@@ -292,100 +317,152 @@ static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride
     a.stages = std::min<uint32_t>(P_MAX_STAGES, (per_sm == 2 ? 100u << 10 : 200u << 10) / a.stage_bytes);
     a.split = 1;
     while (a.split < 8 && tiles * a.split * 2 <= (uint64_t)sms * per_sm && a.steps >= 8 * a.split) a.split *= 2;
-    a.tmem_columns = std::max(32u, a.split > 1 ? a.nt : 2 * a.nt);
+    a.tmem_columns = tmem_columns(a.split > 1 ? a.nt : 2 * a.nt);
     rc = tensor_map(&a.x, x, std::is_same_v<T, __nv_bfloat16>, k, p->tokens, x_stride, a.nt);
     if (!rc) rc = MN ? tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, feats, k, w_stride, STEP_K)
                      : tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, k, feats, w_stride, P_FEATS);
     if (rc) return rc;
-    rc = opt_in_smem(k_project<T, MN>, 201u << 10, done);
+    rc = opt_in_smem(k_project<T, MN>, OPS_SMEM, done);
     if (rc) return rc;
-    cudaLaunchConfig_t c{};
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = a.split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-    c.gridDim = dim3(a.split > 1 ? static_cast<unsigned>(tiles * a.split) : static_cast<unsigned>(std::min<uint64_t>(tiles, (uint64_t)sms * per_sm)));
-    c.blockDim = dim3(P_THREADS), c.dynamicSmemBytes = a.stages * a.stage_bytes + ATOM_BYTES, c.stream = cs, c.attrs = &attr, c.numAttrs = 1;
+    const unsigned grid = static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<uint64_t>(tiles, (uint64_t)sms * per_sm));
+    const cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
     CK("launch k_project", cudaLaunchKernelEx(&c, k_project<T, MN>, a));
     return LMZ_GPU_OK;
 }
+
+// h = s x F^T for each token's own adapter; f: [adapter][rank][f_stride], its first k of each row.
+template <class T>
+static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride, uint64_t k, const T *f, uint64_t f_stride, T *h, cudaStream_t cs)
+{
+    static bool done[64];
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    HiddenArgs<T> a{};
+    a.index = token_index(p), a.h = h, a.tokens = p->tokens, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
+    a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K);
+    a.each = std::min(H_COLUMNS / a.rp, p->adapters);
+    const uint32_t columns = (a.each * a.rp + 15) & ~15u;
+    a.stage_bytes = (H_TOKENS + columns) * ROW_BYTES, a.tmem_columns = tmem_columns(columns);
+    a.stages = std::min<uint32_t>(H_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
+    const uint64_t tiles = (p->tokens + H_TOKENS - 1) / H_TOKENS;
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(p->index ? std::min(p->adapters, H_TOKENS) : 1, p->tokens)), groups = (most + a.each - 1) / a.each;
+    a.split = 1;
+    while (a.split < 8 && tiles * groups * a.split * 2 <= 2ull * sms && a.steps >= 4 * a.split) a.split *= 2;
+    constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+    rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, H_TOKENS);
+    if (!rc) rc = tensor_map(&a.f, f, bf16, k, p->rank, f_stride, p->rank, p->adapters);
+    if (!rc) rc = opt_in_smem(k_hidden<T>, OPS_SMEM, done);
+    if (rc) return rc;
+    cudaLaunchAttribute attr{};
+    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(tiles * a.split), groups), H_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    CK("launch k_hidden", cudaLaunchKernelEx(&c, k_hidden<T>, a));
+    return LMZ_GPU_OK;
+}
+
+// dF_i(f, j) = the sum over i's tokens of thin[t][j] z[t][f].
+template <class T>
+static int launch_factor_grad(const lmz_projection *p, const T *z, uint64_t stride, uint64_t feats, const T *thin, const uint32_t *order, const uint32_t *start,
+                              T *out, uint64_t wide, uint64_t place, cudaStream_t cs)
+{
+    static bool done[64];
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    FactorGradArgs<T> a{};
+    a.z = z, a.thin = thin, a.order = order, a.start = start, a.out = out, a.stride = stride, a.feats = feats;
+    a.each = feats * p->rank, a.wide = wide, a.place = place;
+    a.tokens = static_cast<uint32_t>(p->tokens), a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
+    a.stage_bytes = FG_FEATS * STEP_K * 2 + 2 * thin_tile_bytes(a.rp), a.tmem_columns = tmem_columns((a.rp + 15) & ~15u);
+    // two blocks to an SM where the thin rows are short
+    a.stages = a.rp <= 64 ? 3 : std::min<uint32_t>(FG_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
+    const uint64_t tiles = (feats + FG_FEATS - 1) / FG_FEATS;
+    a.split = 1;
+    while (a.split < 8 && tiles * p->adapters * a.split * 2 <= 4ull * sms && p->tokens >= 2ull * STEP_K * a.split) a.split *= 2;
+    rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
+    if (rc) return rc;
+    cudaLaunchAttribute attr{};
+    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(tiles * a.split), p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    CK("launch k_factor_grad", cudaLaunchKernelEx(&c, k_factor_grad<T>, a));
+    return LMZ_GPU_OK;
+}
+
+// A projection's tensors as the kernels take them: where they lie, or packed into the workspace.
+template <class T>
+struct ProjectInputs {
+    const T *x, *w, *a, *dy;
+    uint64_t x_stride, w_stride, a_stride, dy_stride;
+    int rc;
+    ProjectInputs(const lmz_projection *p, const ProjectLayout &l, bool grad, cudaStream_t cs)
+        : x(static_cast<const T *>(p->x)), w(static_cast<const T *>(p->weight)), a(static_cast<const T *>(p->a)), dy(static_cast<const T *>(p->dy)),
+          x_stride(p->x_stride), w_stride(p->weight_stride), a_stride(p->in), dy_stride(p->out), rc(LMZ_GPU_OK)
+    {
+        auto pack = [&](bool on, const T *&t, uint64_t outer, uint64_t rows, uint64_t &stride, uint64_t cols, uint64_t off) {
+            if (!on || rc) return;
+            T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off);
+            rc = launch_pack(t, outer, rows * stride, rows, stride, cols, 1, to, cs);
+            t = to, stride = up8(cols);
+        };
+        pack(l.pack_x, x, 1, p->tokens, x_stride, p->in, l.x);
+        pack(l.pack_w, w, 1, p->out, w_stride, p->in, l.w);
+        pack(l.pack_a, a, p->adapters, p->rank, a_stride, p->in, l.a);
+        if (grad) pack(l.pack_dy, dy, 1, p->tokens, dy_stride, p->out, l.dy);
+    }
+};
 
 template <class T>
 static int project_as(const lmz_projection *p, cudaStream_t cs)
 {
     const ProjectLayout l(p, false);
-    uint8_t *work = static_cast<uint8_t *>(p->work);
-    auto at = [&](uint64_t off) { return reinterpret_cast<T *>(work + off); };
-    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *fb = static_cast<const T *>(p->b);
-    uint64_t x_stride = p->x_stride, w_stride = p->weight_stride;
+    const ProjectInputs<T> in(p, l, false, cs);
+    int rc = in.rc;
+    const T *b = static_cast<const T *>(p->b);
     T *h = static_cast<T *>(p->hidden);
-    const uint64_t r = p->rank, rp = up8(r);
-    int rc = LMZ_GPU_OK;
-    if (l.pack_x) {
-        rc = launch_pack(x, 1, 0, p->tokens, x_stride, p->in, 1, at(l.x), cs);
-        x = at(l.x), x_stride = up8(p->in);
-    }
-    if (!rc && l.pack_w) {
-        rc = launch_pack(w, 1, 0, p->out, w_stride, p->in, 1, at(l.w), cs);
-        w = at(l.w), w_stride = up8(p->in);
-    }
+    const uint64_t r = p->rank;
     if (!rc && l.pack_b) {
-        rc = launch_pack(fb, p->adapters, p->out * r, p->out, r, r, 1, at(l.b), cs);
-        fb = at(l.b);
+        T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + l.b);
+        rc = launch_pack(b, p->adapters, p->out * r, p->out, r, r, 1, to, cs);
+        b = to;
     }
-    if (rc) return rc;
-    const Factor<T> a{static_cast<const T *>(p->a), r * p->in, 1, p->in};
-    k_hidden<T><<<static_cast<unsigned>((p->tokens * rp + 7) / 8), 256, 0, cs>>>(x, x_stride, p->in, a, token_index(p), p->tokens, p->rank, (uint32_t)rp, h);
-    rc = launched("launch k_hidden");
-    if (rc) return rc;
-    return launch_project<T, false>(p, x, x_stride, p->in, w, w_stride, p->out, fb, p->out, rp, h, static_cast<T *>(p->y), cs);
+    if (!rc) rc = launch_hidden(p, in.x, in.x_stride, p->in, in.a, in.a_stride, h, cs);
+    if (!rc) rc = launch_project<T, false>(p, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, b, p->out, up8(r), h, static_cast<T *>(p->y), cs);
+    return rc;
 }
 
 template <class T>
 static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
 {
+    const uint64_t r = p->rank;
+    if (p->tokens == 0) {
+        if (p->da) CK("cudaMemsetAsync", cudaMemsetAsync(p->da, 0, 2ull * p->adapters * r * p->in, cs));
+        if (p->db) CK("cudaMemsetAsync", cudaMemsetAsync(p->db, 0, 2ull * p->adapters * r * p->out, cs));
+        return LMZ_GPU_OK;
+    }
     const ProjectLayout l(p, true);
+    const ProjectInputs<T> in(p, l, true, cs);
+    int rc = in.rc;
     uint8_t *work = static_cast<uint8_t *>(p->work);
-    auto at = [&](uint64_t off) { return reinterpret_cast<T *>(work + off); };
-    const T *x = static_cast<const T *>(p->x), *w = static_cast<const T *>(p->weight), *dy = static_cast<const T *>(p->dy), *fa = static_cast<const T *>(p->a);
-    uint64_t w_stride = p->weight_stride, dy_stride = p->out, a_row = p->in;
-    const T *h = static_cast<const T *>(p->hidden);
-    T *g = at(l.g);
-    const uint64_t r = p->rank, rp = up8(r);
-    const Factor<T> b{static_cast<const T *>(p->b), r * p->out, r, 1};
-    int rc = LMZ_GPU_OK;
-    if (p->tokens && (p->dx || p->da)) {
-        k_hidden<T><<<static_cast<unsigned>((p->tokens * rp + 7) / 8), 256, 0, cs>>>(dy, p->out, p->out, b, token_index(p), p->tokens, p->rank, (uint32_t)rp, g);
-        rc = launched("launch k_hidden");
+    T *g = reinterpret_cast<T *>(work + l.g);
+    if (!rc && (p->dx || p->da)) {
+        T *bt = reinterpret_cast<T *>(work + l.b);
+        rc = launch_pack(static_cast<const T *>(p->b), p->adapters, r * p->out, r, 1, p->out, r, bt, cs);
+        if (!rc) rc = launch_hidden(p, in.dy, in.dy_stride, p->out, bt, up8(p->out), g, cs);
+    }
+    if (!rc && p->dx) rc = launch_project<T, true>(p, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, g, static_cast<T *>(p->dx), cs);
+    const uint32_t *order = nullptr, *start = nullptr;
+    if (!rc && p->index && (p->da || p->db)) {
+        SortArgs s{};
+        s.ids = p->index, s.n = p->tokens, s.nkeys = p->adapters, s.wide = p->index_bytes == 8;
+        for (int i = 0; i < 2; i++) s.keys[i] = reinterpret_cast<uint32_t *>(work + l.keys[i]), s.pos[i] = reinterpret_cast<uint32_t *>(work + l.pos[i]);
+        int side = 0;
+        rc = launch_sort(s, cs, &side);
         if (rc) return rc;
+        uint32_t *starts = reinterpret_cast<uint32_t *>(work + l.start);
+        k_key_starts<<<p->adapters / 256 + 1, 256, 0, cs>>>(s.keys[side], static_cast<uint32_t>(p->tokens), p->adapters, starts);
+        rc = launched("launch k_key_starts");
+        order = s.pos[side], start = starts;
     }
-    if (p->tokens && p->dx) {
-        const T *d = dy;
-        if (l.pack_dy) {
-            rc = launch_pack(dy, 1, 0, p->tokens, p->out, p->out, 1, at(l.dy), cs);
-            d = at(l.dy), dy_stride = up8(p->out);
-        }
-        if (!rc && l.pack_w) {
-            rc = launch_pack(w, 1, 0, p->out, w_stride, p->in, 1, at(l.w), cs);
-            w = at(l.w), w_stride = up8(p->in);
-        }
-        if (!rc && l.pack_a) {
-            rc = launch_pack(fa, p->adapters, r * p->in, r, p->in, p->in, 1, at(l.a), cs);
-            fa = at(l.a), a_row = up8(p->in);
-        }
-        if (!rc) rc = launch_project<T, true>(p, d, dy_stride, p->out, w, w_stride, p->in, fa, r, a_row, g, static_cast<T *>(p->dx), cs);
-        if (rc) return rc;
-    }
-    if (p->da) {
-        k_factor_grad<T><<<dim3(static_cast<unsigned>((p->in + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
-            g, (uint32_t)rp, x, p->x_stride, token_index(p), p->tokens, p->rank, p->in, static_cast<T *>(p->da), r * p->in, 1, p->in);
-        rc = launched("launch k_factor_grad");
-        if (rc) return rc;
-    }
-    if (p->db) {
-        k_factor_grad<T><<<dim3(static_cast<unsigned>((p->out + 255) / 256), p->rank, p->adapters), 256, 0, cs>>>(
-            h, (uint32_t)rp, dy, p->out, token_index(p), p->tokens, p->rank, p->out, static_cast<T *>(p->db), r * p->out, r, 1);
-        rc = launched("launch k_factor_grad");
-    }
+    if (!rc && p->da) rc = launch_factor_grad<T>(p, in.x, in.x_stride, p->in, g, order, start, static_cast<T *>(p->da), 1, p->in, cs);
+    if (!rc && p->db) rc = launch_factor_grad<T>(p, in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), order, start, static_cast<T *>(p->db), r, 1, cs);
     return rc;
 }
 
@@ -420,15 +497,19 @@ template <class T>
 static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, const void *a, const void *b, unsigned rank, float scale, void *to,
                     cudaStream_t cs)
 {
-    for (uint64_t r0 = 0; r0 < out; r0 += 65535) {               // (a grid's second dimension ends there)
-        const uint64_t rows = std::min<uint64_t>(65535, out - r0);
-        k_merge<T><<<dim3(static_cast<unsigned>((in + 255) / 256), static_cast<unsigned>(rows)), 256, 0, cs>>>(
-            static_cast<const T *>(w) + r0 * stride, stride, static_cast<const T *>(a), static_cast<const T *>(b) + r0 * rank, rank, scale, in,
-            static_cast<T *>(to) + r0 * in);
-        const int rc = launched("launch k_merge");
+    MergeArgs<T> m{};
+    m.w = static_cast<const T *>(w), m.a = static_cast<const T *>(a), m.b = static_cast<const T *>(b), m.out = static_cast<T *>(to);
+    m.rows = out, m.cols = in, m.w_stride = stride, m.rank = rank, m.places = (rank + 15) & ~15u, m.scale = scale;
+    m.a_even = on_boundary(a, in, in), m.b_even = on_boundary(b, rank, rank);
+    return by_width<T>(vector_bytes(in * 2, {address(w), address(to), stride * 2}), [&](auto vec) {
+        constexpr int VB = sizeof(vec.raw);
+        static bool done[64];
+        const int rc = opt_in_smem(k_merge<T, VB>, merge_smem(256), done);
         if (rc) return rc;
-    }
-    return LMZ_GPU_OK;
+        k_merge<T, VB><<<dim3(static_cast<unsigned>((in + M_COLS - 1) / M_COLS), static_cast<unsigned>((out + M_ROWS - 1) / M_ROWS)), M_THREADS,
+                         merge_smem(m.places), cs>>>(m);
+        return launched("launch k_merge");
+    });
 }
 
 API int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a, const void *d_b, unsigned rank,
