@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const FactorGradArgs
             for (uint32_t h = 0; h < 2; h++)
 #pragma unroll
                 for (uint32_t c = 0; c < STEP_K / 16; c++)
-                    mma16(tmem, tile_desc(src + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES),
-                          tile_desc(src + z_bytes + h * half + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES), desc, n || h || c);
+                    mma16(tmem, desc_lo(src + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES),
+                          desc_lo(src + z_bytes + h * half + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES), desc, n || h || c);
             mma_commit(&freed[n % a.stages]);
         }
         if (n + a.stages - 1 < steps) {                          // the stage of the step before is next to be filled

@@ -13,7 +13,7 @@ constexpr uint32_t H_PITCH = H_TOKENS + 1;     // of the partial sums in shared 
 struct HiddenShared {
     uint64_t full[H_MAX_STAGES], empty[H_MAX_STAGES], sums;
     uint32_t tmem, over, present;
-    int32_t adapter[H_TOKENS];                 // per token
+    alignas(16) int32_t adapter[H_TOKENS];     // per token
     int32_t list[H_TOKENS];                    // the tile's adapters in the order of their first tokens
     int32_t slot[H_TOKENS];                    // per token: where its adapter stands in that list, -1: none
     uint32_t firsts[H_TOKENS / 32];
@@ -65,7 +65,16 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     __syncthreads();
     uint32_t first = 0;
     if (tid < H_TOKENS) {
-        if (a.index.ids) while (s.adapter[first] != mine) first++;
+        first = tid;
+        if (!a.index.ids) first = 0;
+        else
+            for (int i = H_TOKENS - 4; i >= 0; i -= 4) {         // (backwards: the lowest match stays)
+                const int4 v = *reinterpret_cast<const int4 *>(s.adapter + i);
+                if (v.w == mine) first = i + 3;
+                if (v.z == mine) first = i + 2;
+                if (v.y == mine) first = i + 1;
+                if (v.x == mine) first = i;
+            }
         const uint32_t firsts = __ballot_sync(~0u, first == tid && mine >= 0);
         if (lane == 0) s.firsts[warp] = firsts;
     }
@@ -85,40 +94,45 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     __syncthreads();
     tc_after();
     const uint32_t tmem = s.tmem;
+    let_next_start();                                            // (not before this block has its columns: the next one's may take all that is left)
 
     if (warp == 4) {
-        if (lane == 0) {
-            uint32_t n = 0;
-            for (uint32_t k = k0; k < k1; k++, n++) {
-                const uint32_t st = n % a.stages, dst = ring + st * a.stage_bytes;
-                if (n >= a.stages && !bar_wait(&s.empty[st], (n / a.stages - 1) & 1, over)) break;
+        RingPlace at;
+        for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
+            const uint32_t st = at.stage, dst = ring + st * a.stage_bytes;
+            if (at.turn && !warp_wait(&s.empty[st], (at.turn - 1) & 1, over)) break;
+            if (elected()) {
                 bar_expect(&s.full[st], H_TOKENS * ROW_BYTES + count * a.rank * ROW_BYTES);
                 tma_load_2d(&a.x, &s.full[st], dst, k * STEP_K, tile * H_TOKENS);
                 for (uint32_t i = 0; i < count; i++)
                     tma_load_3d(&a.f, &s.full[st], dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
             }
-            if (*over)                                           // nothing may still be on its way into this block's memory
-                for (uint32_t i = n > a.stages ? n - a.stages : 0; i < n; i++)
-                    for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.full[i % a.stages], (i / a.stages) & 1); tries++) {}
+            __syncwarp();
         }
+        if (*over)                                               // nothing may still be on its way into this block's memory
+            for (uint32_t i = 0; i < a.stages; i++) {
+                const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
+                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[i], used & 1); tries++) {}
+            }
     } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), false, false, H_TOKENS, (count * a.rp + 15) & ~15u);
-            uint32_t n = 0;
-            for (uint32_t k = k0; k < k1; k++, n++) {
-                const uint32_t st = n % a.stages, src = ring + st * a.stage_bytes;
-                if (!bar_wait(&s.full[st], (n / a.stages) & 1, over)) break;
-                tc_after();
+        const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), false, false, H_TOKENS, (count * a.rp + 15) & ~15u);
+        RingPlace at;
+        const uint32_t a_lo = desc_lo(ring, 16), b_lo = desc_lo(ring + H_TOKENS * ROW_BYTES, 16);
+        for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
+            const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+            if (!warp_wait(&s.full[st], at.turn & 1, over)) break;
+            if (elected()) {
 #pragma unroll
-                for (uint32_t c = 0; c < STEP_K / 16; c++)
-                    mma16(tmem, tile_desc(src + c * 32, 16), tile_desc(src + H_TOKENS * ROW_BYTES + c * 32, 16), desc, n || c);
+                for (uint32_t c = 0; c < STEP_K / 16; c++) mma16(tmem, a_lo + off + c * 2, b_lo + off + c * 2, desc, k != k0 || c);
                 mma_commit(&s.empty[st]);
             }
-            mma_commit(&s.sums);
-            if (*over)
-                for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums, 0); tries++) {}
+            __syncwarp();
         }
-    } else if (__all_sync(~0u, bar_wait(&s.sums, 0, over))) {
+        if (elected()) mma_commit(&s.sums);
+        __syncwarp();
+        if (*over)
+            for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums, 0); tries++) {}
+    } else if (warp_wait(&s.sums, 0, over)) {
         // every token's own columns, over the stages (all products have ended)
         tc_after();
         float *part = reinterpret_cast<float *>(h_smem + (ring - smem_addr(h_smem)));

@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(M_THREADS) k_merge(const MergeArgs<T> a)
     if (tid == 0) {
         const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), false, true, M_ROWS, M_COLS);
         for (uint32_t c = 0; c < a.places / 16; c++)
-            mma16(tmem, tile_desc(base + (c >> 2) * M_ROWS * ROW_BYTES + (c & 3) * 32, 16), tile_desc(base + b_bytes + c * 16 * ROW_BYTES, block), desc, c);
+            mma16(tmem, desc_lo(base + (c >> 2) * M_ROWS * ROW_BYTES + (c & 3) * 32, 16), desc_lo(base + b_bytes + c * 16 * ROW_BYTES, block), desc, c);
         mma_commit(&done);
     }
     const bool ok = __syncthreads_and(bar_wait(&done, 0, &s_over));

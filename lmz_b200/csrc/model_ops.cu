@@ -276,6 +276,8 @@ static int launch_pack(const T *in, uint64_t outer, uint64_t so, uint64_t rows, 
     return launched("launch k_pack");
 }
 
+constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
+
 static uint32_t tmem_columns(uint32_t n)
 {
     uint32_t c = 32;
@@ -292,43 +294,59 @@ static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cu
     return c;
 }
 
-constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
+template <class T, bool MN, bool PAIR>
+static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)
+{
+    static bool done[64];
+    const int rc = opt_in_smem(k_project<T, MN, PAIR>, OPS_SMEM, done);
+    if (rc) return rc;
+    a.stage_bytes = project_stage_bytes(a.nt, PAIR);
+    a.stages = std::min<uint32_t>(P_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
+    cudaLaunchAttribute attrs[2]{};
+    cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, PAIR ? 2 : a.split, attrs);
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    c.numAttrs = 2;
+    CK("launch k_project", cudaLaunchKernelEx(&c, k_project<T, MN, PAIR>, a));
+    return LMZ_GPU_OK;
+}
 
 // y[t][f] = sum of x[t][k] W(f, k) + sum of h[t][j] F_i(f, j) (MN: W and F with their f next to each other).
 template <class T, bool MN>
 static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride, uint64_t k, const T *w, uint64_t w_stride, uint64_t feats, const T *factor,
                           uint64_t factor_rows, uint64_t factor_row, const T *hidden, T *y, cudaStream_t cs)
 {
-    static bool done[64];
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     ProjectArgs<T> a{};
     a.index = token_index(p), a.hidden = hidden, a.factor = factor, a.factor_each = factor_rows * factor_row, a.factor_row = factor_row;
     a.y = y, a.tokens = p->tokens, a.feats = feats, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
-    a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K);
-    a.nt = P_GROUP;
-    while (a.nt < P_TOKENS && a.nt < p->tokens) a.nt *= 2;
-    a.feat_tiles = static_cast<uint32_t>((feats + P_FEATS - 1) / P_FEATS);
-    const uint64_t token_tiles = (p->tokens + a.nt - 1) / a.nt, tiles = a.feat_tiles * token_tiles;
-    if (tiles >= 1u << 31) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many tokens for a weight of this size");
-    a.token_tiles = static_cast<uint32_t>(token_tiles);
-    a.stage_bytes = project_stage_bytes(a.nt);
-    const uint32_t per_sm = a.nt <= 64 ? 2 : 1;
-    a.stages = std::min<uint32_t>(P_MAX_STAGES, (per_sm == 2 ? 100u << 10 : 200u << 10) / a.stage_bytes);
-    a.split = 1;
-    while (a.split < 8 && tiles * a.split * 2 <= (uint64_t)sms * per_sm && a.steps >= 8 * a.split) a.split *= 2;
+    a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K), a.split = 1;
+    auto tiles = [&](uint64_t f, uint64_t t) { return (feats + f - 1) / f * ((p->tokens + t - 1) / t); };
+    // Enough tiles of 256 by 256 for the multiprocessors in pairs: those.  Else tiles of 128 features by as many tokens as
+    // there are, at most 128, and of more tokens fewer at a time, down to 32, until the tiles occupy half of the multiprocessors; where
+    // they still do not, CTAs share K.
+    const bool pair = 2 * tiles(2 * P_FEATS, P_TOKENS) >= (uint64_t)sms;
+    if (pair) {
+        a.nt = P_TOKENS;
+    } else {
+        a.nt = P_GROUP;
+        while (a.nt < P_TOKENS / 2 && a.nt < p->tokens) a.nt *= 2;
+        if (p->tokens > a.nt)
+            while (a.nt > 32 && 2 * tiles(P_FEATS, a.nt) <= (uint64_t)sms) a.nt /= 2;
+        while (a.split < 8 && tiles(P_FEATS, a.nt) * a.split * 2 <= (uint64_t)sms && a.steps >= 8 * a.split) a.split *= 2;
+    }
+    const uint64_t count = tiles(pair ? 2 * P_FEATS : P_FEATS, a.nt);
+    if (count >= 1u << 28) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many tokens for a weight of this size");
+    a.feat_tiles = static_cast<uint32_t>((feats + (pair ? 2 : 1) * P_FEATS - 1) / ((pair ? 2 : 1) * P_FEATS));
+    a.token_tiles = static_cast<uint32_t>((p->tokens + a.nt - 1) / a.nt);
     a.tmem_columns = tmem_columns(a.split > 1 ? a.nt : 2 * a.nt);
-    rc = tensor_map(&a.x, x, std::is_same_v<T, __nv_bfloat16>, k, p->tokens, x_stride, a.nt);
-    if (!rc) rc = MN ? tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, feats, k, w_stride, STEP_K)
-                     : tensor_map(&a.w, w, std::is_same_v<T, __nv_bfloat16>, k, feats, w_stride, P_FEATS);
+    constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+    rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, pair ? a.nt / 2 : a.nt);
+    if (!rc) rc = MN ? tensor_map(&a.w, w, bf16, feats, k, w_stride, STEP_K) : tensor_map(&a.w, w, bf16, k, feats, w_stride, P_FEATS);
     if (rc) return rc;
-    rc = opt_in_smem(k_project<T, MN>, OPS_SMEM, done);
-    if (rc) return rc;
-    cudaLaunchAttribute attr{};
-    const unsigned grid = static_cast<unsigned>(a.split > 1 ? tiles * a.split : std::min<uint64_t>(tiles, (uint64_t)sms * per_sm));
-    const cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
-    CK("launch k_project", cudaLaunchKernelEx(&c, k_project<T, MN>, a));
-    return LMZ_GPU_OK;
+    if (pair) return launch_project_as<T, MN, true>(a, static_cast<unsigned>(std::min<uint64_t>(count, sms / 2) * 2), cs);
+    return launch_project_as<T, MN, false>(a, static_cast<unsigned>(a.split > 1 ? count * a.split : std::min<uint64_t>(count, sms)), cs);
 }
 
 // h = s x F^T for each token's own adapter; f: [adapter][rank][f_stride], its first k of each row.
@@ -348,7 +366,7 @@ static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride,
     const uint64_t tiles = (p->tokens + H_TOKENS - 1) / H_TOKENS;
     const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(p->index ? std::min(p->adapters, H_TOKENS) : 1, p->tokens)), groups = (most + a.each - 1) / a.each;
     a.split = 1;
-    while (a.split < 8 && tiles * groups * a.split * 2 <= 2ull * sms && a.steps >= 4 * a.split) a.split *= 2;
+    while (a.split < 8 && tiles * groups * a.split * 2 <= (uint64_t)sms && a.steps >= 4 * a.split) a.split *= 2;
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
     rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, H_TOKENS);
     if (!rc) rc = tensor_map(&a.f, f, bf16, k, p->rank, f_stride, p->rank, p->adapters);

@@ -7,8 +7,8 @@ namespace lmz {
 
 constexpr uint32_t P_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
 constexpr uint32_t P_TOKENS = 256;             // most tokens of a tile: its N, a TMEM column each
-constexpr uint32_t P_GROUP = 16;               // tokens that are looked at together: N counts in sixteens
-constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 8;
+constexpr uint32_t P_GROUP = 16;               // tokens of a TMEM load, and the steps that N comes in (a pair's: 32)
+constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 10;
 constexpr uint32_t P_EPILOGUE = 128, P_FEED = 128, P_THREADS = P_EPILOGUE + P_FEED + 64;
 
 // What a tile's tokens have for adapters.
@@ -25,7 +25,7 @@ struct ProjectShared {
     uint64_t loaded[P_INFOS], fed[P_INFOS];    // a tile's steps of the weight, and of the adapters, have all got their stages
     uint64_t sums_full[2], sums_empty[2];
     uint32_t tmem, over;
-    uint32_t same[P_TOKENS / 32];              // bit 0, 1: the tokens of these two groups have one adapter
+    uint32_t same[P_TOKENS / 32];              // bit 0, 1: the tokens of these two sixteens have one adapter; bit 2: both the same
     TileInfo info[P_INFOS];
 };
 
@@ -42,11 +42,12 @@ struct ProjectArgs {
     uint32_t steps;                            // of 64 along K
     uint32_t nt;                               // tokens of a tile
     uint32_t split;                            // CTAs of a cluster that share K
-    uint32_t feat_tiles, token_tiles;
+    uint32_t feat_tiles, token_tiles;          // of P_FEATS (a pair: twice that) and nt
     uint32_t stages, stage_bytes, tmem_columns;
 };
 
-__host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt) { return P_FEATS * ROW_BYTES + nt * ROW_BYTES; }
+// Tiles of a stage: W's 128 rows, and the tokens' (of a pair's 256 each CTA has half).
+__host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt, bool pair) { return (P_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
 
 // Eight elements of a factor times eight of h (upper and lower halves).
 template <class T>
@@ -125,15 +126,20 @@ __device__ __forceinline__ void store_group(const ProjectArgs<T> &a, uint64_t t0
 // Roles: a TMA warp loads tiles of W and x (64 along K) into a ring of stages; four warps feed the ring with what adapters
 // need (h and a factor's tile: 2 rp wide, the factor beside both halves of h); one thread issues the MMAs; four warps take
 // the sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.
+// The weight's first tiles are under way while the kernel that makes h still runs.
 // Few tiles: the CTAs of a cluster share K, and their sums meet in distributed shared memory.
-template <class T, bool MN>
+// Many (PAIR): two CTAs multiply 256 features by 256 tokens together, each loading half of both, so that a step brings
+// 32 KiB into an SM for the products that took 48 (L2 bounds those: 888 us against XX for 8192 tokens of 4096 to 14336 features).
+template <class T, bool MN, bool PAIR>
 __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant__ ProjectArgs<T> a)
 {
+    constexpr uint32_t CTAS = PAIR ? 2 : 1, GROUP = CTAS * P_GROUP;
     extern __shared__ uint8_t p_smem[];
     __shared__ ProjectShared s;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
-    const uint32_t first = blockIdx.x / a.split, stride = gridDim.x / a.split, tiles = a.feat_tiles * a.token_tiles;
+    const uint32_t side = PAIR ? cluster_rank() : 0, rank = !PAIR && a.split > 1 ? cluster_rank() : 0;
+    const uint32_t team = PAIR ? 2 : a.split;
+    const uint32_t first = blockIdx.x / team, stride = gridDim.x / team, tiles = a.feat_tiles * a.token_tiles;
     const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split);
     const uint32_t k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(p_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
@@ -142,12 +148,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
 
     if (tid == 0) {
         s.over = 0;
-        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], 1), bar_init(&s.empty[i], 1);
-        for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], 2 + P_EPILOGUE / 32), bar_init(&s.loaded[i], 1), bar_init(&s.fed[i], 1);
-        for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], P_EPILOGUE / 32);
+        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], CTAS), bar_init(&s.empty[i], 1);
+        for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], (side ? 1 : 2) + P_EPILOGUE / 32), bar_init(&s.loaded[i], 1), bar_init(&s.fed[i], 1);
+        for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], CTAS * P_EPILOGUE / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) tmem_alloc(&s.tmem, a.tmem_columns);
+    if constexpr (PAIR) {
+        __syncthreads();
+        cluster_barrier();
+    }
+    if (warp == 9) tmem_alloc<PAIR>(&s.tmem, a.tmem_columns);
     tc_before();
     __syncthreads();
     tc_after();
@@ -160,82 +170,121 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         ft = in / w, tt = 8 * b + in % w;
     };
     auto mine = [&](uint32_t run) { return run % a.split == rank; };
+    auto features = [&](uint32_t ft) { return (ft * CTAS + side) * P_FEATS; };      // where this CTA's begin
 
     if (warp == 8) {
-        if (lane == 0) {
-            uint32_t at = 0, n = 0, filled = 0;
-            for (uint32_t tile = first; tile < tiles && !*over; tile += stride, n++) {
-                uint32_t ft, tt;
-                place(tile, ft, tt);
-                for (uint32_t k = k0; k < k1; k++, at++) {
-                    const uint32_t st = at % a.stages;
-                    if (at >= a.stages && !bar_wait(&s.empty[st], (at / a.stages - 1) & 1, over)) break;
+        RingPlace at;
+        uint32_t n = 0;
+        const uint32_t full = peer_addr(s.full, 0);
+        for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
+            uint32_t ft, tt;
+            place(tile, ft, tt);
+            const uint32_t f = features(ft), t = tt * a.nt + side * (P_TOKENS / 2);
+            bool ok = true;
+            for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
+                const uint32_t st = at.stage;
+                ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
+                if (!ok) break;
+                if (elected()) {
                     const uint32_t dst = ring + st * a.stage_bytes;
-                    bar_expect(&s.full[st], a.stage_bytes);
-                    if constexpr (MN) {
-                        tma_load_2d(&a.w, &s.full[st], dst, ft * P_FEATS, k * STEP_K);
-                        tma_load_2d(&a.w, &s.full[st], dst + STEP_K * ROW_BYTES, ft * P_FEATS + 64, k * STEP_K);
+                    if constexpr (PAIR) {
+                        const uint32_t bar = full + st * 8;
+                        if (side) peer_expect(bar, a.stage_bytes);
+                        else bar_expect(&s.full[st], a.stage_bytes);
+                        if constexpr (MN) {
+                            tma_load_2d_pair(&a.w, bar, dst, f, k * STEP_K);
+                            tma_load_2d_pair(&a.w, bar, dst + STEP_K * ROW_BYTES, f + 64, k * STEP_K);
+                        } else {
+                            tma_load_2d_pair(&a.w, bar, dst, k * STEP_K, f);
+                        }
+                        tma_load_2d_pair(&a.x, bar, dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
                     } else {
-                        tma_load_2d(&a.w, &s.full[st], dst, k * STEP_K, ft * P_FEATS);
+                        bar_expect(&s.full[st], a.stage_bytes);
+                        if constexpr (MN) {
+                            tma_load_2d(&a.w, &s.full[st], dst, f, k * STEP_K);
+                            tma_load_2d(&a.w, &s.full[st], dst + STEP_K * ROW_BYTES, f + 64, k * STEP_K);
+                        } else {
+                            tma_load_2d(&a.w, &s.full[st], dst, k * STEP_K, f);
+                        }
+                        tma_load_2d(&a.x, &s.full[st], dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
                     }
-                    tma_load_2d(&a.x, &s.full[st], dst + P_FEATS * ROW_BYTES, k * STEP_K, tt * a.nt);
-                    filled = at + 1;
                 }
-                if (*over) break;
-                bar_arrive(&s.loaded[n % P_INFOS]);
-                if (!bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
-                const TileInfo &info = s.info[n % P_INFOS];
-                uint32_t steps = 0;
-                for (uint32_t r = 0; r < info.runs; r++) steps += mine(r) ? wide : 0;
-                at += steps;
-                bar_arrive(&s.info_empty[n % P_INFOS]);
-                // A parity tells two phases apart, no more: whoever has skipped a whole turn of the ring first waits for the
-                // others' last stage in it.
-                if (steps >= a.stages && !bar_wait(&s.fed[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+                __syncwarp();
             }
-            if (*over)                                           // nothing may still be on its way into this block's memory
-                for (uint32_t i = filled > a.stages ? filled - a.stages : 0; i < filled; i++)
-                    for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.full[i % a.stages], (i / a.stages) & 1); tries++) {}
+            if (!ok) break;
+            if (lane == 0) bar_arrive(&s.loaded[n % P_INFOS]);
+            if (!warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+            const TileInfo &info = s.info[n % P_INFOS];
+            uint32_t steps = 0;
+            for (uint32_t r = 0; r < info.runs; r++) steps += mine(r) ? wide : 0;
+            at.skip(steps, a.stages);
+            __syncwarp();
+            if (lane == 0) bar_arrive(&s.info_empty[n % P_INFOS]);
+            // A parity tells two phases apart, no more: whoever has skipped a whole turn of the ring first waits for the
+            // others' last stage in it.
+            if (steps >= a.stages && !warp_wait(&s.fed[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
         }
+        // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both).
+        if (*over && !side)
+            for (uint32_t i = 0; i < a.stages; i++) {
+                const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
+                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[i], used & 1); tries++) {}
+            }
     } else if (warp == 9) {
-        if (lane == 0) {
+        if (!side) {
             const uint32_t a_step = MN ? 16 * ROW_BYTES : 32, a_block = MN ? STEP_K * ROW_BYTES : 16;
-            const bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
-            uint32_t at = 0, n = 0;
-            for (uint32_t tile = first; tile < tiles && !*over; tile += stride, n++) {
+            constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+            RingPlace at;
+            uint32_t n = 0;
+            const uint32_t desc = mma_desc(bf16, MN, false, CTAS * P_FEATS, a.nt);
+            const uint32_t a_lo = desc_lo(ring, a_block), b_lo = desc_lo(ring + P_FEATS * ROW_BYTES, 16);
+            bool ok = true;
+            for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
                 const uint32_t buf = n & 1, sums = tmem + buf * a.nt;
-                if (n >= 2 && !bar_wait(&s.sums_empty[buf], (n / 2 - 1) & 1, over)) break;
+                ok = n < 2 || warp_wait(&s.sums_empty[buf], (n / 2 - 1) & 1, over);
+                if (!ok) break;
                 tc_after();
-                const uint32_t desc = mma_desc(bf16, MN, false, P_FEATS, a.nt);
-                for (uint32_t k = k0; k < k1; k++, at++) {
-                    const uint32_t st = at % a.stages, src = ring + st * a.stage_bytes;
-                    if (!bar_wait(&s.full[st], (at / a.stages) & 1, over)) break;
-                    tc_after();
+                for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
+                    const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+                    ok = warp_wait(&s.full[st], at.turn & 1, over);
+                    if (!ok) break;
+                    if (elected()) {
 #pragma unroll
-                    for (uint32_t c = 0; c < STEP_K / 16; c++)
-                        mma16(sums, tile_desc(src + c * a_step, a_block), tile_desc(src + P_FEATS * ROW_BYTES + c * 32, 16), desc, k != k0 || c);
-                    mma_commit(&s.empty[st]);
+                        for (uint32_t c = 0; c < STEP_K / 16; c++)
+                            mma16<PAIR>(sums, a_lo + off + (c * a_step >> 4), b_lo + off + c * 2, desc, k != k0 || c);
+                        mma_commit<PAIR>(&s.empty[st]);
+                    }
+                    __syncwarp();
                 }
-                if (*over || !bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
+                ok = ok && warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over);
+                if (!ok) break;
                 const TileInfo &info = s.info[n % P_INFOS];
-                for (uint32_t r = 0; r < info.runs && !*over; r++) {
+                for (uint32_t r = 0; r < info.runs && ok; r++) {
                     if (!mine(r)) continue;
-                    const uint32_t column = info.run[r].column, rdesc = mma_desc(bf16, MN, false, P_FEATS, info.run[r].tokens);
-                    for (uint32_t v = 0; v < 2 * a.rp; v += STEP_K, at++) {
-                        const uint32_t st = at % a.stages, src = ring + st * a.stage_bytes;
-                        if (!bar_wait(&s.full[st], (at / a.stages) & 1, over)) break;
-                        tc_after();
-                        for (uint32_t c = 0; c < STEP_K / 16 && v + c * 16 < 2 * a.rp; c++)
-                            mma16(sums + column, tile_desc(src + c * a_step, a_block),
-                                  tile_desc(src + P_FEATS * ROW_BYTES + column * ROW_BYTES + c * 32, 16), rdesc, true);
-                        mma_commit(&s.empty[st]);
+                    const uint32_t column = info.run[r].column, rdesc = mma_desc(bf16, MN, false, CTAS * P_FEATS, info.run[r].tokens);
+                    for (uint32_t v = 0; v < 2 * a.rp; v += STEP_K, at.next(a.stages)) {
+                        const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+                        ok = warp_wait(&s.full[st], at.turn & 1, over);
+                        if (!ok) break;
+                        if (elected()) {
+                            for (uint32_t c = 0; c < STEP_K / 16 && v + c * 16 < 2 * a.rp; c++)
+                                mma16<PAIR>(sums + column, a_lo + off + (c * a_step >> 4), b_lo + off + c * 2, rdesc, true);
+                            mma_commit<PAIR>(&s.empty[st]);
+                        }
+                        __syncwarp();
                     }
                 }
-                bar_arrive(&s.info_empty[n % P_INFOS]);
-                mma_commit(&s.sums_full[buf]);
+                if (!ok) break;
+                __syncwarp();
+                if (elected()) {
+                    bar_arrive(&s.info_empty[n % P_INFOS]);
+                    mma_commit<PAIR>(&s.sums_full[buf]);
+                }
+                __syncwarp();
             }
-            if (*over) {                                         // the products under way end before their memory goes
-                mma_commit(&s.sums_full[n & 1]);
+            if (!ok) {                                           // the products under way end before their memory goes
+                if (elected()) mma_commit<PAIR>(&s.sums_full[n & 1]);
+                __syncwarp();
                 for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums_full[n & 1], (n / 2) & 1); tries++) {}
             }
         }
@@ -245,7 +294,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             uint32_t ft, tt;
             place(tile, ft, tt);
             TileInfo &info = s.info[n % P_INFOS];
-            if (!sync_all(1, P_FEED, n < P_INFOS || bar_wait(&s.info_empty[n % P_INFOS], (n / P_INFOS - 1) & 1, over))) return false;
+            if (!sync_all(1, P_FEED, n < P_INFOS || id || bar_wait(&s.info_empty[n % P_INFOS], (n / P_INFOS - 1) & 1, over))) return false;
             const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt;
             for (uint32_t c = id; c < P_TOKENS; c += P_FEED) {
                 const bool in = c < a.nt && t0 + c < a.tokens;
@@ -253,18 +302,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 info.adapter[c] = i;
                 const int head = __shfl_sync(~0u, i, lane & 16);
                 const uint32_t agree = __ballot_sync(~0u, !in || i == head);
-                if (lane == 0) s.same[c / 32] = ((agree & 0xFFFF) == 0xFFFF) | ((agree >> 16) == 0xFFFF) << 1;
+                const int other = __shfl_sync(~0u, i, 16);
+                const bool whole = t0 + c + 16 >= a.tokens || other == i;        // (lane 0's: the halves have the same one)
+                if (lane == 0) s.same[c / 32] = ((agree & 0xFFFF) == 0xFFFF) | ((agree >> 16) == 0xFFFF) << 1 | whole << 2;
             }
             sync_threads(1, P_FEED);
             if (id == 0) {
                 uint32_t runs = 0, mixed = 0, end = ~0u;
-                for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
-                    const int i = info.adapter[g * P_GROUP];
-                    if (!(s.same[g / 2] >> (g & 1) & 1)) {
-                        mixed |= 1u << g;
+                for (uint32_t g = 0; g * GROUP < a.nt; g++) {
+                    const int i = info.adapter[g * GROUP];
+                    if (!(PAIR ? s.same[g] == 7 : s.same[g / 2] >> (g & 1) & 1)) {
+                        mixed |= (PAIR ? 3u : 1u) << g * CTAS;
                     } else if (i >= 0) {
-                        if (end == g && info.run[runs - 1].adapter == i) info.run[runs - 1].tokens += P_GROUP;
-                        else info.run[runs].adapter = i, info.run[runs].column = g * P_GROUP, info.run[runs].tokens = P_GROUP, runs++;
+                        if (end == g && info.run[runs - 1].adapter == i) info.run[runs - 1].tokens += GROUP;
+                        else info.run[runs].adapter = i, info.run[runs].column = g * GROUP, info.run[runs].tokens = GROUP, runs++;
                         end = g + 1;
                     }
                 }
@@ -274,22 +325,24 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             sync_threads(1, P_FEED);
             return true;
         };
-        uint32_t at = 0, n = 0;
+        RingPlace at;
+        uint32_t n = 0;
         bool go = first < tiles && look(first, 0);
+        wait_for_previous();                                     // (h)
         for (uint32_t tile = first; go && tile < tiles; tile += stride, n++) {
             if (tile + stride < tiles) go = look(tile + stride, n + 1);
             uint32_t ft, tt;
             place(tile, ft, tt);
-            const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = static_cast<uint64_t>(ft) * P_FEATS;
+            const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = features(ft);
             const TileInfo &info = s.info[n % P_INFOS];
-            at += k1 - k0;
-            if (!sync_all(1, P_FEED, go && bar_wait(&s.loaded[n % P_INFOS], (n / P_INFOS) & 1, over))) break;
+            at.skip(k1 - k0, a.stages);
+            if (!sync_all(1, P_FEED, go && (id || bar_wait(&s.loaded[n % P_INFOS], (n / P_INFOS) & 1, over)))) break;
             for (uint32_t r = 0; go && r < info.runs; r++) {
                 if (!mine(r)) continue;
                 const T *factor = a.factor + info.run[r].adapter * a.factor_each;
-                for (uint32_t v0 = 0; v0 < 2 * a.rp; v0 += STEP_K, at++) {
-                    const uint32_t st = at % a.stages, fdst = ring + st * a.stage_bytes, hdst = fdst + P_FEATS * ROW_BYTES;
-                    if (!sync_all(1, P_FEED, at < a.stages || bar_wait(&s.empty[st], (at / a.stages - 1) & 1, over))) { go = false; break; }
+                for (uint32_t v0 = 0; v0 < 2 * a.rp; v0 += STEP_K, at.next(a.stages)) {
+                    const uint32_t st = at.stage, fdst = ring + st * a.stage_bytes, hdst = fdst + P_FEATS * ROW_BYTES;
+                    if (!sync_all(1, P_FEED, !at.turn || id || bar_wait(&s.empty[st], (at.turn - 1) & 1, over))) { go = false; break; }
                     const uint32_t parts = (2 * a.rp - v0 < STEP_K ? 2 * a.rp - v0 : STEP_K) / 8;
                     if constexpr (MN) {                          // a row per j of the rank, 64 features a block
                         for (uint32_t e = id; e < parts * 8 * 16; e += P_FEED) {
@@ -306,9 +359,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                             if (c < parts) copy16(fdst + swizzled(row, c), on ? factor + f * a.factor_row + j : factor, on);
                         }
                     }
-                    for (uint32_t e = id; e < info.run[r].tokens * 8; e += P_FEED) {
-                        const uint32_t row = info.run[r].column + (e >> 3), c = e & 7;
-                        const uint64_t t = t0 + row;
+                    const uint32_t share = info.run[r].tokens / CTAS, column = info.run[r].column + side * share;
+                    for (uint32_t e = id; e < share * 8; e += P_FEED) {
+                        const uint32_t row = e >> 3, c = e & 7;
+                        const uint64_t t = t0 + column + row;
                         const bool on = t < a.tokens;
                         if (c < parts) copy16(hdst + swizzled(row, c), on ? a.hidden + t * 2 * a.rp + v0 + c * 8 : a.hidden, on);
                     }
@@ -316,7 +370,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                     copies_wait<0>();
                     publish_smem();
                     sync_threads(1, P_FEED);
-                    if (id == 0) bar_arrive(&s.full[st]);
+                    if (id == 0) {
+                        if (side) peer_arrive(peer_addr(&s.full[st], 0));
+                        else bar_arrive(&s.full[st]);
+                    }
                 }
             }
             if (id == 0) bar_arrive(&s.fed[n % P_INFOS]);
@@ -324,19 +381,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
     } else {
         const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
         uint32_t n = 0;
+        wait_for_previous();
         for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
             uint32_t ft, tt;
             place(tile, ft, tt);
             const uint32_t buf = n & 1;
-            if (!__all_sync(~0u, bar_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over) && bar_wait(&s.sums_full[buf], (n / 2) & 1, over))) break;
+            if (!warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over) || !warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
             tc_after();
             const TileInfo &info = s.info[n % P_INFOS];
-            const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            const uint64_t f = features(ft) + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
             for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
-                if (a.split == 1 && t0 + g * P_GROUP >= a.tokens) break;
+                if ((PAIR || a.split == 1) && t0 + g * P_GROUP >= a.tokens) break;
                 float v[P_GROUP];
                 tmem_load16(tmem + (warp << 21) + buf * a.nt + g * P_GROUP, v);
-                if (a.split > 1) {                               // (the stages are free: all products have ended)
+                if (!PAIR && a.split > 1) {                      // (the stages are free: all products have ended)
                     float *sums = reinterpret_cast<float *>(p_smem + (ring - smem_addr(p_smem)));
 #pragma unroll
                     for (uint32_t c = 0; c < P_GROUP; c++) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
@@ -348,11 +406,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             }
             tc_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(&s.sums_empty[buf]), bar_arrive(&s.info_empty[n % P_INFOS]);
+            if (lane == 0) {
+                if (side) peer_arrive(peer_addr(&s.sums_empty[buf], 0));
+                else bar_arrive(&s.sums_empty[buf]);
+                bar_arrive(&s.info_empty[n % P_INFOS]);
+            }
         }
     }
     __syncwarp();
-    if (a.split > 1) {                                           // one tile per cluster: its CTAs take its groups in turn
+    if (!PAIR && a.split > 1) {                                  // one tile per cluster: its CTAs take its groups in turn
         cluster_barrier();
         if (warp < 4 && !*over && first < tiles) {
             uint32_t ft, tt;
@@ -372,11 +434,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         }
         cluster_barrier();
     }
+    if constexpr (PAIR) cluster_barrier();                       // nobody's barriers or tiles go while the other may use them
     tc_before();
     __syncthreads();
     if (warp == 9) {
         tc_after();
-        tmem_free(tmem, a.tmem_columns);
+        tmem_free<PAIR>(tmem, a.tmem_columns);
     }
 }
 

@@ -53,12 +53,60 @@ __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile 
     return false;
 }
 
+// The address, in the cluster's window, of a word that another CTA has where this one has `p`.
+__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank)
+{
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// (Relaxed: nothing of this thread's is handed over, and a release would wait a microsecond for nothing.)
+__device__ __forceinline__ void peer_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// One lane of the warp, always the same: what one thread issues stands in a loop that all lanes run, so that the compiler
+// knows addresses and descriptors to be the warp's (a loop of lane 0's alone took twice as long to issue a step).
+__device__ __forceinline__ bool elected()
+{
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p;
+}
+
+// Where a role stands in a ring of stages, counted up without divisions (the threads that issue copies and products run alone:
+// every instruction of their loops counts).
+struct RingPlace {
+    uint32_t stage = 0, turn = 0;              // turn: bit 0 is the parity of this use's phase
+    __device__ __forceinline__ void next(uint32_t stages)
+    {
+        if (++stage == stages) stage = 0, turn++;
+    }
+    __device__ __forceinline__ void skip(uint32_t n, uint32_t stages)
+    {
+        stage += n;
+        turn += stage / stages;
+        stage %= stages;
+    }
+};
+
 // ---- asynchronous copies
 
 __device__ __forceinline__ void tma_load_2d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y)
 {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
+}
+// The same, telling a barrier of the pair's first CTA (its address in the cluster's window).
+__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap *map, uint32_t bar, uint32_t dst, int32_t x, int32_t y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y, int32_t z)
 {
@@ -94,40 +142,59 @@ __device__ __forceinline__ bool sync_all(uint32_t barrier, uint32_t threads, boo
 
 // ---- tensor cores
 
+// PAIR: two CTAs of a cluster as one, each with half of the M rows of A, half of the N rows of B and its M rows of D.  Both
+// allocate; the first one's thread issues.
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_alloc(uint32_t *at, uint32_t columns)
 {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns)
 {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // A tile's descriptor.  K-major: eight rows of 128 bytes, 1024 bytes to the next eight.  MN-major: eight K indices, 1024 bytes to
-// the next eight; `block` bytes to the next 64 M or N elements.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block)
-{
-    return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(block >> 4) << 16 | static_cast<uint64_t>(ATOM_BYTES >> 4) << 32 |
-           1ull << 46 | 2ull << 61;
-}
+// the next eight; `block` bytes to the next 64 M or N elements.  The upper word is the same for all tiles; 16 more bytes of address are one more in the lower word.
+constexpr uint32_t DESC_HI = ATOM_BYTES >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t block) { return (addr & 0x3FFFF) >> 4 | (block >> 4) << 16; }
 // 16-bit operands of one type, sums in 32 bits.
 __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, uint32_t m, uint32_t n)
 {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (m >> 4) << 24;
 }
-// D (+)= A B^T over 16 K elements.
-__device__ __forceinline__ void mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add)
+// D (+)= A B^T over 16 K elements; the tiles by their descriptors' lower words.
+template <bool PAIR = false>
+__device__ __forceinline__ void mma16(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add)
 {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add)) : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(DESC_HI) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(DESC_HI) : "memory");
 }
-// The barrier gets an arrival when all MMAs issued so far have ended.
+// The barrier (of a pair: both CTAs') gets an arrival when all MMAs issued so far have ended.
+template <bool PAIR = false>
 __device__ __forceinline__ void mma_commit(uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(smem_addr(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // Sixteen columns of the warp's 32 lanes.
 __device__ __forceinline__ void tmem_load16(uint32_t at, float *v)
@@ -151,6 +218,20 @@ __device__ __forceinline__ void tmem_load8(uint32_t at, float *v)
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
 }
+
+// A warp waits by its first lane: 32 that ask take issue slots from those who work.
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile uint32_t *over)
+{
+    const bool ok = (threadIdx.x & 31) || bar_wait(b, parity, over);
+    return __all_sync(~0u, ok);
+}
+
+// ---- a kernel and the one launched behind it
+
+// From here on the next kernel's blocks may start where there is room.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The kernel before has ended and its results can be read.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- clusters
 

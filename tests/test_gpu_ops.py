@@ -266,6 +266,7 @@ SHAPES = [
     # more tiles than multiprocessors, more steps than a ring has stages, more runs than that too
     (2600, 64, 2200, 16, 5, "runs"), (2600, 648, 2056, 40, 30, "short"), (4700, 1400, 1288, 8, 3, "runs"), (900, 1032, 5000, 100, 12, "short"),
     (2300, 776, 2200, 16, 40, "mixed"), (200, 2048, 264, 64, 6, "short"),
+    (4000, 200, 640, 16, 5, "runs"), (4100, 328, 600, 24, 9, "short"), (2000, 136, 6000, 16, 30, "mixed"), (9000, 256, 1400, 32, 3, "runs"),
     # sizes where rows do not start on a boundary
     (5, 1, 1, 1, 1, "none"), (9, 33, 65, 3, 2, "mixed"), (333, 777, 501, 5, 5, "runs"), (70, 250, 1001, 7, 4, "mixed"), (600, 100, 77, 12, 3, "runs"),
 ]
