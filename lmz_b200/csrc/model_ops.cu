@@ -277,6 +277,7 @@ static int launch_pack(const T *in, uint64_t outer, uint64_t so, uint64_t rows, 
 }
 
 constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
+constexpr uint32_t PROJECT_SMEM = 219u << 10;
 
 static uint32_t tmem_columns(uint32_t n)
 {
@@ -298,12 +299,15 @@ template <class T, bool MN, bool PAIR>
 static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)
 {
     static bool done[64];
-    const int rc = opt_in_smem(k_project<T, MN, PAIR>, OPS_SMEM, done);
+    const int rc = opt_in_smem(k_project<T, MN, PAIR>, PROJECT_SMEM, done);
     if (rc) return rc;
     a.stage_bytes = project_stage_bytes(a.nt, PAIR);
-    a.stages = std::min<uint32_t>(P_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
+    // A slot per group that may be mixed, where a pair's six stages leave room for three.
+    a.slots = PAIR ? 3 : std::min(P_MAX_SLOTS, (a.nt / P_GROUP + a.split - 1) / a.split);
+    const uint32_t rest = ATOM_BYTES + a.slots * P_SLOT_BYTES + P_GROUP * P_PLACES * 4;
+    a.stages = std::min<uint32_t>(P_MAX_STAGES, (PROJECT_SMEM - rest) / a.stage_bytes);
     cudaLaunchAttribute attrs[2]{};
-    cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, PAIR ? 2 : a.split, attrs);
+    cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + rest, cs, PAIR ? 2 : a.split, attrs);
     attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     c.numAttrs = 2;

@@ -8,7 +8,8 @@ namespace lmz {
 constexpr uint32_t P_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
 constexpr uint32_t P_TOKENS = 256;             // most tokens of a tile: its N, a TMEM column each
 constexpr uint32_t P_GROUP = 16;               // tokens of a TMEM load, and the steps that N comes in (a pair's: 32)
-constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 10;
+constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 10, P_MAX_SLOTS = 8;
+constexpr uint32_t P_SLOT_BYTES = P_GROUP * P_FEATS * 4, P_PLACES = 16;     // places of the rank that mixed groups take at a time
 constexpr uint32_t P_EPILOGUE = 128, P_FEED = 128, P_THREADS = P_EPILOGUE + P_FEED + 64;
 
 // What a tile's tokens have for adapters.
@@ -24,6 +25,7 @@ struct ProjectShared {
     uint64_t info_full[P_INFOS], info_empty[P_INFOS];
     uint64_t loaded[P_INFOS], fed[P_INFOS];    // a tile's steps of the weight, and of the adapters, have all got their stages
     uint64_t sums_full[2], sums_empty[2];
+    uint64_t slot_full[P_MAX_SLOTS], slot_empty[P_MAX_SLOTS];
     uint32_t tmem, over;
     uint32_t same[P_TOKENS / 32];              // bit 0, 1: the tokens of these two sixteens have one adapter; bit 2: both the same
     TileInfo info[P_INFOS];
@@ -44,55 +46,97 @@ struct ProjectArgs {
     uint32_t split;                            // CTAs of a cluster that share K
     uint32_t feat_tiles, token_tiles;          // of P_FEATS (a pair: twice that) and nt
     uint32_t stages, stage_bytes, tmem_columns;
+    uint32_t slots;                            // mixed groups' sums that wait for their way out
 };
 
 // Tiles of a stage: W's 128 rows, and the tokens' (of a pair's 256 each CTA has half).
 __host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt, bool pair) { return (P_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
 
-// Eight elements of a factor times eight of h (upper and lower halves).
-template <class T>
-__device__ __forceinline__ float dot8(const Vec<T, 16> &f, const Vec<T, 16> &hi, const Vec<T, 16> &lo, float sum)
-{
-#pragma unroll
-    for (int e = 0; e < 8; e++) sum += (widen(hi.e[e]) + widen(lo.e[e])) * widen(f.e[e]);
-    return sum;
-}
-
-// What the adapters add to one feature of sixteen tokens that have different ones.  Not on the tensor core: a factor
-// multiplied by the zeros of tokens it does not belong to would still hand them its infinities and NaN.
+// What the adapters add to a tile's features of sixteen tokens that have different ones, into `slot` ([token][feature]), by
+// the four feeding warps.  Not on the tensor core: a factor multiplied by the zeros of tokens it does not belong to would
+// still hand them its infinities and NaN.  Bound by the latency of the factors' loads, sixteen of which a thread keeps under
+// way; `places`: room for sixteen places of the rank of the tokens' h.
 template <class T, bool MN>
-__device__ __forceinline__ void add_mixed(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f, float *v)
+__device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f0, uint32_t id, float *places, float *slot)
 {
-    constexpr int BATCH = 4;
+    constexpr uint32_t BATCH = 8;
+    float sum[P_GROUP] = {};                                     // !MN: per token, of feature `id`; MN: two tokens' eight features
+    const uint32_t fg = id & 15, tg = id >> 4;
+    for (uint32_t j0 = 0; j0 < a.rp; j0 += P_PLACES) {
+        sync_threads(1, P_FEED);
+        {
+            const uint32_t c = id >> 3, j = j0 + (id & 7) * 2;
+            float2 v = make_float2(0, 0);
+            if (adapter[c] >= 0 && j < a.rp) {
+                const T *h = a.hidden + (t0 + c) * 2 * a.rp + j;
+                v = make_float2(widen(h[0]) + widen(h[a.rp]), widen(h[1]) + widen(h[a.rp + 1]));
+            }
+            *reinterpret_cast<float2 *>(places + c * P_PLACES + (id & 7) * 2) = v;
+        }
+        sync_threads(1, P_FEED);
+        if constexpr (MN) {
 #pragma unroll
-    for (int c0 = 0; c0 < static_cast<int>(P_GROUP); c0 += BATCH) {
-        float sum[BATCH] = {};
-        for (uint32_t j = 0; j < a.rp; j += 8) {
-            Vec<T, 16> fac[BATCH], hi[BATCH], lo[BATCH];
+            for (uint32_t half = 0; half < 2; half++) {
+                const uint32_t c = tg + half * 8;
+                const int i = adapter[c];
+                const uint64_t f = f0 + fg * 8;
+                if (i < 0 || f >= a.feats) continue;
+                const T *p = a.factor + i * a.factor_each + j0 * a.factor_row + f;
+                Vec<T, 16> fac[P_PLACES];
 #pragma unroll
-            for (int c = 0; c < BATCH; c++) {
-                const int i = adapter[c0 + c];
-                fac[c].raw = hi[c].raw = lo[c].raw = {};
-                if (i < 0) continue;
-                const T *h = a.hidden + (t0 + c0 + c) * 2 * a.rp + j;
-                hi[c].raw = *reinterpret_cast<const uint4 *>(h);
-                lo[c].raw = *reinterpret_cast<const uint4 *>(h + a.rp);
-                const T *p = a.factor + i * a.factor_each;
-                if constexpr (MN) {
+                for (uint32_t j = 0; j < P_PLACES; j++) {
+                    fac[j].raw = {};
+                    if (j0 + j < a.rank) fac[j].raw = *reinterpret_cast<const uint4 *>(p + j * a.factor_row);
+                }
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; e++)
-                        if (j + e < a.rank) fac[c].e[e] = p[(j + e) * a.factor_row + f];
-                } else {
-                    fac[c].raw = *reinterpret_cast<const uint4 *>(p + f * a.factor_row + j);
+                for (uint32_t j = 0; j < P_PLACES; j++) {
+                    const float h = places[c * P_PLACES + j];
+                    if (j0 + j < a.rank) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; e++) sum[half * 8 + e] += h * widen(fac[j].e[e]);
+                    }
                 }
             }
+        } else {
+            const uint64_t f = f0 + id;
+            if (f < a.feats) {
 #pragma unroll
-            for (int c = 0; c < BATCH; c++) sum[c] = dot8(fac[c], hi[c], lo[c], sum[c]);
+                for (uint32_t c0 = 0; c0 < P_GROUP; c0 += BATCH) {
+                    Vec<T, 16> fac[BATCH][2];
+#pragma unroll
+                    for (uint32_t c = 0; c < BATCH; c++) {
+                        const int i = adapter[c0 + c];
+                        const T *p = a.factor + (i < 0 ? 0 : i) * a.factor_each + f * a.factor_row + j0;
+                        fac[c][0].raw = fac[c][1].raw = {};
+                        if (i >= 0) {
+                            fac[c][0].raw = *reinterpret_cast<const uint4 *>(p);
+                            if (j0 + 8 < a.rp) fac[c][1].raw = *reinterpret_cast<const uint4 *>(p + 8);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < BATCH; c++)
+#pragma unroll
+                        for (uint32_t j = 0; j < P_PLACES; j += 4) {
+                            const float4 h = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + j);
+                            const auto &v = fac[c][j / 8];
+                            sum[c0 + c] += h.x * widen(v.e[j % 8]) + h.y * widen(v.e[j % 8 + 1]) + h.z * widen(v.e[j % 8 + 2]) + h.w * widen(v.e[j % 8 + 3]);
+                        }
+                }
+            }
         }
-#pragma unroll
-        for (int c = 0; c < BATCH; c++)
-            if (adapter[c0 + c] >= 0) v[c0 + c] += sum[c];
     }
+    if constexpr (MN) {
+#pragma unroll
+        for (uint32_t half = 0; half < 2; half++) {
+            float *to = slot + (tg + half * 8) * P_FEATS + fg * 8;
+            *reinterpret_cast<float4 *>(to) = make_float4(sum[half * 8], sum[half * 8 + 1], sum[half * 8 + 2], sum[half * 8 + 3]);
+            *reinterpret_cast<float4 *>(to + 4) = make_float4(sum[half * 8 + 4], sum[half * 8 + 5], sum[half * 8 + 6], sum[half * 8 + 7]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < P_GROUP; c++) slot[c * P_FEATS + id] = sum[c];
+    }
+    sync_threads(1, P_FEED);
 }
 
 // Sixteen tokens' sums of a lane's feature, to y: two lanes exchange halves, so that a store has two features.
@@ -143,6 +187,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
     const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split);
     const uint32_t k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(p_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
+    uint8_t *const local = p_smem + (ring - smem_addr(p_smem));
+    float *const slots = reinterpret_cast<float *>(local + a.stages * a.stage_bytes), *const places = slots + a.slots * (P_SLOT_BYTES / 4);
     const uint32_t wide = (2 * a.rp + STEP_K - 1) / STEP_K;      // steps of a run
     volatile uint32_t *over = &s.over;
 
@@ -151,6 +197,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], CTAS), bar_init(&s.empty[i], 1);
         for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], (side ? 1 : 2) + P_EPILOGUE / 32), bar_init(&s.loaded[i], 1), bar_init(&s.fed[i], 1);
         for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], CTAS * P_EPILOGUE / 32);
+        for (uint32_t i = 0; i < a.slots; i++) bar_init(&s.slot_full[i], 1), bar_init(&s.slot_empty[i], P_EPILOGUE / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if constexpr (PAIR) {
@@ -170,7 +217,19 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         ft = in / w, tt = 8 * b + in % w;
     };
     auto mine = [&](uint32_t run) { return run % a.split == rank; };
+    auto mixed = [&](const TileInfo &info, uint32_t g) { return (info.mixed >> g & 1) && (a.split == 1 || g % a.split == rank); };
     auto features = [&](uint32_t ft) { return (ft * CTAS + side) * P_FEATS; };      // where this CTA's begin
+
+    auto add_slot = [&](RingPlace &slot, float *v) {             // a mixed group's sums
+        if (!warp_wait(&s.slot_full[slot.stage], slot.turn & 1, over)) return false;
+        const float *from = slots + slot.stage * (P_SLOT_BYTES / 4) + tid;
+#pragma unroll
+        for (uint32_t c = 0; c < P_GROUP; c++) v[c] += from[c * P_FEATS];
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.slot_empty[slot.stage]);
+        slot.next(a.slots);
+        return true;
+    };
 
     if (warp == 8) {
         RingPlace at;
@@ -312,7 +371,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 for (uint32_t g = 0; g * GROUP < a.nt; g++) {
                     const int i = info.adapter[g * GROUP];
                     if (!(PAIR ? s.same[g] == 7 : s.same[g / 2] >> (g & 1) & 1)) {
-                        mixed |= (PAIR ? 3u : 1u) << g * CTAS;
+                        mixed |= (PAIR && t0 + g * GROUP + P_GROUP < a.tokens ? 3u : 1u) << g * CTAS;    // (sixteens that have tokens)
                     } else if (i >= 0) {
                         if (end == g && info.run[runs - 1].adapter == i) info.run[runs - 1].tokens += GROUP;
                         else info.run[runs].adapter = i, info.run[runs].column = g * GROUP, info.run[runs].tokens = GROUP, runs++;
@@ -325,7 +384,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             sync_threads(1, P_FEED);
             return true;
         };
-        RingPlace at;
+        RingPlace at, slot;
         uint32_t n = 0;
         bool go = first < tiles && look(first, 0);
         wait_for_previous();                                     // (h)
@@ -335,6 +394,21 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             place(tile, ft, tt);
             const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = features(ft);
             const TileInfo &info = s.info[n % P_INFOS];
+            // As many mixed groups as have a slot while the weight is on its way; the others last, when what makes room for them no
+            // longer waits for this tile's own steps.
+            uint32_t g = 0;
+            auto mix = [&](uint32_t most) {
+                for (; go && most && g * P_GROUP < a.nt; g++) {
+                    if (!mixed(info, g)) continue;
+                    go = sync_all(1, P_FEED, !slot.turn || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
+                    if (!go) break;
+                    mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, places, slots + slot.stage * (P_SLOT_BYTES / 4));
+                    if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
+                    slot.next(a.slots);
+                    most--;
+                }
+            };
+            mix(a.slots);
             at.skip(k1 - k0, a.stages);
             if (!sync_all(1, P_FEED, go && (id || bar_wait(&s.loaded[n % P_INFOS], (n / P_INFOS) & 1, over)))) break;
             for (uint32_t r = 0; go && r < info.runs; r++) {
@@ -377,10 +451,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 }
             }
             if (id == 0) bar_arrive(&s.fed[n % P_INFOS]);
+            mix(P_TOKENS);
         }
     } else {
         const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
         uint32_t n = 0;
+        RingPlace slot;
         wait_for_previous();
         for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
             uint32_t ft, tt;
@@ -395,12 +471,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 float v[P_GROUP];
                 tmem_load16(tmem + (warp << 21) + buf * a.nt + g * P_GROUP, v);
                 if (!PAIR && a.split > 1) {                      // (the stages are free: all products have ended)
-                    float *sums = reinterpret_cast<float *>(p_smem + (ring - smem_addr(p_smem)));
+                    float *sums = reinterpret_cast<float *>(local);
 #pragma unroll
                     for (uint32_t c = 0; c < P_GROUP; c++) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
                 } else {
-                    if (info.mixed >> g & 1 && f < a.feats) add_mixed<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f, v);
-                    __syncwarp();
+                    if (mixed(info, g) && !add_slot(slot, v)) break;
                     store_group(a, t0 + g * P_GROUP, f, pairs, v);
                 }
             }
@@ -422,13 +497,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             const TileInfo &info = s.info[0];
             const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
             const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            RingPlace slot;
             for (uint32_t g = rank; g * P_GROUP < a.nt && t0 + g * P_GROUP < a.tokens; g += a.split) {
                 float v[P_GROUP] = {};
                 for (uint32_t q = 0; q < a.split; q++)
 #pragma unroll
                     for (uint32_t c = 0; c < P_GROUP; c++) v[c] += peer_float(ring + ((g * P_GROUP + c) * P_FEATS + tid) * 4, q);
-                if (info.mixed >> g & 1 && f < a.feats) add_mixed<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f, v);
-                __syncwarp();
+                if (mixed(info, g) && !add_slot(slot, v)) break;
                 store_group(a, t0 + g * P_GROUP, f, pairs, v);
             }
         }
