@@ -379,7 +379,7 @@ typedef struct lmz_projection {
     const void *scales;         /* adapters float32, times `scale`; or NULL */
     void *y;                    /* tokens x out */
     void *hidden;               /* lmz_gpu_project_hidden_bytes(), 256-byte aligned: what the gradients need of the
-                                 * forward pass */
+                                 * forward pass; NULL where there will be none */
     const void *dy;             /* tokens x out */
     void *dx, *da, *db;         /* like x (contiguous), a and b; NULL: not wanted */
     void *work;                 /* lmz_gpu_project_work_bytes(), 256-byte aligned */
@@ -387,7 +387,8 @@ typedef struct lmz_projection {
     uint32_t adapters, rank, dtype, index_bytes;
     float scale;
 } lmz_projection;
-/* Both read the sizes, strides and types alone, and the addresses' last bits; `grad`: for the gradients' call. */
+/* Both read the sizes, strides and types alone, the addresses' last bits and whether there is an index and a `hidden`;
+ * `grad`: for the gradients' call. */
 size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p);
 size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad);
 int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream);

@@ -3,6 +3,7 @@ layers share."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 from . import gpu
 
@@ -33,59 +34,89 @@ def bind(lib) -> None:
         fn.restype, fn.argtypes = res, args
 
 
+_codes = {}
+
+
+def _known():
+    """Element types by the library's numbers (filled on first use: importing this package does not import torch)."""
+    import torch
+    _codes.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32})
+    return _codes
+
+
 def type_code(t, what: str, half_only: bool = False) -> int:
     """The library's number for a tensor's element type, or a TypeError."""
-    import torch
-    code = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}.get(t.dtype)
+    code = (_codes or _known()).get(t.dtype)
     if code is None or (half_only and code == F32):
         raise TypeError(f"{what} must be {'bfloat16 or float16' if half_only else 'bfloat16, float16 or float32'}, not {t.dtype}")
     return code
 
 
-def on_cuda(**tensors):
-    """The CUDA device that all given tensors are on (None for one that is not given), or an error that names who is not."""
+def on_cuda(names: str, *tensors) -> int:
+    """The index of the CUDA device that all given tensors are on (None for one that is not given), or an error that names
+    who is not.  `names`: the tensors', by spaces."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        try:
+            d = t.get_device()
+        except AttributeError:
+            d = -1
+        if device is None:
+            device = d
+        if d < 0 or d != device:
+            _refuse_place(names.split(), tensors)
+    return device
+
+
+def _refuse_place(names, tensors):
     import torch
     device = None
-    for name, t in tensors.items():
+    for name, t in zip(names, tensors):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor")
-        if device is None:
-            device = t.device
-        elif t.device != device:
+        if device is not None and t.device != device:
             raise ValueError(f"{name} is on {t.device}, the tensors before it on {device}")
-    return device
+        device = t.device
 
 
 def whole_numbers(t, what: str) -> int:
     """Bytes of an id: int32 and int64 are taken."""
     import torch
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype is not torch.int32 and t.dtype is not torch.int64:
         raise TypeError(f"{what} must be int32 or int64, not {t.dtype}")
-    return t.element_size()
+    return 4 if t.dtype is torch.int32 else 8
 
 
 def finite(scale, what: str = "scale") -> float:
-    import math
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"{what} must be finite")
     return scale
 
 
-def launch(device, name: str, *args) -> None:
+def stream_of(index: int) -> int:
+    """The device's current stream, as the library takes it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def launch(index: int, name: str, *args) -> None:
     """Call an entry point on the device's current stream (its last argument)."""
     import torch
-    lib = gpu.library()
-    if torch.cuda.current_device() == device.index:
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = getattr(gpu.library(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream_of(index))
     else:
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, stream_of(index))
+    if rc == gpu.OK:
+        return
     if rc == gpu.EUNSUPPORTED:
         raise ValueError(gpu.last_error())
-    if rc != gpu.OK:
-        raise RuntimeError(f"{name} failed ({rc}): {gpu.last_error()}")
+    raise RuntimeError(f"{name} failed ({rc}): {gpu.last_error()}")

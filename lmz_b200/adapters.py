@@ -6,8 +6,6 @@ makes a fine-tune's own weight out of base and adapter; `load` takes the factors
 """
 from __future__ import annotations
 
-import ctypes
-
 from . import _ops, gpu
 
 MAX_RANK = 256
@@ -25,18 +23,18 @@ def project(x, weight, a, b, index=None, scale=1.0):
     Returns [..., out], summed in 32 bits and rounded once.  An adapter's values, infinities and NaN among them, reach only
     its own tokens.  Differentiable once in x, a and b; gradients of a and b sum over each adapter's tokens, with zeros for
     an adapter that none has, and are the same in every run."""
-    device = _ops.on_cuda(x=x, weight=weight, a=a, b=b, index=index)
+    import torch
+    _ops.on_cuda("x weight a b index", x, weight, a, b, index)
     code = _ops.type_code(x, "x", half_only=True)
-    for name, t in (("weight", weight), ("a", a), ("b", b)):
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
+    if weight.dtype is not x.dtype or a.dtype is not x.dtype or b.dtype is not x.dtype:
+        raise TypeError(f"weight is {weight.dtype}, a {a.dtype} and b {b.dtype}, but x {x.dtype}")
     if weight.dim() != 2 or x.dim() < 1:
         raise ValueError(f"weight must be [out, in] and x [..., in], not {list(weight.shape)} and {list(x.shape)}")
-    out, inp = weight.shape
     if a.dim() == 2 and b.dim() == 2:
         a, b = a.unsqueeze(0), b.unsqueeze(0)
-    if a.dim() != 3 or b.dim() != 3 or x.shape[-1] != inp or a.shape[2] != inp or b.shape[1] != out or \
-            a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+    out, inp = weight.shape
+    lead = x.shape[:-1]
+    if a.dim() != 3 or b.dim() != 3 or x.shape[-1] != inp or a.shape[2] != inp or b.shape[1] != out or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
         raise ValueError(f"x {list(x.shape)}, weight {list(weight.shape)}, a {list(a.shape)} and b {list(b.shape)} do not fit "
                          "[..., in], [out, in], [adapters, rank, in] and [adapters, out, rank]")
     if weight.stride(1) != 1 and inp > 1:
@@ -45,74 +43,71 @@ def project(x, weight, a, b, index=None, scale=1.0):
         raise ValueError(f"no adapter, an empty weight, or a rank outside 1..{MAX_RANK}")
     if index is not None:
         _ops.whole_numbers(index, "index")
-        if index.shape != x.shape[:-1]:
-            raise ValueError(f"index is {list(index.shape)}, x has tokens {list(x.shape[:-1])}")
-    import torch
+        if index.shape != lead:
+            raise ValueError(f"index is {list(index.shape)}, x has tokens {list(lead)}")
     scales = None
     if isinstance(scale, torch.Tensor):
         scales, scale = scale, 1.0
-        _ops.on_cuda(x=x, scale=scales)
-        if scales.dtype != torch.float32 or scales.shape != a.shape[:1]:
+        _ops.on_cuda("x scale", x, scales)
+        if scales.dtype is not torch.float32 or scales.shape != a.shape[:1]:
             raise ValueError(f"scale must be a number or float32 [{a.shape[0]}], not {scales.dtype} {list(scales.shape)}")
-    scale = _ops.finite(scale)
-    needs_grad = torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or weight.requires_grad or
-                                              (scales is not None and scales.requires_grad))
-    if needs_grad:
+    else:
+        scale = _ops.finite(scale)
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or weight.requires_grad or
+                                    (scales is not None and scales.requires_grad)):
         if weight.requires_grad or (scales is not None and scales.requires_grad):
             raise ValueError("weight and scale are not trained beside an adapter: they must not require a gradient")
         return _function().apply(x, weight, a, b, index, scales, scale)
-    return _forward(device, code, x, weight, a, b, index, scales, scale)[0]
+    return _forward(code, x, weight, a, b, index, scales, scale, False)[0]
 
 
 def _flat(x):
     """x as [tokens, in] with the elements of a row next to each other, without a copy where it can be."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
-def _call(code, x, weight, a, b, index, scales, scale):
-    p = _ops.Projection()
-    p.x, p.weight, p.a, p.b = x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr()
-    if index is not None:
-        p.index, p.index_bytes = index.data_ptr(), index.element_size()
-    if scales is not None:
-        p.scales = scales.data_ptr()
-    p.tokens, p.in_, p.out = x.shape[0], x.shape[1], weight.shape[0]
-    p.x_stride, p.weight_stride = x.stride(0), weight.stride(0)
-    p.adapters, p.rank, p.dtype, p.scale = a.shape[0], a.shape[1], code, scale
-    return p
+def _packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _forward(device, code, x, weight, a, b, index, scales, scale):
+def _call(code, x, weight, a, b, index, scales, scale, y=None, hidden=None, dy=None, dx=None, da=None, db=None):
+    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+    (tokens, inp), (n, rank, _) = x.shape, a.shape
+    return _ops.Projection(x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), ptr(index), ptr(scales), ptr(y), ptr(hidden), ptr(dy), ptr(dx), ptr(da),
+                           ptr(db), None, tokens, inp, weight.shape[0], x.stride(0), weight.stride(0), n, rank, code,
+                           0 if index is None else index.element_size(), scale)
+
+
+def _run(name: str, grad: int, p, index: int):
     import torch
-    y = torch.empty((*x.shape[:-1], weight.shape[0]), dtype=x.dtype, device=device)
-    lead, x = x.shape[:-1], _flat(x)
-    a, b = a.contiguous(), b.contiguous()
-    index = index.contiguous() if index is not None else None
-    scales = scales.contiguous() if scales is not None else None
-    p = _call(code, x, weight, a, b, index, scales, scale)
-    lib = gpu.library()
-    nh = lib.lmz_gpu_project_hidden_bytes(p)
-    hidden = torch.empty(nh, dtype=torch.uint8, device=device)
-    work = torch.empty(lib.lmz_gpu_project_work_bytes(p, 0), dtype=torch.uint8, device=device)
-    p.y, p.hidden, p.work = y.data_ptr(), hidden.data_ptr(), work.data_ptr()
-    _ops.launch(device, "lmz_gpu_project_dev", p)
+    size = gpu.library().lmz_gpu_project_work_bytes(p, grad)
+    work = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+    p.work = work.data_ptr()
+    _ops.launch(index, name, p)
+
+
+def _forward(code, x, weight, a, b, index, scales, scale, keep):
+    """y, and what the gradients need of it if `keep`."""
+    y = x.new_empty((*x.shape[:-1], weight.shape[0]))
+    x, a, b, index, scales = _flat(x), _packed(a), _packed(b), _packed(index), _packed(scales)
+    hidden = None
+    if keep:
+        import torch
+        p = _call(code, x, weight, a, b, index, scales, scale)
+        hidden = torch.empty(gpu.library().lmz_gpu_project_hidden_bytes(p), dtype=torch.uint8, device=x.device)
+    _run("lmz_gpu_project_dev", 0, _call(code, x, weight, a, b, index, scales, scale, y, hidden), x.get_device())
     return y, hidden
 
 
-def _backward(device, code, dy, x, weight, a, b, index, scales, scale, hidden, wanted):
+def _backward(code, dy, x, weight, a, b, index, scales, scale, hidden, wanted):
     import torch
-    shape, x, dy = x.shape, _flat(x), dy.reshape(-1, dy.shape[-1]).contiguous()
-    ac, bc = a.contiguous(), b.contiguous()
-    index = index.contiguous() if index is not None else None
-    scales = scales.contiguous() if scales is not None else None
-    p = _call(code, x, weight, ac, bc, index, scales, scale)
-    dx, da, db = (torch.empty(s, dtype=x.dtype, device=device) if w else None for s, w in zip((shape, a.shape, b.shape), wanted))
-    p.dy, p.hidden = dy.data_ptr(), hidden.data_ptr()
-    p.dx, p.da, p.db = (t.data_ptr() if t is not None else None for t in (dx, da, db))
-    work = torch.empty(gpu.library().lmz_gpu_project_work_bytes(p, 1), dtype=torch.uint8, device=device)
-    p.work = work.data_ptr()
-    _ops.launch(device, "lmz_gpu_project_grad_dev", p)
+    dx, da, db = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((x, a, b), wanted))
+    x, dy = _flat(x), dy.reshape(-1, dy.shape[-1]).contiguous()
+    a, b, index, scales = _packed(a), _packed(b), _packed(index), _packed(scales)      # (copies live until the launch)
+    p = _call(code, x, weight, a, b, index, scales, scale, None, hidden, dy, dx, da, db)
+    _run("lmz_gpu_project_grad_dev", 1, p, x.get_device())
     return dx, da, db
 
 
@@ -127,7 +122,7 @@ def _function():
             @staticmethod
             def forward(ctx, x, weight, a, b, index, scales, scale):
                 code = _ops.type_code(x, "x", half_only=True)
-                y, hidden = _forward(x.device, code, x, weight, a, b, index, scales, scale)
+                y, hidden = _forward(code, x, weight, a, b, index, scales, scale, True)
                 ctx.save_for_backward(x, weight, a, b, index, scales, hidden)
                 ctx.code, ctx.scale = code, scale
                 return y
@@ -137,7 +132,7 @@ def _function():
             def backward(ctx, dy):
                 x, weight, a, b, index, scales, hidden = ctx.saved_tensors
                 wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])
-                dx, da, db = _backward(dy.device, ctx.code, dy, x, weight, a, b, index, scales, ctx.scale, hidden, wanted)
+                dx, da, db = _backward(ctx.code, dy, x, weight, a, b, index, scales, ctx.scale, hidden, wanted)
                 return dx, None, da, db, None, None, None
 
         _made = Project
@@ -152,7 +147,8 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
 
     `weight`: [out, in], `a`: [rank, in], `b`: [out, rank], all bfloat16 or all float16.  `out`: a contiguous tensor like
     the weight to write to, the weight itself among them; without it a new one.  Not differentiable."""
-    device = _ops.on_cuda(weight=weight, a=a, b=b, out=out)
+    import torch
+    index = _ops.on_cuda("weight a b out", weight, a, b, out)
     code = _ops.type_code(weight, "weight", half_only=True)
     if a.dtype != weight.dtype or b.dtype != weight.dtype:
         raise TypeError(f"a is {a.dtype} and b {b.dtype}, the weight {weight.dtype}")
@@ -164,18 +160,17 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
     if not 1 <= a.shape[0] <= MAX_RANK:
         raise ValueError(f"a rank outside 1..{MAX_RANK}")
     scale = _ops.finite(scale)
-    import torch
     if torch.is_grad_enabled() and any(t.requires_grad for t in (weight, a, b)):
         raise ValueError("merge has no gradient: call it under torch.no_grad()")
     if out is None:
-        out = torch.empty(weight.shape, dtype=weight.dtype, device=device)
+        out = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
     elif out.shape != weight.shape or out.dtype != weight.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of the weight's shape and type")
     elif not _apart(out, a) or not _apart(out, b) or not (_apart(out, weight) or (out.data_ptr() == weight.data_ptr() and weight.is_contiguous())):
         raise ValueError("out may be the weight itself, but not overlap a, b or a part of the weight")
     if out.numel():
-        a, b = a.contiguous(), b.contiguous()
-        _ops.launch(device, "lmz_gpu_merge_dev", weight.data_ptr(), weight.shape[0], weight.shape[1], weight.stride(0), a.data_ptr(), b.data_ptr(),
+        a, b = _packed(a), _packed(b)
+        _ops.launch(index, "lmz_gpu_merge_dev", weight.data_ptr(), weight.shape[0], weight.shape[1], weight.stride(0), a.data_ptr(), b.data_ptr(),
                     a.shape[0], scale, code, out.data_ptr())
     return out
 

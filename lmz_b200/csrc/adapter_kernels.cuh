@@ -33,13 +33,30 @@ __device__ __forceinline__ void split_halves(float v, T &hi, T &lo)
     lo = narrow<T>(isfinite(widen(hi)) ? v - widen(hi) : 0.0f);
 }
 
-// A copy whose rows start on a boundary of 16 bytes and end in zeros: out[o][r][c] = in(o, r, c) for r < rows, c < cols, else 0.
+// Copies whose rows start on a boundary of 16 bytes and end in zeros: out[o][r][c] = in(o, r, c) for c < cols, else 0.
 template <class T>
-__global__ void __launch_bounds__(256) k_pack(const T *in, uint64_t so, uint64_t sr, uint64_t sc, uint64_t rows, uint64_t cols, uint64_t pitch, uint64_t total, T *out)
+struct PackJob {
+    const T *in;
+    T *out;
+    uint64_t so, sr, sc, rows, cols, pitch, total;      // total: outer * rows
+};
+template <class T>
+struct PackArgs {
+    PackJob<T> job[5];
+};
+constexpr uint32_t PACK_ROWS = 8;
+// A warp a row (neighbouring warps take neighbouring rows: of a transposed tensor they read the same lines).
+template <class T>
+__global__ void __launch_bounds__(32 * PACK_ROWS) k_pack(const __grid_constant__ PackArgs<T> a)
 {
-    for (uint64_t e = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; e < total; e += static_cast<uint64_t>(gridDim.x) * 256) {
-        const uint64_t c = e % pitch, q = e / pitch, r = q % rows, o = q / rows;
-        out[e] = c < cols ? in[o * so + r * sr + c * sc] : narrow<T>(0.0f);
+    const PackJob<T> &j = a.job[blockIdx.y];
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * PACK_ROWS + (threadIdx.x >> 5); row < j.total; row += static_cast<uint64_t>(gridDim.x) * PACK_ROWS) {
+        const uint64_t o = row / j.rows;
+        const T *in = j.in + o * j.so + (row - o * j.rows) * j.sr;
+        T *out = j.out + row * j.pitch;
+#pragma unroll 4
+        for (uint64_t c = lane; c < j.pitch; c += 32) out[c] = c < j.cols ? in[c * j.sc] : narrow<T>(0.0f);
     }
 }
 

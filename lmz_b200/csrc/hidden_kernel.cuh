@@ -50,6 +50,8 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     const uint32_t ring = (smem_addr(h_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
     volatile uint32_t *over = &s.over;
 
+    // (Neither kernel leaves an SM room for a block of the other, so the next one's cannot take this block's TMEM.)
+    let_next_start();
     // Which adapters the tile has: a token is its adapter's first if none before it has it.
     if (tid == 0) {
         s.over = 0;
@@ -94,7 +96,6 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     __syncthreads();
     tc_after();
     const uint32_t tmem = s.tmem;
-    let_next_start();                                            // (not before this block has its columns: the next one's may take all that is left)
 
     if (warp == 4) {
         RingPlace at;

@@ -12,6 +12,7 @@
 #include "merge_kernel.cuh"
 #include "project_kernel.cuh"
 #include "rows_kernels.cuh"
+#include "sort_kernel.cuh"
 
 using namespace lmz;
 
@@ -62,6 +63,15 @@ static int by_type(int dtype, uint32_t vb, F f)
     return fail_msg(LMZ_GPU_EUNSUPPORTED, "an element type other than BF16, F16 and F32");
 }
 
+static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute *attr)
+{
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster, attr->val.clusterDim.y = 1, attr->val.clusterDim.z = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attr, c.numAttrs = 1;
+    return c;
+}
+
 static uint32_t lanes_log(uint32_t vectors)
 {
     uint32_t log = 0;
@@ -104,45 +114,56 @@ API int lmz_gpu_rows_dev(const void *d_table, uint64_t rows, uint64_t dim, uint6
     });
 }
 
-// Tokens of a window of the rows' gradient: windows of 32, but not more than 4096 of them.
-static uint32_t rows_window(uint64_t n) { return static_cast<uint32_t>(std::max<uint64_t>(32, (n + 4095) / 4096)); }
+// Tokens of a window of the rows' gradient: 32, and in windows of more for more than 4096 windows' tokens.
+static uint32_t rows_window(uint64_t n) { return static_cast<uint32_t>((std::max<uint64_t>(ROWS_STEP, (n + 4095) / 4096) + ROWS_STEP - 1) / ROWS_STEP * ROWS_STEP); }
 
 struct RowsGradLayout {
-    uint64_t keys[2], pos[2], start, partial, end;
-    RowsGradLayout(uint64_t n, uint64_t rows, uint64_t dim)
+    uint64_t keys[2], pos[2], partial, end;
+    RowsGradLayout(uint64_t n, uint64_t dim)
     {
         uint64_t at = 0;
         auto take = [&](uint64_t bytes) { const uint64_t r = at; at += (bytes + 255) & ~255ull; return r; };
         for (int i = 0; i < 2; i++) keys[i] = take(n * 4), pos[i] = take(n * 4);
-        start = take((rows + 1) * 4);
         const uint64_t w = rows_window(n);
         partial = take(n > w ? (n + w - 1) / w * 2 * dim * 4 : 0);
         end = at;
     }
 };
 
-// Sort ids; on return *side is where the result lies.
+// Sort ids (and clear memory beside it); on return *side is where the result lies.
 static int launch_sort(SortArgs &s, cudaStream_t cs, int *side)
 {
     static bool done[64];
-    int rc = opt_in_smem(k_sort, SORT_SMEM, done);
+    int sms = 0, rc = sm_count(&sms);
+    if (!rc) rc = opt_in_smem(k_sort, sort_smem(SORT_DIGIT), done);
     if (rc) return rc;
     uint32_t bits = 1;
     while (bits < 32 && s.nkeys >> bits) bits++;
-    s.passes = (bits + 7) / 8;
-    cudaLaunchConfig_t c{};
+    s.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT, s.digit = std::max(5u, (bits + s.passes - 1) / s.passes);
+    // (a thousand elements are sorted by one CTA before a cluster has met)
+    s.ctas = s.n <= SORT_THREADS ? 1 : SORT_CTAS;
+    const uint64_t clear = std::min<uint64_t>((s.zero_bytes + (64 << 10) - 1) / (64 << 10), 2ull * sms);
     cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    const uint32_t ctas = s.n <= 2 * SORT_THREADS ? 1 : SORT_CTAS;
-    attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-    c.gridDim = dim3(ctas), c.blockDim = dim3(SORT_THREADS), c.dynamicSmemBytes = SORT_SMEM, c.stream = cs;
-    c.attrs = &attr, c.numAttrs = 1;
-    CK("launch k_sort", cudaLaunchKernelEx(&c, k_sort, s));
+    const cudaLaunchConfig_t c = clustered(dim3(s.ctas + static_cast<unsigned>((clear + s.ctas - 1) / s.ctas * s.ctas)), SORT_THREADS, sort_smem(s.digit), cs, s.ctas, &attr);
+    CK("launch k_sort", cudaLaunchKernelEx(&c, k_sort, static_cast<const SortArgs>(s)));
     *side = (s.passes - 1) & 1;
     return LMZ_GPU_OK;
 }
 
-API size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t rows, uint64_t dim) { return RowsGradLayout(n, rows, dim).end; }
+API size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t, uint64_t dim) { return RowsGradLayout(n, dim).end; }
+
+// A launch whose blocks may start before the kernel in front of it has ended (they wait for it themselves).
+template <class K, class A>
+static int launch_behind(const char *what, K kernel, dim3 grid, unsigned threads, cudaStream_t cs, const A &args)
+{
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid, c.blockDim = dim3(threads), c.stream = cs, c.attrs = &attr, c.numAttrs = 1;
+    CK(what, cudaLaunchKernelEx(&c, kernel, args));
+    return LMZ_GPU_OK;
+}
 
 API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dtype, const void *d_ids, int id_bytes, uint64_t rows,
                               float scale, void *d_dtable, void *d_work, void *cuda_stream)
@@ -158,34 +179,28 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
         CK("cudaMemsetAsync", cudaMemsetAsync(d_dtable, 0, rows * bytes, cs));
         return LMZ_GPU_OK;
     }
-    const RowsGradLayout l(n, rows, dim);
+    const RowsGradLayout l(n, dim);
     uint8_t *work = static_cast<uint8_t *>(d_work);
     auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(work + off); };
     SortArgs s{};
-    s.ids = d_ids, s.n = n, s.nkeys = rows, s.wide = id_bytes == 8;
+    s.ids = d_ids, s.n = n, s.nkeys = rows, s.wide = id_bytes == 8, s.zero = static_cast<uint8_t *>(d_dtable), s.zero_bytes = rows * bytes;
     for (int i = 0; i < 2; i++) s.keys[i] = words(l.keys[i]), s.pos[i] = words(l.pos[i]);
     int side = 0;
     rc = launch_sort(s, cs, &side);
     if (rc) return rc;
-    k_key_starts<<<static_cast<unsigned>(rows / 256 + 1), 256, 0, cs>>>(s.keys[side], static_cast<uint32_t>(n), static_cast<uint32_t>(rows), words(l.start));
-    rc = launched("launch k_key_starts");
-    if (rc) return rc;
     return by_type(dtype, vector_bytes(bytes, {address(d_dy), address(d_dtable)}), [&](auto type, auto vec) {
         using T = decltype(type);
-        constexpr int VB = sizeof(vec.raw), U = 4;
+        constexpr int VB = sizeof(vec.raw);
         RowsGradArgs a{};
-        a.dy = static_cast<const uint8_t *>(d_dy), a.keys = s.keys[side], a.pos = s.pos[side], a.start = words(l.start);
+        a.dy = static_cast<const uint8_t *>(d_dy), a.keys = s.keys[side], a.pos = s.pos[side];
         a.partial = reinterpret_cast<float *>(work + l.partial), a.out = static_cast<uint8_t *>(d_dtable);
-        a.rows = rows, a.row_bytes = bytes, a.dim = dim, a.n = static_cast<uint32_t>(n), a.window = rows_window(n), a.scale = scale;
-        a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = lanes_log(a.vectors);
-        const uint32_t slices = (a.vectors + ROW_THREADS - 1) / ROW_THREADS, per = (ROW_THREADS >> a.lane_log) * U;
-        if (a.n > a.window) {
-            k_rows_grad_windows<T, VB><<<dim3((a.n + a.window - 1) / a.window, slices), ROW_THREADS, 0, cs>>>(a);
-            const int failed = launched("launch k_rows_grad_windows");
-            if (failed) return failed;
-        }
-        k_rows_grad<T, VB, U><<<dim3(static_cast<unsigned>((rows + per - 1) / per), slices), ROW_THREADS, 0, cs>>>(a);
-        return launched("launch k_rows_grad");
+        a.rows = static_cast<uint32_t>(rows), a.row_bytes = bytes, a.dim = dim, a.n = static_cast<uint32_t>(n), a.window = rows_window(n), a.scale = scale;
+        a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = std::max(5u, lanes_log(a.vectors));
+        const uint32_t slices = (a.vectors + ROW_THREADS - 1) / ROW_THREADS, per = ROW_THREADS >> a.lane_log;
+        const dim3 grid(((a.n + a.window - 1) / a.window + per - 1) / per, slices);
+        int failed = launch_behind("launch k_rows_sums", k_rows_sums<T, VB>, grid, ROW_THREADS, cs, a);
+        if (!failed && a.n > a.window) failed = launch_behind("launch k_rows_join", k_rows_join<T, VB>, grid, ROW_THREADS, cs, a);
+        return failed;
     });
 }
 
@@ -237,7 +252,7 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
 
 // What a projection's kernels read in place of tensors that do not lie on boundaries, and between each other.
 struct ProjectLayout {
-    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, end = 0;
+    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, hidden, end = 0;
     bool pack_x, pack_w, pack_a, pack_b, pack_dy;
     ProjectLayout(const lmz_projection *p, bool grad)
     {
@@ -260,21 +275,12 @@ struct ProjectLayout {
         const bool sorted = grad && p->index;
         for (int i = 0; i < 2; i++) keys[i] = take(sorted, p->tokens * 4), pos[i] = take(sorted, p->tokens * 4);
         start = take(sorted, (p->adapters + 1ull) * 4);
+        hidden = take(!grad && !p->hidden, p->tokens * 4 * up8(p->rank));
     }
 };
 
 API size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p) { return p->tokens * 4 * up8(p->rank); }
 API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { return ProjectLayout(p, grad).end; }
-
-// out[o][r][0 .. up8(cols)) of a tensor with any strides.
-template <class T>
-static int launch_pack(const T *in, uint64_t outer, uint64_t so, uint64_t rows, uint64_t sr, uint64_t cols, uint64_t sc, T *out, cudaStream_t cs)
-{
-    const uint64_t total = outer * rows * up8(cols);
-    if (!total) return LMZ_GPU_OK;
-    k_pack<T><<<static_cast<unsigned>(std::min<uint64_t>((total + 255) / 256, 148 * 16)), 256, 0, cs>>>(in, so, sr, sc, rows, cols, up8(cols), total, out);
-    return launched("launch k_pack");
-}
 
 constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
 constexpr uint32_t PROJECT_SMEM = 219u << 10;
@@ -283,15 +289,6 @@ static uint32_t tmem_columns(uint32_t n)
 {
     uint32_t c = 32;
     while (c < n) c *= 2;
-    return c;
-}
-
-static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute *attr)
-{
-    attr->id = cudaLaunchAttributeClusterDimension;
-    attr->val.clusterDim.x = cluster, attr->val.clusterDim.y = 1, attr->val.clusterDim.z = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attr, c.numAttrs = 1;
     return c;
 }
 
@@ -408,26 +405,36 @@ static int launch_factor_grad(const lmz_projection *p, const T *z, uint64_t stri
     return LMZ_GPU_OK;
 }
 
-// A projection's tensors as the kernels take them: where they lie, or packed into the workspace.
+// A projection's tensors as the kernels take them: where they lie, or packed into the workspace (in one launch).
 template <class T>
 struct ProjectInputs {
-    const T *x, *w, *a, *dy;
+    const T *x, *w, *a, *b, *dy;
     uint64_t x_stride, w_stride, a_stride, dy_stride;
     int rc;
     ProjectInputs(const lmz_projection *p, const ProjectLayout &l, bool grad, cudaStream_t cs)
-        : x(static_cast<const T *>(p->x)), w(static_cast<const T *>(p->weight)), a(static_cast<const T *>(p->a)), dy(static_cast<const T *>(p->dy)),
-          x_stride(p->x_stride), w_stride(p->weight_stride), a_stride(p->in), dy_stride(p->out), rc(LMZ_GPU_OK)
+        : x(static_cast<const T *>(p->x)), w(static_cast<const T *>(p->weight)), a(static_cast<const T *>(p->a)), b(static_cast<const T *>(p->b)),
+          dy(static_cast<const T *>(p->dy)), x_stride(p->x_stride), w_stride(p->weight_stride), a_stride(p->in), dy_stride(p->out), rc(LMZ_GPU_OK)
     {
-        auto pack = [&](bool on, const T *&t, uint64_t outer, uint64_t rows, uint64_t &stride, uint64_t cols, uint64_t off) {
-            if (!on || rc) return;
+        PackArgs<T> args{};
+        uint32_t jobs = 0;
+        uint64_t most = 0;
+        auto job = [&](const T *&t, uint64_t outer, uint64_t so, uint64_t rows, uint64_t sr, uint64_t cols, uint64_t sc, uint64_t off) {
             T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off);
-            rc = launch_pack(t, outer, rows * stride, rows, stride, cols, 1, to, cs);
-            t = to, stride = up8(cols);
+            args.job[jobs++] = {t, to, so, sr, sc, rows, cols, up8(cols), outer * rows};
+            most = std::max(most, outer * rows);
+            t = to;
         };
-        pack(l.pack_x, x, 1, p->tokens, x_stride, p->in, l.x);
-        pack(l.pack_w, w, 1, p->out, w_stride, p->in, l.w);
-        pack(l.pack_a, a, p->adapters, p->rank, a_stride, p->in, l.a);
-        if (grad) pack(l.pack_dy, dy, 1, p->tokens, dy_stride, p->out, l.dy);
+        const uint64_t r = p->rank;
+        if (l.pack_x) job(x, 1, 0, p->tokens, x_stride, p->in, 1, l.x), x_stride = up8(p->in);
+        if (l.pack_w) job(w, 1, 0, p->out, w_stride, p->in, 1, l.w), w_stride = up8(p->in);
+        if (l.pack_a) job(a, 1, 0, p->adapters * r, p->in, p->in, 1, l.a), a_stride = up8(p->in);
+        if (grad && l.pack_dy) job(dy, 1, 0, p->tokens, p->out, p->out, 1, l.dy), dy_stride = up8(p->out);
+        if (grad) job(b, p->adapters, p->out * r, r, 1, p->out, r, l.b);
+        else if (l.pack_b) job(b, 1, 0, p->adapters * p->out, r, r, 1, l.b);
+        if (!jobs) return;
+        const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((most + PACK_ROWS - 1) / PACK_ROWS, 1u << 20)), jobs);
+        k_pack<T><<<grid, 32 * PACK_ROWS, 0, cs>>>(args);
+        rc = launched("launch k_pack");
     }
 };
 
@@ -436,17 +443,10 @@ static int project_as(const lmz_projection *p, cudaStream_t cs)
 {
     const ProjectLayout l(p, false);
     const ProjectInputs<T> in(p, l, false, cs);
+    T *h = static_cast<T *>(p->hidden ? p->hidden : static_cast<uint8_t *>(p->work) + l.hidden);
     int rc = in.rc;
-    const T *b = static_cast<const T *>(p->b);
-    T *h = static_cast<T *>(p->hidden);
-    const uint64_t r = p->rank;
-    if (!rc && l.pack_b) {
-        T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + l.b);
-        rc = launch_pack(b, p->adapters, p->out * r, p->out, r, r, 1, to, cs);
-        b = to;
-    }
     if (!rc) rc = launch_hidden(p, in.x, in.x_stride, p->in, in.a, in.a_stride, h, cs);
-    if (!rc) rc = launch_project<T, false>(p, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, b, p->out, up8(r), h, static_cast<T *>(p->y), cs);
+    if (!rc) rc = launch_project<T, false>(p, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, in.b, p->out, up8(p->rank), h, static_cast<T *>(p->y), cs);
     return rc;
 }
 
@@ -464,24 +464,18 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
     int rc = in.rc;
     uint8_t *work = static_cast<uint8_t *>(p->work);
     T *g = reinterpret_cast<T *>(work + l.g);
-    if (!rc && (p->dx || p->da)) {
-        T *bt = reinterpret_cast<T *>(work + l.b);
-        rc = launch_pack(static_cast<const T *>(p->b), p->adapters, r * p->out, r, 1, p->out, r, bt, cs);
-        if (!rc) rc = launch_hidden(p, in.dy, in.dy_stride, p->out, bt, up8(p->out), g, cs);
-    }
+    if (!rc && (p->dx || p->da)) rc = launch_hidden(p, in.dy, in.dy_stride, p->out, in.b, up8(p->out), g, cs);
     if (!rc && p->dx) rc = launch_project<T, true>(p, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, g, static_cast<T *>(p->dx), cs);
     const uint32_t *order = nullptr, *start = nullptr;
     if (!rc && p->index && (p->da || p->db)) {
         SortArgs s{};
         s.ids = p->index, s.n = p->tokens, s.nkeys = p->adapters, s.wide = p->index_bytes == 8;
         for (int i = 0; i < 2; i++) s.keys[i] = reinterpret_cast<uint32_t *>(work + l.keys[i]), s.pos[i] = reinterpret_cast<uint32_t *>(work + l.pos[i]);
+        s.start = reinterpret_cast<uint32_t *>(work + l.start);
         int side = 0;
         rc = launch_sort(s, cs, &side);
         if (rc) return rc;
-        uint32_t *starts = reinterpret_cast<uint32_t *>(work + l.start);
-        k_key_starts<<<p->adapters / 256 + 1, 256, 0, cs>>>(s.keys[side], static_cast<uint32_t>(p->tokens), p->adapters, starts);
-        rc = launched("launch k_key_starts");
-        order = s.pos[side], start = starts;
+        order = s.pos[side], start = s.start;
     }
     if (!rc && p->da) rc = launch_factor_grad<T>(p, in.x, in.x_stride, p->in, g, order, start, static_cast<T *>(p->da), 1, p->in, cs);
     if (!rc && p->db) rc = launch_factor_grad<T>(p, in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), order, start, static_cast<T *>(p->db), r, 1, cs);

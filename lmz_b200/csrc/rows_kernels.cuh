@@ -1,6 +1,6 @@
 // Rows of an embedding table, and the table's gradient.
 #pragma once
-#include "sort_kernel.cuh"
+#include "tcgen.cuh"
 #include "vectors.cuh"
 
 namespace lmz {
@@ -59,101 +59,127 @@ __global__ void __launch_bounds__(ROW_THREADS) k_rows(RowsArgs a)
 
 struct RowsGradArgs {
     const uint8_t *dy;
-    const uint32_t *keys, *pos, *start;          // the sorted ids, the tokens that have them, and where each row's begin
+    const uint32_t *keys, *pos;                  // the sorted ids, and the tokens that have them
     float *partial;                              // [window][2][dim]
     uint8_t *out;
-    uint64_t rows, row_bytes, dim;
-    uint32_t n, window;                          // tokens of a window: a row with more of them is summed window by window
+    uint64_t row_bytes, dim;
+    uint32_t rows, n, window;                    // window: sorted tokens that are summed up in a row
     uint32_t vectors, lane_log;
     float scale;
 };
 
+constexpr uint32_t ROWS_STEP = 32;               // tokens whose ids a window has in shared memory at a time
+
+// dE[v] = scale * sum of dy[t] over the tokens t with id v, for the rows that have tokens (the others are zeros already).
+// Sums in 32 bits and one order (the tokens' own), no atomics: the same result every time.
+//
+// A window of sorted tokens after the other: a row whose tokens lie within one is finished there; the others leave a sum
+// per window, in slot 0 where they began before it and in slot 1 where they go on behind it, which k_rows_join adds up.
+// Bound by reading dy (and, before it, by the zeros of the table's other rows); 8 tokens' rows are under way at a time.
 template <class T, int VB>
-__device__ __forceinline__ void add_rows(const RowsGradArgs &a, uint32_t from, uint32_t to, uint32_t v, float *sum)
+__global__ void __launch_bounds__(ROW_THREADS) k_rows_sums(const RowsGradArgs a)
 {
     using V = Vec<T, VB>;
-    constexpr int AHEAD = 4;
-    for (uint32_t i = from; i < to; i += AHEAD) {
-        V x[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; j++) {
-            x[j].raw = {};
-            if (i + j < to) x[j].raw = reinterpret_cast<const typename Raw<VB>::type *>(a.dy + a.pos[i + j] * a.row_bytes)[v];
+    constexpr int N = V::N, AHEAD = 8;
+    __shared__ uint32_t s_key[ROW_THREADS / 32][ROWS_STEP + 1], s_pos[ROW_THREADS / 32][ROWS_STEP];
+    const uint32_t threads = 1u << a.lane_log, lane = threadIdx.x & (threads - 1), sub = threadIdx.x >> a.lane_log;
+    const uint64_t w = static_cast<uint64_t>(blockIdx.x) * (ROW_THREADS >> a.lane_log) + sub;
+    const uint32_t v = blockIdx.y * ROW_THREADS + lane;
+    const uint64_t w0 = w * a.window, w1 = w0 + a.window < a.n ? w0 + a.window : a.n;
+    let_next_start();
+    wait_for_previous();
+    const uint32_t before = w0 && w0 < a.n ? a.keys[w0 - 1] : ~0u;
+    float sum[N] = {};
+    bool began = true;                                           // the row began in this window
+    uint32_t key = ~0u;
+    for (uint64_t s0 = w0; s0 < w0 + a.window; s0 += ROWS_STEP) {
+        __syncthreads();                                         // (all threads of a block take as many steps)
+        for (uint32_t i = lane; i <= ROWS_STEP; i += threads) {
+            const uint64_t at = s0 + i;
+            s_key[sub][i] = at < a.n ? a.keys[at] : ~0u;
+            if (i < ROWS_STEP) s_pos[sub][i] = at < a.n ? a.pos[at] : 0;
         }
+        __syncthreads();
+        if (v >= a.vectors || s0 >= w1) continue;
+        const uint32_t count = w1 - s0 < ROWS_STEP ? static_cast<uint32_t>(w1 - s0) : ROWS_STEP;
+        for (uint32_t i = 0; i < count; i += AHEAD) {
+            V x[AHEAD];
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; j++) {
+                x[j].raw = {};
+                if (i + j < count && s_key[sub][i + j] < a.rows)
+                    x[j].raw = reinterpret_cast<const typename Raw<VB>::type *>(a.dy + s_pos[sub][i + j] * a.row_bytes)[v];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; j++) {
+                if (i + j >= count) break;
+                const uint32_t mine = s_key[sub][i + j];
+                if (mine >= a.rows) break;
+                if (mine != key) {
+                    began = mine != before;                      // (a row before this window can only be its first)
+                    key = mine;
+#pragma unroll
+                    for (int e = 0; e < N; e++) sum[e] = 0;
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) sum[e] += widen(x[j].e[e]);
+                const bool ends = s_key[sub][i + j + 1] != mine, last = s0 + i + j + 1 == w1;
+                if (!ends && !last) continue;
+                if (ends && began) {
+                    V y;
+#pragma unroll
+                    for (int e = 0; e < N; e++) y.e[e] = narrow<T>(sum[e] * a.scale);
+                    reinterpret_cast<typename Raw<VB>::type *>(a.out + mine * a.row_bytes)[v] = y.raw;
+                } else {
+                    float *to = a.partial + (w * 2 + began) * a.dim + static_cast<uint64_t>(v) * N;
+#pragma unroll
+                    for (int e = 0; e < N; e++) to[e] = sum[e];
+                }
+            }
+        }
+    }
+}
+
+// The rows whose tokens lie in more than one window: by the window that they begin in.
+template <class T, int VB>
+__global__ void __launch_bounds__(ROW_THREADS) k_rows_join(const RowsGradArgs a)
+{
+    using V = Vec<T, VB>;
+    constexpr int N = V::N, AHEAD = 8;
+    const uint32_t threads = 1u << a.lane_log, lane = threadIdx.x & (threads - 1), sub = threadIdx.x >> a.lane_log;
+    const uint64_t w = static_cast<uint64_t>(blockIdx.x) * (ROW_THREADS >> a.lane_log) + sub;
+    const uint32_t v = blockIdx.y * ROW_THREADS + lane;
+    const uint64_t w0 = w * a.window, w1 = w0 + a.window;
+    wait_for_previous();
+    if (v >= a.vectors || w1 >= a.n) return;
+    const uint32_t key = a.keys[w1 - 1];
+    if (key >= a.rows || a.keys[w1] != key || (w0 && a.keys[w0 - 1] == key)) return;
+    uint64_t lo = w1, hi = a.n;                                  // where the row's tokens end
+    while (lo < hi) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        if (a.keys[mid] <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    const uint64_t last = (lo - 1) / a.window;
+    const float *from = a.partial + (w * 2 + 1) * a.dim + static_cast<uint64_t>(v) * N;
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) sum[e] = from[e];
+    for (uint64_t i = w + 1; i <= last; i += AHEAD) {
+        float x[AHEAD][N];
 #pragma unroll
         for (int j = 0; j < AHEAD; j++)
-            if (i + j < to) {
 #pragma unroll
-                for (int e = 0; e < V::N; e++) sum[e] += widen(x[j].e[e]);
-            }
+            for (int e = 0; e < N; e++) x[j][e] = i + j <= last ? a.partial[(i + j) * 2 * a.dim + static_cast<uint64_t>(v) * N + e] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) sum[e] += x[j][e];
     }
-}
-
-// The rows that more than `window` tokens have: what each window of sorted tokens adds to the row it begins in and to
-// the row it ends in.  (No window holds parts of a third: that row would lie between them, with fewer tokens.)
-template <class T, int VB>
-__global__ void __launch_bounds__(ROW_THREADS) k_rows_grad_windows(RowsGradArgs a)
-{
-    constexpr int N = Vec<T, VB>::N;
-    const uint32_t v = blockIdx.y * ROW_THREADS + threadIdx.x;
-    const uint32_t w0 = blockIdx.x * a.window, w1 = a.n - w0 < a.window ? a.n : w0 + a.window;
-    if (v >= a.vectors) return;
-    const uint32_t ends[2] = {a.keys[w0], a.keys[w1 - 1]};
+    V y;
 #pragma unroll
-    for (int side = 0; side < 2; side++) {
-        const uint32_t key = ends[side];
-        if (key >= a.rows || (side && key == ends[0])) continue;
-        const uint32_t s = a.start[key], e = a.start[key + 1];
-        if (e - s <= a.window) continue;
-        float sum[N] = {};
-        add_rows<T, VB>(a, s > w0 ? s : w0, e < w1 ? e : w1, v, sum);
-        float *to = a.partial + (static_cast<uint64_t>(blockIdx.x) * 2 + side) * a.dim + static_cast<uint64_t>(v) * N;
-#pragma unroll
-        for (int i = 0; i < N; i++) to[i] = sum[i];
-    }
-}
-
-// dE[v] = scale * sum of dy[t] over the tokens t with id v, every row of the gradient written once, zeros for rows
-// without tokens.  Sums in 32 bits and one order (the tokens' own), no atomics: the same result every time.
-//
-// Bound by HBM: dy read and dE written once; for a large vocabulary the zeros are most of it.
-template <class T, int VB, int U>
-__global__ void __launch_bounds__(ROW_THREADS) k_rows_grad(RowsGradArgs a)
-{
-    using V = Vec<T, VB>;
-    constexpr int N = V::N;
-    const uint32_t lane = threadIdx.x & ((1u << a.lane_log) - 1), sub = threadIdx.x >> a.lane_log;
-    const uint32_t per = ROW_THREADS >> a.lane_log;
-    const uint32_t v = blockIdx.y * ROW_THREADS + lane;
-    if (v >= a.vectors) return;
-    uint32_t s[U], e[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * U + u) * per + sub;
-        s[u] = e[u] = 0;
-        if (row < a.rows) s[u] = a.start[row], e[u] = a.start[row + 1];
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * U + u) * per + sub;
-        if (row >= a.rows) continue;
-        float sum[N] = {};
-        if (e[u] - s[u] <= a.window) {
-            add_rows<T, VB>(a, s[u], e[u], v, sum);
-        } else {
-            const uint32_t first = s[u] / a.window, last = (e[u] - 1) / a.window;
-            for (uint32_t w = first; w <= last; w++) {
-                const uint32_t side = w == first && s[u] != w * a.window;
-                const float *from = a.partial + (static_cast<uint64_t>(w) * 2 + side) * a.dim + static_cast<uint64_t>(v) * N;
-#pragma unroll
-                for (int i = 0; i < N; i++) sum[i] += from[i];
-            }
-        }
-        V y;
-#pragma unroll
-        for (int i = 0; i < N; i++) y.e[i] = narrow<T>(sum[i] * a.scale);
-        reinterpret_cast<typename Raw<VB>::type *>(a.out + row * a.row_bytes)[v] = y.raw;
-    }
+    for (int e = 0; e < N; e++) y.e[e] = narrow<T>(sum[e] * a.scale);
+    reinterpret_cast<typename Raw<VB>::type *>(a.out + key * a.row_bytes)[v] = y.raw;
 }
 
 }  // namespace lmz

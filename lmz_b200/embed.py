@@ -18,40 +18,40 @@ def lookup(table, tokens, scale: float = 1.0):
 
     Differentiable in `table`, once: the gradient is dense and contiguous, summed in 32 bits over each row's tokens in their
     order, and the same in every run."""
-    device = _ops.on_cuda(table=table, tokens=tokens)
+    import torch
+    index = _ops.on_cuda("table tokens", table, tokens)
+    code = _ops.type_code(table, "table")
+    id_bytes = _ops.whole_numbers(tokens, "tokens")
     if table.dim() != 2:
         raise ValueError(f"table must be [rows, dim], not {list(table.shape)}")
-    _ops.type_code(table, "table")
-    _ops.whole_numbers(tokens, "tokens")
-    if table.shape[1] > 1 and table.stride(1) != 1:
+    if table.stride(1) != 1 and table.shape[1] > 1:
         raise ValueError("the elements of a row of the table must be next to each other")
-    scale = _ops.finite(scale)
-    import torch
+    if scale != 1.0:
+        scale = _ops.finite(scale)
     if table.requires_grad and torch.is_grad_enabled():
         return _function().apply(table, tokens, scale)
-    return _rows(device, table, tokens, scale)
+    return _rows(index, code, id_bytes, table, tokens, scale)
 
 
-def _rows(device, table, tokens, scale):
-    import torch
+def _rows(index, code, id_bytes, table, tokens, scale):
     rows, dim = table.shape
-    out = torch.empty((*tokens.shape, dim), dtype=table.dtype, device=device)
-    if out.numel():
-        ids = tokens.contiguous()
-        _ops.launch(device, "lmz_gpu_rows_dev", table.data_ptr(), rows, dim, table.stride(0), _ops.type_code(table, "table"), ids.data_ptr(),
-                    ids.element_size(), ids.numel(), scale, out.data_ptr())
+    out = table.new_empty((*tokens.shape, dim))
+    n = tokens.numel()
+    if n and dim:
+        ids = tokens if tokens.is_contiguous() else tokens.contiguous()
+        _ops.launch(index, "lmz_gpu_rows_dev", table.data_ptr(), rows, dim, table.stride(0), code, ids.data_ptr(), id_bytes, n, scale, out.data_ptr())
     return out
 
 
-def _rows_grad(device, dy, tokens, rows: int, scale):
+def _rows_grad(dy, tokens, rows: int, scale):
     import torch
     dim = dy.shape[-1]
-    grad = torch.empty((rows, dim), dtype=dy.dtype, device=device)
+    grad = dy.new_empty((rows, dim))
     if grad.numel():
-        ids, dy = tokens.contiguous(), dy.contiguous()
-        work = torch.empty(gpu.library().lmz_gpu_rows_grad_work_bytes(ids.numel(), rows, dim), dtype=torch.uint8, device=device)
-        _ops.launch(device, "lmz_gpu_rows_grad_dev", dy.data_ptr(), ids.numel(), dim, _ops.type_code(dy, "dy"), ids.data_ptr(), ids.element_size(), rows,
-                    scale, grad.data_ptr(), work.data_ptr())
+        ids, dy, n = tokens.contiguous(), dy.contiguous(), tokens.numel()
+        work = torch.empty(gpu.library().lmz_gpu_rows_grad_work_bytes(n, rows, dim), dtype=torch.uint8, device=dy.device)
+        _ops.launch(dy.get_device(), "lmz_gpu_rows_grad_dev", dy.data_ptr(), n, dim, _ops.type_code(dy, "dy"), ids.data_ptr(), ids.element_size(), rows, scale,
+                    grad.data_ptr(), work.data_ptr())
     return grad
 
 
@@ -67,13 +67,13 @@ def _function():
             def forward(ctx, table, tokens, scale):
                 ctx.save_for_backward(tokens)
                 ctx.rows, ctx.scale = table.shape[0], scale
-                return _rows(table.device, table, tokens, scale)
+                return _rows(table.get_device(), _ops.type_code(table, "table"), tokens.element_size(), table, tokens, scale)
 
             @staticmethod
             @once_differentiable
             def backward(ctx, dy):
                 (tokens,) = ctx.saved_tensors
-                return _rows_grad(dy.device, dy, tokens, ctx.rows, ctx.scale), None, None
+                return _rows_grad(dy, tokens, ctx.rows, ctx.scale), None, None
 
         _made = Rows
     return _made
