@@ -44,19 +44,30 @@ template <class T>
 struct PackArgs {
     PackJob<T> job[5];
 };
-constexpr uint32_t PACK_ROWS = 8;
-// A warp a row (neighbouring warps take neighbouring rows: of a transposed tensor they read the same lines).
+constexpr uint32_t PACK_WARPS = 8, PACK_COLS = 256;
+// A warp 256 columns of a row.  Neighbouring warps take neighbouring rows where those lie closer to each other than a row's
+// elements (a transposed tensor: they read the same lines), else the row's next columns.
 template <class T>
-__global__ void __launch_bounds__(32 * PACK_ROWS) k_pack(const __grid_constant__ PackArgs<T> a)
+__global__ void __launch_bounds__(32 * PACK_WARPS) k_pack(const __grid_constant__ PackArgs<T> a)
 {
     const PackJob<T> &j = a.job[blockIdx.y];
-    const uint32_t lane = threadIdx.x & 31;
-    for (uint64_t row = static_cast<uint64_t>(blockIdx.x) * PACK_ROWS + (threadIdx.x >> 5); row < j.total; row += static_cast<uint64_t>(gridDim.x) * PACK_ROWS) {
-        const uint64_t o = row / j.rows;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t parts = (j.pitch + PACK_COLS - 1) / PACK_COLS, units = j.total * parts;
+    for (uint64_t u = static_cast<uint64_t>(blockIdx.x) * PACK_WARPS + warp; u < units; u += static_cast<uint64_t>(gridDim.x) * PACK_WARPS) {
+        const uint64_t row = j.sc == 1 ? u / parts : u % j.total, part = j.sc == 1 ? u - row * parts : u / j.total, o = row / j.rows;
         const T *in = j.in + o * j.so + (row - o * j.rows) * j.sr;
         T *out = j.out + row * j.pitch;
-#pragma unroll 4
-        for (uint64_t c = lane; c < j.pitch; c += 32) out[c] = c < j.cols ? in[c * j.sc] : narrow<T>(0.0f);
+        T v[PACK_COLS / 32];
+#pragma unroll
+        for (uint32_t q = 0; q < PACK_COLS / 32; q++) {
+            const uint64_t c = part * PACK_COLS + q * 32 + lane;
+            v[q] = c < j.cols ? in[c * j.sc] : narrow<T>(0.0f);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < PACK_COLS / 32; q++) {
+            const uint64_t c = part * PACK_COLS + q * 32 + lane;
+            if (c < j.pitch) out[c] = v[q];
+        }
     }
 }
 

@@ -5,138 +5,160 @@
 
 namespace lmz {
 
-constexpr uint32_t FG_FEATS = 128, FG_THREADS = 256, FG_MAX_STAGES = 4;
+constexpr uint32_t FG_FEATS = 128, FG_THREADS = 128, FG_MAX_STAGES = 8;
 constexpr uint32_t FG_PITCH = FG_FEATS + 1;
+
+struct FactorGradShared {
+    uint64_t full[FG_MAX_STAGES], empty[FG_MAX_STAGES], sums;
+    uint32_t tmem, over;
+};
 
 template <class T>
 struct FactorGradArgs {
-    const T *z, *thin;                         // rows of the tokens: `stride` elements apart, and [2][rp]
+    CUtensorMap z, z_rows, thin, thin_rows;    // tiles of 64 x 64, and of one row (for gathers)
     const uint32_t *order, *start;             // tokens sorted by adapter and where each adapter's begin; NULL: all have adapter 0
     T *out;                                    // dF_i(f, j) at i * each + f * wide + j * place
-    uint64_t stride, feats, each, wide, place;
+    uint64_t feats, each, wide, place;
     uint32_t tokens, rank, rp, split;
+    uint32_t blocks;                           // of FG_FEATS features
     uint32_t stages, stage_bytes, tmem_columns;
 };
 
-// Bytes of a half of the thin rows' tile: blocks of 64 columns by 64 tokens.
-__host__ __device__ constexpr uint32_t thin_tile_bytes(uint32_t rp) { return (rp + 63) / 64 * STEP_K * ROW_BYTES; }
+// A row of the thin product, both halves, in blocks of 64 columns; a stage of 64 tokens.
+__host__ __device__ constexpr uint32_t thin_blocks(uint32_t rp) { return (2 * rp + 63) / 64; }
+constexpr uint32_t FG_TILE = STEP_K * ROW_BYTES;
+__host__ __device__ constexpr uint32_t factor_stage_bytes(uint32_t blocks, uint32_t rp) { return (2 * blocks + thin_blocks(rp)) * FG_TILE; }
 
 // dF_i(f, j) = sum over i's tokens of thin[t][j] z[t][f].
 //
-// Tokens are the tensor core's K.  They come one by one in the order of a sort by adapter, so that a sum has its own tokens and
-// no others (a foreign token times zero would still bring its infinities in), in one order.  Rows are copied as they lie,
-// both operands MN-major; z's tile meets both halves of the thin rows.  Bound by reading z once, 128 features a block;
-// the CTAs of a cluster share an adapter's tokens.
+// Tokens are the tensor core's K, and come in the order of a sort by adapter, so that a sum has its own tokens and no others
+// (a foreign token times zero would still bring its infinities in), in one order.  Rows are brought as they lie, both
+// operands MN-major: 64 neighbours by a tile's copy, others by gathers of four rows, whose places behind the last token read
+// as zeros.  The halves of the thin rows are columns of their own, added at the end.  Bound by reading z (256 features a block,
+// so that the thin rows are read half as often as by 128); the CTAs of a cluster share an adapter's tokens.
 template <class T>
-__global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const FactorGradArgs<T> a)
+__global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constant__ FactorGradArgs<T> a)
 {
     extern __shared__ uint8_t f_smem[];
-    __shared__ uint64_t freed[FG_MAX_STAGES];
-    __shared__ uint64_t sums;
-    __shared__ uint32_t s_tmem, s_over;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5;
+    __shared__ FactorGradShared s;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
-    const uint64_t f0 = static_cast<uint64_t>(blockIdx.x / a.split) * FG_FEATS;
-    const uint32_t i = blockIdx.y;
-    const uint32_t begin = a.start ? a.start[i] : 0, total = a.start ? a.start[i + 1] - begin : a.tokens;
-    const uint32_t lo = begin + static_cast<uint32_t>(static_cast<uint64_t>(total) * rank / a.split);
-    const uint32_t hi = begin + static_cast<uint32_t>(static_cast<uint64_t>(total) * (rank + 1) / a.split);
-    const uint32_t steps = (hi - lo + STEP_K - 1) / STEP_K;
+    const uint32_t f0 = blockIdx.x / a.split * a.blocks * FG_FEATS, i = blockIdx.y;
+    const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : a.tokens;
+    const uint32_t all = (end - begin + STEP_K - 1) / STEP_K;
+    const uint32_t n0 = static_cast<uint32_t>(static_cast<uint64_t>(all) * rank / a.split), n1 = static_cast<uint32_t>(static_cast<uint64_t>(all) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(f_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
-    const uint32_t half = thin_tile_bytes(a.rp), z_bytes = FG_FEATS * STEP_K * 2;
-    float *part = reinterpret_cast<float *>(f_smem + (ring - smem_addr(f_smem)));
-    volatile uint32_t *over = &s_over;
+    const uint32_t thins = thin_blocks(a.rp), thin_at = 2 * a.blocks * FG_TILE;
+    volatile uint32_t *over = &s.over;
 
     if (tid == 0) {
-        s_over = 0;
-        for (uint32_t st = 0; st < a.stages; st++) bar_init(&freed[st], 1);
-        bar_init(&sums, 1);
+        s.over = 0;
+        for (uint32_t st = 0; st < a.stages; st++) bar_init(&s.full[st], 1), bar_init(&s.empty[st], 1);
+        bar_init(&s.sums, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 0) tmem_alloc(&s_tmem, a.tmem_columns);
+    if (warp == 1) tmem_alloc(&s.tmem, a.tmem_columns);
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = s.tmem;
 
-    auto load = [&](uint32_t n) {
-        if (n < steps) {
-            const uint32_t dst = ring + n % a.stages * a.stage_bytes, at = lo + n * STEP_K;
-            for (uint32_t e = tid; e < STEP_K * 16; e += FG_THREADS) {
-                const uint32_t row = e >> 4, c = e & 15;
-                const uint64_t f = f0 + c * 8;
-                const bool on = at + row < hi && f < a.feats;
-                const uint64_t t = on ? (a.order ? a.order[at + row] : at + row) : 0;
-                copy16(dst + (c >> 3) * STEP_K * ROW_BYTES + swizzled(row, c & 7), on ? a.z + t * a.stride + f : a.z, on);
-            }
-            const uint32_t parts = a.rp / 8;
-            for (uint32_t e = tid; e < STEP_K * parts * 2; e += FG_THREADS) {
-                const uint32_t row = e / (parts * 2), q = e % (parts * 2), lower = q >= parts, c = lower ? q - parts : q;
-                const bool on = at + row < hi;
-                const uint64_t t = on ? (a.order ? a.order[at + row] : at + row) : 0;
-                copy16(dst + z_bytes + lower * half + (c >> 3) * STEP_K * ROW_BYTES + swizzled(row, c & 7),
-                       on ? a.thin + t * 2 * a.rp + q * 8 : a.thin, on);
-            }
-        }
-        copies_commit();
-    };
-    const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), true, true, FG_FEATS, (a.rp + 15) & ~15u);
-    for (uint32_t n = 0; n + 1 < a.stages; n++) load(n);
-    bool ok = true;
-    for (uint32_t n = 0; n < steps && ok; n++) {
-        if (a.stages == 2) copies_wait<0>();
-        else if (a.stages == 3) copies_wait<1>();
-        else copies_wait<2>();
-        publish_smem();
-        __syncthreads();
-        if (tid == 0) {
-            const uint32_t src = ring + n % a.stages * a.stage_bytes;
-            tc_after();
-            for (uint32_t h = 0; h < 2; h++)
+    if (warp == 0) {
+        RingPlace at;
+        for (uint32_t n = n0; n < n1; n++, at.next(a.stages)) {
+            const uint32_t p = begin + n * STEP_K, left = end - p, st = at.stage, dst = ring + st * a.stage_bytes;
+            // four rows of a lane: its gathers', and the first and last tell whether all are neighbours
+            uint32_t row[4];
 #pragma unroll
-                for (uint32_t c = 0; c < STEP_K / 16; c++)
-                    mma16(tmem, desc_lo(src + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES),
-                          desc_lo(src + z_bytes + h * half + c * 16 * ROW_BYTES, STEP_K * ROW_BYTES), desc, n || h || c);
-            mma_commit(&freed[n % a.stages]);
+            for (uint32_t q = 0; q < 4; q++) {
+                const uint32_t o = (lane & 15) * 4 + q;
+                row[q] = o < left ? (a.order ? a.order[p + o] : p + o) : a.tokens;
+            }
+            const uint32_t first = __shfl_sync(~0u, row[0], 0), last = __shfl_sync(~0u, row[3], 15);
+            const bool tile = left >= STEP_K && last - first == STEP_K - 1;      // (an adapter's tokens ascend)
+            if (at.turn && !warp_wait(&s.empty[st], (at.turn - 1) & 1, over)) break;
+            if (lane == 0) bar_expect(&s.full[st], a.stage_bytes);
+            __syncwarp();
+            if (tile) {
+                if (elected()) {
+                    for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_load_2d(&a.z, &s.full[st], dst + b * FG_TILE, f0 + b * 64, first);
+                    for (uint32_t b = 0; b < thins; b++) tma_load_2d(&a.thin, &s.full[st], dst + thin_at + b * FG_TILE, b * 64, first);
+                }
+            } else if (lane < 16) {
+                for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_gather4(&a.z_rows, &s.full[st], dst + b * FG_TILE + lane * 4 * ROW_BYTES, f0 + b * 64, row);
+                for (uint32_t b = 0; b < thins; b++) tma_gather4(&a.thin_rows, &s.full[st], dst + thin_at + b * FG_TILE + lane * 4 * ROW_BYTES, b * 64, row);
+            }
+            __syncwarp();
         }
-        if (n + a.stages - 1 < steps) {                          // the stage of the step before is next to be filled
-            ok = n == 0 || bar_wait(&freed[(n - 1) % a.stages], ((n - 1) / a.stages) & 1, over);
-            ok = __syncthreads_and(ok);
+        if (*over)                                               // nothing may still be on its way into this block's memory
+            for (uint32_t st = 0; st < a.stages; st++) {
+                const uint32_t used = at.turn - (st >= at.stage);                // the last turn that filled this stage
+                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[st], used & 1); tries++) {}
+            }
+    } else if (warp == 1) {
+        // at most 256 columns a product, in whole blocks
+        const uint32_t columns = 2 * a.rp, one = columns < 256 ? columns : 256, two = columns - one;
+        constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+        const uint32_t desc = mma_desc(bf16, true, true, FG_FEATS, one), desc2 = mma_desc(bf16, true, true, FG_FEATS, two);
+        const uint32_t z_lo = desc_lo(ring, FG_TILE), t_lo = desc_lo(ring + thin_at, FG_TILE);
+        RingPlace at;
+        for (uint32_t n = n0; n < n1; n++, at.next(a.stages)) {
+            const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+            if (!warp_wait(&s.full[st], at.turn & 1, over)) break;
+            if (elected()) {
+                for (uint32_t b = 0; b < a.blocks; b++) {
+                    const uint32_t z = z_lo + off + (b * 2 * FG_TILE >> 4), d = tmem + b * columns;
+#pragma unroll
+                    for (uint32_t c = 0; c < STEP_K / 16; c++) {
+                        mma16(d, z + (c * 16 * ROW_BYTES >> 4), t_lo + off + (c * 16 * ROW_BYTES >> 4), desc, n != n0 || c);
+                        if (two) mma16(d + one, z + (c * 16 * ROW_BYTES >> 4), t_lo + off + (4 * FG_TILE + c * 16 * ROW_BYTES >> 4), desc2, n != n0 || c);
+                    }
+                }
+                mma_commit(&s.empty[st]);
+            }
+            __syncwarp();
         }
-        if (ok) load(n + a.stages - 1);
+        if (elected()) mma_commit(&s.sums);
+        __syncwarp();
     }
-    copies_wait<0>();
-    if (tid == 0) mma_commit(&sums);
-    ok = __syncthreads_and(bar_wait(&sums, 0, over) && ok);
+    __syncwarp();
+    const bool ok = __syncthreads_and(warp_wait(&s.sums, 0, over));
+    float *part = reinterpret_cast<float *>(f_smem + (ring - smem_addr(f_smem)));
     tc_after();
-    if (warp < 4 && ok) {
-        for (uint32_t c = 0; c < a.rp; c += 8) {
-            float v[8] = {};
-            if (steps) tmem_load8(tmem + (warp << 21) + c, v);
+    if (ok && !*over) {                                          // the halves' sums, over the stages
+        for (uint32_t b = 0; b < a.blocks; b++)
+            for (uint32_t c = 0; c < a.rp; c += 8) {
+                float v[8] = {}, w[8] = {};
+                if (n1 > n0) {
+                    tmem_load8(tmem + (warp << 21) + b * 2 * a.rp + c, v);
+                    tmem_load8(tmem + (warp << 21) + b * 2 * a.rp + a.rp + c, w);
+                }
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) part[(c + e) * FG_PITCH + tid] = v[e];
-        }
-        tc_before();
+                for (uint32_t e = 0; e < 8; e++) part[(b * a.rp + c + e) * FG_PITCH + tid] = v[e] + w[e];
+            }
     }
+    tc_before();
     __syncwarp();
     if (a.split > 1) cluster_barrier();
     else __syncthreads();
-    if (ok) {
+    if (ok && !*over) {
         T *out = a.out + i * a.each;
-        const uint32_t share = FG_FEATS / a.split, mine = a.wide == 1 ? FG_FEATS : share;
+        const uint32_t wide = a.blocks * FG_FEATS, share = wide / a.split;
         // neighbouring threads write neighbouring elements: along f (a CTA every split-th j), or along j (a CTA its share of the f)
-        for (uint32_t e = tid; e < (a.wide == 1 ? (a.rank + a.split - 1 - rank) / a.split : a.rank) * mine; e += FG_THREADS) {
-            const uint32_t j = a.wide == 1 ? rank + e / FG_FEATS * a.split : e % a.rank, row = a.wide == 1 ? e % FG_FEATS : rank * share + e / a.rank;
-            if (f0 + row >= a.feats) continue;
-            float sum = 0;
-            for (uint32_t q = 0; q < a.split; q++) sum += peer_float(ring + (j * FG_PITCH + row) * 4, q);
-            out[(f0 + row) * a.wide + j * a.place] = narrow<T>(sum);
+        const bool along_f = a.wide == 1;
+        const uint32_t count = along_f ? (a.rank + a.split - 1 - rank) / a.split * wide : a.rank * share;
+#pragma unroll 4
+        for (uint32_t e = tid; e < count; e += FG_THREADS) {
+            const uint32_t j = along_f ? rank + e / wide * a.split : e % a.rank, row = along_f ? e % wide : rank * share + e / a.rank;
+            const uint64_t f = f0 + static_cast<uint64_t>(row);
+            if (f >= a.feats) continue;
+            out[f * a.wide + j * a.place] = narrow<T>(peer_sum(ring + ((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, a.split));
         }
     }
-    if (a.split > 1) cluster_barrier();
+    if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums
     tc_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         tc_after();
         tmem_free(tmem, a.tmem_columns);
     }

@@ -156,12 +156,12 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     else __syncthreads();
     if (!*over) {                                                // a CTA's share of the tokens: the sums of all, in order
         const uint32_t each = H_TOKENS / a.split, lo = rank * each;
+#pragma unroll 2
         for (uint32_t e = tid; e < each * a.rp; e += H_THREADS) {
             const uint32_t row = lo + e / a.rp, c = e % a.rp;
             const int slot = s.slot[row] - static_cast<int>(from);
             if (slot < 0 || slot >= static_cast<int>(count)) continue;
-            float sum = 0;
-            for (uint32_t q = 0; q < a.split; q++) sum += peer_float(ring + (c * H_PITCH + row) * 4, q);
+            const float sum = peer_sum(ring + (c * H_PITCH + row) * 4, a.split);
             T hi, lo_half;
             split_halves(c < a.rank ? sum * a.index.scale_of(s.adapter[row]) : 0.0f, hi, lo_half);
             T *to = a.h + (t0 + row) * 2 * a.rp + c;

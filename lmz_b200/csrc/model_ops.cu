@@ -130,21 +130,19 @@ struct RowsGradLayout {
     }
 };
 
-// Sort ids (and clear memory beside it); on return *side is where the result lies.
+// Sort ids; on return *side is where the result lies.
 static int launch_sort(SortArgs &s, cudaStream_t cs, int *side)
 {
     static bool done[64];
-    int sms = 0, rc = sm_count(&sms);
-    if (!rc) rc = opt_in_smem(k_sort, sort_smem(SORT_DIGIT), done);
+    const int rc = opt_in_smem(k_sort, sort_smem(SORT_DIGIT), done);
     if (rc) return rc;
     uint32_t bits = 1;
     while (bits < 32 && s.nkeys >> bits) bits++;
     s.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT, s.digit = std::max(5u, (bits + s.passes - 1) / s.passes);
     // (a thousand elements are sorted by one CTA before a cluster has met)
-    s.ctas = s.n <= SORT_THREADS ? 1 : SORT_CTAS;
-    const uint64_t clear = std::min<uint64_t>((s.zero_bytes + (64 << 10) - 1) / (64 << 10), 2ull * sms);
+    const uint32_t ctas = s.n <= SORT_THREADS ? 1 : SORT_CTAS;
     cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(s.ctas + static_cast<unsigned>((clear + s.ctas - 1) / s.ctas * s.ctas)), SORT_THREADS, sort_smem(s.digit), cs, s.ctas, &attr);
+    const cudaLaunchConfig_t c = clustered(dim3(ctas), SORT_THREADS, sort_smem(s.digit), cs, ctas, &attr);
     CK("launch k_sort", cudaLaunchKernelEx(&c, k_sort, static_cast<const SortArgs>(s)));
     *side = (s.passes - 1) & 1;
     return LMZ_GPU_OK;
@@ -153,15 +151,15 @@ static int launch_sort(SortArgs &s, cudaStream_t cs, int *side)
 API size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t, uint64_t dim) { return RowsGradLayout(n, dim).end; }
 
 // A launch whose blocks may start before the kernel in front of it has ended (they wait for it themselves).
-template <class K, class A>
-static int launch_behind(const char *what, K kernel, dim3 grid, unsigned threads, cudaStream_t cs, const A &args)
+template <class K, class... A>
+static int launch_behind(const char *what, K kernel, dim3 grid, unsigned threads, cudaStream_t cs, A... args)
 {
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t c{};
     c.gridDim = grid, c.blockDim = dim3(threads), c.stream = cs, c.attrs = &attr, c.numAttrs = 1;
-    CK(what, cudaLaunchKernelEx(&c, kernel, args));
+    CK(what, cudaLaunchKernelEx(&c, kernel, args...));
     return LMZ_GPU_OK;
 }
 
@@ -183,10 +181,13 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
     uint8_t *work = static_cast<uint8_t *>(d_work);
     auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(work + off); };
     SortArgs s{};
-    s.ids = d_ids, s.n = n, s.nkeys = rows, s.wide = id_bytes == 8, s.zero = static_cast<uint8_t *>(d_dtable), s.zero_bytes = rows * bytes;
+    s.ids = d_ids, s.n = n, s.nkeys = rows, s.wide = id_bytes == 8;
     for (int i = 0; i < 2; i++) s.keys[i] = words(l.keys[i]), s.pos[i] = words(l.pos[i]);
     int side = 0;
     rc = launch_sort(s, cs, &side);
+    const uint64_t total = rows * bytes, blocks = (total + CLEAR_BYTES - 1) / CLEAR_BYTES;
+    if (!rc && blocks >= 1u << 30) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a table of 64 TiB and more");
+    if (!rc) rc = launch_behind("launch k_clear", k_clear, dim3(static_cast<unsigned>(blocks)), CLEAR_THREADS, cs, static_cast<uint8_t *>(d_dtable), total);
     if (rc) return rc;
     return by_type(dtype, vector_bytes(bytes, {address(d_dy), address(d_dtable)}), [&](auto type, auto vec) {
         using T = decltype(type);
@@ -388,19 +389,24 @@ static int launch_factor_grad(const lmz_projection *p, const T *z, uint64_t stri
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     FactorGradArgs<T> a{};
-    a.z = z, a.thin = thin, a.order = order, a.start = start, a.out = out, a.stride = stride, a.feats = feats;
+    a.order = order, a.start = start, a.out = out, a.feats = feats;
     a.each = feats * p->rank, a.wide = wide, a.place = place;
     a.tokens = static_cast<uint32_t>(p->tokens), a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
-    a.stage_bytes = FG_FEATS * STEP_K * 2 + 2 * thin_tile_bytes(a.rp), a.tmem_columns = tmem_columns((a.rp + 15) & ~15u);
-    // two blocks to an SM where the thin rows are short
-    a.stages = a.rp <= 64 ? 3 : std::min<uint32_t>(FG_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
-    const uint64_t tiles = (feats + FG_FEATS - 1) / FG_FEATS;
+    a.blocks = a.rp <= 128 ? 2 : 1;                              // (as many as TMEM has columns for)
+    a.stage_bytes = factor_stage_bytes(a.blocks, a.rp), a.tmem_columns = tmem_columns(a.blocks * 2 * a.rp);
+    a.stages = std::min<uint32_t>(FG_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
+    const uint64_t wide_tiles = (feats + a.blocks * FG_FEATS - 1) / (a.blocks * FG_FEATS);
     a.split = 1;
-    while (a.split < 8 && tiles * p->adapters * a.split * 2 <= 4ull * sms && p->tokens >= 2ull * STEP_K * a.split) a.split *= 2;
-    rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
+    while (a.split < 8 && wide_tiles * p->adapters * a.split * 2 <= (uint64_t)sms && p->tokens >= 4ull * STEP_K * a.split) a.split *= 2;
+    constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+    rc = tensor_map(&a.z, z, bf16, feats, p->tokens, stride, STEP_K);
+    if (!rc) rc = tensor_map(&a.z_rows, z, bf16, feats, p->tokens, stride, 1);
+    if (!rc) rc = tensor_map(&a.thin, thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, STEP_K);
+    if (!rc) rc = tensor_map(&a.thin_rows, thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, 1);
+    if (!rc) rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
     if (rc) return rc;
     cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(tiles * a.split), p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(wide_tiles * a.split), p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
     CK("launch k_factor_grad", cudaLaunchKernelEx(&c, k_factor_grad<T>, a));
     return LMZ_GPU_OK;
 }
@@ -421,7 +427,7 @@ struct ProjectInputs {
         auto job = [&](const T *&t, uint64_t outer, uint64_t so, uint64_t rows, uint64_t sr, uint64_t cols, uint64_t sc, uint64_t off) {
             T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off);
             args.job[jobs++] = {t, to, so, sr, sc, rows, cols, up8(cols), outer * rows};
-            most = std::max(most, outer * rows);
+            most = std::max(most, outer * rows * ((up8(cols) + PACK_COLS - 1) / PACK_COLS));
             t = to;
         };
         const uint64_t r = p->rank;
@@ -432,8 +438,8 @@ struct ProjectInputs {
         if (grad) job(b, p->adapters, p->out * r, r, 1, p->out, r, l.b);
         else if (l.pack_b) job(b, 1, 0, p->adapters * p->out, r, r, 1, l.b);
         if (!jobs) return;
-        const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((most + PACK_ROWS - 1) / PACK_ROWS, 1u << 20)), jobs);
-        k_pack<T><<<grid, 32 * PACK_ROWS, 0, cs>>>(args);
+        const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((most + PACK_WARPS - 1) / PACK_WARPS, 1u << 20)), jobs);
+        k_pack<T><<<grid, 32 * PACK_WARPS, 0, cs>>>(args);
         rc = launched("launch k_pack");
     }
 };

@@ -499,10 +499,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
             RingPlace slot;
             for (uint32_t g = rank; g * P_GROUP < a.nt && t0 + g * P_GROUP < a.tokens; g += a.split) {
-                float v[P_GROUP] = {};
-                for (uint32_t q = 0; q < a.split; q++)
+                float v[P_GROUP];
 #pragma unroll
-                    for (uint32_t c = 0; c < P_GROUP; c++) v[c] += peer_float(ring + ((g * P_GROUP + c) * P_FEATS + tid) * 4, q);
+                for (uint32_t c = 0; c < P_GROUP; c++) v[c] = peer_sum(ring + ((g * P_GROUP + c) * P_FEATS + tid) * 4, a.split);
                 if (mixed(info, g) && !add_slot(slot, v)) break;
                 store_group(a, t0 + g * P_GROUP, f, pairs, v);
             }

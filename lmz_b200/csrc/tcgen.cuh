@@ -113,6 +113,12 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *ba
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
+// Four rows, by their numbers, of a map whose tiles are one row high (a row behind the tensor's last reads as zeros).
+__device__ __forceinline__ void tma_gather4(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, const uint32_t *row)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]) : "memory");
+}
 // 16 bytes from global to shared memory, or zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on)
 {
@@ -240,14 +246,24 @@ __device__ __forceinline__ void cluster_barrier()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// A word of another CTA's shared memory, by this CTA's address of it.
-__device__ __forceinline__ float peer_float(uint32_t addr, uint32_t rank)
+// The sum over a cluster's CTAs, in their order, of a word that each has at the same address (at most eight CTAs; all loads are
+// under way together).
+__device__ __forceinline__ float peer_sum(uint32_t addr, uint32_t ctas)
 {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
+    float v[8];
+#pragma unroll
+    for (uint32_t q = 0; q < 8; q++) {
+        v[q] = 0;
+        if (q < ctas) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(q));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(at) : "memory");
+        }
+    }
+    float sum = v[0];
+#pragma unroll
+    for (uint32_t q = 1; q < 8; q++) sum += v[q];
+    return sum;
 }
 
 }  // namespace lmz
