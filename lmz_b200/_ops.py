@@ -100,6 +100,24 @@ def finite(scale, what: str = "scale") -> float:
     return scale
 
 
+def once(backward):
+    """A backward pass that has no gradient of its own: as torch's `once_differentiable`, without its cost where nobody asked
+    for a graph of the gradients."""
+    wrapped = None
+
+    def run(ctx, *grads):
+        nonlocal wrapped
+        import torch
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        if wrapped is None:
+            from torch.autograd.function import once_differentiable
+            wrapped = once_differentiable(backward)
+        return wrapped(ctx, *grads)
+
+    return run
+
+
 def stream_of(index: int) -> int:
     """The device's current stream, as the library takes it."""
     import torch

@@ -83,8 +83,9 @@ def _call(code, x, weight, a, b, index, scales, scale, y=None, hidden=None, dy=N
 def _run(name: str, grad: int, p, index: int):
     import torch
     size = gpu.library().lmz_gpu_project_work_bytes(p, grad)
-    work = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
-    p.work = work.data_ptr()
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+        p.work = work.data_ptr()
     _ops.launch(index, name, p)
 
 
@@ -92,12 +93,12 @@ def _forward(code, x, weight, a, b, index, scales, scale, keep):
     """y, and what the gradients need of it if `keep`."""
     y = x.new_empty((*x.shape[:-1], weight.shape[0]))
     x, a, b, index, scales = _flat(x), _packed(a), _packed(b), _packed(index), _packed(scales)
-    hidden = None
+    p, hidden = _call(code, x, weight, a, b, index, scales, scale, y), None
     if keep:
         import torch
-        p = _call(code, x, weight, a, b, index, scales, scale)
         hidden = torch.empty(gpu.library().lmz_gpu_project_hidden_bytes(p), dtype=torch.uint8, device=x.device)
-    _run("lmz_gpu_project_dev", 0, _call(code, x, weight, a, b, index, scales, scale, y, hidden), x.get_device())
+        p.hidden = hidden.data_ptr()
+    _run("lmz_gpu_project_dev", 0, p, x.get_device())
     return y, hidden
 
 
@@ -116,7 +117,6 @@ def _function():
     global _made
     if _made is None:
         import torch
-        from torch.autograd.function import once_differentiable
 
         class Project(torch.autograd.Function):
             @staticmethod
@@ -128,7 +128,7 @@ def _function():
                 return y
 
             @staticmethod
-            @once_differentiable
+            @_ops.once
             def backward(ctx, dy):
                 x, weight, a, b, index, scales, hidden = ctx.saved_tensors
                 wanted = (ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3])

@@ -13,12 +13,19 @@ struct FactorGradShared {
     uint32_t tmem, over;
 };
 
+// One factor's gradient.
 template <class T>
-struct FactorGradArgs {
+struct FactorGradJob {
     CUtensorMap z, z_rows, thin, thin_rows;    // tiles of 64 x 64, and of one row (for gathers)
-    const uint32_t *order, *start;             // tokens sorted by adapter and where each adapter's begin; NULL: all have adapter 0
     T *out;                                    // dF_i(f, j) at i * each + f * wide + j * place
     uint64_t feats, each, wide, place;
+    uint32_t clusters;                         // that it takes
+};
+
+template <class T>
+struct FactorGradArgs {
+    FactorGradJob<T> job[2];
+    const uint32_t *order, *start;             // tokens sorted by adapter and where each adapter's begin; NULL: all have adapter 0
     uint32_t tokens, rank, rp, split;
     uint32_t blocks;                           // of FG_FEATS features
     uint32_t stages, stage_bytes, tmem_columns;
@@ -36,6 +43,7 @@ __host__ __device__ constexpr uint32_t factor_stage_bytes(uint32_t blocks, uint3
 // operands MN-major: 64 neighbours by a tile's copy, others by gathers of four rows, whose places behind the last token read
 // as zeros.  The halves of the thin rows are columns of their own, added at the end.  Bound by reading z (256 features a block,
 // so that the thin rows are read half as often as by 128); the CTAs of a cluster share an adapter's tokens.
+// The two factors' gradients are one launch: its first clusters make the one, the others the other.
 template <class T>
 __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constant__ FactorGradArgs<T> a)
 {
@@ -43,7 +51,9 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     __shared__ FactorGradShared s;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = a.split > 1 ? cluster_rank() : 0;
-    const uint32_t f0 = blockIdx.x / a.split * a.blocks * FG_FEATS, i = blockIdx.y;
+    const uint32_t place = blockIdx.x / a.split, which = place >= a.job[0].clusters;
+    const FactorGradJob<T> &g = a.job[which];
+    const uint32_t f0 = (which ? place - a.job[0].clusters : place) * a.blocks * FG_FEATS, i = blockIdx.y;
     const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : a.tokens;
     const uint32_t all = (end - begin + STEP_K - 1) / STEP_K;
     const uint32_t n0 = static_cast<uint32_t>(static_cast<uint64_t>(all) * rank / a.split), n1 = static_cast<uint32_t>(static_cast<uint64_t>(all) * (rank + 1) / a.split);
@@ -81,12 +91,12 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
             __syncwarp();
             if (tile) {
                 if (elected()) {
-                    for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_load_2d(&a.z, &s.full[st], dst + b * FG_TILE, f0 + b * 64, first);
-                    for (uint32_t b = 0; b < thins; b++) tma_load_2d(&a.thin, &s.full[st], dst + thin_at + b * FG_TILE, b * 64, first);
+                    for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_load_2d(&g.z, &s.full[st], dst + b * FG_TILE, f0 + b * 64, first);
+                    for (uint32_t b = 0; b < thins; b++) tma_load_2d(&g.thin, &s.full[st], dst + thin_at + b * FG_TILE, b * 64, first);
                 }
             } else if (lane < 16) {
-                for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_gather4(&a.z_rows, &s.full[st], dst + b * FG_TILE + lane * 4 * ROW_BYTES, f0 + b * 64, row);
-                for (uint32_t b = 0; b < thins; b++) tma_gather4(&a.thin_rows, &s.full[st], dst + thin_at + b * FG_TILE + lane * 4 * ROW_BYTES, b * 64, row);
+                for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_gather4(&g.z_rows, &s.full[st], dst + b * FG_TILE + lane * 4 * ROW_BYTES, f0 + b * 64, row);
+                for (uint32_t b = 0; b < thins; b++) tma_gather4(&g.thin_rows, &s.full[st], dst + thin_at + b * FG_TILE + lane * 4 * ROW_BYTES, b * 64, row);
             }
             __syncwarp();
         }
@@ -142,17 +152,17 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     if (a.split > 1) cluster_barrier();
     else __syncthreads();
     if (ok && !*over) {
-        T *out = a.out + i * a.each;
+        T *out = g.out + i * g.each;
         const uint32_t wide = a.blocks * FG_FEATS, share = wide / a.split;
         // neighbouring threads write neighbouring elements: along f (a CTA every split-th j), or along j (a CTA its share of the f)
-        const bool along_f = a.wide == 1;
+        const bool along_f = g.wide == 1;
         const uint32_t count = along_f ? (a.rank + a.split - 1 - rank) / a.split * wide : a.rank * share;
 #pragma unroll 4
         for (uint32_t e = tid; e < count; e += FG_THREADS) {
             const uint32_t j = along_f ? rank + e / wide * a.split : e % a.rank, row = along_f ? e % wide : rank * share + e / a.rank;
             const uint64_t f = f0 + static_cast<uint64_t>(row);
-            if (f >= a.feats) continue;
-            out[f * a.wide + j * a.place] = narrow<T>(peer_sum(ring + ((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, a.split));
+            if (f >= g.feats) continue;
+            out[f * g.wide + j * g.place] = narrow<T>(peer_sum(ring + ((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, a.split));
         }
     }
     if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums

@@ -380,33 +380,48 @@ static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride,
     return LMZ_GPU_OK;
 }
 
-// dF_i(f, j) = the sum over i's tokens of thin[t][j] z[t][f].
+// One factor's gradient: dF_i(f, j) = the sum over i's tokens of thin[t][j] z[t][f].
 template <class T>
-static int launch_factor_grad(const lmz_projection *p, const T *z, uint64_t stride, uint64_t feats, const T *thin, const uint32_t *order, const uint32_t *start,
-                              T *out, uint64_t wide, uint64_t place, cudaStream_t cs)
+struct FactorGrad {
+    const T *z;
+    uint64_t stride, feats;
+    const T *thin;
+    T *out;
+    uint64_t wide, place;
+};
+
+template <class T>
+static int launch_factor_grad(const lmz_projection *p, const FactorGrad<T> *jobs, uint32_t count, const uint32_t *order, const uint32_t *start, cudaStream_t cs)
 {
     static bool done[64];
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     FactorGradArgs<T> a{};
-    a.order = order, a.start = start, a.out = out, a.feats = feats;
-    a.each = feats * p->rank, a.wide = wide, a.place = place;
+    a.order = order, a.start = start;
     a.tokens = static_cast<uint32_t>(p->tokens), a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.blocks = a.rp <= 128 ? 2 : 1;                              // (as many as TMEM has columns for)
     a.stage_bytes = factor_stage_bytes(a.blocks, a.rp), a.tmem_columns = tmem_columns(a.blocks * 2 * a.rp);
     a.stages = std::min<uint32_t>(FG_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
-    const uint64_t wide_tiles = (feats + a.blocks * FG_FEATS - 1) / (a.blocks * FG_FEATS);
-    a.split = 1;
-    while (a.split < 8 && wide_tiles * p->adapters * a.split * 2 <= (uint64_t)sms && p->tokens >= 4ull * STEP_K * a.split) a.split *= 2;
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
-    rc = tensor_map(&a.z, z, bf16, feats, p->tokens, stride, STEP_K);
-    if (!rc) rc = tensor_map(&a.z_rows, z, bf16, feats, p->tokens, stride, 1);
-    if (!rc) rc = tensor_map(&a.thin, thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, STEP_K);
-    if (!rc) rc = tensor_map(&a.thin_rows, thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, 1);
-    if (!rc) rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
+    uint32_t clusters = 0;
+    for (uint32_t i = 0; i < count; i++) {
+        const FactorGrad<T> &f = jobs[i];
+        FactorGradJob<T> &g = a.job[i];
+        g.out = f.out, g.feats = f.feats, g.each = f.feats * p->rank, g.wide = f.wide, g.place = f.place;
+        g.clusters = static_cast<uint32_t>((f.feats + a.blocks * FG_FEATS - 1) / (a.blocks * FG_FEATS));
+        clusters += g.clusters;
+        rc = tensor_map(&g.z, f.z, bf16, f.feats, p->tokens, f.stride, STEP_K);
+        if (!rc) rc = tensor_map(&g.z_rows, f.z, bf16, f.feats, p->tokens, f.stride, 1);
+        if (!rc) rc = tensor_map(&g.thin, f.thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, STEP_K);
+        if (!rc) rc = tensor_map(&g.thin_rows, f.thin, bf16, 2 * a.rp, p->tokens, 2 * a.rp, 1);
+        if (rc) return rc;
+    }
+    a.split = 1;
+    while (a.split < 8 && (uint64_t)clusters * p->adapters * a.split * 2 <= (uint64_t)sms && p->tokens >= 4ull * STEP_K * a.split) a.split *= 2;
+    rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
     if (rc) return rc;
     cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(wide_tiles * a.split), p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    const cudaLaunchConfig_t c = clustered(dim3(clusters * a.split, p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
     CK("launch k_factor_grad", cudaLaunchKernelEx(&c, k_factor_grad<T>, a));
     return LMZ_GPU_OK;
 }
@@ -483,9 +498,12 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
         if (rc) return rc;
         order = s.pos[side], start = s.start;
     }
-    if (!rc && p->da) rc = launch_factor_grad<T>(p, in.x, in.x_stride, p->in, g, order, start, static_cast<T *>(p->da), 1, p->in, cs);
-    if (!rc && p->db) rc = launch_factor_grad<T>(p, in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), order, start, static_cast<T *>(p->db), r, 1, cs);
-    return rc;
+    if (rc || !(p->da || p->db)) return rc;
+    FactorGrad<T> jobs[2];
+    uint32_t count = 0;
+    if (p->db) jobs[count++] = {in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), static_cast<T *>(p->db), r, 1};
+    if (p->da) jobs[count++] = {in.x, in.x_stride, p->in, g, static_cast<T *>(p->da), 1, p->in};
+    return launch_factor_grad<T>(p, jobs, count, order, start, cs);
 }
 
 API int lmz_gpu_ops_gave_up(void)

@@ -60,7 +60,6 @@ def _function():
     global _made
     if _made is None:
         import torch
-        from torch.autograd.function import once_differentiable
 
         class Rows(torch.autograd.Function):
             @staticmethod
@@ -70,7 +69,7 @@ def _function():
                 return _rows(table.get_device(), _ops.type_code(table, "table"), tokens.element_size(), table, tokens, scale)
 
             @staticmethod
-            @once_differentiable
+            @_ops.once
             def backward(ctx, dy):
                 (tokens,) = ctx.saved_tensors
                 return _rows_grad(dy, tokens, ctx.rows, ctx.scale), None, None

@@ -522,6 +522,21 @@ def test_inputs_changed_between_the_passes_are_noticed():
         y.sum().backward()
 
 
+def test_gradients_have_no_gradient():
+    """A graph of the gradients may be asked for (other parts of a loss may need it); going through it is refused."""
+    from lmz_b200 import adapters, embed
+    table, ids = _randn(60, (5, 8), torch.float32).requires_grad_(True), _ids(61, 3, 5)
+    (g,) = torch.autograd.grad(embed.lookup(table, ids).square().sum(), table, create_graph=True)
+    want = torch.autograd.grad(embed.lookup(table, ids).square().sum(), table)[0]
+    assert torch.equal(g, want)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    x, w, a, b, scales = _inputs(6, 64, 96, 8, 3, torch.bfloat16)
+    (g,) = torch.autograd.grad(adapters.project(x.requires_grad_(True), w, a, b, scale=0.5).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+
+
 # ------------------------------------------------------------------------------------------- with archives
 
 def _safetensors(tensors):
