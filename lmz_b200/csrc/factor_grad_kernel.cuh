@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
             __syncwarp();
             if (tile) {
                 if (elected()) {
-                    for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_load_2d(&g.z, &s.full[st], dst + b * FG_TILE, f0 + b * 64, first);
-                    for (uint32_t b = 0; b < thins; b++) tma_load_2d(&g.thin, &s.full[st], dst + thin_at + b * FG_TILE, b * 64, first);
+                    for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_load_2d(&g.z, smem_addr(&s.full[st]), dst + b * FG_TILE, f0 + b * 64, first);
+                    for (uint32_t b = 0; b < thins; b++) tma_load_2d(&g.thin, smem_addr(&s.full[st]), dst + thin_at + b * FG_TILE, b * 64, first);
                 }
             } else if (lane < 16) {
                 for (uint32_t b = 0; b < 2 * a.blocks; b++) tma_gather4(&g.z_rows, &s.full[st], dst + b * FG_TILE + lane * 4 * ROW_BYTES, f0 + b * 64, row);

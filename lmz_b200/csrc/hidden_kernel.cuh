@@ -104,9 +104,9 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
             if (at.turn && !warp_wait(&s.empty[st], (at.turn - 1) & 1, over)) break;
             if (elected()) {
                 bar_expect(&s.full[st], H_TOKENS * ROW_BYTES + count * a.rank * ROW_BYTES);
-                tma_load_2d(&a.x, &s.full[st], dst, k * STEP_K, tile * H_TOKENS);
+                tma_load_2d(&a.x, smem_addr(&s.full[st]), dst, k * STEP_K, tile * H_TOKENS);
                 for (uint32_t i = 0; i < count; i++)
-                    tma_load_3d(&a.f, &s.full[st], dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
+                    tma_load_3d(&a.f, smem_addr(&s.full[st]), dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
             }
             __syncwarp();
         }

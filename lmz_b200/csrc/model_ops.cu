@@ -232,7 +232,8 @@ static bool on_boundary(const void *p, uint64_t cols, uint64_t stride) { return 
 
 // A tensor map of planes x rows x cols 16-bit elements, a plane's rows behind those of the plane before: tiles of 64 columns
 // with the 128-byte swizzle.
-static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0)
+static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0,
+                      uint32_t tile_planes = 1)
 {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -244,7 +245,7 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
     }();
     if (!encode) return fail_msg(LMZ_GPU_EUNSUPPORTED, "the driver makes no tensor maps");
     const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {stride * 2, stride * rows * 2};
-    const cuuint32_t box[3] = {STEP_K, tile_rows, 1}, steps[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {STEP_K, tile_rows, tile_planes}, steps[3] = {1, 1, 1};
     const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes ? 3 : 2, const_cast<void *>(p), dims,
                               strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -346,6 +347,9 @@ static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
     rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, pair ? a.nt / 2 : a.nt);
     if (!rc) rc = MN ? tensor_map(&a.w, w, bf16, feats, k, w_stride, STEP_K) : tensor_map(&a.w, w, bf16, k, feats, w_stride, P_FEATS);
+    if (!rc) rc = tensor_map(&a.h, hidden, bf16, a.rp, 2, a.rp, 1, p->tokens, pair ? a.nt / 2 : a.nt);
+    if (!rc) rc = MN ? tensor_map(&a.f, factor, bf16, feats, factor_rows, factor_row, STEP_K, p->adapters)
+                     : tensor_map(&a.f, factor, bf16, a.rp, factor_rows, factor_row, P_FEATS, p->adapters);
     if (rc) return rc;
     if (pair) return launch_project_as<T, MN, true>(a, static_cast<unsigned>(std::min<uint64_t>(count, sms / 2) * 2), cs);
     return launch_project_as<T, MN, false>(a, static_cast<unsigned>(a.split > 1 ? count * a.split : std::min<uint64_t>(count, sms)), cs);

@@ -23,7 +23,6 @@ struct TileInfo {
 struct ProjectShared {
     uint64_t full[P_MAX_STAGES], empty[P_MAX_STAGES];
     uint64_t info_full[P_INFOS], info_empty[P_INFOS];
-    uint64_t loaded[P_INFOS], fed[P_INFOS];    // a tile's steps of the weight, and of the adapters, have all got their stages
     uint64_t sums_full[2], sums_empty[2];
     uint64_t slot_full[P_MAX_SLOTS], slot_empty[P_MAX_SLOTS];
     uint32_t tmem, over;
@@ -34,6 +33,7 @@ struct ProjectShared {
 template <class T>
 struct ProjectArgs {
     CUtensorMap x, w;
+    CUtensorMap h, f;                          // hidden as tokens x 2 x rp, and the factors as adapters x their two sides
     TokenIndex index;
     const T *hidden;                           // [token][2][rp]: the thin product, its upper and its lower half
     const T *factor;                           // of adapter i from i * factor_each; rows of factor_row elements, multiples of 8
@@ -167,9 +167,10 @@ __device__ __forceinline__ void store_group(const ProjectArgs<T> &a, uint64_t t0
 // Features are the tensor core's M and tokens its N, whatever their number: a single token streams the weight past 16 columns,
 // a prompt past 256, and what an adapter adds to a run of its own tokens is one more product into just their columns.
 //
-// Roles: a TMA warp loads tiles of W and x (64 along K) into a ring of stages; four warps feed the ring with what adapters
-// need (h and a factor's tile: 2 rp wide, the factor beside both halves of h); one thread issues the MMAs; four warps take
-// the sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.
+// Roles: a TMA warp loads tiles of W and x (64 along K) into a ring of stages, and behind them, for every run of tokens with
+// one adapter, tiles of its factor and of either half of h; a warp issues the MMAs; four warps look at the next tile's tokens
+// and work out what has no run (mixed_group); four take the sums out of TMEM, which holds two tiles' sums, so that a tile's way
+// out runs under the next tile's products.
 // The weight's first tiles are under way while the kernel that makes h still runs.
 // Few tiles: the CTAs of a cluster share K, and their sums meet in distributed shared memory.
 // Many (PAIR): two CTAs multiply 256 features by 256 tokens together, each loading half of both, so that a step brings
@@ -188,14 +189,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
     const uint32_t k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(p_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
     uint8_t *const local = p_smem + (ring - smem_addr(p_smem));
-    float *const slots = reinterpret_cast<float *>(local + a.stages * a.stage_bytes), *const places = slots + a.slots * (P_SLOT_BYTES / 4);
-    const uint32_t wide = (2 * a.rp + STEP_K - 1) / STEP_K;      // steps of a run
+    float *const slots = reinterpret_cast<float *>(local + a.stages * a.stage_bytes), *const room = slots + a.slots * (P_SLOT_BYTES / 4);
     volatile uint32_t *over = &s.over;
 
     if (tid == 0) {
         s.over = 0;
         for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], CTAS), bar_init(&s.empty[i], 1);
-        for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], (side ? 1 : 2) + P_EPILOGUE / 32), bar_init(&s.loaded[i], 1), bar_init(&s.fed[i], 1);
+        for (uint32_t i = 0; i < P_INFOS; i++) bar_init(&s.info_full[i], 1), bar_init(&s.info_empty[i], (side ? 1 : 2) + P_EPILOGUE / 32);
         for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], CTAS * P_EPILOGUE / 32);
         for (uint32_t i = 0; i < a.slots; i++) bar_init(&s.slot_full[i], 1), bar_init(&s.slot_empty[i], P_EPILOGUE / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         const uint32_t w = a.token_tiles - 8 * b < 8 ? a.token_tiles - 8 * b : 8;
         ft = in / w, tt = 8 * b + in % w;
     };
+    const uint32_t places = (a.rp + STEP_K - 1) / STEP_K;        // steps of a run, for each half of h
     auto mine = [&](uint32_t run) { return run % a.split == rank; };
     auto mixed = [&](const TileInfo &info, uint32_t g) { return (info.mixed >> g & 1) && (a.split == 1 || g % a.split == rank); };
     auto features = [&](uint32_t ft) { return (ft * CTAS + side) * P_FEATS; };      // where this CTA's begin
@@ -246,42 +247,48 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 if (!ok) break;
                 if (elected()) {
                     const uint32_t dst = ring + st * a.stage_bytes;
-                    if constexpr (PAIR) {
-                        const uint32_t bar = full + st * 8;
-                        if (side) peer_expect(bar, a.stage_bytes);
-                        else bar_expect(&s.full[st], a.stage_bytes);
-                        if constexpr (MN) {
-                            tma_load_2d_pair(&a.w, bar, dst, f, k * STEP_K);
-                            tma_load_2d_pair(&a.w, bar, dst + STEP_K * ROW_BYTES, f + 64, k * STEP_K);
-                        } else {
-                            tma_load_2d_pair(&a.w, bar, dst, k * STEP_K, f);
-                        }
-                        tma_load_2d_pair(&a.x, bar, dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
+                    const uint32_t bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
+                    if (side) peer_expect(bar, a.stage_bytes);
+                    else bar_expect(&s.full[st], a.stage_bytes);
+                    if constexpr (MN) {
+                        tma_load_2d<PAIR>(&a.w, bar, dst, f, k * STEP_K);
+                        tma_load_2d<PAIR>(&a.w, bar, dst + STEP_K * ROW_BYTES, f + 64, k * STEP_K);
                     } else {
-                        bar_expect(&s.full[st], a.stage_bytes);
-                        if constexpr (MN) {
-                            tma_load_2d(&a.w, &s.full[st], dst, f, k * STEP_K);
-                            tma_load_2d(&a.w, &s.full[st], dst + STEP_K * ROW_BYTES, f + 64, k * STEP_K);
-                        } else {
-                            tma_load_2d(&a.w, &s.full[st], dst, k * STEP_K, f);
-                        }
-                        tma_load_2d(&a.x, &s.full[st], dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
+                        tma_load_2d<PAIR>(&a.w, bar, dst, k * STEP_K, f);
                     }
+                    tma_load_2d<PAIR>(&a.x, bar, dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
                 }
                 __syncwarp();
             }
+            ok = ok && warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over);
             if (!ok) break;
-            if (lane == 0) bar_arrive(&s.loaded[n % P_INFOS]);
-            if (!warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
             const TileInfo &info = s.info[n % P_INFOS];
-            uint32_t steps = 0;
-            for (uint32_t r = 0; r < info.runs; r++) steps += mine(r) ? wide : 0;
-            at.skip(steps, a.stages);
+            if (n == 0) wait_for_previous();                     // (h)
+            for (uint32_t r = 0; r < info.runs && ok; r++) {
+                if (!mine(r)) continue;
+                const uint32_t token = tt * a.nt + info.run[r].column + side * (info.run[r].tokens / CTAS), adapter = info.run[r].adapter;
+                for (uint32_t j = 0; j < 2 * places; j++, at.next(a.stages)) {
+                    const uint32_t st = at.stage, half = j >= places, j0 = (half ? j - places : j) * STEP_K;
+                    ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
+                    if (!ok) break;
+                    if (elected()) {
+                        const uint32_t dst = ring + st * a.stage_bytes, bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
+                        if (side) peer_expect(bar, a.stage_bytes);
+                        else bar_expect(&s.full[st], a.stage_bytes);
+                        if constexpr (MN) {
+                            tma_load_3d<PAIR>(&a.f, bar, dst, f, j0, adapter);
+                            tma_load_3d<PAIR>(&a.f, bar, dst + STEP_K * ROW_BYTES, f + 64, j0, adapter);
+                        } else {
+                            tma_load_3d<PAIR>(&a.f, bar, dst, j0, f, adapter);
+                        }
+                        tma_load_3d<PAIR>(&a.h, bar, dst + P_FEATS * ROW_BYTES, j0, half, token);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!ok) break;
             __syncwarp();
             if (lane == 0) bar_arrive(&s.info_empty[n % P_INFOS]);
-            // A parity tells two phases apart, no more: whoever has skipped a whole turn of the ring first waits for the
-            // others' last stage in it.
-            if (steps >= a.stages && !warp_wait(&s.fed[n % P_INFOS], (n / P_INFOS) & 1, over)) break;
         }
         // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both).
         if (*over && !side)
@@ -321,12 +328,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 for (uint32_t r = 0; r < info.runs && ok; r++) {
                     if (!mine(r)) continue;
                     const uint32_t column = info.run[r].column, rdesc = mma_desc(bf16, MN, false, CTAS * P_FEATS, info.run[r].tokens);
-                    for (uint32_t v = 0; v < 2 * a.rp; v += STEP_K, at.next(a.stages)) {
-                        const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+                    for (uint32_t j = 0; j < 2 * places; j++, at.next(a.stages)) {
+                        const uint32_t st = at.stage, off = st * a.stage_bytes >> 4, j0 = (j >= places ? j - places : j) * STEP_K;
                         ok = warp_wait(&s.full[st], at.turn & 1, over);
                         if (!ok) break;
                         if (elected()) {
-                            for (uint32_t c = 0; c < STEP_K / 16 && v + c * 16 < 2 * a.rp; c++)
+                            for (uint32_t c = 0; c < STEP_K / 16 && j0 + c * 16 < a.rp; c++)
                                 mma16<PAIR>(sums + column, a_lo + off + (c * a_step >> 4), b_lo + off + c * 2, rdesc, true);
                             mma_commit<PAIR>(&s.empty[st]);
                         }
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             sync_threads(1, P_FEED);
             return true;
         };
-        RingPlace at, slot;
+        RingPlace slot;
         uint32_t n = 0;
         bool go = first < tiles && look(first, 0);
         wait_for_previous();                                     // (h)
@@ -394,64 +401,14 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             place(tile, ft, tt);
             const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = features(ft);
             const TileInfo &info = s.info[n % P_INFOS];
-            // As many mixed groups as have a slot while the weight is on its way; the others last, when what makes room for them no
-            // longer waits for this tile's own steps.
-            uint32_t g = 0;
-            auto mix = [&](uint32_t most) {
-                for (; go && most && g * P_GROUP < a.nt; g++) {
-                    if (!mixed(info, g)) continue;
-                    go = sync_all(1, P_FEED, !slot.turn || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
-                    if (!go) break;
-                    mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, places, slots + slot.stage * (P_SLOT_BYTES / 4));
-                    if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
-                    slot.next(a.slots);
-                    most--;
-                }
-            };
-            mix(a.slots);
-            at.skip(k1 - k0, a.stages);
-            if (!sync_all(1, P_FEED, go && (id || bar_wait(&s.loaded[n % P_INFOS], (n / P_INFOS) & 1, over)))) break;
-            for (uint32_t r = 0; go && r < info.runs; r++) {
-                if (!mine(r)) continue;
-                const T *factor = a.factor + info.run[r].adapter * a.factor_each;
-                for (uint32_t v0 = 0; v0 < 2 * a.rp; v0 += STEP_K, at.next(a.stages)) {
-                    const uint32_t st = at.stage, fdst = ring + st * a.stage_bytes, hdst = fdst + P_FEATS * ROW_BYTES;
-                    if (!sync_all(1, P_FEED, !at.turn || id || bar_wait(&s.empty[st], (at.turn - 1) & 1, over))) { go = false; break; }
-                    const uint32_t parts = (2 * a.rp - v0 < STEP_K ? 2 * a.rp - v0 : STEP_K) / 8;
-                    if constexpr (MN) {                          // a row per j of the rank, 64 features a block
-                        for (uint32_t e = id; e < parts * 8 * 16; e += P_FEED) {
-                            const uint32_t row = e >> 4, c = e & 15, v = v0 + row, j = v < a.rp ? v : v - a.rp;
-                            const uint64_t f = f0 + c * 8;
-                            const bool on = j < a.rank && f < a.feats;
-                            copy16(fdst + (c >> 3) * STEP_K * ROW_BYTES + swizzled(row, c & 7), on ? factor + j * a.factor_row + f : factor, on);
-                        }
-                    } else {                                     // a row per feature
-                        for (uint32_t e = id; e < P_FEATS * 8; e += P_FEED) {
-                            const uint32_t row = e >> 3, c = e & 7, v = v0 + c * 8, j = v < a.rp ? v : v - a.rp;
-                            const uint64_t f = f0 + row;
-                            const bool on = c < parts && f < a.feats;
-                            if (c < parts) copy16(fdst + swizzled(row, c), on ? factor + f * a.factor_row + j : factor, on);
-                        }
-                    }
-                    const uint32_t share = info.run[r].tokens / CTAS, column = info.run[r].column + side * share;
-                    for (uint32_t e = id; e < share * 8; e += P_FEED) {
-                        const uint32_t row = e >> 3, c = e & 7;
-                        const uint64_t t = t0 + column + row;
-                        const bool on = t < a.tokens;
-                        if (c < parts) copy16(hdst + swizzled(row, c), on ? a.hidden + t * 2 * a.rp + v0 + c * 8 : a.hidden, on);
-                    }
-                    copies_commit();
-                    copies_wait<0>();
-                    publish_smem();
-                    sync_threads(1, P_FEED);
-                    if (id == 0) {
-                        if (side) peer_arrive(peer_addr(&s.full[st], 0));
-                        else bar_arrive(&s.full[st]);
-                    }
-                }
+            for (uint32_t g = 0; go && g * P_GROUP < a.nt; g++) {
+                if (!mixed(info, g)) continue;
+                go = sync_all(1, P_FEED, !slot.turn || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
+                if (!go) break;
+                mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, room, slots + slot.stage * (P_SLOT_BYTES / 4));
+                if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
+                slot.next(a.slots);
             }
-            if (id == 0) bar_arrive(&s.fed[n % P_INFOS]);
-            mix(P_TOKENS);
         }
     } else {
         const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;

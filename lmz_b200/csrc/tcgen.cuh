@@ -97,21 +97,26 @@ struct RingPlace {
 
 // ---- asynchronous copies
 
-__device__ __forceinline__ void tma_load_2d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y)
+// Tiles; the barrier by its address.  PAIR: that of the pair's first CTA (in the cluster's window).
+template <bool PAIR = false>
+__device__ __forceinline__ void tma_load_2d(const CUtensorMap *map, uint32_t bar, uint32_t dst, int32_t x, int32_t y)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-// The same, telling a barrier of the pair's first CTA (its address in the cluster's window).
-__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap *map, uint32_t bar, uint32_t dst, int32_t x, int32_t y)
+template <bool PAIR = false>
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint32_t bar, uint32_t dst, int32_t x, int32_t y, int32_t z)
 {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, int32_t y, int32_t z)
-{
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 // Four rows, by their numbers, of a map whose tiles are one row high (a row behind the tensor's last reads as zeros).
 __device__ __forceinline__ void tma_gather4(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int32_t x, const uint32_t *row)
