@@ -4,6 +4,7 @@
 //   y[t] = x[t] W^T + h[t] B_i^T,  h[t] = s_i x[t] A_i^T,  i = index[t];  no adapter where index[t] is outside [0, n)
 //   g[t] = s_i dy[t] B_i,  dx[t] = dy[t] W + g[t] A_i,  dA_i = sum of g[t]^T x[t],  dB_i = sum of dy[t]^T h[t] over i's tokens
 #pragma once
+#include "tcgen.cuh"
 #include "vectors.cuh"
 
 namespace lmz {
@@ -52,6 +53,7 @@ __global__ void __launch_bounds__(32 * PACK_WARPS) k_pack(const __grid_constant_
 {
     const PackJob<T> &j = a.job[blockIdx.y];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    wait_for_previous();
     const uint64_t parts = (j.pitch + PACK_COLS - 1) / PACK_COLS, units = j.total * parts;
     for (uint64_t u = static_cast<uint64_t>(blockIdx.x) * PACK_WARPS + warp; u < units; u += static_cast<uint64_t>(gridDim.x) * PACK_WARPS) {
         const uint64_t row = j.sc == 1 ? u / parts : u % j.total, part = j.sc == 1 ? u - row * parts : u / j.total, o = row / j.rows;

@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     const uint32_t place = blockIdx.x / a.split, which = place >= a.job[0].clusters;
     const FactorGradJob<T> &g = a.job[which];
     const uint32_t f0 = (which ? place - a.job[0].clusters : place) * a.blocks * FG_FEATS, i = blockIdx.y;
+    wait_for_previous();
     const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : a.tokens;
     const uint32_t all = (end - begin + STEP_K - 1) / STEP_K;
     const uint32_t n0 = static_cast<uint32_t>(static_cast<uint64_t>(all) * rank / a.split), n1 = static_cast<uint32_t>(static_cast<uint64_t>(all) * (rank + 1) / a.split);
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
         T *out = g.out + i * g.each;
         const uint32_t wide = a.blocks * FG_FEATS, share = wide / a.split;
         // neighbouring threads write neighbouring elements: along f (a CTA every split-th j), or along j (a CTA its share of the f)
+        const Peers peers(ring, a.split);
         const bool along_f = g.wide == 1;
         const uint32_t count = along_f ? (a.rank + a.split - 1 - rank) / a.split * wide : a.rank * share;
 #pragma unroll 4
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
             const uint32_t j = along_f ? rank + e / wide * a.split : e % a.rank, row = along_f ? e % wide : rank * share + e / a.rank;
             const uint64_t f = f0 + static_cast<uint64_t>(row);
             if (f >= g.feats) continue;
-            out[f * g.wide + j * g.place] = narrow<T>(peer_sum(ring + ((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, a.split));
+            out[f * g.wide + j * g.place] = narrow<T>(peers.sum(((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4));
         }
     }
     if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums

@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     volatile uint32_t *over = &s.over;
 
     // (Neither kernel leaves an SM room for a block of the other, so the next one's cannot take this block's TMEM.)
+    wait_for_previous();
     let_next_start();
     // Which adapters the tile has: a token is its adapter's first if none before it has it.
     if (tid == 0) {
@@ -105,9 +106,10 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
             if (elected()) {
                 bar_expect(&s.full[st], H_TOKENS * ROW_BYTES + count * a.rank * ROW_BYTES);
                 tma_load_2d(&a.x, smem_addr(&s.full[st]), dst, k * STEP_K, tile * H_TOKENS);
-                for (uint32_t i = 0; i < count; i++)
-                    tma_load_3d(&a.f, smem_addr(&s.full[st]), dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
             }
+            __syncwarp();
+            for (uint32_t i = lane; i < count; i += 32)
+                tma_load_3d(&a.f, smem_addr(&s.full[st]), dst + H_TOKENS * ROW_BYTES + i * a.rp * ROW_BYTES, k * STEP_K, 0, s.list[from + i]);
             __syncwarp();
         }
         if (*over)                                               // nothing may still be on its way into this block's memory
@@ -155,13 +157,14 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     if (a.split > 1) cluster_barrier();
     else __syncthreads();
     if (!*over) {                                                // a CTA's share of the tokens: the sums of all, in order
+        const Peers peers(ring, a.split);
         const uint32_t each = H_TOKENS / a.split, lo = rank * each;
 #pragma unroll 2
         for (uint32_t e = tid; e < each * a.rp; e += H_THREADS) {
             const uint32_t row = lo + e / a.rp, c = e % a.rp;
             const int slot = s.slot[row] - static_cast<int>(from);
             if (slot < 0 || slot >= static_cast<int>(count)) continue;
-            const float sum = peer_sum(ring + (c * H_PITCH + row) * 4, a.split);
+            const float sum = peers.sum((c * H_PITCH + row) * 4);
             T hi, lo_half;
             split_halves(c < a.rank ? sum * a.index.scale_of(s.adapter[row]) : 0.0f, hi, lo_half);
             T *to = a.h + (t0 + row) * 2 * a.rp + c;

@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(M_THREADS) k_merge(const MergeArgs<T> a)
     // where element c of the tile's row lies
     auto place = [](uint32_t row, uint32_t c) { return (c >> 6) * M_BLOCK + swizzled(row, (c & 63) * sizeof(T) >> 4) + (c * sizeof(T) & 15); };
 
+    wait_for_previous();
     // B's rows, K-major; A's, MN-major in blocks of 64 columns
     for (uint32_t e = tid; e < M_ROWS * a.places / 8; e += M_THREADS) {
         const uint32_t row = e / (a.places / 8), c = e % (a.places / 8), j = c * 8;

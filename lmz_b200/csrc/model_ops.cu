@@ -21,12 +21,6 @@ using namespace lmz;
 #include "host_error.inl"
 #include "host_device.inl"
 
-static int launched(const char *what)
-{
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? LMZ_GPU_OK : fail_cuda(what, e);
-}
-
 static uint32_t element_bytes(int dtype) { return dtype == LMZ_GPU_F32 ? 4 : dtype == LMZ_GPU_BF16 || dtype == LMZ_GPU_F16 ? 2 : 0; }
 
 // The widest vector, of at most 16 bytes, that rows of `row_bytes` at the given addresses and strides are made of.
@@ -63,13 +57,27 @@ static int by_type(int dtype, uint32_t vb, F f)
     return fail_msg(LMZ_GPU_EUNSUPPORTED, "an element type other than BF16, F16 and F32");
 }
 
-static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute *attr)
+// A launch in clusters along x whose blocks may start before the kernel in front of it has ended: each of these kernels waits
+// for that itself, before it reads or writes what another may have to do with.
+static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute (&attrs)[2])
 {
-    attr->id = cudaLaunchAttributeClusterDimension;
-    attr->val.clusterDim.x = cluster, attr->val.clusterDim.y = 1, attr->val.clusterDim.z = 1;
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster, attrs[1].val.clusterDim.y = 1, attrs[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t c{};
-    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attr, c.numAttrs = 1;
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attrs, c.numAttrs = cluster > 1 ? 2 : 1;
     return c;
+}
+
+// The same without clusters.
+template <class K, class... A>
+static int launch(const char *what, K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, A... args)
+{
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(grid, threads, smem, cs, 1, attrs);
+    CK(what, cudaLaunchKernelEx(&c, kernel, args...));
+    return LMZ_GPU_OK;
 }
 
 static uint32_t lanes_log(uint32_t vectors)
@@ -109,8 +117,7 @@ API int lmz_gpu_rows_dev(const void *d_table, uint64_t rows, uint64_t dim, uint6
         a.scale = scale, a.wide = id_bytes == 8;
         constexpr int U = 4;
         const uint32_t per = (ROW_THREADS >> a.lane_log) * U;
-        k_rows<T, VB, U><<<static_cast<unsigned>((n + per - 1) / per), ROW_THREADS, 0, static_cast<cudaStream_t>(cuda_stream)>>>(a);
-        return launched("launch k_rows");
+        return launch("launch k_rows", k_rows<T, VB, U>, dim3(static_cast<unsigned>((n + per - 1) / per)), ROW_THREADS, 0, static_cast<cudaStream_t>(cuda_stream), a);
     });
 }
 
@@ -141,27 +148,14 @@ static int launch_sort(SortArgs &s, cudaStream_t cs, int *side)
     s.passes = (bits + SORT_DIGIT - 1) / SORT_DIGIT, s.digit = std::max(5u, (bits + s.passes - 1) / s.passes);
     // (a thousand elements are sorted by one CTA before a cluster has met)
     const uint32_t ctas = s.n <= SORT_THREADS ? 1 : SORT_CTAS;
-    cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(ctas), SORT_THREADS, sort_smem(s.digit), cs, ctas, &attr);
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(dim3(ctas), SORT_THREADS, sort_smem(s.digit), cs, ctas, attrs);
     CK("launch k_sort", cudaLaunchKernelEx(&c, k_sort, static_cast<const SortArgs>(s)));
     *side = (s.passes - 1) & 1;
     return LMZ_GPU_OK;
 }
 
 API size_t lmz_gpu_rows_grad_work_bytes(uint64_t n, uint64_t, uint64_t dim) { return RowsGradLayout(n, dim).end; }
-
-// A launch whose blocks may start before the kernel in front of it has ended (they wait for it themselves).
-template <class K, class... A>
-static int launch_behind(const char *what, K kernel, dim3 grid, unsigned threads, cudaStream_t cs, A... args)
-{
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = grid, c.blockDim = dim3(threads), c.stream = cs, c.attrs = &attr, c.numAttrs = 1;
-    CK(what, cudaLaunchKernelEx(&c, kernel, args...));
-    return LMZ_GPU_OK;
-}
 
 API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dtype, const void *d_ids, int id_bytes, uint64_t rows,
                               float scale, void *d_dtable, void *d_work, void *cuda_stream)
@@ -187,7 +181,7 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
     rc = launch_sort(s, cs, &side);
     const uint64_t total = rows * bytes, blocks = (total + CLEAR_BYTES - 1) / CLEAR_BYTES;
     if (!rc && blocks >= 1u << 30) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a table of 64 TiB and more");
-    if (!rc) rc = launch_behind("launch k_clear", k_clear, dim3(static_cast<unsigned>(blocks)), CLEAR_THREADS, cs, static_cast<uint8_t *>(d_dtable), total);
+    if (!rc) rc = launch("launch k_clear", k_clear, dim3(static_cast<unsigned>(blocks)), CLEAR_THREADS, 0, cs, static_cast<uint8_t *>(d_dtable), total);
     if (rc) return rc;
     return by_type(dtype, vector_bytes(bytes, {address(d_dy), address(d_dtable)}), [&](auto type, auto vec) {
         using T = decltype(type);
@@ -199,8 +193,8 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
         a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = std::max(5u, lanes_log(a.vectors));
         const uint32_t slices = (a.vectors + ROW_THREADS - 1) / ROW_THREADS, per = ROW_THREADS >> a.lane_log;
         const dim3 grid(((a.n + a.window - 1) / a.window + per - 1) / per, slices);
-        int failed = launch_behind("launch k_rows_sums", k_rows_sums<T, VB>, grid, ROW_THREADS, cs, a);
-        if (!failed && a.n > a.window) failed = launch_behind("launch k_rows_join", k_rows_join<T, VB>, grid, ROW_THREADS, cs, a);
+        int failed = launch("launch k_rows_sums", k_rows_sums<T, VB>, grid, ROW_THREADS, 0, cs, a);
+        if (!failed && a.n > a.window) failed = launch("launch k_rows_join", k_rows_join<T, VB>, grid, ROW_THREADS, 0, cs, a);
         return failed;
     });
 }
@@ -306,10 +300,7 @@ static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)
     const uint32_t rest = ATOM_BYTES + a.slots * P_SLOT_BYTES + P_GROUP * P_PLACES * 4;
     a.stages = std::min<uint32_t>(P_MAX_STAGES, (PROJECT_SMEM - rest) / a.stage_bytes);
     cudaLaunchAttribute attrs[2]{};
-    cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + rest, cs, PAIR ? 2 : a.split, attrs);
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    c.numAttrs = 2;
+    const cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + rest, cs, PAIR ? 2 : a.split, attrs);
     CK("launch k_project", cudaLaunchKernelEx(&c, k_project<T, MN, PAIR>, a));
     return LMZ_GPU_OK;
 }
@@ -378,8 +369,8 @@ static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride,
     if (!rc) rc = tensor_map(&a.f, f, bf16, k, p->rank, f_stride, p->rank, p->adapters);
     if (!rc) rc = opt_in_smem(k_hidden<T>, OPS_SMEM, done);
     if (rc) return rc;
-    cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(tiles * a.split), groups), H_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(dim3(static_cast<unsigned>(tiles * a.split), groups), H_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, attrs);
     CK("launch k_hidden", cudaLaunchKernelEx(&c, k_hidden<T>, a));
     return LMZ_GPU_OK;
 }
@@ -424,8 +415,8 @@ static int launch_factor_grad(const lmz_projection *p, const FactorGrad<T> *jobs
     while (a.split < 8 && (uint64_t)clusters * p->adapters * a.split * 2 <= (uint64_t)sms && p->tokens >= 4ull * STEP_K * a.split) a.split *= 2;
     rc = opt_in_smem(k_factor_grad<T>, OPS_SMEM, done);
     if (rc) return rc;
-    cudaLaunchAttribute attr{};
-    const cudaLaunchConfig_t c = clustered(dim3(clusters * a.split, p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, &attr);
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(dim3(clusters * a.split, p->adapters), FG_THREADS, a.stages * a.stage_bytes + ATOM_BYTES, cs, a.split, attrs);
     CK("launch k_factor_grad", cudaLaunchKernelEx(&c, k_factor_grad<T>, a));
     return LMZ_GPU_OK;
 }
@@ -458,8 +449,7 @@ struct ProjectInputs {
         else if (l.pack_b) job(b, 1, 0, p->adapters * p->out, r, r, 1, l.b);
         if (!jobs) return;
         const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((most + PACK_WARPS - 1) / PACK_WARPS, 1u << 20)), jobs);
-        k_pack<T><<<grid, 32 * PACK_WARPS, 0, cs>>>(args);
-        rc = launched("launch k_pack");
+        rc = launch("launch k_pack", k_pack<T>, grid, 32 * PACK_WARPS, 0, cs, args);
     }
 };
 
@@ -550,9 +540,8 @@ static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, c
         static bool done[64];
         const int rc = opt_in_smem(k_merge<T, VB>, merge_smem(256), done);
         if (rc) return rc;
-        k_merge<T, VB><<<dim3(static_cast<unsigned>((in + M_COLS - 1) / M_COLS), static_cast<unsigned>((out + M_ROWS - 1) / M_ROWS)), M_THREADS,
-                         merge_smem(m.places), cs>>>(m);
-        return launched("launch k_merge");
+        return launch("launch k_merge", k_merge<T, VB>, dim3(static_cast<unsigned>((in + M_COLS - 1) / M_COLS), static_cast<unsigned>((out + M_ROWS - 1) / M_ROWS)),
+                      M_THREADS, merge_smem(m.places), cs, m);
     });
 }
 

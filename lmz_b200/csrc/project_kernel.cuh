@@ -54,12 +54,12 @@ __host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt, bool pai
 
 // What the adapters add to a tile's features of sixteen tokens that have different ones, into `slot` ([token][feature]), by
 // the four feeding warps.  Not on the tensor core: a factor multiplied by the zeros of tokens it does not belong to would
-// still hand them its infinities and NaN.  Bound by the latency of the factors' loads, sixteen of which a thread keeps under
-// way; `places`: room for sixteen places of the rank of the tokens' h.
+// still hand them its infinities and NaN.  Bound by the latency of the factors' loads, of which a thread has a whole group's
+// sixteen places under way; `places`: room for sixteen places of the rank of the tokens' h.
 template <class T, bool MN>
 __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f0, uint32_t id, float *places, float *slot)
 {
-    constexpr uint32_t BATCH = 8;
+    constexpr uint32_t BATCH = 16;
     float sum[P_GROUP] = {};                                     // !MN: per token, of feature `id`; MN: two tokens' eight features
     const uint32_t fg = id & 15, tg = id >> 4;
     for (uint32_t j0 = 0; j0 < a.rp; j0 += P_PLACES) {
@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 if (!PAIR && a.split > 1) {                      // (the stages are free: all products have ended)
                     float *sums = reinterpret_cast<float *>(local);
 #pragma unroll
-                    for (uint32_t c = 0; c < P_GROUP; c++) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
+                    for (uint32_t c = 0; c < P_GROUP; c++)
+                        if (t0 + g * P_GROUP + c < a.tokens) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
                 } else {
                     if (mixed(info, g) && !add_slot(slot, v)) break;
                     store_group(a, t0 + g * P_GROUP, f, pairs, v);
@@ -454,11 +455,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             const TileInfo &info = s.info[0];
             const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
             const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            const uint32_t live = a.tokens - t0 < a.nt ? static_cast<uint32_t>(a.tokens - t0) : a.nt;
+            const Peers peers(ring, a.split);
             RingPlace slot;
             for (uint32_t g = rank; g * P_GROUP < a.nt && t0 + g * P_GROUP < a.tokens; g += a.split) {
                 float v[P_GROUP];
 #pragma unroll
-                for (uint32_t c = 0; c < P_GROUP; c++) v[c] = peer_sum(ring + ((g * P_GROUP + c) * P_FEATS + tid) * 4, a.split);
+                for (uint32_t c = 0; c < P_GROUP; c++) v[c] = g * P_GROUP + c < live ? peers.sum(((g * P_GROUP + c) * P_FEATS + tid) * 4) : 0.0f;
                 if (mixed(info, g) && !add_slot(slot, v)) break;
                 store_group(a, t0 + g * P_GROUP, f, pairs, v);
             }

@@ -23,13 +23,14 @@ struct RowsArgs {
 // Bound by HBM: every row read and written once, in vectors of VB bytes (the widest that row size, stride and bases
 // allow).  The id has to arrive before the row can be asked for, so a thread keeps U rows on their way.
 template <class T, int VB, int U>
-__global__ void __launch_bounds__(ROW_THREADS) k_rows(RowsArgs a)
+__global__ void __launch_bounds__(ROW_THREADS) k_rows(const RowsArgs a)
 {
     using V = Vec<T, VB>;
     const uint32_t lane = threadIdx.x & ((1u << a.lane_log) - 1), sub = threadIdx.x >> a.lane_log;
     const uint32_t per = ROW_THREADS >> a.lane_log;
     const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * per * U + sub;
     const uint8_t *src[U];
+    wait_for_previous();
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const uint64_t t = t0 + static_cast<uint64_t>(u) * per;

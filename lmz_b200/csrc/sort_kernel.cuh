@@ -40,6 +40,7 @@ static __global__ void __launch_bounds__(SORT_THREADS) k_sort(const SortArgs a)
 {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t sort_words[];
+    wait_for_previous();
     let_next_start();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     cg::cluster_group cluster = cg::this_cluster();

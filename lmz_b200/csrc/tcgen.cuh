@@ -251,24 +251,28 @@ __device__ __forceinline__ void cluster_barrier()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The sum over a cluster's CTAs, in their order, of a word that each has at the same address (at most eight CTAs; all loads are
-// under way together).
-__device__ __forceinline__ float peer_sum(uint32_t addr, uint32_t ctas)
-{
-    float v[8];
+// Sums over a cluster's CTAs (at most eight), in their order, of words that each has at the same address; all loads are under
+// way together.
+struct Peers {
+    uint32_t at[8], ctas;                      // where the others' words lie that this CTA has at `base`
+    __device__ __forceinline__ Peers(uint32_t base, uint32_t n) : ctas(n)
+    {
 #pragma unroll
-    for (uint32_t q = 0; q < 8; q++) {
-        v[q] = 0;
-        if (q < ctas) {
-            uint32_t at;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(q));
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(at) : "memory");
-        }
+        for (uint32_t q = 0; q < 8; q++) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at[q]) : "r"(base), "r"(q < n ? q : 0));
     }
-    float sum = v[0];
+    __device__ __forceinline__ float sum(uint32_t offset) const
+    {
+        float v[8];
 #pragma unroll
-    for (uint32_t q = 1; q < 8; q++) sum += v[q];
-    return sum;
-}
+        for (uint32_t q = 0; q < 8; q++) {
+            v[q] = 0;
+            if (q < ctas) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(at[q] + offset) : "memory");
+        }
+        float all = v[0];
+#pragma unroll
+        for (uint32_t q = 1; q < 8; q++) all += v[q];
+        return all;
+    }
+};
 
 }  // namespace lmz

@@ -507,6 +507,40 @@ def test_on_a_stream_of_its_own_and_captured():
             assert torch.equal(g, v)
 
 
+def test_captured_behind_copies_and_from_other_streams():
+    """What stands in front of an operator in a graph may be a copy, or work of another stream that it waits for."""
+    from lmz_b200 import adapters, embed
+    x, w, a, b, scales = _inputs(40, 256, 136, 16, 3, torch.bfloat16)
+    table, ids, index = _randn(60, (500, 256), torch.bfloat16), _ids(61, 40, 500), _index("runs", 40, 3)
+    mine, weight, out = torch.empty_like(table), torch.empty_like(w), torch.empty_like(w)
+
+    def step():
+        mine.copy_(table)
+        e = embed.lookup(mine, ids, scale=3.0)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            weight.copy_(w)
+            merged = adapters.merge(weight, a[0], b[0], scale=0.5)
+        torch.cuda.current_stream().wait_stream(other)
+        y = adapters.project(e, merged, a, b, index, scale=scales)
+        out.copy_(merged)
+        return y, adapters.merge(out, a[1], b[1], scale=0.25, out=out)
+
+    other = torch.cuda.Stream()
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in (mine, weight, out, *got):
+        t.fill_(7)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for g, v in zip(got, want):
+        assert torch.equal(g, v)
+
+
 def test_inputs_changed_between_the_passes_are_noticed():
     from lmz_b200 import adapters, embed
     x, w, a, b, scales = _inputs(6, 64, 96, 8, 3, torch.bfloat16)
