@@ -297,7 +297,7 @@ static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)
     a.stage_bytes = project_stage_bytes(a.nt, PAIR);
     // A slot per group that may be mixed, where a pair's six stages leave room for three.
     a.slots = PAIR ? 3 : std::min(P_MAX_SLOTS, (a.nt / P_GROUP + a.split - 1) / a.split);
-    const uint32_t rest = ATOM_BYTES + a.slots * P_SLOT_BYTES + P_GROUP * P_PLACES * 4;
+    const uint32_t rest = ATOM_BYTES + a.slots * P_SLOT_BYTES + (PAIR ? 1 : 2) * P_GROUP * P_PLACES * 4;
     a.stages = std::min<uint32_t>(P_MAX_STAGES, (PROJECT_SMEM - rest) / a.stage_bytes);
     cudaLaunchAttribute attrs[2]{};
     const cudaLaunchConfig_t c = clustered(dim3(grid), P_THREADS, a.stages * a.stage_bytes + rest, cs, PAIR ? 2 : a.split, attrs);
@@ -317,19 +317,26 @@ static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride
     a.y = y, a.tokens = p->tokens, a.feats = feats, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K), a.split = 1;
     auto tiles = [&](uint64_t f, uint64_t t) { return (feats + f - 1) / f * ((p->tokens + t - 1) / t); };
-    // Enough tiles of 256 by 256 for the multiprocessors in pairs: those.  Else tiles of 128 features by as many tokens as
-    // there are, at most 128, and of more tokens fewer at a time, down to 32, until the tiles occupy half of the multiprocessors; where
-    // they still do not, CTAs share K.
-    const bool pair = 2 * tiles(2 * P_FEATS, P_TOKENS) >= (uint64_t)sms;
-    if (pair) {
-        a.nt = P_TOKENS;
-    } else {
-        a.nt = P_GROUP;
-        while (a.nt < P_TOKENS / 2 && a.nt < p->tokens) a.nt *= 2;
-        if (p->tokens > a.nt)
-            while (a.nt > 32 && 2 * tiles(P_FEATS, a.nt) <= (uint64_t)sms) a.nt /= 2;
-        while (a.split < 8 && tiles(P_FEATS, a.nt) * a.split * 2 <= (uint64_t)sms && a.steps >= 8 * a.split) a.split *= 2;
-    }
+    // Tiles of 256 by 256 by pairs of CTAs, or of 128 features by 16 to 128 tokens by one, or by a cluster that shares K: by what
+    // they are reckoned to take (in 10 ns).  A step of a pair takes 0.3 us, of a CTA 0.19 or what L2 gives all of them their tiles
+    // in; a cluster's meeting 1.5 us and more.  One B200, rank 16, us in all, tokens x in x out: 512x4096x4096 pairs 35, 128 tokens a
+    // CTA 34, 64 a CTA 38; 200x4096x4096 64 a CTA 23, 128 a CTA 26, pairs 33; 16x4096x4096 by two CTAs 15.5, by one 20, by four 18;
+    // 2048x1024x1024 128 a CTA 21, pairs 26; 128x1024x4096 32 a CTA 12, 128 by four 21; 300x4096x14336 pairs 56, 128 a CTA 70.
+    uint64_t best = ~0ull;
+    bool pair = false;
+    auto consider = [&](bool p2, uint32_t nt, uint32_t split) {
+        const uint64_t n = tiles(p2 ? 2 * P_FEATS : P_FEATS, nt) * split, places = p2 ? sms / 2 : sms;
+        if (split > 1 && n > places) return;
+        const uint64_t waves = (n + places - 1) / places, steps = (a.steps + split - 1) / split;
+        const uint64_t step = p2 ? 30 : std::max<uint64_t>(19, std::min(n, places) * (P_FEATS + nt) / 940);
+        const uint64_t meeting = split == 1 ? 0 : split == 2 ? 150 + 5 * nt / 2 : 180 * split;
+        const uint64_t cost = waves * (step * steps + (p2 ? 600 : 4 * nt + meeting)) + 600;
+        if (cost < best) best = cost, pair = p2, a.nt = nt, a.split = split;
+    };
+    for (uint32_t nt = P_GROUP; nt < P_TOKENS; nt *= 2)
+        for (uint32_t split = 1; split <= 8 && 2 * split <= std::max(2u, a.steps); split *= 2)
+            if (nt == P_GROUP || nt < 2 * p->tokens) consider(false, nt, split);
+    if (p->tokens > P_TOKENS / 2) consider(true, P_TOKENS, 1);
     const uint64_t count = tiles(pair ? 2 * P_FEATS : P_FEATS, a.nt);
     if (count >= 1u << 28) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many tokens for a weight of this size");
     a.feat_tiles = static_cast<uint32_t>((feats + (pair ? 2 : 1) * P_FEATS - 1) / ((pair ? 2 : 1) * P_FEATS));
@@ -356,12 +363,14 @@ static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride,
     HiddenArgs<T> a{};
     a.index = token_index(p), a.h = h, a.tokens = p->tokens, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K);
-    a.each = std::min(H_COLUMNS / a.rp, p->adapters);
-    const uint32_t columns = (a.each * a.rp + 15) & ~15u;
+    const uint64_t tiles = (p->tokens + H_TOKENS - 1) / H_TOKENS;
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(p->index ? std::min(p->adapters, H_TOKENS) : 1, p->tokens));
+    // As many adapters to a block as have room: the fewer blocks, the more multiprocessors the next kernel finds free for its
+    // weight (one B200, 64 tokens of 48 adapters, 4096x14336: 24 blocks 60 us in all, 96 blocks 72).
+    a.each = std::min(H_COLUMNS / a.rp, most);
+    const uint32_t groups = (most + a.each - 1) / a.each, columns = (a.each * a.rp + 15) & ~15u;
     a.stage_bytes = (H_TOKENS + columns) * ROW_BYTES, a.tmem_columns = tmem_columns(columns);
     a.stages = std::min<uint32_t>(H_MAX_STAGES, (OPS_SMEM - ATOM_BYTES) / a.stage_bytes);
-    const uint64_t tiles = (p->tokens + H_TOKENS - 1) / H_TOKENS;
-    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(p->index ? std::min(p->adapters, H_TOKENS) : 1, p->tokens)), groups = (most + a.each - 1) / a.each;
     a.split = 1;
     while (a.split < 8 && tiles * groups * a.split * 2 <= (uint64_t)sms && a.steps >= 4 * a.split) a.split *= 2;
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;

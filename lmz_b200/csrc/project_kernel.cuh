@@ -53,17 +53,17 @@ struct ProjectArgs {
 __host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt, bool pair) { return (P_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
 
 // What the adapters add to a tile's features of sixteen tokens that have different ones, into `slot` ([token][feature]), by
-// the four feeding warps.  Not on the tensor core: a factor multiplied by the zeros of tokens it does not belong to would
+// four warps.  Not on the tensor core: a factor multiplied by the zeros of tokens it does not belong to would
 // still hand them its infinities and NaN.  Bound by the latency of the factors' loads, of which a thread has a whole group's
 // sixteen places under way; `places`: room for sixteen places of the rank of the tokens' h.
 template <class T, bool MN>
-__device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f0, uint32_t id, float *places, float *slot)
+__device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f0, uint32_t id, uint32_t barrier, float *places, float *slot)
 {
     constexpr uint32_t BATCH = 16;
     float sum[P_GROUP] = {};                                     // !MN: per token, of feature `id`; MN: two tokens' eight features
     const uint32_t fg = id & 15, tg = id >> 4;
     for (uint32_t j0 = 0; j0 < a.rp; j0 += P_PLACES) {
-        sync_threads(1, P_FEED);
+        sync_threads(barrier, P_FEED);
         {
             const uint32_t c = id >> 3, j = j0 + (id & 7) * 2;
             float2 v = make_float2(0, 0);
@@ -73,7 +73,7 @@ __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32
             }
             *reinterpret_cast<float2 *>(places + c * P_PLACES + (id & 7) * 2) = v;
         }
-        sync_threads(1, P_FEED);
+        sync_threads(barrier, P_FEED);
         if constexpr (MN) {
 #pragma unroll
             for (uint32_t half = 0; half < 2; half++) {
@@ -136,27 +136,23 @@ __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32
 #pragma unroll
         for (uint32_t c = 0; c < P_GROUP; c++) slot[c * P_FEATS + id] = sum[c];
     }
-    sync_threads(1, P_FEED);
+    sync_threads(barrier, P_FEED);
 }
 
-// Sixteen tokens' sums of a lane's feature, to y: two lanes exchange halves, so that a store has two features.
+// Two tokens' sums of a lane's feature, to y: where rows allow it two lanes exchange halves, so that a store has two features.
 template <class T>
-__device__ __forceinline__ void store_group(const ProjectArgs<T> &a, uint64_t t0, uint64_t f, bool pairs, const float *v)
+__device__ __forceinline__ void store_two(const ProjectArgs<T> &a, uint64_t t, uint64_t f, bool pairs, float v0, float v1)
 {
     const uint32_t odd = threadIdx.x & 1;
-#pragma unroll
-    for (int c = 0; c < static_cast<int>(P_GROUP); c += 2) {
-        if (pairs) {
-            const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
-            union { T e[2]; uint32_t raw; } both;
-            both.e[0] = narrow<T>(odd ? got : v[c]);
-            both.e[1] = narrow<T>(odd ? v[c + 1] : got);
-            const uint64_t t = t0 + c + odd;
-            if (t < a.tokens && f < a.feats) *reinterpret_cast<uint32_t *>(a.y + t * a.feats + (f & ~1ull)) = both.raw;
-        } else if (f < a.feats) {
-            if (t0 + c < a.tokens) a.y[(t0 + c) * a.feats + f] = narrow<T>(v[c]);
-            if (t0 + c + 1 < a.tokens) a.y[(t0 + c + 1) * a.feats + f] = narrow<T>(v[c + 1]);
-        }
+    if (pairs) {
+        const float got = __shfl_xor_sync(~0u, odd ? v0 : v1, 1);
+        union { T e[2]; uint32_t raw; } both;
+        both.e[0] = narrow<T>(odd ? got : v0);
+        both.e[1] = narrow<T>(odd ? v1 : got);
+        if (t + odd < a.tokens && f < a.feats) *reinterpret_cast<uint32_t *>(a.y + (t + odd) * a.feats + (f & ~1ull)) = both.raw;
+    } else if (f < a.feats) {
+        if (t < a.tokens) a.y[t * a.feats + f] = narrow<T>(v0);
+        if (t + 1 < a.tokens) a.y[(t + 1) * a.feats + f] = narrow<T>(v1);
     }
 }
 
@@ -174,7 +170,7 @@ __device__ __forceinline__ void store_group(const ProjectArgs<T> &a, uint64_t t0
 // The weight's first tiles are under way while the kernel that makes h still runs.
 // Few tiles: the CTAs of a cluster share K, and their sums meet in distributed shared memory.
 // Many (PAIR): two CTAs multiply 256 features by 256 tokens together, each loading half of both, so that a step brings
-// 32 KiB into an SM for the products that took 48 (L2 bounds those: 888 us against XX for 8192 tokens of 4096 to 14336 features).
+// 32 KiB into an SM for the products that took 48 (8192 tokens of 4096 to 14336 features: 888 us by single CTAs, 633 by pairs).
 template <class T, bool MN, bool PAIR>
 __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant__ ProjectArgs<T> a)
 {
@@ -236,6 +232,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         RingPlace at;
         uint32_t n = 0;
         const uint32_t full = peer_addr(s.full, 0);
+        bool h_here = false;                                     // (the kernel before has made h)
         for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
             uint32_t ft, tt;
             place(tile, ft, tt);
@@ -263,7 +260,6 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             ok = ok && warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over);
             if (!ok) break;
             const TileInfo &info = s.info[n % P_INFOS];
-            if (n == 0) wait_for_previous();                     // (h)
             for (uint32_t r = 0; r < info.runs && ok; r++) {
                 if (!mine(r)) continue;
                 const uint32_t token = tt * a.nt + info.run[r].column + side * (info.run[r].tokens / CTAS), adapter = info.run[r].adapter;
@@ -281,8 +277,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                         } else {
                             tma_load_3d<PAIR>(&a.f, bar, dst, j0, f, adapter);
                         }
-                        tma_load_3d<PAIR>(&a.h, bar, dst + P_FEATS * ROW_BYTES, j0, half, token);
                     }
+                    __syncwarp();
+                    if (!h_here) wait_for_previous(), h_here = true;
+                    if (elected()) tma_load_3d<PAIR>(&a.h, PAIR ? full + st * 8 : smem_addr(&s.full[st]), ring + st * a.stage_bytes + P_FEATS * ROW_BYTES, j0, half, token);
                     __syncwarp();
                 }
             }
@@ -401,12 +399,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             place(tile, ft, tt);
             const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt, f0 = features(ft);
             const TileInfo &info = s.info[n % P_INFOS];
+            uint32_t order = 0;
             for (uint32_t g = 0; go && g * P_GROUP < a.nt; g++) {
                 if (!mixed(info, g)) continue;
                 go = sync_all(1, P_FEED, !slot.turn || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
                 if (!go) break;
-                mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, room, slots + slot.stage * (P_SLOT_BYTES / 4));
-                if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
+                if (PAIR || !(order++ & 1)) {
+                    mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, 1, room, slots + slot.stage * (P_SLOT_BYTES / 4));
+                    if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
+                }
                 slot.next(a.slots);
             }
         }
@@ -419,22 +420,37 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             uint32_t ft, tt;
             place(tile, ft, tt);
             const uint32_t buf = n & 1;
-            if (!warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over) || !warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
-            tc_after();
+            if (!sync_all(2, P_EPILOGUE, warp_wait(&s.info_full[n % P_INFOS], (n / P_INFOS) & 1, over))) break;
             const TileInfo &info = s.info[n % P_INFOS];
             const uint64_t f = features(ft) + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            if constexpr (!PAIR) {                               // every other mixed group (each has a slot here) while the sums are made
+                RingPlace at = slot;
+                uint32_t order = 0;
+                for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
+                    if (!mixed(info, g)) continue;
+                    if (order++ & 1) {
+                        mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, features(ft), tid, 2, room + P_GROUP * P_PLACES,
+                                           slots + at.stage * (P_SLOT_BYTES / 4));
+                        if (tid == 0) bar_arrive(&s.slot_full[at.stage]);
+                    }
+                    at.next(a.slots);
+                }
+            }
+            if (!warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
+            tc_after();
             for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
                 if ((PAIR || a.split == 1) && t0 + g * P_GROUP >= a.tokens) break;
                 float v[P_GROUP];
                 tmem_load16(tmem + (warp << 21) + buf * a.nt + g * P_GROUP, v);
+                if (mixed(info, g) && !add_slot(slot, v)) break;
                 if (!PAIR && a.split > 1) {                      // (the stages are free: all products have ended)
                     float *sums = reinterpret_cast<float *>(local);
 #pragma unroll
                     for (uint32_t c = 0; c < P_GROUP; c++)
                         if (t0 + g * P_GROUP + c < a.tokens) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
                 } else {
-                    if (mixed(info, g) && !add_slot(slot, v)) break;
-                    store_group(a, t0 + g * P_GROUP, f, pairs, v);
+#pragma unroll
+                    for (uint32_t c = 0; c < P_GROUP; c += 2) store_two(a, t0 + g * P_GROUP + c, f, pairs, v[c], v[c + 1]);
                 }
             }
             tc_before();
@@ -447,23 +463,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         }
     }
     __syncwarp();
-    if (!PAIR && a.split > 1) {                                  // one tile per cluster: its CTAs take its groups in turn
+    if (!PAIR && a.split > 1) {                                  // one tile per cluster: every CTA adds up its share of the tokens
         cluster_barrier();
-        if (warp < 4 && !*over && first < tiles) {
+        if (warp < 8 && !*over) {
             uint32_t ft, tt;
             place(first, ft, tt);
-            const TileInfo &info = s.info[0];
             const bool pairs = a.feats % 2 == 0 && (reinterpret_cast<uint64_t>(a.y) & 3) == 0;
-            const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + tid, t0 = static_cast<uint64_t>(tt) * a.nt;
+            const uint32_t feat = tid & (P_FEATS - 1), share = a.nt / a.split;
+            const uint64_t f = static_cast<uint64_t>(ft) * P_FEATS + feat, t0 = static_cast<uint64_t>(tt) * a.nt;
             const uint32_t live = a.tokens - t0 < a.nt ? static_cast<uint32_t>(a.tokens - t0) : a.nt;
             const Peers peers(ring, a.split);
-            RingPlace slot;
-            for (uint32_t g = rank; g * P_GROUP < a.nt && t0 + g * P_GROUP < a.tokens; g += a.split) {
-                float v[P_GROUP];
-#pragma unroll
-                for (uint32_t c = 0; c < P_GROUP; c++) v[c] = g * P_GROUP + c < live ? peers.sum(((g * P_GROUP + c) * P_FEATS + tid) * 4) : 0.0f;
-                if (mixed(info, g) && !add_slot(slot, v)) break;
-                store_group(a, t0 + g * P_GROUP, f, pairs, v);
+#pragma unroll 2
+            for (uint32_t c = rank * share + 2 * (tid / P_FEATS); c < (rank + 1) * share && c < live; c += 4) {
+                const float v0 = peers.sum((c * P_FEATS + feat) * 4), v1 = c + 1 < live ? peers.sum(((c + 1) * P_FEATS + feat) * 4) : 0.0f;
+                store_two(a, t0 + c, f, pairs, v0, v1);
             }
         }
         cluster_barrier();

@@ -230,10 +230,13 @@ __device__ __forceinline__ void tmem_load8(uint32_t at, float *v)
     for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// A warp waits by its first lane: 32 that ask take issue slots from those who work.
+// The same for a warp whose lanes stay together.  (All of them ask: one lane alone, and the others told by a vote, took 350
+// cycles where the phase was over already.)
 __device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile uint32_t *over)
 {
-    const bool ok = (threadIdx.x & 31) || bar_wait(b, parity, over);
+    bool ok = bar_try(b, parity);
+    if (!ok) ok = bar_wait(b, parity, over);
+    __syncwarp();
     return __all_sync(~0u, ok);
 }
 
