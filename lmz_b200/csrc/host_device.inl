@@ -1,14 +1,18 @@
 // What the entry points ask of the current device (included by every source file of the library).
+#include <atomic>
 #include <cstdint>
 #include <mutex>
 
 static int device_ready()
 {
+    static std::atomic<bool> found{false};       // (a device that was there stays)
+    if (found.load(std::memory_order_relaxed)) return LMZ_GPU_OK;
     int n = 0;
     if (cudaGetDeviceCount(&n) != cudaSuccess || n < 1) {
         cudaGetLastError();
         return fail_msg(LMZ_GPU_ENODEV, "no CUDA device");
     }
+    found = true;
     return LMZ_GPU_OK;
 }
 

@@ -549,8 +549,11 @@ static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, c
         static bool done[64];
         const int rc = opt_in_smem(k_merge<T, VB>, merge_smem(256), done);
         if (rc) return rc;
-        return launch("launch k_merge", k_merge<T, VB>, dim3(static_cast<unsigned>((in + M_COLS - 1) / M_COLS), static_cast<unsigned>((out + M_ROWS - 1) / M_ROWS)),
-                      M_THREADS, merge_smem(m.places), cs, m);
+        int sms = 0;
+        const int failed = sm_count(&sms);
+        if (failed) return failed;
+        const uint64_t tiles = ((in + M_COLS - 1) / M_COLS) * ((out + M_ROWS - 1) / M_ROWS), room = (uint64_t)sms * (merge_smem(m.places) <= 113u << 10 ? 2 : 1);
+        return launch("launch k_merge", k_merge<T, VB>, dim3(static_cast<unsigned>(std::min(tiles, room))), M_THREADS, merge_smem(m.places), cs, m);
     });
 }
 

@@ -427,7 +427,7 @@ def test_project_refusals():
 # ------------------------------------------------------------------------------------------- merges
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("out, inp, rank", [(1, 1, 1), (8, 8, 8), (130, 264, 16), (1000, 771, 5), (256, 1024, 64), (129, 512, 256), (70, 2000, 100), (66_000, 16, 4)])
+@pytest.mark.parametrize("out, inp, rank", [(1, 1, 1), (8, 8, 8), (130, 264, 16), (1000, 771, 5), (256, 1024, 64), (129, 512, 256), (70, 2000, 100), (66_000, 16, 4), (3000, 2600, 8), (2900, 1900, 72), (5000, 1032, 200), (2500, 1001, 33)])
 def test_merge(dtype, out, inp, rank):
     from lmz_b200 import adapters
     w, a, b = _randn(50, (out, inp), dtype), _randn(51, (rank, inp), dtype, inp ** -0.5), _randn(52, (out, rank), dtype)
