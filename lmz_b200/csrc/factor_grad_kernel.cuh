@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
         if (*over)                                               // nothing may still be on its way into this block's memory
             for (uint32_t st = 0; st < a.stages; st++) {
                 const uint32_t used = at.turn - (st >= at.stage);                // the last turn that filled this stage
-                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[st], used & 1); tries++) {}
+                if (used != ~0u) bar_drain(&s.full[st], used & 1);
             }
     } else if (warp == 1) {
         // at most 256 columns a product, in whole blocks

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
         if (*over)                                               // nothing may still be on its way into this block's memory
             for (uint32_t i = 0; i < a.stages; i++) {
                 const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
-                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[i], used & 1); tries++) {}
+                if (used != ~0u) bar_drain(&s.full[i], used & 1);
             }
     } else if (warp == 5) {
         const uint32_t desc = mma_desc(__is_same(T, __nv_bfloat16), false, false, H_TOKENS, (count * a.rp + 15) & ~15u);
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
         if (elected()) mma_commit(&s.sums);
         __syncwarp();
         if (*over)
-            for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums, 0); tries++) {}
+            bar_drain(&s.sums, 0);
     } else if (warp_wait(&s.sums, 0, over)) {
         // every token's own columns, over the stages (all products have ended)
         tc_after();

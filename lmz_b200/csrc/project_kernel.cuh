@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         if (*over && !side)
             for (uint32_t i = 0; i < a.stages; i++) {
                 const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
-                for (uint32_t tries = 0; used != ~0u && tries < WAIT_TRIES && !bar_try(&s.full[i], used & 1); tries++) {}
+                if (used != ~0u) bar_drain(&s.full[i], used & 1);
             }
     } else if (warp == 9) {
         if (!side) {
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             if (!ok) {                                           // the products under way end before their memory goes
                 if (elected()) mma_commit<PAIR>(&s.sums_full[n & 1]);
                 __syncwarp();
-                for (uint32_t tries = 0; tries < WAIT_TRIES && !bar_try(&s.sums_full[n & 1], (n / 2) & 1); tries++) {}
+                bar_drain(&s.sums_full[n & 1], (n / 2) & 1);
             }
         }
     } else if (warp >= 4) {

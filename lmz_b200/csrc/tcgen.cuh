@@ -39,18 +39,36 @@ __device__ __forceinline__ bool bar_try(uint64_t *b, uint32_t parity)
 // Set once a wait has run out (no wait does unless the hardware loses a copy): lmz_gpu_ops_gave_up() tells the host.
 static __device__ uint32_t g_gave_up;
 
-// Wait for a phase, but not for ever: after WAIT_TRIES (each a few microseconds at most) the block's waits are all over,
-// and with them its work; `over` is the block's flag.
-constexpr uint32_t WAIT_TRIES = 1u << 20;
+// Wait for a phase, but not for ever: after WAIT_NS the block's waits are all over, and with them its work; `over` is the
+// block's flag.
+constexpr uint64_t WAIT_NS = 4000000000ull;
+__device__ __forceinline__ uint64_t nanoseconds()
+{
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
 __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile uint32_t *over)
 {
-    for (uint32_t i = 0; i < WAIT_TRIES; i++) {
-        if (bar_try(b, parity)) return true;
-        if ((i & 63) == 63 && *over) return false;
+    uint64_t since = 0;
+    for (uint32_t i = 1; !bar_try(b, parity); i++) {
+        if (i & 255) continue;
+        if (*over) return false;
+        const uint64_t now = nanoseconds();
+        if (!since) since = now;
+        if (now - since > WAIT_NS) {
+            *over = 1;
+            g_gave_up = 1;
+            return false;
+        }
     }
-    *over = 1;
-    g_gave_up = 1;
-    return false;
+    return true;
+}
+// The same behind a wait that was over: for a copy or a product that must end before its memory goes.
+__device__ __forceinline__ void bar_drain(uint64_t *b, uint32_t parity)
+{
+    const uint64_t since = nanoseconds();
+    while (!bar_try(b, parity) && nanoseconds() - since < WAIT_NS) {}
 }
 
 // The address, in the cluster's window, of a word that another CTA has where this one has `p`.

@@ -541,6 +541,14 @@ def test_captured_behind_copies_and_from_other_streams():
         assert torch.equal(g, v)
 
 
+def test_no_wait_has_run_out():
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(300, 256, 264, 16, 3, torch.bfloat16)
+    adapters.project(x, w, a, b, _index("runs", 300, 3), scale=scales)
+    adapters.check()
+    adapters.check(torch.device("cuda", 0))
+
+
 def test_inputs_changed_between_the_passes_are_noticed():
     from lmz_b200 import adapters, embed
     x, w, a, b, scales = _inputs(6, 64, 96, 8, 3, torch.bfloat16)
