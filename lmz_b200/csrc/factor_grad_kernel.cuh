@@ -154,17 +154,33 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     else __syncthreads();
     if (ok && !*over) {
         T *out = g.out + i * g.each;
-        const uint32_t wide = a.blocks * FG_FEATS, share = wide / a.split;
-        // neighbouring threads write neighbouring elements: along f (a CTA every split-th j), or along j (a CTA its share of the f)
+        const uint32_t wide = a.blocks * FG_FEATS;
         const Peers peers(ring, a.split);
+        // Eight neighbours of the result a thread: along f, threads side by side on neighbouring j; or along j, threads on
+        // neighbouring f (either way they read neighbouring banks).
         const bool along_f = g.wide == 1;
-        const uint32_t count = along_f ? (a.rank + a.split - 1 - rank) / a.split * wide : a.rank * share;
-#pragma unroll 4
-        for (uint32_t e = tid; e < count; e += FG_THREADS) {
-            const uint32_t j = along_f ? rank + e / wide * a.split : e % a.rank, row = along_f ? e % wide : rank * share + e / a.rank;
+        const uint64_t next = along_f ? g.place : g.wide;
+        const bool whole = (reinterpret_cast<uint64_t>(g.out) & 15) == 0 && next % 8 == 0;
+        const uint32_t tasks = along_f ? a.rank * (wide / 8) : (a.rank + 7) / 8 * wide;
+        const uint32_t e1 = static_cast<uint32_t>(static_cast<uint64_t>(tasks) * (rank + 1) / a.split);
+        for (uint32_t e = static_cast<uint32_t>(static_cast<uint64_t>(tasks) * rank / a.split) + tid; e < e1; e += FG_THREADS) {
+            const uint32_t j = along_f ? e % a.rank : e / wide * 8, row = along_f ? e / a.rank * 8 : e % wide;
             const uint64_t f = f0 + static_cast<uint64_t>(row);
             if (f >= g.feats) continue;
-            out[f * g.wide + j * g.place] = narrow<T>(peers.sum(((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4));
+            float sum[8];
+            peers.sum8(((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, along_f ? 4 : FG_PITCH * 4, sum);
+            Vec<T, 16> v;
+#pragma unroll
+            for (uint32_t q = 0; q < 8; q++) v.e[q] = narrow<T>(sum[q]);
+            T *to = out + f * g.wide + j * g.place;
+            const uint64_t left = along_f ? g.feats - f : a.rank - j;
+            if (whole && left >= 8) {
+                *reinterpret_cast<uint4 *>(to) = v.raw;
+            } else {
+#pragma unroll
+                for (uint32_t q = 0; q < 8; q++)
+                    if (q < left) to[q] = v.e[q];
+            }
         }
     }
     if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums

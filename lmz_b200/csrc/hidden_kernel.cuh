@@ -156,19 +156,22 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
     __syncwarp();
     if (a.split > 1) cluster_barrier();
     else __syncthreads();
-    if (!*over) {                                                // a CTA's share of the tokens: the sums of all, in order
+    if (!*over) {                                                // a CTA's share of the tokens: the sums of all, in order, eight at a time
         const Peers peers(ring, a.split);
         const uint32_t each = H_TOKENS / a.split, lo = rank * each;
-#pragma unroll 2
-        for (uint32_t e = tid; e < each * a.rp; e += H_THREADS) {
-            const uint32_t row = lo + e / a.rp, c = e % a.rp;
+        for (uint32_t e = tid; e < each * (a.rp / 8); e += H_THREADS) {
+            const uint32_t row = lo + e % each, c = e / each * 8;
             const int slot = s.slot[row] - static_cast<int>(from);
             if (slot < 0 || slot >= static_cast<int>(count)) continue;
-            const float sum = peers.sum((c * H_PITCH + row) * 4);
-            T hi, lo_half;
-            split_halves(c < a.rank ? sum * a.index.scale_of(s.adapter[row]) : 0.0f, hi, lo_half);
+            const float scale = a.index.scale_of(s.adapter[row]);
+            float sum[8];
+            peers.sum8((c * H_PITCH + row) * 4, H_PITCH * 4, sum);
+            Vec<T, 16> upper, lower;
+#pragma unroll
+            for (uint32_t q = 0; q < 8; q++) split_halves(c + q < a.rank ? sum[q] * scale : 0.0f, upper.e[q], lower.e[q]);
             T *to = a.h + (t0 + row) * 2 * a.rp + c;
-            to[0] = hi, to[a.rp] = lo_half;
+            *reinterpret_cast<uint4 *>(to) = upper.raw;
+            *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
         }
     }
     if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums

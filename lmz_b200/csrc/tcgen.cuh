@@ -294,6 +294,21 @@ struct Peers {
         for (uint32_t q = 1; q < 8; q++) all += v[q];
         return all;
     }
+    // Eight of them, `step` bytes apart.
+    __device__ __forceinline__ void sum8(uint32_t offset, uint32_t step, float *to) const
+    {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) to[e] = 0;
+#pragma unroll
+        for (uint32_t q = 0; q < 8; q++) {
+            if (q >= ctas) break;
+            float v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[e]) : "r"(at[q] + offset + e * step) : "memory");
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) to[e] += v[e];
+        }
+    }
 };
 
 }  // namespace lmz
