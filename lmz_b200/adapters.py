@@ -72,33 +72,33 @@ def _packed(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
-def _call(code, x, weight, a, b, index, scales, scale, y=None, hidden=None, dy=None, dx=None, da=None, db=None):
-    ptr = lambda t: None if t is None else t.data_ptr()      # noqa: E731
+def _call(code, x, weight, a, b, index, scales, scale):
     (tokens, inp), (n, rank, _) = x.shape, a.shape
-    return _ops.Projection(x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), ptr(index), ptr(scales), ptr(y), ptr(hidden), ptr(dy), ptr(dx), ptr(da),
-                           ptr(db), None, tokens, inp, weight.shape[0], x.stride(0), weight.stride(0), n, rank, code,
-                           0 if index is None else index.element_size(), scale)
+    return _ops.Projection(x.data_ptr(), weight.data_ptr(), a.data_ptr(), b.data_ptr(), None if index is None else index.data_ptr(),
+                           None if scales is None else scales.data_ptr(), None, None, None, None, None, None, None, tokens, inp, weight.shape[0], x.stride(0),
+                           weight.stride(0), n, rank, code, 0 if index is None else index.element_size(), scale)
 
 
-def _run(name: str, grad: int, p, index: int):
+def _run(name: str, grad: int, p, x):
     import torch
     size = gpu.library().lmz_gpu_project_work_bytes(p, grad)
     if size:
-        work = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+        work = x.new_empty(size, dtype=torch.uint8)
         p.work = work.data_ptr()
-    _ops.launch(index, name, p)
+    _ops.launch(x.get_device(), name, p)
 
 
 def _forward(code, x, weight, a, b, index, scales, scale, keep):
     """y, and what the gradients need of it if `keep`."""
     y = x.new_empty((*x.shape[:-1], weight.shape[0]))
     x, a, b, index, scales = _flat(x), _packed(a), _packed(b), _packed(index), _packed(scales)
-    p, hidden = _call(code, x, weight, a, b, index, scales, scale, y), None
+    p, hidden = _call(code, x, weight, a, b, index, scales, scale), None
+    p.y = y.data_ptr()
     if keep:
         import torch
         hidden = torch.empty(gpu.library().lmz_gpu_project_hidden_bytes(p), dtype=torch.uint8, device=x.device)
         p.hidden = hidden.data_ptr()
-    _run("lmz_gpu_project_dev", 0, p, x.get_device())
+    _run("lmz_gpu_project_dev", 0, p, x)
     return y, hidden
 
 
@@ -107,8 +107,10 @@ def _backward(code, dy, x, weight, a, b, index, scales, scale, hidden, wanted):
     dx, da, db = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((x, a, b), wanted))
     x, dy = _flat(x), dy.reshape(-1, dy.shape[-1]).contiguous()
     a, b, index, scales = _packed(a), _packed(b), _packed(index), _packed(scales)      # (copies live until the launch)
-    p = _call(code, x, weight, a, b, index, scales, scale, None, hidden, dy, dx, da, db)
-    _run("lmz_gpu_project_grad_dev", 1, p, x.get_device())
+    p = _call(code, x, weight, a, b, index, scales, scale)
+    p.hidden, p.dy = hidden.data_ptr(), dy.data_ptr()
+    p.dx, p.da, p.db = (None if t is None else t.data_ptr() for t in (dx, da, db))
+    _run("lmz_gpu_project_grad_dev", 1, p, x)
     return dx, da, db
 
 
