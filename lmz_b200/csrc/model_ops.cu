@@ -279,7 +279,8 @@ API size_t lmz_gpu_project_hidden_bytes(const lmz_projection *p) { return p->tok
 API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { return ProjectLayout(p, grad).end; }
 
 constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
-constexpr uint32_t PROJECT_SMEM = 219u << 10;
+constexpr uint32_t PROJECT_SMEM = 222u << 10;
+static_assert(PROJECT_SMEM + sizeof(ProjectShared) <= 227u << 10);
 
 static uint32_t tmem_columns(uint32_t n)
 {

@@ -9,7 +9,7 @@ constexpr uint32_t P_FEATS = 128;              // features of a tile: the tensor
 constexpr uint32_t P_TOKENS = 256;             // most tokens of a tile: its N, a TMEM column each
 constexpr uint32_t P_GROUP = 16;               // tokens of a TMEM load, and the steps that N comes in (a pair's: 32)
 constexpr uint32_t P_INFOS = 3, P_MAX_STAGES = 10, P_MAX_SLOTS = 8;
-constexpr uint32_t P_SLOT_BYTES = P_GROUP * P_FEATS * 4, P_PLACES = 16;     // places of the rank that mixed groups take at a time
+constexpr uint32_t P_SLOT_BYTES = P_GROUP * P_FEATS * 4, P_PLACES = 64;     // places of the rank that mixed groups take at a time
 constexpr uint32_t P_EPILOGUE = 128, P_FEED = 128, P_THREADS = P_EPILOGUE + P_FEED + 64;
 
 // What a tile's tokens have for adapters.
@@ -52,77 +52,112 @@ struct ProjectArgs {
 // Tiles of a stage: W's 128 rows, and the tokens' (of a pair's 256 each CTA has half).
 __host__ __device__ constexpr uint32_t project_stage_bytes(uint32_t nt, bool pair) { return (P_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
 
+// Of sixteen tokens' adapters, factors [feature][rank]: L threads have a feature's up to 64 places of the rank, eight each, so
+// that a warp's load is of whole lines; their sums meet by shuffles, in which each thread ends with another feature's.
+// `factor`: at the tile's first feature and place, of adapter 0; `live`: the tile's features; `left`: places, from here on.
+template <class T, uint32_t L>
+__device__ __forceinline__ void mixed_rows(const T *factor, uint64_t factor_each, uint32_t factor_row, uint32_t live, uint32_t left, const int32_t *adapter,
+                                        uint32_t id, bool add, const float *places, float *slot)
+{
+    constexpr uint32_t FLIGHT = 16, BATCH = FLIGHT / L;          // loads under way
+    const uint32_t part = id % L, row = id / L;
+    for (uint32_t c0 = 0; c0 < P_GROUP; c0 += BATCH) {
+        Vec<T, 16> fac[BATCH][L];
+#pragma unroll
+        for (uint32_t c = 0; c < BATCH; c++) {
+            const int i = adapter[c0 + c];
+            const T *p = factor + (i < 0 ? 0 : i) * factor_each + part * 8;
+#pragma unroll
+            for (uint32_t m = 0; m < L; m++) {
+                const uint32_t f = row + m * (P_FEATS / L);
+                fac[c][m].raw = {};
+                if (i >= 0 && f < live && part * 8 < left) fac[c][m].raw = *reinterpret_cast<const uint4 *>(p + static_cast<uint64_t>(f) * factor_row);
+            }
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < BATCH; c++) {
+            float h[8], v[L];
+            *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + part * 8);
+            *reinterpret_cast<float4 *>(h + 4) = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + part * 8 + 4);
+#pragma unroll
+            for (uint32_t m = 0; m < L; m++) {
+                v[m] = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) v[m] += h[e] * widen(fac[c][m].e[e]);
+            }
+#pragma unroll
+            for (uint32_t o = L / 2; o; o /= 2)
+#pragma unroll
+                for (uint32_t m = 0; m < o; m++) {
+                    const float give = part & o ? v[m] : v[m + o], keep = part & o ? v[m + o] : v[m];
+                    v[m] = keep + __shfl_xor_sync(~0u, give, o);
+                }
+            float &to = slot[(c0 + c) * P_FEATS + row + part * (P_FEATS / L)];
+            to = add ? to + v[0] : v[0];
+        }
+    }
+}
+
 // What the adapters add to a tile's features of sixteen tokens that have different ones, into `slot` ([token][feature]), by
 // four warps.  Not on the tensor core: a factor multiplied by the zeros of tokens it does not belong to would
-// still hand them its infinities and NaN.  Bound by the latency of the factors' loads, of which a thread has a whole group's
-// sixteen places under way; `places`: room for sixteen places of the rank of the tokens' h.
+// still hand them its infinities and NaN.  Bound by the latency of the factors' loads, of which a thread has sixteen
+// under way; `places`: room for 64 places of the rank of the tokens' h.
 template <class T, bool MN>
 __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32_t *adapter, uint64_t t0, uint64_t f0, uint32_t id, uint32_t barrier, float *places, float *slot)
 {
-    constexpr uint32_t BATCH = 16;
-    float sum[P_GROUP] = {};                                     // !MN: per token, of feature `id`; MN: two tokens' eight features
+    float sum[P_GROUP] = {};                                     // MN: two tokens' eight features
     const uint32_t fg = id & 15, tg = id >> 4;
     for (uint32_t j0 = 0; j0 < a.rp; j0 += P_PLACES) {
         sync_threads(barrier, P_FEED);
         {
-            const uint32_t c = id >> 3, j = j0 + (id & 7) * 2;
-            float2 v = make_float2(0, 0);
+            const uint32_t c = id >> 3, j = j0 + (id & 7) * 8;
+            Vec<T, 16> upper, lower;
+            upper.raw = lower.raw = {};
             if (adapter[c] >= 0 && j < a.rp) {
                 const T *h = a.hidden + (t0 + c) * 2 * a.rp + j;
-                v = make_float2(widen(h[0]) + widen(h[a.rp]), widen(h[1]) + widen(h[a.rp + 1]));
+                upper.raw = *reinterpret_cast<const uint4 *>(h), lower.raw = *reinterpret_cast<const uint4 *>(h + a.rp);
             }
-            *reinterpret_cast<float2 *>(places + c * P_PLACES + (id & 7) * 2) = v;
+            float v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) v[e] = widen(upper.e[e]) + widen(lower.e[e]);
+            float4 *to = reinterpret_cast<float4 *>(places + c * P_PLACES + (id & 7) * 8);
+            to[0] = make_float4(v[0], v[1], v[2], v[3]), to[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
         sync_threads(barrier, P_FEED);
         if constexpr (MN) {
+            constexpr uint32_t BATCH = 16;
+            for (uint32_t j1 = 0; j1 < P_PLACES && j0 + j1 < a.rp; j1 += BATCH) {
 #pragma unroll
-            for (uint32_t half = 0; half < 2; half++) {
-                const uint32_t c = tg + half * 8;
-                const int i = adapter[c];
-                const uint64_t f = f0 + fg * 8;
-                if (i < 0 || f >= a.feats) continue;
-                const T *p = a.factor + i * a.factor_each + j0 * a.factor_row + f;
-                Vec<T, 16> fac[P_PLACES];
+                for (uint32_t half = 0; half < 2; half++) {
+                    const uint32_t c = tg + half * 8;
+                    const int i = adapter[c];
+                    const uint64_t f = f0 + fg * 8;
+                    if (i < 0 || f >= a.feats) continue;
+                    const T *p = a.factor + i * a.factor_each + (j0 + j1) * a.factor_row + f;
+                    Vec<T, 16> fac[BATCH];
 #pragma unroll
-                for (uint32_t j = 0; j < P_PLACES; j++) {
-                    fac[j].raw = {};
-                    if (j0 + j < a.rank) fac[j].raw = *reinterpret_cast<const uint4 *>(p + j * a.factor_row);
-                }
+                    for (uint32_t j = 0; j < BATCH; j++) {
+                        fac[j].raw = {};
+                        if (j0 + j1 + j < a.rank) fac[j].raw = *reinterpret_cast<const uint4 *>(p + j * a.factor_row);
+                    }
 #pragma unroll
-                for (uint32_t j = 0; j < P_PLACES; j++) {
-                    const float h = places[c * P_PLACES + j];
-                    if (j0 + j < a.rank) {
+                    for (uint32_t j = 0; j < BATCH; j++) {
+                        const float h = places[c * P_PLACES + j1 + j];
+                        if (j0 + j1 + j < a.rank) {
 #pragma unroll
-                        for (uint32_t e = 0; e < 8; e++) sum[half * 8 + e] += h * widen(fac[j].e[e]);
+                            for (uint32_t e = 0; e < 8; e++) sum[half * 8 + e] += h * widen(fac[j].e[e]);
+                        }
                     }
                 }
             }
         } else {
-            const uint64_t f = f0 + id;
-            if (f < a.feats) {
-#pragma unroll
-                for (uint32_t c0 = 0; c0 < P_GROUP; c0 += BATCH) {
-                    Vec<T, 16> fac[BATCH][2];
-#pragma unroll
-                    for (uint32_t c = 0; c < BATCH; c++) {
-                        const int i = adapter[c0 + c];
-                        const T *p = a.factor + (i < 0 ? 0 : i) * a.factor_each + f * a.factor_row + j0;
-                        fac[c][0].raw = fac[c][1].raw = {};
-                        if (i >= 0) {
-                            fac[c][0].raw = *reinterpret_cast<const uint4 *>(p);
-                            if (j0 + 8 < a.rp) fac[c][1].raw = *reinterpret_cast<const uint4 *>(p + 8);
-                        }
-                    }
-#pragma unroll
-                    for (uint32_t c = 0; c < BATCH; c++)
-#pragma unroll
-                        for (uint32_t j = 0; j < P_PLACES; j += 4) {
-                            const float4 h = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + j);
-                            const auto &v = fac[c][j / 8];
-                            sum[c0 + c] += h.x * widen(v.e[j % 8]) + h.y * widen(v.e[j % 8 + 1]) + h.z * widen(v.e[j % 8 + 2]) + h.w * widen(v.e[j % 8 + 3]);
-                        }
-                }
-            }
+            const T *factor = a.factor + f0 * a.factor_row + j0;
+            const uint32_t live = a.feats > f0 ? static_cast<uint32_t>(a.feats - f0 < P_FEATS ? a.feats - f0 : P_FEATS) : 0, left = a.rp - j0;
+            const uint32_t row = static_cast<uint32_t>(a.factor_row);
+            if (left > 32) mixed_rows<T, 8>(factor, a.factor_each, row, live, left, adapter, id, j0 != 0, places, slot);
+            else if (left > 16) mixed_rows<T, 4>(factor, a.factor_each, row, live, left, adapter, id, j0 != 0, places, slot);
+            else if (left > 8) mixed_rows<T, 2>(factor, a.factor_each, row, live, left, adapter, id, j0 != 0, places, slot);
+            else mixed_rows<T, 1>(factor, a.factor_each, row, live, left, adapter, id, j0 != 0, places, slot);
         }
     }
     if constexpr (MN) {
@@ -132,9 +167,6 @@ __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32
             *reinterpret_cast<float4 *>(to) = make_float4(sum[half * 8], sum[half * 8 + 1], sum[half * 8 + 2], sum[half * 8 + 3]);
             *reinterpret_cast<float4 *>(to + 4) = make_float4(sum[half * 8 + 4], sum[half * 8 + 5], sum[half * 8 + 6], sum[half * 8 + 7]);
         }
-    } else {
-#pragma unroll
-        for (uint32_t c = 0; c < P_GROUP; c++) slot[c * P_FEATS + id] = sum[c];
     }
     sync_threads(barrier, P_FEED);
 }

@@ -319,6 +319,40 @@ def test_bad_values_stay_with_their_own_tokens(tokens):
     assert torch.equal(got[1][keep], want[1][keep]) and torch.equal(got[2][keep], want[2][keep])
 
 
+@pytest.mark.parametrize("tokens, inp, out, rank, n", [(130, 256, 512, 16, 5), (300, 1024, 2056, 8, 9), (700, 264, 1288, 24, 12), (2500, 512, 4104, 72, 7),
+                                                       (1100, 320, 1096, 16, 200)])
+def test_bad_values_among_tokens_in_any_order(tokens, inp, out, rank, n):
+    """The same where every sixteen tokens have several adapters, in tiles of a few adapters and of very many."""
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(tokens, inp, out, rank, n, torch.bfloat16)
+    index, dy = _index("mixed", tokens, n), _randn(41, (tokens, out), torch.bfloat16)
+    index[:3] = torch.tensor([1, -1, 3])
+
+    def both():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, a, b)]
+        y = adapters.project(leaves[0], w, leaves[1], leaves[2], index, scale=scales)
+        return y.detach(), torch.autograd.grad(y, leaves, dy)
+
+    good, want = both()
+    _check_project(x, w, a, b, scales, index, good, dy, want)
+    a[1, -1, -1], b[1, 0, 0], a[3, 0, 0], b[3, -1, -1] = math.nan, math.inf, -math.inf, math.nan
+    x[index == -1] = math.nan
+    dy[index == -1] = math.inf
+    others = (index != 1) & (index != 3) & (index != -1)
+    y, got = both()
+    assert torch.equal(y[others], good[others]) and torch.equal(got[0][others], want[0][others])
+    for i in (1, 3):
+        assert torch.isnan(y[index == i]).any() and torch.isnan(got[0][index == i]).any()
+    keep = [i for i in range(n) if i not in (1, 3)]
+    assert torch.equal(got[1][keep], want[1][keep]) and torch.equal(got[2][keep], want[2][keep])
+    # a row of x with infinities is its own token's alone
+    x, w, a, b, scales = _inputs(tokens, inp, out, rank, n, torch.bfloat16)
+    dy = _randn(41, (tokens, out), torch.bfloat16)
+    x[0], dy[0] = math.inf, math.nan
+    y, got = both()
+    assert torch.equal(y[1:], good[1:]) and torch.equal(got[0][1:], want[0][1:])
+
+
 def test_one_adapter_without_a_stack():
     from lmz_b200 import adapters
     x, w, a, b, _ = _inputs(20, 64, 96, 8, 1, torch.bfloat16)
