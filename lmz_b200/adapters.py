@@ -33,18 +33,19 @@ def project(x, weight, a, b, index=None, scale=1.0):
     if a.dim() == 2 and b.dim() == 2:
         a, b = a.unsqueeze(0), b.unsqueeze(0)
     out, inp = weight.shape
-    lead = x.shape[:-1]
-    if a.dim() != 3 or b.dim() != 3 or x.shape[-1] != inp or a.shape[2] != inp or b.shape[1] != out or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+    *lead, columns = x.shape
+    n, rank, width = a.shape if a.dim() == 3 else (0, 0, 0)
+    if columns != inp or width != inp or a.dim() != 3 or b.shape != (n, out, rank):
         raise ValueError(f"x {list(x.shape)}, weight {list(weight.shape)}, a {list(a.shape)} and b {list(b.shape)} do not fit "
                          "[..., in], [out, in], [adapters, rank, in] and [adapters, out, rank]")
     if weight.stride(1) != 1 and inp > 1:
         raise ValueError("the elements of a row of the weight must be next to each other")
-    if not a.shape[0] or not inp or not out or not 1 <= a.shape[1] <= MAX_RANK:
+    if not n or not inp or not out or not 1 <= rank <= MAX_RANK:
         raise ValueError(f"no adapter, an empty weight, or a rank outside 1..{MAX_RANK}")
     if index is not None:
         _ops.whole_numbers(index, "index")
-        if index.shape != lead:
-            raise ValueError(f"index is {list(index.shape)}, x has tokens {list(lead)}")
+        if [*index.shape] != lead:
+            raise ValueError(f"index is {list(index.shape)}, x has tokens {lead}")
     scales = None
     if isinstance(scale, torch.Tensor):
         scales, scale = scale, 1.0
@@ -96,15 +97,14 @@ def _forward(code, x, weight, a, b, index, scales, scale, keep):
     p.y = y.data_ptr()
     if keep:
         import torch
-        hidden = torch.empty(gpu.library().lmz_gpu_project_hidden_bytes(p), dtype=torch.uint8, device=x.device)
+        hidden = x.new_empty(gpu.library().lmz_gpu_project_hidden_bytes(p), dtype=torch.uint8)
         p.hidden = hidden.data_ptr()
     _run("lmz_gpu_project_dev", 0, p, x)
     return y, hidden
 
 
 def _backward(code, dy, x, weight, a, b, index, scales, scale, hidden, wanted):
-    import torch
-    dx, da, db = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None for t, w in zip((x, a, b), wanted))
+    dx, da, db = (t.new_empty(t.shape) if w else None for t, w in zip((x, a, b), wanted))
     x, dy = _flat(x), dy.reshape(-1, dy.shape[-1]).contiguous()
     a, b, index, scales = _packed(a), _packed(b), _packed(index), _packed(scales)      # (copies live until the launch)
     p = _call(code, x, weight, a, b, index, scales, scale)

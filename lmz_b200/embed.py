@@ -49,7 +49,7 @@ def _rows_grad(dy, tokens, rows: int, scale):
     grad = dy.new_empty((rows, dim))
     if grad.numel():
         ids, dy, n = tokens.contiguous(), dy.contiguous(), tokens.numel()
-        work = torch.empty(gpu.library().lmz_gpu_rows_grad_work_bytes(n, rows, dim), dtype=torch.uint8, device=dy.device)
+        work = dy.new_empty(gpu.library().lmz_gpu_rows_grad_work_bytes(n, rows, dim), dtype=torch.uint8)
         _ops.launch(dy.get_device(), "lmz_gpu_rows_grad_dev", dy.data_ptr(), n, dim, _ops.type_code(dy, "dy"), ids.data_ptr(), ids.element_size(), rows, scale,
                     grad.data_ptr(), work.data_ptr())
     return grad
