@@ -34,6 +34,43 @@ __device__ __forceinline__ void split_halves(float v, T &hi, T &lo)
     lo = narrow<T>(isfinite(widen(hi)) ? v - widen(hi) : 0.0f);
 }
 
+// Tokens in the order of their adapters, if they came scattered: what the projection's kernels then read in place of x.
+struct SortedTokens {
+    const uint32_t *scattered;                 // NULL: never; else 1 if they are
+    const uint32_t *order, *keys;              // per place: the token, and its adapter (n: none)
+    __device__ __forceinline__ bool on() const { return scattered && __ldcg(scattered); }
+    __device__ __forceinline__ TokenIndex index(TokenIndex index, bool on) const
+    {
+        if (on) index.ids = keys, index.wide = false;
+        return index;
+    }
+};
+
+// A row per place, rows of `cols` elements that start on 16 bytes (what is behind a row's last is not written).  Bound by HBM.
+constexpr uint32_t GATHER_WARPS = 8;
+template <class T>
+__global__ void __launch_bounds__(32 * GATHER_WARPS) k_gather(const SortedTokens sorted, const T *from, uint64_t stride, uint32_t cols, uint64_t tokens, T *to, uint64_t pitch)
+{
+    constexpr uint32_t AHEAD = 8;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t t = static_cast<uint64_t>(blockIdx.x) * GATHER_WARPS + threadIdx.x / 32;
+    let_next_start();
+    wait_for_previous();
+    if (t >= tokens || !sorted.on()) return;
+    const T *in = from + sorted.order[t] * stride;
+    T *out = to + t * pitch;
+    for (uint32_t v = lane; v < cols / 8; v += 32 * AHEAD) {
+        uint4 q[AHEAD];
+#pragma unroll
+        for (uint32_t e = 0; e < AHEAD; e++)
+            if (v + e * 32 < cols / 8) q[e] = reinterpret_cast<const uint4 *>(in)[v + e * 32];
+#pragma unroll
+        for (uint32_t e = 0; e < AHEAD; e++)
+            if (v + e * 32 < cols / 8) reinterpret_cast<uint4 *>(out)[v + e * 32] = q[e];
+    }
+    if (lane < cols % 8) out[cols / 8 * 8 + lane] = in[cols / 8 * 8 + lane];
+}
+
 // Copies whose rows start on a boundary of 16 bytes and end in zeros: out[o][r][c] = in(o, r, c) for c < cols, else 0.
 template <class T>
 struct PackJob {

@@ -22,8 +22,11 @@ struct HiddenShared {
 template <class T>
 struct HiddenArgs {
     CUtensorMap x, f;                          // f: adapters x rank x K
+    CUtensorMap xs;                            // x in the order of `sorted`
     TokenIndex index;
-    T *h;                                      // [token][2][rp]
+    SortedTokens sorted;
+    T *h;                                      // [token][2][rp], in that order if x is
+    T *kept;                                   // NULL, or the same in the tokens' own order
     uint64_t tokens;
     uint32_t rank, rp, steps, split;
     uint32_t each;                             // adapters of a block: as many as have room in H_COLUMNS columns
@@ -61,9 +64,11 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
         bar_init(&s.sums, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    const bool sorted = a.sorted.on();
+    const TokenIndex index = a.sorted.index(a.index, sorted);
     int mine = -1;
     if (tid < H_TOKENS) {
-        if (t0 + tid < a.tokens) mine = a.index.of(t0 + tid);
+        if (t0 + tid < a.tokens) mine = index.of(t0 + tid);
         s.adapter[tid] = mine;
     }
     __syncthreads();
@@ -106,7 +111,7 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
             if (at.turn && !warp_wait(&s.empty[st], (at.turn - 1) & 1, over)) break;
             if (elected()) {
                 bar_expect(&s.full[st], H_TOKENS * ROW_BYTES + count * a.rank * ROW_BYTES);
-                tma_load_2d(&a.x, smem_addr(&s.full[st]), dst, k * STEP_K, tile * H_TOKENS);
+                tma_load_2d(sorted ? &a.xs : &a.x, smem_addr(&s.full[st]), dst, k * STEP_K, tile * H_TOKENS);
             }
             __syncwarp();
             for (uint32_t i = lane; i < count; i += 32)
@@ -173,6 +178,11 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
             T *to = a.h + (t0 + row) * 2 * a.rp + c;
             *reinterpret_cast<uint4 *>(to) = upper.raw;
             *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
+            if (a.kept) {
+                to = a.kept + (sorted ? a.sorted.order[t0 + row] : t0 + row) * 2 * a.rp + c;
+                *reinterpret_cast<uint4 *>(to) = upper.raw;
+                *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
+            }
         }
     }
     if (a.split > 1) cluster_barrier();                          // nobody leaves while another reads its sums

@@ -246,10 +246,19 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
     return r == CUDA_SUCCESS ? LMZ_GPU_OK : report(LMZ_GPU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
+// Whether a projection that finds more than a quarter of its sixteens of tokens with several adapters takes the tokens in the
+// order of their adapters.  To find out costs 7 us, the order and the copy of x 10 and more, and without them the sixteens take
+// some 2.4 us a feature tile and 16 places of the rank on a multiprocessor: from 30 us of that on, if sixteens of one adapter
+// come of it.  One B200, tokens x in x out, adapters, rank, in any order and in runs, with it and without: 8192x4096x4096 of 30 r16 240
+// and 219 against 505 and 213, 8000x512x512 of 8 r128 77 and 66 against 301 and 56, 2048x1024x2048 of 16 r16 52 and 40 against 75
+// and 34, 1024x4096x1024 of 8 r32 42 and 34 against 47 and 27 (left without).
+static bool worth_sorting(const lmz_projection *p, uint64_t feats, uint64_t rp) { return p->tokens >= 8ull * p->adapters && p->tokens * feats * rp >= 1ull << 26; }
+
 // What a projection's kernels read in place of tensors that do not lie on boundaries, and between each other.
 struct ProjectLayout {
-    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, hidden, end = 0;
+    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, hidden, scattered, in_order, thin, end = 0;
     bool pack_x, pack_w, pack_a, pack_b, pack_dy;
+    bool sorts;                                // the projection takes scattered tokens by adapter
     ProjectLayout(const lmz_projection *p, bool grad)
     {
         auto take = [&](bool on, uint64_t bytes) {
@@ -268,10 +277,14 @@ struct ProjectLayout {
         b = take(pack_b, 2 * p->adapters * (grad ? p->rank * up8(p->out) : p->out * up8(p->rank)));
         dy = take(pack_dy, p->tokens * up8(p->out) * 2);
         g = take(grad, p->tokens * 4 * up8(p->rank));
-        const bool sorted = grad && p->index;
+        sorts = p->index && p->adapters > 1 && (!grad || p->dx) && worth_sorting(p, grad ? p->in : p->out, up8(p->rank));
+        const bool sorted = (grad && p->index) || sorts;
         for (int i = 0; i < 2; i++) keys[i] = take(sorted, p->tokens * 4), pos[i] = take(sorted, p->tokens * 4);
-        start = take(sorted, (p->adapters + 1ull) * 4);
+        start = take(grad && p->index, (p->adapters + 1ull) * 4);
         hidden = take(!grad && !p->hidden, p->tokens * 4 * up8(p->rank));
+        scattered = take(sorts, 4);
+        in_order = take(sorts, p->tokens * up8(grad ? p->out : p->in) * 2);
+        thin = take(sorts && (grad || p->hidden), p->tokens * 4 * up8(p->rank));
     }
 };
 
@@ -306,15 +319,22 @@ static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)
     return LMZ_GPU_OK;
 }
 
+// Scattered tokens by adapter (launch_in_order), or nothing.
+template <class T>
+struct InOrder {
+    SortedTokens sorted{};
+    const T *x = nullptr;                        // rows of up8(k) elements
+};
+
 // y[t][f] = sum of x[t][k] W(f, k) + sum of h[t][j] F_i(f, j) (MN: W and F with their f next to each other).
 template <class T, bool MN>
-static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride, uint64_t k, const T *w, uint64_t w_stride, uint64_t feats, const T *factor,
+static int launch_project(const lmz_projection *p, const InOrder<T> &o, const T *x, uint64_t x_stride, uint64_t k, const T *w, uint64_t w_stride, uint64_t feats, const T *factor,
                           uint64_t factor_rows, uint64_t factor_row, const T *hidden, T *y, cudaStream_t cs)
 {
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     ProjectArgs<T> a{};
-    a.index = token_index(p), a.hidden = hidden, a.factor = factor, a.factor_each = factor_rows * factor_row, a.factor_row = factor_row;
+    a.index = token_index(p), a.sorted = o.sorted, a.hidden = hidden, a.factor = factor, a.factor_each = factor_rows * factor_row, a.factor_row = factor_row;
     a.y = y, a.tokens = p->tokens, a.feats = feats, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K), a.split = 1;
     auto tiles = [&](uint64_t f, uint64_t t) { return (feats + f - 1) / f * ((p->tokens + t - 1) / t); };
@@ -345,6 +365,7 @@ static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride
     a.tmem_columns = tmem_columns(a.split > 1 ? a.nt : 2 * a.nt);
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
     rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, pair ? a.nt / 2 : a.nt);
+    if (!rc && o.x) rc = tensor_map(&a.xs, o.x, bf16, k, p->tokens, up8(k), pair ? a.nt / 2 : a.nt);
     if (!rc) rc = MN ? tensor_map(&a.w, w, bf16, feats, k, w_stride, STEP_K) : tensor_map(&a.w, w, bf16, k, feats, w_stride, P_FEATS);
     if (!rc) rc = tensor_map(&a.h, hidden, bf16, a.rp, 2, a.rp, 1, p->tokens, pair ? a.nt / 2 : a.nt);
     if (!rc) rc = MN ? tensor_map(&a.f, factor, bf16, feats, factor_rows, factor_row, STEP_K, p->adapters)
@@ -356,13 +377,14 @@ static int launch_project(const lmz_projection *p, const T *x, uint64_t x_stride
 
 // h = s x F^T for each token's own adapter; f: [adapter][rank][f_stride], its first k of each row.
 template <class T>
-static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride, uint64_t k, const T *f, uint64_t f_stride, T *h, cudaStream_t cs)
+static int launch_hidden(const lmz_projection *p, const InOrder<T> &o, const T *x, uint64_t x_stride, uint64_t k, const T *f, uint64_t f_stride, T *h, T *kept,
+                         cudaStream_t cs)
 {
     static bool done[64];
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     HiddenArgs<T> a{};
-    a.index = token_index(p), a.h = h, a.tokens = p->tokens, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
+    a.index = token_index(p), a.sorted = o.sorted, a.h = h, a.kept = kept, a.tokens = p->tokens, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K);
     const uint64_t tiles = (p->tokens + H_TOKENS - 1) / H_TOKENS;
     const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(p->index ? std::min(p->adapters, H_TOKENS) : 1, p->tokens));
@@ -376,6 +398,7 @@ static int launch_hidden(const lmz_projection *p, const T *x, uint64_t x_stride,
     while (a.split < 8 && tiles * groups * a.split * 2 <= (uint64_t)sms && a.steps >= 4 * a.split) a.split *= 2;
     constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
     rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, H_TOKENS);
+    if (!rc && o.x) rc = tensor_map(&a.xs, o.x, bf16, k, p->tokens, up8(k), H_TOKENS);
     if (!rc) rc = tensor_map(&a.f, f, bf16, k, p->rank, f_stride, p->rank, p->adapters);
     if (!rc) rc = opt_in_smem(k_hidden<T>, OPS_SMEM, done);
     if (rc) return rc;
@@ -463,15 +486,47 @@ struct ProjectInputs {
     }
 };
 
+// The sort of the tokens by adapter; `order` is where it lies.  `start`: and where each adapter's begin.
+static int launch_token_sort(const lmz_projection *p, const ProjectLayout &l, bool start, SortedTokens *sorted, cudaStream_t cs)
+{
+    uint8_t *work = static_cast<uint8_t *>(p->work);
+    auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t *>(work + off); };
+    SortArgs s{};
+    s.ids = p->index, s.n = p->tokens, s.nkeys = p->adapters, s.wide = p->index_bytes == 8;
+    for (int i = 0; i < 2; i++) s.keys[i] = words(l.keys[i]), s.pos[i] = words(l.pos[i]);
+    s.start = start ? words(l.start) : nullptr, s.scattered = l.sorts ? words(l.scattered) : nullptr;
+    int side = 0;
+    const int rc = launch_sort(s, cs, &side);
+    *sorted = {s.scattered, s.pos[side], s.keys[side]};
+    return rc;
+}
+
+// x's rows by adapter, if the sort has found them scattered.
+template <class T>
+static int launch_in_order(const lmz_projection *p, const ProjectLayout &l, const T *x, uint64_t x_stride, uint64_t k, InOrder<T> *o, cudaStream_t cs)
+{
+    T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + l.in_order);
+    o->x = to;
+    return launch("launch k_gather", k_gather<T>, dim3(static_cast<unsigned>((p->tokens + GATHER_WARPS - 1) / GATHER_WARPS)), 32 * GATHER_WARPS, 0, cs, o->sorted, x,
+                  x_stride, static_cast<uint32_t>(k), p->tokens, to, up8(k));
+}
+
 template <class T>
 static int project_as(const lmz_projection *p, cudaStream_t cs)
 {
     const ProjectLayout l(p, false);
     const ProjectInputs<T> in(p, l, false, cs);
-    T *h = static_cast<T *>(p->hidden ? p->hidden : static_cast<uint8_t *>(p->work) + l.hidden);
+    auto work = [&](uint64_t off) { return reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off); };
     int rc = in.rc;
-    if (!rc) rc = launch_hidden(p, in.x, in.x_stride, p->in, in.a, in.a_stride, h, cs);
-    if (!rc) rc = launch_project<T, false>(p, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, in.b, p->out, up8(p->rank), h, static_cast<T *>(p->y), cs);
+    InOrder<T> o;
+    T *h = p->hidden ? static_cast<T *>(p->hidden) : work(l.hidden), *kept = nullptr;
+    if (!rc && l.sorts) {
+        rc = launch_token_sort(p, l, false, &o.sorted, cs);
+        if (!rc) rc = launch_in_order(p, l, in.x, in.x_stride, p->in, &o, cs);
+        if (p->hidden) kept = h, h = work(l.thin);
+    }
+    if (!rc) rc = launch_hidden(p, o, in.x, in.x_stride, p->in, in.a, in.a_stride, h, kept, cs);
+    if (!rc) rc = launch_project<T, false>(p, o, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, in.b, p->out, up8(p->rank), h, static_cast<T *>(p->y), cs);
     return rc;
 }
 
@@ -486,28 +541,28 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
     }
     const ProjectLayout l(p, true);
     const ProjectInputs<T> in(p, l, true, cs);
+    auto work = [&](uint64_t off) { return reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off); };
     int rc = in.rc;
-    uint8_t *work = static_cast<uint8_t *>(p->work);
-    T *g = reinterpret_cast<T *>(work + l.g);
-    if (!rc && (p->dx || p->da)) rc = launch_hidden(p, in.dy, in.dy_stride, p->out, in.b, up8(p->out), g, cs);
-    if (!rc && p->dx) rc = launch_project<T, true>(p, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, g, static_cast<T *>(p->dx), cs);
-    const uint32_t *order = nullptr, *start = nullptr;
-    if (!rc && p->index && (p->da || p->db)) {
-        SortArgs s{};
-        s.ids = p->index, s.n = p->tokens, s.nkeys = p->adapters, s.wide = p->index_bytes == 8;
-        for (int i = 0; i < 2; i++) s.keys[i] = reinterpret_cast<uint32_t *>(work + l.keys[i]), s.pos[i] = reinterpret_cast<uint32_t *>(work + l.pos[i]);
-        s.start = reinterpret_cast<uint32_t *>(work + l.start);
-        int side = 0;
-        rc = launch_sort(s, cs, &side);
-        if (rc) return rc;
-        order = s.pos[side], start = s.start;
+    InOrder<T> o;
+    SortedTokens tokens{};
+    T *g = work(l.g), *h = g, *kept = nullptr;
+    const bool factors = p->da || p->db;
+    if (!rc && l.sorts) {
+        rc = launch_token_sort(p, l, factors, &tokens, cs);
+        o.sorted = tokens;
+        if (!rc) rc = launch_in_order(p, l, in.dy, in.dy_stride, p->out, &o, cs);
+        h = work(l.thin), kept = p->da ? g : nullptr;
     }
-    if (rc || !(p->da || p->db)) return rc;
+    if (!rc && (p->dx || p->da)) rc = launch_hidden(p, o, in.dy, in.dy_stride, p->out, in.b, up8(p->out), h, kept, cs);
+    if (!rc && p->dx) rc = launch_project<T, true>(p, o, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, h, static_cast<T *>(p->dx), cs);
+    if (rc || !factors) return rc;
+    if (p->index && !l.sorts) rc = launch_token_sort(p, l, true, &tokens, cs);
+    if (rc) return rc;
     FactorGrad<T> jobs[2];
     uint32_t count = 0;
     if (p->db) jobs[count++] = {in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), static_cast<T *>(p->db), r, 1};
     if (p->da) jobs[count++] = {in.x, in.x_stride, p->in, g, static_cast<T *>(p->da), 1, p->in};
-    return launch_factor_grad<T>(p, jobs, count, order, start, cs);
+    return launch_factor_grad<T>(p, jobs, count, tokens.order, p->index ? reinterpret_cast<const uint32_t *>(work(l.start)) : nullptr, cs);
 }
 
 API int lmz_gpu_ops_gave_up(void)

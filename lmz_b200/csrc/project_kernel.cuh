@@ -3,6 +3,8 @@
 #include "adapter_kernels.cuh"
 #include "tcgen.cuh"
 
+#include <type_traits>
+
 namespace lmz {
 
 constexpr uint32_t P_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
@@ -33,9 +35,11 @@ struct ProjectShared {
 template <class T>
 struct ProjectArgs {
     CUtensorMap x, w;
+    CUtensorMap xs;                            // x in the order of `sorted`
     CUtensorMap h, f;                          // hidden as tokens x 2 x rp, and the factors as adapters x their two sides
     TokenIndex index;
-    const T *hidden;                           // [token][2][rp]: the thin product, its upper and its lower half
+    SortedTokens sorted;
+    const T *hidden;                           // [token][2][rp]: the thin product, its upper and its lower half (in that order if x is)
     const T *factor;                           // of adapter i from i * factor_each; rows of factor_row elements, multiples of 8
     uint64_t factor_each, factor_row;
     T *y;
@@ -172,19 +176,23 @@ __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32
 }
 
 // Two tokens' sums of a lane's feature, to y: where rows allow it two lanes exchange halves, so that a store has two features.
-template <class T>
+template <class T, bool SORTED>
 __device__ __forceinline__ void store_two(const ProjectArgs<T> &a, uint64_t t, uint64_t f, bool pairs, float v0, float v1)
 {
+    auto row = [&](uint64_t t) {
+        if constexpr (SORTED) t = a.sorted.order[t];
+        return a.y + t * a.feats;
+    };
     const uint32_t odd = threadIdx.x & 1;
     if (pairs) {
         const float got = __shfl_xor_sync(~0u, odd ? v0 : v1, 1);
         union { T e[2]; uint32_t raw; } both;
         both.e[0] = narrow<T>(odd ? got : v0);
         both.e[1] = narrow<T>(odd ? v1 : got);
-        if (t + odd < a.tokens && f < a.feats) *reinterpret_cast<uint32_t *>(a.y + (t + odd) * a.feats + (f & ~1ull)) = both.raw;
+        if (t + odd < a.tokens && f < a.feats) *reinterpret_cast<uint32_t *>(row(t + odd) + (f & ~1ull)) = both.raw;
     } else if (f < a.feats) {
-        if (t < a.tokens) a.y[t * a.feats + f] = narrow<T>(v0);
-        if (t + 1 < a.tokens) a.y[(t + 1) * a.feats + f] = narrow<T>(v1);
+        if (t < a.tokens) row(t)[f] = narrow<T>(v0);
+        if (t + 1 < a.tokens) row(t + 1)[f] = narrow<T>(v1);
     }
 }
 
@@ -199,6 +207,7 @@ __device__ __forceinline__ void store_two(const ProjectArgs<T> &a, uint64_t t, u
 // one adapter, tiles of its factor and of either half of h; a warp issues the MMAs; four warps look at the next tile's tokens
 // and work out what has no run (mixed_group); four take the sums out of TMEM, which holds two tiles' sums, so that a tile's way
 // out runs under the next tile's products.
+// Tokens that came scattered are taken in the order of their adapters: x has been copied into it, y's rows are found by it.
 // The weight's first tiles are under way while the kernel that makes h still runs.
 // Few tiles: the CTAs of a cluster share K, and their sums meet in distributed shared memory.
 // Many (PAIR): two CTAs multiply 256 features by 256 tokens together, each loading half of both, so that a step brings
@@ -224,6 +233,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
     uint8_t *const local = p_smem + (ring - smem_addr(p_smem));
     float *const slots = reinterpret_cast<float *>(local + a.stages * a.stage_bytes), *const room = slots + a.slots * (P_SLOT_BYTES / 4);
     volatile uint32_t *over = &s.over;
+    const bool sorted = a.sorted.on();                           // (found before the kernel in front could let this one start)
 
     if (tid == 0) {
         s.over = 0;
@@ -290,7 +300,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                     } else {
                         tma_load_2d<PAIR>(&a.w, bar, dst, k * STEP_K, f);
                     }
-                    tma_load_2d<PAIR>(&a.x, bar, dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
+                    tma_load_2d<PAIR>(sorted ? &a.xs : &a.x, bar, dst + P_FEATS * ROW_BYTES, k * STEP_K, t);
                 }
                 __syncwarp();
             }
@@ -391,6 +401,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         }
     } else if (warp >= 4) {
         const uint32_t id = tid - P_EPILOGUE;
+        const TokenIndex index = a.sorted.index(a.index, sorted);
         auto look = [&](uint32_t tile, uint32_t n) {             // the tile's tokens and their adapters
             uint32_t ft, tt;
             place(tile, ft, tt);
@@ -399,7 +410,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             const uint64_t t0 = static_cast<uint64_t>(tt) * a.nt;
             for (uint32_t c = id; c < P_TOKENS; c += P_FEED) {
                 const bool in = c < a.nt && t0 + c < a.tokens;
-                const int i = in ? a.index.of(t0 + c) : -1;
+                const int i = in ? index.of(t0 + c) : -1;
                 info.adapter[c] = i;
                 const int head = __shfl_sync(~0u, i, lane & 16);
                 const uint32_t agree = __ballot_sync(~0u, !in || i == head);
@@ -486,8 +497,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                     for (uint32_t c = 0; c < P_GROUP; c++)
                         if (t0 + g * P_GROUP + c < a.tokens) sums[(g * P_GROUP + c) * P_FEATS + tid] = v[c];
                 } else {
+                    auto store = [&](auto in_order) {
 #pragma unroll
-                    for (uint32_t c = 0; c < P_GROUP; c += 2) store_two(a, t0 + g * P_GROUP + c, f, pairs, v[c], v[c + 1]);
+                        for (uint32_t c = 0; c < P_GROUP; c += 2) store_two<T, decltype(in_order)::value>(a, t0 + g * P_GROUP + c, f, pairs, v[c], v[c + 1]);
+                    };
+                    if (sorted) store(std::true_type{});
+                    else store(std::false_type{});
                 }
             }
             tc_before();
@@ -513,7 +528,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
 #pragma unroll 2
             for (uint32_t c = rank * share + 2 * (tid / P_FEATS); c < (rank + 1) * share && c < live; c += 4) {
                 const float v0 = peers.sum((c * P_FEATS + feat) * 4), v1 = c + 1 < live ? peers.sum(((c + 1) * P_FEATS + feat) * 4) : 0.0f;
-                store_two(a, t0 + c, f, pairs, v0, v1);
+                if (sorted) store_two<T, true>(a, t0 + c, f, pairs, v0, v1);
+                else store_two<T, false>(a, t0 + c, f, pairs, v0, v1);
             }
         }
         cluster_barrier();

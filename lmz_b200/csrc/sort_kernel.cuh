@@ -17,6 +17,8 @@ struct SortArgs {
     uint64_t nkeys;             // ids outside [0, nkeys) get the key nkeys, and so come last
     uint32_t *keys[2], *pos[2]; // n each: pass p writes to side p & 1
     uint32_t *start;            // NULL, or nkeys + 1: how many keys are below each
+    uint32_t *scattered;        // NULL, or a word: 1 if more than a quarter of the sixteens have several keys; without `start`
+                                // there is no sort for a 0
     uint32_t passes, digit;     // of `digit` bits of the key, lowest first
     bool wide;                  // ids are int64
 };
@@ -53,6 +55,27 @@ static __global__ void __launch_bounds__(SORT_THREADS) k_sort(const SortArgs a)
     const uint64_t run = ((a.n + ctas * SORT_WARPS - 1) / (ctas * SORT_WARPS) + 31) & ~31ull;
     const uint64_t lo = (me * SORT_WARPS + warp) * run, hi = lo + run < a.n ? lo + run : a.n;
     uint32_t *mine = cnt + warp * bins;
+    if (a.scattered) {
+        uint32_t mixed = 0;
+        for (uint64_t i = static_cast<uint64_t>(me) * SORT_THREADS + tid; i - lane < a.n; i += ctas * SORT_THREADS) {
+            const uint32_t k = sort_key(a, i < a.n ? i : a.n - 1), head = __shfl_sync(~0u, k, lane & 16);
+            const uint32_t others = __ballot_sync(~0u, i < a.n && k != head);
+            mixed += ((others & 0xFFFF) != 0) + (others >> 16 != 0);
+        }
+        if (lane == 0) sums[warp] = mixed;
+        __syncthreads();
+        if (tid == 0) {
+            for (uint32_t w = 1; w < SORT_WARPS; w++) mixed += sums[w];
+            tot[0] = mixed;
+        }
+        cluster.sync();
+        mixed = 0;
+        for (uint32_t c = 0; c < ctas; c++) mixed += cluster.map_shared_rank(tot, c)[0];
+        const bool scattered = mixed * 64ull > a.n;
+        cluster.sync();                                         // (nobody reads `tot` any more)
+        if (me == 0 && tid == 0) *a.scattered = scattered;
+        if (!scattered && !a.start) return;
+    }
     for (uint32_t p = 0; p < a.passes; p++) {
         const uint32_t *ks = a.keys[(p + 1) & 1], *ps = a.pos[(p + 1) & 1];
         uint32_t *kd = a.keys[p & 1], *pd = a.pos[p & 1];

@@ -267,6 +267,7 @@ SHAPES = [
     (2600, 64, 2200, 16, 5, "runs"), (2600, 648, 2056, 40, 30, "short"), (4700, 1400, 1288, 8, 3, "runs"), (900, 1032, 5000, 100, 12, "short"),
     (2300, 776, 2200, 16, 40, "mixed"), (200, 2048, 264, 64, 6, "short"),
     (4000, 200, 640, 16, 5, "runs"), (4100, 328, 600, 24, 9, "short"), (2000, 136, 6000, 16, 30, "mixed"), (9000, 256, 1400, 32, 3, "runs"),
+    (1500, 777, 501, 100, 6, "mixed"), (5000, 1032, 1000, 16, 9, "far"), (700, 1100, 1200, 128, 20, "mixed"), (300, 1000, 2000, 256, 2, "mixed"),
     # sizes where rows do not start on a boundary
     (5, 1, 1, 1, 1, "none"), (9, 33, 65, 3, 2, "mixed"), (333, 777, 501, 5, 5, "runs"), (70, 250, 1001, 7, 4, "mixed"), (600, 100, 77, 12, 3, "runs"),
 ]
@@ -539,6 +540,33 @@ def test_on_a_stream_of_its_own_and_captured():
     for out in outs:
         for g, v in zip(out, want):
             assert torch.equal(g, v)
+
+
+def test_captured_for_any_order_of_the_tokens():
+    """One graph for tokens in runs and in any order: which it is shows only on the device."""
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(1500, 392, 400, 128, 6, torch.bfloat16)
+    dy, index = _randn(62, (1500, 400), torch.bfloat16), _index("runs", 1500, 6).long()
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, a, b)]
+        y = adapters.project(*leaves[:1], w, *leaves[1:], index, scale=scales)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for kind in ("mixed", "runs", "far", "off"):
+        index.copy_(_index(kind, 1500, 6, seed=64))
+        for t in out:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, v in zip(out, step()):
+            assert torch.equal(g, v)
+        _check_project(x, w, a, b, scales, index, out[0], dy, out[1:])
 
 
 def test_captured_behind_copies_and_from_other_streams():
