@@ -83,17 +83,30 @@ struct PackArgs {
     PackJob<T> job[5];
 };
 constexpr uint32_t PACK_WARPS = 8, PACK_COLS = 256;
-// A warp 256 columns of a row.  Neighbouring warps take neighbouring rows where those lie closer to each other than a row's
-// elements (a transposed tensor: they read the same lines), else the row's next columns.
+// Where a row's elements are next to each other a thread has eight of them, whatever the row's length.  Else (a transposed tensor)
+// a warp has 256 columns of a row, and neighbouring warps neighbouring rows: they read the same lines.
 template <class T>
 __global__ void __launch_bounds__(32 * PACK_WARPS) k_pack(const __grid_constant__ PackArgs<T> a)
 {
     const PackJob<T> &j = a.job[blockIdx.y];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_for_previous();
+    if (j.sc == 1) {
+        const uint64_t each = j.pitch / 8, all = j.total * each;
+        for (uint64_t u = blockIdx.x * 32ull * PACK_WARPS + threadIdx.x; u < all; u += gridDim.x * 32ull * PACK_WARPS) {
+            const uint64_t row = all >> 32 ? u / each : static_cast<uint32_t>(u) / static_cast<uint32_t>(each), o = j.rows == j.total ? 0 : row / j.rows;
+            const uint64_t c = (u - row * each) * 8;
+            const T *in = j.in + o * j.so + (row - o * j.rows) * j.sr + c;
+            Vec<T, 16> v;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) v.e[e] = c + e < j.cols ? in[e] : narrow<T>(0.0f);
+            *reinterpret_cast<uint4 *>(j.out + u * 8) = v.raw;
+        }
+        return;
+    }
     const uint64_t parts = (j.pitch + PACK_COLS - 1) / PACK_COLS, units = j.total * parts;
     for (uint64_t u = static_cast<uint64_t>(blockIdx.x) * PACK_WARPS + warp; u < units; u += static_cast<uint64_t>(gridDim.x) * PACK_WARPS) {
-        const uint64_t row = j.sc == 1 ? u / parts : u % j.total, part = j.sc == 1 ? u - row * parts : u / j.total, o = row / j.rows;
+        const uint64_t part = u / j.total, row = u - part * j.total, o = row / j.rows;
         const T *in = j.in + o * j.so + (row - o * j.rows) * j.sr;
         T *out = j.out + row * j.pitch;
         T v[PACK_COLS / 32];

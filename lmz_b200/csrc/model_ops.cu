@@ -470,7 +470,7 @@ struct ProjectInputs {
         auto job = [&](const T *&t, uint64_t outer, uint64_t so, uint64_t rows, uint64_t sr, uint64_t cols, uint64_t sc, uint64_t off) {
             T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off);
             args.job[jobs++] = {t, to, so, sr, sc, rows, cols, up8(cols), outer * rows};
-            most = std::max(most, outer * rows * ((up8(cols) + PACK_COLS - 1) / PACK_COLS));
+            most = std::max(most, sc == 1 ? outer * rows * up8(cols) / 256 + 1 : outer * rows * ((up8(cols) + PACK_COLS - 1) / PACK_COLS));    // (warps)
             t = to;
         };
         const uint64_t r = p->rank;
