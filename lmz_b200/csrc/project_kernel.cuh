@@ -65,40 +65,54 @@ __device__ __forceinline__ void mixed_rows(const T *factor, uint64_t factor_each
 {
     constexpr uint32_t FLIGHT = 16, BATCH = FLIGHT / L;          // loads under way
     const uint32_t part = id % L, row = id / L;
+    auto load = [&](int i, Vec<T, 16> *fac) {
+        const T *p = factor + (i < 0 ? 0 : i) * factor_each + part * 8;
+#pragma unroll
+        for (uint32_t m = 0; m < L; m++) {
+            const uint32_t f = row + m * (P_FEATS / L);
+            fac[m].raw = {};
+            if (i >= 0 && f < live && part * 8 < left) fac[m].raw = *reinterpret_cast<const uint4 *>(p + static_cast<uint64_t>(f) * factor_row);
+        }
+    };
+    auto give = [&](uint32_t c, const Vec<T, 16> *fac) {
+        float h[8], v[L];
+        *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(places + c * P_PLACES + part * 8);
+        *reinterpret_cast<float4 *>(h + 4) = *reinterpret_cast<const float4 *>(places + c * P_PLACES + part * 8 + 4);
+#pragma unroll
+        for (uint32_t m = 0; m < L; m++) {
+            v[m] = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) v[m] += h[e] * widen(fac[m].e[e]);
+        }
+#pragma unroll
+        for (uint32_t o = L / 2; o; o /= 2)
+#pragma unroll
+            for (uint32_t m = 0; m < o; m++) {
+                const float other = part & o ? v[m] : v[m + o], own = part & o ? v[m + o] : v[m];
+                v[m] = own + __shfl_xor_sync(~0u, other, o);
+            }
+        float &to = slot[c * P_FEATS + row + part * (P_FEATS / L)];
+        to = add ? to + v[0] : v[0];
+    };
+    uint32_t runs = 1;
+#pragma unroll
+    for (uint32_t c = 1; c < P_GROUP; c++) runs += adapter[c] != adapter[c - 1];
+    if (runs <= L / 2) {                                         // (where an adapter's tokens end: fewer loads to wait for than batches)
+        for (uint32_t c = 0; c < P_GROUP;) {
+            Vec<T, 16> fac[L];
+            const int i = adapter[c];
+            load(i, fac);
+            do give(c++, fac);
+            while (c < P_GROUP && adapter[c] == i);
+        }
+        return;
+    }
     for (uint32_t c0 = 0; c0 < P_GROUP; c0 += BATCH) {
         Vec<T, 16> fac[BATCH][L];
 #pragma unroll
-        for (uint32_t c = 0; c < BATCH; c++) {
-            const int i = adapter[c0 + c];
-            const T *p = factor + (i < 0 ? 0 : i) * factor_each + part * 8;
+        for (uint32_t c = 0; c < BATCH; c++) load(adapter[c0 + c], fac[c]);
 #pragma unroll
-            for (uint32_t m = 0; m < L; m++) {
-                const uint32_t f = row + m * (P_FEATS / L);
-                fac[c][m].raw = {};
-                if (i >= 0 && f < live && part * 8 < left) fac[c][m].raw = *reinterpret_cast<const uint4 *>(p + static_cast<uint64_t>(f) * factor_row);
-            }
-        }
-#pragma unroll
-        for (uint32_t c = 0; c < BATCH; c++) {
-            float h[8], v[L];
-            *reinterpret_cast<float4 *>(h) = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + part * 8);
-            *reinterpret_cast<float4 *>(h + 4) = *reinterpret_cast<const float4 *>(places + (c0 + c) * P_PLACES + part * 8 + 4);
-#pragma unroll
-            for (uint32_t m = 0; m < L; m++) {
-                v[m] = 0;
-#pragma unroll
-                for (uint32_t e = 0; e < 8; e++) v[m] += h[e] * widen(fac[c][m].e[e]);
-            }
-#pragma unroll
-            for (uint32_t o = L / 2; o; o /= 2)
-#pragma unroll
-                for (uint32_t m = 0; m < o; m++) {
-                    const float give = part & o ? v[m] : v[m + o], keep = part & o ? v[m + o] : v[m];
-                    v[m] = keep + __shfl_xor_sync(~0u, give, o);
-                }
-            float &to = slot[(c0 + c) * P_FEATS + row + part * (P_FEATS / L)];
-            to = add ? to + v[0] : v[0];
-        }
+        for (uint32_t c = 0; c < BATCH; c++) give(c0 + c, fac[c]);
     }
 }
 
