@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
         // neighbouring f (either way they read neighbouring banks).
         const bool along_f = g.wide == 1;
         const uint64_t next = along_f ? g.place : g.wide;
-        const bool whole = (reinterpret_cast<uint64_t>(g.out) & 15) == 0 && next % 8 == 0;
+        const uint64_t bits = reinterpret_cast<uint64_t>(g.out) | next * 2;      // stores of 16 bytes, 8, 4, or each by itself
         const uint32_t tasks = along_f ? a.rank * (wide / 8) : (a.rank + 7) / 8 * wide;
         const uint32_t e1 = static_cast<uint32_t>(static_cast<uint64_t>(tasks) * (rank + 1) / a.split);
         for (uint32_t e = static_cast<uint32_t>(static_cast<uint64_t>(tasks) * rank / a.split) + tid; e < e1; e += FG_THREADS) {
@@ -175,8 +175,13 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
             for (uint32_t q = 0; q < 8; q++) v.e[q] = narrow<T>(sum[q]);
             T *to = out + f * g.wide + j * g.place;
             const uint64_t left = along_f ? g.feats - f : a.rank - j;
-            if (whole && left >= 8) {
+            if (left >= 8 && (bits & 15) == 0) {
                 *reinterpret_cast<uint4 *>(to) = v.raw;
+            } else if (left >= 8 && (bits & 7) == 0) {
+                reinterpret_cast<uint2 *>(to)[0] = make_uint2(v.raw.x, v.raw.y), reinterpret_cast<uint2 *>(to)[1] = make_uint2(v.raw.z, v.raw.w);
+            } else if (left >= 8 && (bits & 3) == 0) {
+                uint32_t *words = reinterpret_cast<uint32_t *>(to);
+                words[0] = v.raw.x, words[1] = v.raw.y, words[2] = v.raw.z, words[3] = v.raw.w;
             } else {
 #pragma unroll
                 for (uint32_t q = 0; q < 8; q++)
