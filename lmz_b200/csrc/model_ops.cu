@@ -277,14 +277,15 @@ struct ProjectLayout {
         b = take(pack_b, 2 * p->adapters * (grad ? p->rank * up8(p->out) : p->out * up8(p->rank)));
         dy = take(pack_dy, p->tokens * up8(p->out) * 2);
         g = take(grad, p->tokens * 4 * up8(p->rank));
-        sorts = p->index && p->adapters > 1 && (!grad || p->dx) && worth_sorting(p, grad ? p->in : p->out, up8(p->rank));
-        const bool sorted = (grad && p->index) || sorts;
+        const bool may_sort = p->index && p->adapters > 1 && worth_sorting(p, grad ? p->in : p->out, up8(p->rank));
+        sorts = may_sort && (!grad || p->dx);                    // (the workspace is the same whichever gradients are wanted)
+        const bool sorted = (grad && p->index) || may_sort;
         for (int i = 0; i < 2; i++) keys[i] = take(sorted, p->tokens * 4), pos[i] = take(sorted, p->tokens * 4);
         start = take(grad && p->index, (p->adapters + 1ull) * 4);
         hidden = take(!grad && !p->hidden, p->tokens * 4 * up8(p->rank));
-        scattered = take(sorts, 4);
-        in_order = take(sorts, p->tokens * up8(grad ? p->out : p->in) * 2);
-        thin = take(sorts && (grad || p->hidden), p->tokens * 4 * up8(p->rank));
+        scattered = take(may_sort, 4);
+        in_order = take(may_sort, p->tokens * up8(grad ? p->out : p->in) * 2);
+        thin = take(may_sort && (grad || p->hidden), p->tokens * 4 * up8(p->rank));
     }
 };
 

@@ -427,6 +427,26 @@ def test_only_the_gradients_asked_for():
         assert torch.equal(g, full[k])
 
 
+def test_only_the_gradients_asked_for_of_tokens_in_any_order():
+    """(How many CTAs share a factor's tokens, and so the order of its sums in 32 bits, goes by how many factors are wanted:
+    within the bounds of the definition, not bit for bit.)"""
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(1500, 392, 400, 128, 5, torch.bfloat16)
+    index, dy = _index("mixed", 1500, 5), _randn(43, (1500, 400), torch.bfloat16)
+
+    def grads(which):
+        leaves = [t.detach().requires_grad_(i in which) for i, t in enumerate((x, a, b))]
+        y = adapters.project(leaves[0], w, leaves[1], leaves[2], index, scale=scales)
+        return y.detach(), torch.autograd.grad(y, [leaves[i] for i in which], dy)
+
+    y, every = grads((0, 1, 2))
+    for which in ((0,), (1,), (2,), (0, 1), (1, 2)):
+        got = list(every)
+        for i, g in zip(which, grads(which)[1]):
+            got[i] = g
+        _check_project(x, w, a, b, scales, index, y, dy, got)
+
+
 def test_no_tokens():
     from lmz_b200 import adapters
     x, w, a, b, scales = _inputs(0, 64, 96, 8, 3, torch.bfloat16)

@@ -71,6 +71,18 @@ def test_merges_the_library_refuses(lib, out, inp, rank, dtype):
     assert lib.lmz_gpu_merge_dev(None, out, inp, inp, None, None, rank, 1.0, dtype, None, None) == -2
 
 
+@pytest.mark.parametrize("index", [None, 64])
+@pytest.mark.parametrize("tokens", [4, 5000])
+def test_workspaces_do_not_depend_on_the_gradients_wanted(lib, index, tokens):
+    p = _projection(tokens=tokens, in_=1024, out=1024, x_stride=1024, weight_stride=1024, adapters=7, index=index, index_bytes=4, rank=16)
+    size = lib.lmz_gpu_project_work_bytes(p, 1)
+    for name in ("dx", "da", "db"):
+        p.dx = p.da = p.db = None
+        setattr(p, name, 4096)
+        assert lib.lmz_gpu_project_work_bytes(p, 1) == size
+    assert lib.lmz_gpu_project_work_bytes(p, 0) >= 4 * tokens * 16      # (the thin product)
+
+
 def test_nothing_to_do_needs_no_gpu(lib):
     assert lib.lmz_gpu_rows_dev(None, 10, 8, 8, 0, None, 4, 0, 1.0, None, None) == 0
     assert lib.lmz_gpu_project_dev(_projection(tokens=0), None) == 0
