@@ -1,6 +1,7 @@
 // The projection through a shared weight with low-rank adapters beside it, and by the same kernel the gradient of its input.
 #pragma once
 #include "adapter_kernels.cuh"
+#include "slot_ring.cuh"
 #include "tcgen.cuh"
 
 #include <type_traits>
@@ -464,12 +465,14 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             uint32_t order = 0;
             for (uint32_t g = 0; go && g * P_GROUP < a.nt; g++) {
                 if (!mixed(info, g)) continue;
-                go = sync_all(1, P_FEED, !slot.turn || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
-                if (!go) break;
-                if (PAIR || !(order++ & 1)) {
+                if (slot_by_feed(PAIR, order)) {
+                    const bool waits = slot_feed_waits(PAIR, order, slot.turn);
+                    go = sync_all(1, P_FEED, !waits || id || bar_wait(&s.slot_empty[slot.stage], (slot.turn - 1) & 1, over));
+                    if (!go) break;
                     mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, f0, id, 1, room, slots + slot.stage * (P_SLOT_BYTES / 4));
                     if (id == 0) bar_arrive(&s.slot_full[slot.stage]);
                 }
+                order++;
                 slot.next(a.slots);
             }
         }
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 uint32_t order = 0;
                 for (uint32_t g = 0; g * P_GROUP < a.nt; g++) {
                     if (!mixed(info, g)) continue;
-                    if (order++ & 1) {
+                    if (!slot_by_feed(PAIR, order++)) {
                         mixed_group<T, MN>(a, info.adapter + g * P_GROUP, t0 + g * P_GROUP, features(ft), tid, 2, room + P_GROUP * P_PLACES,
                                            slots + at.stage * (P_SLOT_BYTES / 4));
                         if (tid == 0) bar_arrive(&s.slot_full[at.stage]);

@@ -1,0 +1,23 @@
+"""Rules of the operators' kernels that are plain arithmetic, checked on the CPU."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def _compiled(tmp_path_factory, name):
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    exe = str(tmp_path_factory.mktemp("native") / name)
+    subprocess.run([cxx, "-std=c++17", "-O1", "-g", "-o", exe, os.path.join(HERE, "native", name + ".cc")], check=True)
+    return exe
+
+
+def test_slots_between_a_projections_warps(tmp_path_factory):
+    """Under every schedule the warps that fill slots and those that empty them get to their end."""
+    done = subprocess.run([_compiled(tmp_path_factory, "slot_ring_check")], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
