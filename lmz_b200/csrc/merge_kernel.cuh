@@ -1,12 +1,12 @@
 // An adapter merged into its weight.
 #pragma once
 #include "adapter_kernels.cuh"
+#include "merge_layout.cuh"
 #include "tcgen.cuh"
 
 namespace lmz {
 
-constexpr uint32_t M_ROWS = 128, M_COLS = 128, M_THREADS = 256;
-constexpr uint32_t M_BLOCK = M_ROWS * ROW_BYTES;       // 64 columns of the weight's tile, swizzled as operands are
+constexpr uint32_t M_THREADS = 256;
 
 template <class T>
 struct MergeArgs {
@@ -18,17 +18,11 @@ struct MergeArgs {
     bool a_even, b_even;                       // the factors' rows start on boundaries of 16 bytes
 };
 
-// Shared memory of a block: stages of the weight's and A's tiles, one of B's, and what the block's threads share.
 struct MergeShared {
     uint64_t done;
     uint32_t tmem, over;
 };
-__host__ __device__ constexpr uint32_t merge_stage(uint32_t places) { return M_COLS / 64 * (M_BLOCK + places * ROW_BYTES); }
-__host__ __device__ constexpr uint32_t merge_stages(uint32_t places) { return places <= 192 ? 2 : 1; }      // (as many as have room)
-__host__ __device__ constexpr uint32_t merge_smem(uint32_t places)
-{
-    return merge_stages(places) * merge_stage(places) + (places + STEP_K - 1) / STEP_K * M_BLOCK + sizeof(MergeShared);
-}
+static_assert(sizeof(MergeShared) == M_SHARED && M_ROW_BYTES == ROW_BYTES);
 
 // W' = W + s B A, in tiles of 128 x 128, a row of them after the other; a block has a run of tiles.
 //

@@ -16,6 +16,8 @@
 
 using namespace lmz;
 
+static_assert(M_MAX_PLACES == LMZ_GPU_MAX_RANK);
+
 #define API extern "C" __attribute__((visibility("default")))
 
 #include "host_error.inl"
@@ -604,7 +606,7 @@ static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, c
     return by_width<T>(vector_bytes(in * 2, {address(w), address(to), stride * 2}), [&](auto vec) {
         constexpr int VB = sizeof(vec.raw);
         static bool done[64];
-        const int rc = opt_in_smem(k_merge<T, VB>, merge_smem(256), done);
+        const int rc = opt_in_smem(k_merge<T, VB>, merge_smem_most(), done);
         if (rc) return rc;
         int sms = 0;
         const int failed = sm_count(&sms);

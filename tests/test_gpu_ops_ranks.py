@@ -1,0 +1,26 @@
+"""Operators with adapters at the ranks where their kernels change layout, against the definition in 64 bits (bounds as in
+test_gpu_ops)."""
+import pytest
+import torch
+
+from test_gpu_ops import DTYPES, _check, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _library(gpu):
+    return gpu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("out, inp", [(264, 520), (130, 251)])
+@pytest.mark.parametrize("rank", [127, 128, 129, 136, 144, 145, 160, 161, 176, 191, 192, 193, 208, 209, 224, 240, 255, 256])
+def test_merge_of_every_layout(dtype, out, inp, rank):
+    from lmz_b200 import adapters
+    w, a, b = _randn(50, (out, inp), dtype), _randn(51, (rank, inp), dtype, inp ** -0.5), _randn(52, (out, rank), dtype)
+    want = w.double() + 0.5 * (b.double() @ a.double())
+    size = w.double().abs() + 0.5 * (b.double().abs() @ a.double().abs())
+    got = adapters.merge(w, a, b, scale=0.5)
+    _check(got, want, size, torch.zeros_like(want), rank + 4, "merge")
+    assert adapters.merge(w, a, b, scale=0.5, out=w) is w and torch.equal(w, got)

@@ -21,3 +21,9 @@ def test_slots_between_a_projections_warps(tmp_path_factory):
     """Under every schedule the warps that fill slots and those that empty them get to their end."""
     done = subprocess.run([_compiled(tmp_path_factory, "slot_ring_check")], capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr
+
+
+def test_a_merges_shared_memory(tmp_path_factory):
+    """No rank takes more than the kernel is given leave for."""
+    done = subprocess.run([_compiled(tmp_path_factory, "merge_layout_check")], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stderr
