@@ -3,7 +3,7 @@ test_gpu_ops)."""
 import pytest
 import torch
 
-from test_gpu_ops import DTYPES, _check, _randn
+from test_gpu_ops import DTYPES, _check, _check_project, _index, _inputs, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,16 @@ def test_merge_of_every_layout(dtype, out, inp, rank):
     got = adapters.merge(w, a, b, scale=0.5)
     _check(got, want, size, torch.zeros_like(want), rank + 4, "merge")
     assert adapters.merge(w, a, b, scale=0.5, out=w) is w and torch.equal(w, got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, inp, out, n, kind", [(1, 264, 520, 1, "none"), (90, 264, 392, 3, "mixed"), (700, 200, 320, 2, "runs"), (500, 136, 1288, 1, "none"),
+                                                       (333, 131, 203, 4, "runs"), (1800, 264, 2056, 5, "mixed")])
+@pytest.mark.parametrize("rank", [120, 129, 136, 144, 160, 192, 200, 247, 255])
+def test_project_and_its_gradients_of_every_layout(dtype, tokens, inp, out, n, kind, rank):
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(tokens, inp, out, rank, n, dtype)
+    index, dy = _index(kind, tokens, n), _randn(40, (tokens, out), dtype)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = adapters.project(x, w, a, b, index, scale=scales)
+    _check_project(x, w, a, b, scales, index, y.detach(), dy, torch.autograd.grad(y, leaves, dy))
