@@ -54,7 +54,8 @@ def type_code(t, what: str, half_only: bool = False) -> int:
 
 def on_cuda(names: str, *tensors) -> int:
     """The index of the CUDA device that all given tensors are on (None for one that is not given), or an error that names
-    who is not.  `names`: the tensors', by spaces."""
+    who is not.  `names`: the tensors', by spaces.  Tensors with a forward-mode tangent are refused."""
+    no_tangents(names, *tensors)
     device = None
     for t in tensors:
         if t is None:
@@ -68,6 +69,23 @@ def on_cuda(names: str, *tensors) -> int:
         if d < 0 or d != device:
             _refuse_place(names.split(), tensors)
     return device
+
+
+_forward_mode = None
+
+
+def no_tangents(names: str, *tensors) -> None:
+    """The operators have gradients, but no forward-mode derivatives: a tangent would be lost without a word."""
+    global _forward_mode
+    if _forward_mode is None:
+        from torch.autograd import forward_ad
+        _forward_mode = forward_ad
+    if _forward_mode._current_level < 0:                   # (nobody has made a dual tensor)
+        return
+    import torch
+    for name, t in zip(names.split(), tensors):
+        if isinstance(t, torch.Tensor) and _forward_mode.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has a tangent: this operator has no forward-mode derivative")
 
 
 def _refuse_place(names, tensors):

@@ -104,6 +104,7 @@ def _forward(code, x, weight, a, b, index, scales, scale, keep):
 
 
 def _backward(code, dy, x, weight, a, b, index, scales, scale, hidden, wanted):
+    _ops.no_tangents("dy", dy)
     dx, da, db = (t.new_empty(t.shape) if w else None for t, w in zip((x, a, b), wanted))
     x, dy = _flat(x), dy.reshape(-1, dy.shape[-1]).contiguous()
     a, b, index, scales = _packed(a), _packed(b), _packed(index), _packed(scales)      # (copies live until the launch)

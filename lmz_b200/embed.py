@@ -45,6 +45,7 @@ def _rows(index, code, id_bytes, table, tokens, scale):
 
 def _rows_grad(dy, tokens, rows: int, scale):
     import torch
+    _ops.no_tangents("dy", dy)
     dim = dy.shape[-1]
     grad = dy.new_empty((rows, dim))
     if grad.numel():

@@ -1,0 +1,30 @@
+"""Calls of the operators that their documentation allows, or that they have to refuse, beside the sizes of test_gpu_ops."""
+import pytest
+import torch
+
+from test_gpu_ops import _inputs, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _library(gpu):
+    return gpu
+
+
+def test_tangents_are_refused_beside_a_scale_and_in_a_gradient():
+    from torch.autograd import forward_ad
+
+    from lmz_b200 import adapters, embed
+    x, w, a, b, scales = _inputs(6, 64, 96, 8, 3, torch.bfloat16)
+    index, dy = torch.zeros(6, dtype=torch.int32, device="cuda"), _randn(1, (6, 96), torch.bfloat16)
+    table, ids = _randn(2, (5, 8), torch.float32).requires_grad_(True), torch.zeros(3, dtype=torch.int64, device="cuda")
+    y, e = adapters.project(x.requires_grad_(True), w, a, b, index, scale=scales), embed.lookup(table, ids)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="tangent"):
+            adapters.project(x, w, a, b, index, scale=forward_ad.make_dual(scales, torch.ones_like(scales)))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(dy, dy.clone()))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            torch.autograd.grad(e, table, forward_ad.make_dual(e.detach(), e.detach().clone()))
+        assert adapters.project(x, w, a, b, index, scale=scales).shape == (6, 96)
