@@ -674,7 +674,7 @@ def decode_rows(ar, name, rows, scale: float = 1.0, device=None, checksum: bool 
     except RuntimeError:                                   # not on a boundary of its elements
         table = raw.clone().view(dtype)
     with torch.cuda.device(dev):
-        return embed.lookup(table.view(-1, dim), torch.from_numpy(ids.astype(np.int64) - base).to(dev), scale=scale)
+        return embed.lookup(table.view(-1, dim), torch.from_numpy(np.asarray(ids.astype(np.int64) - base)).to(dev), scale=scale)
 
 
 def _decode_ranges(ar, ranges, device, checksum):

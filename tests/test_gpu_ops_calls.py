@@ -1,8 +1,9 @@
 """Calls of the operators that their documentation allows, or that they have to refuse, beside the sizes of test_gpu_ops."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_ops import _inputs, _randn
+from test_gpu_ops import _archive, _inputs, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +29,16 @@ def test_tangents_are_refused_beside_a_scale_and_in_a_gradient():
         with pytest.raises(NotImplementedError, match="tangent"):
             torch.autograd.grad(e, table, forward_ad.make_dual(e.detach(), e.detach().clone()))
         assert adapters.project(x, w, a, b, index, scale=scales).shape == (6, 96)
+
+
+def test_one_row_of_an_archive_by_its_number():
+    """Row numbers of any shape: of none, too."""
+    from lmz_b200 import archive, decode
+    table = _randn(71, (900, 250), torch.bfloat16, 0.02)
+    ar = archive.Archive(_archive({"norm": _randn(70, (33,), torch.bfloat16), "emb": table}, mapped=True))
+    for row in (7, np.int64(7), np.array(7, dtype=np.uint8), torch.tensor(7)):
+        got = decode.decode_rows(ar, "emb", row)
+        assert got.shape == (250,) and torch.equal(got, table[7])
+    assert decode.decode_rows(ar, "emb", torch.tensor([[899], [0]])).shape == (2, 1, 250)
+    with pytest.raises(IndexError):
+        decode.decode_rows(ar, "emb", 900)
