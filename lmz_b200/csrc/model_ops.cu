@@ -194,7 +194,8 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
         a.rows = static_cast<uint32_t>(rows), a.row_bytes = bytes, a.dim = dim, a.n = static_cast<uint32_t>(n), a.window = rows_window(n), a.scale = scale;
         a.vectors = static_cast<uint32_t>(bytes / VB), a.lane_log = std::max(5u, lanes_log(a.vectors));
         const uint32_t slices = (a.vectors + ROW_THREADS - 1) / ROW_THREADS, per = ROW_THREADS >> a.lane_log;
-        const dim3 grid(((a.n + a.window - 1) / a.window + per - 1) / per, slices);
+        // (a row of 2^24 elements less one, two bytes at a time, is 65536 slices: one more than a grid has along y)
+        const dim3 grid(((a.n + a.window - 1) / a.window + per - 1) / per, std::min(slices, 32768u), (slices + 32767) / 32768);
         int failed = launch("launch k_rows_sums", k_rows_sums<T, VB>, grid, ROW_THREADS, 0, cs, a);
         if (!failed && a.n > a.window) failed = launch("launch k_rows_join", k_rows_join<T, VB>, grid, ROW_THREADS, 0, cs, a);
         return failed;

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_rows_sums(const RowsGradArgs a)
     __shared__ uint32_t s_key[ROW_THREADS / 32][ROWS_STEP + 1], s_pos[ROW_THREADS / 32][ROWS_STEP];
     const uint32_t threads = 1u << a.lane_log, lane = threadIdx.x & (threads - 1), sub = threadIdx.x >> a.lane_log;
     const uint64_t w = static_cast<uint64_t>(blockIdx.x) * (ROW_THREADS >> a.lane_log) + sub;
-    const uint32_t v = blockIdx.y * ROW_THREADS + lane;
+    const uint32_t v = (blockIdx.z * gridDim.y + blockIdx.y) * ROW_THREADS + lane;
     const uint64_t w0 = w * a.window, w1 = w0 + a.window < a.n ? w0 + a.window : a.n;
     let_next_start();
     wait_for_previous();
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_rows_join(const RowsGradArgs a)
     constexpr int N = V::N, AHEAD = 8;
     const uint32_t threads = 1u << a.lane_log, lane = threadIdx.x & (threads - 1), sub = threadIdx.x >> a.lane_log;
     const uint64_t w = static_cast<uint64_t>(blockIdx.x) * (ROW_THREADS >> a.lane_log) + sub;
-    const uint32_t v = blockIdx.y * ROW_THREADS + lane;
+    const uint32_t v = (blockIdx.z * gridDim.y + blockIdx.y) * ROW_THREADS + lane;
     const uint64_t w0 = w * a.window, w1 = w0 + a.window;
     wait_for_previous();
     if (v >= a.vectors || w1 >= a.n) return;

@@ -42,3 +42,21 @@ def test_one_row_of_an_archive_by_its_number():
     assert decode.decode_rows(ar, "emb", torch.tensor([[899], [0]])).shape == (2, 1, 250)
     with pytest.raises(IndexError):
         decode.decode_rows(ar, "emb", 900)
+
+
+@pytest.mark.parametrize("n", [3, 33])
+def test_rows_gradient_of_the_widest_rows(n):
+    """2^24 - 1 elements of 16 bits, which move one at a time: more slices of a row than a grid has along y."""
+    from lmz_b200 import embed
+    dim = (1 << 24) - 1
+    table = torch.zeros((2, dim), dtype=torch.float16, device="cuda").requires_grad_(True)
+    ids = torch.ones(n, dtype=torch.int64, device="cuda")
+    ids[1] = 0
+    dy = torch.randint(-8, 9, (n, dim), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda", dtype=torch.int8).to(torch.float16)
+    (got,) = torch.autograd.grad(embed.lookup(table, ids), table, dy)
+    assert torch.equal(got[0], dy[1])
+    want = torch.zeros(dim, device="cuda")                 # (whole numbers up to 33 * 8: exact in F16 too)
+    for t in range(n):
+        if t != 1:
+            want += dy[t]
+    assert torch.equal(got[1].float(), want)
