@@ -163,9 +163,10 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
     if not 1 <= a.shape[0] <= MAX_RANK:
         raise ValueError(f"a rank outside 1..{MAX_RANK}")
     scale = _ops.finite(scale)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (weight, a, b)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, a, b, out)):
         raise ValueError("merge has no gradient: call it under torch.no_grad()")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
     elif out.shape != weight.shape or out.dtype != weight.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of the weight's shape and type")
@@ -175,6 +176,8 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
         a, b = _packed(a), _packed(b)
         _ops.launch(index, "lmz_gpu_merge_dev", weight.data_ptr(), weight.shape[0], weight.shape[1], weight.stride(0), a.data_ptr(), b.data_ptr(),
                     a.shape[0], scale, code, out.data_ptr())
+        if given:                                          # (autograd notices where what was there is still needed)
+            torch.autograd.graph.increment_version(out)
     return out
 
 

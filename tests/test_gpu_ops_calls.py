@@ -60,3 +60,25 @@ def test_rows_gradient_of_the_widest_rows(n):
         if t != 1:
             want += dy[t]
     assert torch.equal(got[1].float(), want)
+
+
+def test_a_merge_in_place_is_noticed():
+    """As any operator of torch that writes to a tensor which a gradient still needs; and a leaf is not written to."""
+    from lmz_b200 import adapters
+    w, a, b = _randn(50, (16, 24), torch.bfloat16), _randn(51, (4, 24), torch.bfloat16), _randn(52, (16, 4), torch.bfloat16)
+    v = torch.ones_like(w).requires_grad_(True)
+    y = (v * w).sum()
+    adapters.merge(w, a, b, out=torch.empty_like(w))       # (leaves w alone)
+    (g,) = torch.autograd.grad(y, v, retain_graph=True)
+    assert torch.equal(g, w)
+    adapters.merge(w, a, b, out=w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    leaf = torch.empty_like(w).requires_grad_(True)
+    with pytest.raises(ValueError, match="gradient"):
+        adapters.merge(w, a, b, out=leaf)
+    with torch.no_grad():
+        assert adapters.merge(w, a, b, out=leaf) is leaf
+    with torch.inference_mode():
+        out = torch.empty_like(w)
+        assert torch.equal(adapters.merge(w, a, b, out=out), leaf)
