@@ -396,8 +396,9 @@ int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream);
  * the tokens of adapter i (zeros for an adapter without any). */
 int lmz_gpu_project_grad_dev(const lmz_projection *p, void *cuda_stream);
 
-/* Every wait inside the kernels above has a limit.  1 if one has run out on the current device since the library was
- * loaded (the results of that launch are not to be used), 0 if none has, negative on failure; waits for the device. */
+/* Every wait inside the kernels above has a limit, after which the launch ends without its results.  1 if one has run out on
+ * the current device since this was last asked (what has been computed there since then is not to be used), 0 if none has,
+ * negative on failure; waits for the device, all its streams. */
 int lmz_gpu_ops_gave_up(void);
 
 /* out = W + scale * B A for an out x in weight (rows weight_stride elements apart), BF16 or F16; d_out is contiguous, and

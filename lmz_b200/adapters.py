@@ -182,8 +182,9 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
 
 
 def check(device=None) -> None:
-    """Synchronise, and raise if a kernel has given up waiting for one of its own copies on this device (every wait in
-    them has a limit; none runs out unless the hardware fails)."""
+    """Synchronise the device, and raise if a kernel has given up waiting for one of its own copies there since the last
+    check (every wait in them has a limit; none runs out unless the hardware fails).  What was computed since then is not to
+    be used; calls after it are not touched by it."""
     import torch
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         rc = gpu.library().lmz_gpu_ops_gave_up()

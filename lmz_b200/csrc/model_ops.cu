@@ -22,6 +22,7 @@ static_assert(M_MAX_PLACES == LMZ_GPU_MAX_RANK);
 
 #include "host_error.inl"
 #include "host_device.inl"
+#include "host_gave_up.inl"
 
 static uint32_t element_bytes(int dtype) { return dtype == LMZ_GPU_F32 ? 4 : dtype == LMZ_GPU_BF16 || dtype == LMZ_GPU_F16 ? 2 : 0; }
 
@@ -571,9 +572,11 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
 
 API int lmz_gpu_ops_gave_up(void)
 {
-    uint32_t word = 0;
-    CK("cudaMemcpyFromSymbol", cudaMemcpyFromSymbol(&word, g_gave_up, sizeof word));
-    return word != 0;
+    const int rc = device_ready();
+    if (rc) return rc;
+    void *word = nullptr;
+    CK("cudaGetSymbolAddress", cudaGetSymbolAddress(&word, g_gave_up));
+    return taken_word(word);
 }
 
 API int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream)

@@ -628,11 +628,14 @@ def _merge_adapter(tensors, adapter, scale):
     """Put merged weights in the place of the tensors that an adapter archive has factors for."""
     from . import adapters
     adapter = adapter if isinstance(adapter, fmt.Archive) else fmt.Archive(adapter)
+    merged = None
     for key, weight in tensors.items():
         pair = adapters._factors(adapter, key[1], weight.device)
         if pair is not None:
             a, b = (t.to(weight.dtype) for t in pair)
-            tensors[key] = adapters.merge(weight, a, b, scale=scale)
+            tensors[key] = merged = adapters.merge(weight, a, b, scale=scale)
+    if merged is not None:
+        adapters.check(merged.device)                      # (as the decoded tensors have been)
 
 
 def decode_rows(ar, name, rows, scale: float = 1.0, device=None, checksum: bool = True):

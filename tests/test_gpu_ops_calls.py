@@ -82,3 +82,16 @@ def test_a_merge_in_place_is_noticed():
     with torch.inference_mode():
         out = torch.empty_like(w)
         assert torch.equal(adapters.merge(w, a, b, out=out), leaf)
+
+
+def test_merged_tensors_are_checked(monkeypatch):
+    from lmz_b200 import adapters, archive, decode, gpu
+    w, a, b = _randn(50, (32, 64), torch.bfloat16), _randn(51, (4, 64), torch.bfloat16), _randn(52, (32, 4), torch.bfloat16)
+    ar, tuned = archive.Archive(_archive({"p.weight": w})), archive.Archive(_archive({"p.lora_A.weight": a, "p.lora_B.weight": b}))
+    (got,) = decode.decode_tensors(ar, ["p.weight"], adapter=tuned).values()
+    assert torch.equal(got, adapters.merge(w, a, b))
+    monkeypatch.setattr(gpu.library(), "lmz_gpu_ops_gave_up", lambda: 1)      # a merge whose wait has run out
+    with pytest.raises(RuntimeError, match="gave up"):
+        decode.decode_tensors(ar, ["p.weight"], adapter=tuned)
+    (plain,) = decode.decode_tensors(ar, ["p.weight"]).values()
+    assert torch.equal(plain, w)

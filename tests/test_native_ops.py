@@ -13,7 +13,7 @@ def _compiled(tmp_path_factory, name):
     if cxx is None:
         pytest.skip("no C++ compiler")
     exe = str(tmp_path_factory.mktemp("native") / name)
-    subprocess.run([cxx, "-std=c++17", "-O1", "-g", "-o", exe, os.path.join(HERE, "native", name + ".cc")], check=True)
+    subprocess.run([cxx, "-std=c++17", "-O1", "-g", "-I", os.path.join(HERE, "native"), "-o", exe, os.path.join(HERE, "native", name + ".cc")], check=True)
     return exe
 
 
@@ -26,4 +26,10 @@ def test_slots_between_a_projections_warps(tmp_path_factory):
 def test_a_merges_shared_memory(tmp_path_factory):
     """No rank takes more than the kernel is given leave for."""
     done = subprocess.run([_compiled(tmp_path_factory, "merge_layout_check")], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stderr
+
+
+def test_a_wait_that_ran_out_is_told_once(tmp_path_factory):
+    """Whichever stream it was on, and to the check that follows it alone."""
+    done = subprocess.run([_compiled(tmp_path_factory, "gave_up_check")], capture_output=True, text=True, timeout=60)
     assert done.returncode == 0, done.stderr
