@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     const FactorGradJob<T> &g = a.job[which];
     const uint32_t f0 = (which ? place - a.job[0].clusters : place) * a.blocks * FG_FEATS, i = blockIdx.y;
     wait_for_previous();
-    const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : a.tokens;
+    const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : i ? 0 : a.tokens;
     const uint32_t all = (end - begin + STEP_K - 1) / STEP_K;
     const uint32_t n0 = static_cast<uint32_t>(static_cast<uint64_t>(all) * rank / a.split), n1 = static_cast<uint32_t>(static_cast<uint64_t>(all) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(f_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);

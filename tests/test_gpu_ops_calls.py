@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_ops import _archive, _inputs, _randn
+from test_gpu_ops import _archive, _check_project, _inputs, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,19 @@ def test_merged_tensors_are_checked(monkeypatch):
         decode.decode_tensors(ar, ["p.weight"], adapter=tuned)
     (plain,) = decode.decode_tensors(ar, ["p.weight"]).values()
     assert torch.equal(plain, w)
+
+
+@pytest.mark.parametrize("tokens", [1, 64, 700])
+@pytest.mark.parametrize("n", [2, 5])
+def test_without_an_index_only_the_first_adapter_has_gradients(tokens, n):
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(tokens, 64, 136, 8, n, torch.bfloat16)
+    dy = _randn(40, (tokens, 136), torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = adapters.project(x, w, a, b, scale=scales)
+    grads = torch.autograd.grad(y, leaves, dy)
+    _check_project(x, w, a, b, scales, None, y.detach(), dy, grads)
+    zeros = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    for g, h in zip(grads, torch.autograd.grad(adapters.project(x, w, a, b, zeros, scale=scales), leaves, dy)):
+        assert torch.equal(g, h)
+    assert (grads[1][1:] == 0).all() and (grads[2][1:] == 0).all()
