@@ -25,13 +25,29 @@ struct TokenIndex {
     __device__ __forceinline__ float scale_of(int i) const { return scales ? scale * scales[i] : scale; }
 };
 
-// Thin products are kept as two halves of 16 bits, [token][2][rp] with rp the rank up to a multiple of 8: a value to the
-// nearest T, and what that lacks.  One T alone would cost as much as the result's own rounding.
+// Thin products are kept as two halves of 16 bits, [token][2][rp] with rp the rank up to a multiple of 8: a value cut to T, and
+// what that lacks.  One T alone would cost as much as the result's own rounding.
+//
+// The upper half is always short of the value (of one that T holds, too: then by T's last place), so that both halves of a value
+// other than zero are other than zero and have its sign.  Both are multiplied by the same factor, and infinity times them
+// has to be the infinity that the value would give: a lower half of zero, or of the other sign, makes NaN of it.
+template <class T>
+__device__ __forceinline__ T shorter(float v)
+{
+    if constexpr (__is_same(T, __nv_bfloat16)) {
+        const uint32_t u = __float_as_uint(v);
+        return __ushort_as_bfloat16(static_cast<uint16_t>((u & 0x7FFFFFFF ? u - 1 : u) >> 16));
+    } else {
+        const T hi = __float2half_rz(v);
+        const uint16_t bits = __half_as_ushort(hi);
+        return widen(hi) == v && (bits & 0x7FFF) ? __ushort_as_half(static_cast<uint16_t>(bits - 1)) : hi;
+    }
+}
 template <class T>
 __device__ __forceinline__ void split_halves(float v, T &hi, T &lo)
 {
-    hi = narrow<T>(v);
-    lo = narrow<T>(isfinite(widen(hi)) ? v - widen(hi) : 0.0f);
+    hi = isfinite(v) ? shorter<T>(v) : narrow<T>(v);
+    lo = narrow<T>(isfinite(v) ? v - widen(hi) : v);
 }
 
 // Tokens in the order of their adapters, if they came scattered: what the projection's kernels then read in place of x.

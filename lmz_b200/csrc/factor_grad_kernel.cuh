@@ -41,7 +41,7 @@ __host__ __device__ constexpr uint32_t factor_stage_bytes(uint32_t blocks, uint3
 // Tokens are the tensor core's K, and come in the order of a sort by adapter, so that a sum has its own tokens and no others
 // (a foreign token times zero would still bring its infinities in), in one order.  Rows are brought as they lie, both
 // operands MN-major: 64 neighbours by a tile's copy, others by gathers of four rows, whose places behind the last token read
-// as zeros.  The halves of the thin rows are columns of their own, added at the end.  Bound by reading z (256 features a block,
+// as zeros.  The halves of the thin rows are columns of their own, added at the end; an infinity or NaN is the upper halves' alone.  Bound by reading z (256 features a block,
 // so that the thin rows are read half as often as by 128); the CTAs of a cluster share an adapter's tokens.  One B200, 8192 tokens
 // of 4096 and 14336 features at rank 64: both factors 79 us (3.9 TB/s of HBM).
 // The two factors' gradients are one launch: its first clusters make the one, the others the other.
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
                     tmem_load8(tmem + (warp << 21) + b * 2 * a.rp + a.rp + c, w);
                 }
 #pragma unroll
-                for (uint32_t e = 0; e < 8; e++) part[(b * a.rp + c + e) * FG_PITCH + tid] = v[e] + w[e];
+                for (uint32_t e = 0; e < 8; e++) part[(b * a.rp + c + e) * FG_PITCH + tid] = isfinite(v[e]) ? v[e] + w[e] : v[e];
             }
     }
     tc_before();
