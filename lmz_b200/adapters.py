@@ -20,7 +20,8 @@ def project(x, weight, a, b, index=None, scale=1.0):
     index all tokens have adapter 0.  `scale`: a number, or a float32 tensor of one per adapter (alpha / rank).  Adapters of
     lower rank are padded with zeros.  Ranks go up to 256.  Tokens of one adapter next to each other are fastest.
 
-    Returns [..., out], summed in 32 bits and rounded once.  An adapter's values, infinities and NaN among them, reach only
+    Returns [..., out], summed in 32 bits and rounded once; what comes of a_i goes to b_i with 16 bits or more (an error of 2^-16
+    of its magnitude), over float32's range whatever the tensors' type.  An adapter's values, infinities and NaN among them, reach only
     its own tokens.  Differentiable once in x, a and b; gradients of a and b sum over each adapter's tokens, with zeros for
     an adapter that none has, and are the same in every run."""
     import torch

@@ -25,29 +25,21 @@ struct TokenIndex {
     __device__ __forceinline__ float scale_of(int i) const { return scales ? scale * scales[i] : scale; }
 };
 
-// Thin products are kept as two halves of 16 bits, [token][2][rp] with rp the rank up to a multiple of 8: a value cut to T, and
-// what that lacks.  One T alone would cost as much as the result's own rounding.
+// Thin products go into the second product as two halves, [token][2][rp] with rp the rank up to a multiple of 8: a value cut to
+// 16 bits, and what that lacks.  One 16-bit number alone would cost as much as the result's own rounding.
 //
-// The upper half is always short of the value (of one that T holds, too: then by T's last place), so that both halves of a value
-// other than zero are other than zero and have its sign.  Both are multiplied by the same factor, and infinity times them
-// has to be the infinity that the value would give: a lower half of zero, or of the other sign, makes NaN of it.
-template <class T>
-__device__ __forceinline__ T shorter(float v)
+// The halves are BF16 for F16 tensors, too: F16 would lose values above 65504, and bits of those below 2^-14, that the result
+// still needs.  (A factor in F16 then comes as two BF16 parts: k_parts.)
+//
+// The upper half is always short of the value (of one that 16 bits hold, too: then by its last place), so that both halves of a
+// value other than zero are other than zero and have its sign.  Both are multiplied by the same factor, and infinity
+// times them has to be the infinity that the value would give: a lower half of zero, or of the other sign, makes NaN of it.
+using Thin = __nv_bfloat16;
+__device__ __forceinline__ void split_halves(float v, Thin &hi, Thin &lo)
 {
-    if constexpr (__is_same(T, __nv_bfloat16)) {
-        const uint32_t u = __float_as_uint(v);
-        return __ushort_as_bfloat16(static_cast<uint16_t>((u & 0x7FFFFFFF ? u - 1 : u) >> 16));
-    } else {
-        const T hi = __float2half_rz(v);
-        const uint16_t bits = __half_as_ushort(hi);
-        return widen(hi) == v && (bits & 0x7FFF) ? __ushort_as_half(static_cast<uint16_t>(bits - 1)) : hi;
-    }
-}
-template <class T>
-__device__ __forceinline__ void split_halves(float v, T &hi, T &lo)
-{
-    hi = isfinite(v) ? shorter<T>(v) : narrow<T>(v);
-    lo = narrow<T>(isfinite(v) ? v - widen(hi) : v);
+    const uint32_t u = __float_as_uint(v);
+    hi = isfinite(v) ? __ushort_as_bfloat16(static_cast<uint16_t>((u & 0x7FFFFFFF ? u - 1 : u) >> 16)) : narrow<Thin>(v);
+    lo = narrow<Thin>(isfinite(v) ? v - widen(hi) : v);
 }
 
 // Tokens in the order of their adapters, if they came scattered: what the projection's kernels then read in place of x.
@@ -86,6 +78,157 @@ __global__ void __launch_bounds__(32 * GATHER_WARPS) k_gather(const SortedTokens
             if (v + e * 32 < cols / 8) reinterpret_cast<uint4 *>(out)[v + e * 32] = q[e];
     }
     if (lane < cols % 8) out[cols / 8 * 8 + lane] = in[cols / 8 * 8 + lane];
+}
+
+// F16's factors as BF16, for the product with thin halves: each value as two parts (split_halves, exact: 11 bits of 16), so that a
+// sum over both parts is the sum over the factor.  out[slot][part][each], for the adapters that have a sixteen of tokens to
+// themselves; only those are asked for.
+//
+// A block's row of the grid is a slot: an adapter's own where there are no more adapters than sixteens, else a sixteen's, for the
+// adapter whose first sixteen it is (one token beside a thousand adapters of 4096 x 16: 14 us of the call were blocks with nothing
+// to do).  Runs beside the thin product, which has waited for all that is read here.  Bound by HBM: 2 bytes read and 4 written a
+// value.
+struct PartsArgs {
+    const __half *in;                          // of adapter i from i * each
+    Thin *out;
+    uint32_t *slot;                            // per adapter, written
+    TokenIndex index;
+    SortedTokens sorted;
+    uint64_t each, tokens, sixteens;
+};
+constexpr uint32_t PARTS_THREADS = 256, PARTS_VALUES = PARTS_THREADS * 8 * 4;        // of a block
+static __global__ void __launch_bounds__(PARTS_THREADS) k_parts(const PartsArgs a)
+{
+    __shared__ uint32_t s_first;
+    const uint32_t tid = threadIdx.x, slot = blockIdx.y;
+    let_next_start();
+    int i = slot;
+    bool own = true;
+    if (a.index.ids) {                                           // the adapter's first sixteen, if it has one
+        const TokenIndex index = a.sorted.index(a.index, a.sorted.on());
+        const bool by_sixteen = a.index.n > a.sixteens;
+        const uint64_t end = by_sixteen ? slot + 1ull : a.sixteens;
+        if (by_sixteen) i = index.of(slot * 16ull);
+        if (tid == 0) s_first = ~0u;
+        __syncthreads();
+        uint32_t first = ~0u;
+        for (uint64_t g0 = 0; i >= 0 && g0 < end && first == ~0u; g0 += PARTS_THREADS) {
+            const uint64_t g = g0 + tid, t0 = g * 16;
+            if (g < end && index.of(t0) == i) {
+                bool all = true;
+                for (uint32_t c = 1; c < 16; c++)
+                    if (t0 + c < a.tokens) all = all && index.of(t0 + c) == i;
+                if (all) atomicMin(&s_first, static_cast<uint32_t>(g));
+            }
+            __syncthreads();
+            first = s_first;
+            __syncthreads();
+        }
+        own = by_sixteen ? first == slot : first != ~0u;
+    }
+    if (own) {
+        if (blockIdx.x == 0 && tid == 0) a.slot[i] = slot;
+        const __half *in = a.in + i * a.each;
+        Thin *out = a.out + slot * 2ull * a.each;
+        const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * PARTS_VALUES + tid * 8;
+        Vec<__half, 16> v[4];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++)
+            if (lo + q * PARTS_THREADS * 8 < a.each) v[q].raw = *reinterpret_cast<const uint4 *>(in + lo + q * PARTS_THREADS * 8);
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) {
+            const uint64_t at = lo + q * PARTS_THREADS * 8;
+            if (at >= a.each) continue;
+            Vec<Thin, 16> hi, rest;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) split_halves(widen(v[q].e[e]), hi.e[e], rest.e[e]);
+            *reinterpret_cast<uint4 *>(out + at) = hi.raw;
+            *reinterpret_cast<uint4 *>(out + a.each + at) = rest.raw;
+        }
+    }
+    if (blockIdx.x == 0 && slot == 0) wait_for_previous();       // (this one ends no sooner than the thin product)
+}
+
+// F16's thin products for the factors' gradients, where they are multiplied by F16 tensors: [token][rp] in 32 bits, as two halves
+// in F16 times a power of two.  Each adapter has a power of its own, by which its largest value comes to 2^14 and more; the
+// lower half is 2^11 times what the upper one lacks.  So a value keeps 16 bits and more down to 2^-34 of the largest one, and
+// both powers go out of the sums again exactly.  (The upper half is zero only where the value is: see above.)
+//
+// A cluster has an adapter's tokens: their largest value, then their halves.  Bound by latency: the products were just made.
+struct ThinJob {
+    const float *from;
+    __half *to;                                // [token][2][rp]
+    float *scale;                              // per adapter: what its sums are to be multiplied by
+};
+struct ThinArgs {
+    ThinJob job[2];
+    const uint32_t *order, *start;             // as for the factors' gradients
+    uint32_t tokens, rp;
+};
+constexpr uint32_t THIN_CTAS = 8, THIN_THREADS = 512;
+constexpr float THIN_LOWER = 1.0f / 2048;      // of a lower half
+static __global__ void __launch_bounds__(THIN_THREADS) k_thin(const __grid_constant__ ThinArgs a)
+{
+    __shared__ uint32_t s_most;
+    const ThinJob &job = a.job[blockIdx.z];
+    const uint32_t tid = threadIdx.x, i = blockIdx.y, rank = cluster_rank(), parts = a.rp / 8;
+    wait_for_previous();
+    const uint32_t begin = a.start ? a.start[i] : 0, end = a.start ? a.start[i + 1] : i ? 0 : a.tokens;
+    const uint64_t units = static_cast<uint64_t>(end - begin) * parts;
+    auto at = [&](uint64_t u, uint64_t &row, uint32_t &c) {
+        const uint32_t n = static_cast<uint32_t>(u / parts);
+        row = a.order ? a.order[begin + n] : n, c = static_cast<uint32_t>(u - static_cast<uint64_t>(n) * parts) * 8;
+    };
+    auto load = [&](uint64_t row, uint32_t c, float *v) {
+        const float4 *p = reinterpret_cast<const float4 *>(job.from + row * a.rp + c);
+        *reinterpret_cast<float4 *>(v) = p[0], *reinterpret_cast<float4 *>(v + 4) = p[1];
+    };
+    uint32_t most = 0;
+    for (uint64_t u = rank * THIN_THREADS + tid; u < units; u += THIN_CTAS * THIN_THREADS) {
+        uint64_t row;
+        uint32_t c;
+        float v[8];
+        at(u, row, c);
+        load(row, c, v);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++)
+            if (isfinite(v[e])) most = max(most, __float_as_uint(v[e]) & 0x7FFFFFFF);
+    }
+    if (tid == 0) s_most = 0;
+    __syncthreads();
+    most = __reduce_max_sync(~0u, most);
+    if ((tid & 31) == 0) atomicMax(&s_most, most);
+    __syncwarp();
+    cluster_barrier();
+    for (uint32_t q = 0; q < THIN_CTAS; q++) {
+        uint32_t other;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(other) : "r"(peer_addr(&s_most, q)) : "memory");
+        most = max(most, other);
+    }
+    const int e2 = most ? max(-100, min(113, static_cast<int>(most >> 23) - 127 - 14)) : 0;
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+    if (rank == 0 && tid == 0) job.scale[i] = __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+    for (uint64_t u = rank * THIN_THREADS + tid; u < units; u += THIN_CTAS * THIN_THREADS) {
+        uint64_t row;
+        uint32_t c;
+        float v[8];
+        at(u, row, c);
+        load(row, c, v);
+        Vec<__half, 16> upper, lower;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) {
+            const float w = v[e] * down;
+            __half hi = narrow<__half>(w);
+            if (v[e] != 0 && __heq(hi, __ushort_as_half(0))) hi = __ushort_as_half(w < 0 || (w == 0 && v[e] < 0) ? 0x8001 : 1);
+            upper.e[e] = hi;
+            lower.e[e] = narrow<__half>(isfinite(v[e]) ? (w - widen(hi)) * (1 / THIN_LOWER) : 0.0f);
+        }
+        __half *to = job.to + row * 2 * a.rp + c;
+        *reinterpret_cast<uint4 *>(to) = upper.raw;
+        *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
+    }
+    __syncwarp();
+    cluster_barrier();                                           // nobody leaves while another reads its largest
 }
 
 // Copies whose rows start on a boundary of 16 bytes and end in zeros: out[o][r][c] = in(o, r, c) for c < cols, else 0.

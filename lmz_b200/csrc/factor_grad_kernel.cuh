@@ -18,6 +18,7 @@ template <class T>
 struct FactorGradJob {
     CUtensorMap z, z_rows, thin, thin_rows;    // tiles of 64 x 64, and of one row (for gathers)
     T *out;                                    // dF_i(f, j) at i * each + f * wide + j * place
+    const float *scale;                        // F16: per adapter, what its sums are multiplied by (k_thin)
     uint64_t feats, each, wide, place;
     uint32_t clusters;                         // that it takes
 };
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     const uint32_t all = (end - begin + STEP_K - 1) / STEP_K;
     const uint32_t n0 = static_cast<uint32_t>(static_cast<uint64_t>(all) * rank / a.split), n1 = static_cast<uint32_t>(static_cast<uint64_t>(all) * (rank + 1) / a.split);
     const uint32_t ring = (smem_addr(f_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
+    constexpr float LOWER = __is_same(T, __half) ? THIN_LOWER : 1.0f;
     const uint32_t thins = thin_blocks(a.rp), thin_at = 2 * a.blocks * FG_TILE;
     volatile uint32_t *over = &s.over;
 
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
                     tmem_load8(tmem + (warp << 21) + b * 2 * a.rp + a.rp + c, w);
                 }
 #pragma unroll
-                for (uint32_t e = 0; e < 8; e++) part[(b * a.rp + c + e) * FG_PITCH + tid] = isfinite(v[e]) ? v[e] + w[e] : v[e];
+                for (uint32_t e = 0; e < 8; e++) part[(b * a.rp + c + e) * FG_PITCH + tid] = isfinite(v[e]) ? v[e] + w[e] * LOWER : v[e];
             }
     }
     tc_before();
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
     else __syncthreads();
     if (ok && !*over) {
         T *out = g.out + i * g.each;
+        const float scale = __is_same(T, __half) ? g.scale[i] : 1.0f;
         const uint32_t wide = a.blocks * FG_FEATS;
         const Peers peers(ring, a.split);
         // Eight neighbours of the result a thread: along f, threads side by side on neighbouring j; or along j, threads on
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(FG_THREADS) k_factor_grad(const __grid_constan
             peers.sum8(((row / FG_FEATS * a.rp + j) * FG_PITCH + row % FG_FEATS) * 4, along_f ? 4 : FG_PITCH * 4, sum);
             Vec<T, 16> v;
 #pragma unroll
-            for (uint32_t q = 0; q < 8; q++) v.e[q] = narrow<T>(sum[q]);
+            for (uint32_t q = 0; q < 8; q++) v.e[q] = narrow<T>(__is_same(T, __half) ? sum[q] * scale : sum[q]);
             T *to = out + f * g.wide + j * g.place;
             const uint64_t left = along_f ? g.feats - f : a.rank - j;
             if (left >= 8 && (bits & 15) == 0) {

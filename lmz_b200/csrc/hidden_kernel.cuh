@@ -25,8 +25,9 @@ struct HiddenArgs {
     CUtensorMap xs;                            // x in the order of `sorted`
     TokenIndex index;
     SortedTokens sorted;
-    T *h;                                      // [token][2][rp], in that order if x is
-    T *kept;                                   // NULL, or the same in the tokens' own order
+    Thin *h;                                   // [token][2][rp], in that order if x is
+    void *kept;                                // NULL, or for the factors' gradients in the tokens' own order: the same for BF16
+                                               // tensors, for F16 ones [token][rp] in 32 bits
     uint64_t tokens;
     uint32_t rank, rp, steps, split;
     uint32_t each;                             // adapters of a block: as many as have room in H_COLUMNS columns
@@ -172,16 +173,25 @@ __global__ void __launch_bounds__(H_THREADS) k_hidden(const __grid_constant__ Hi
             const float scale = a.index.scale_of(s.adapter[row]);
             float sum[8];
             peers.sum8((c * H_PITCH + row) * 4, H_PITCH * 4, sum);
-            Vec<T, 16> upper, lower;
+            Vec<Thin, 16> upper, lower;
 #pragma unroll
-            for (uint32_t q = 0; q < 8; q++) split_halves(c + q < a.rank ? sum[q] * scale : 0.0f, upper.e[q], lower.e[q]);
-            T *to = a.h + (t0 + row) * 2 * a.rp + c;
+            for (uint32_t q = 0; q < 8; q++) {
+                sum[q] = c + q < a.rank ? sum[q] * scale : 0.0f;
+                split_halves(sum[q], upper.e[q], lower.e[q]);
+            }
+            Thin *to = a.h + (t0 + row) * 2 * a.rp + c;
             *reinterpret_cast<uint4 *>(to) = upper.raw;
             *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
             if (a.kept) {
-                to = a.kept + (sorted ? a.sorted.order[t0 + row] : t0 + row) * 2 * a.rp + c;
-                *reinterpret_cast<uint4 *>(to) = upper.raw;
-                *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
+                const uint64_t t = sorted ? a.sorted.order[t0 + row] : t0 + row;
+                if constexpr (__is_same(T, __half)) {
+                    float4 *wide = reinterpret_cast<float4 *>(static_cast<float *>(a.kept) + t * a.rp + c);
+                    wide[0] = make_float4(sum[0], sum[1], sum[2], sum[3]), wide[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+                } else {
+                    to = static_cast<Thin *>(a.kept) + t * 2 * a.rp + c;
+                    *reinterpret_cast<uint4 *>(to) = upper.raw;
+                    *reinterpret_cast<uint4 *>(to + a.rp) = lower.raw;
+                }
             }
         }
     }

@@ -258,9 +258,12 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
 // and 34, 1024x4096x1024 of 8 r32 42 and 34 against 47 and 27 (left without).
 static bool worth_sorting(const lmz_projection *p, uint64_t feats, uint64_t rp) { return p->tokens >= 8ull * p->adapters && p->tokens * feats * rp >= 1ull << 26; }
 
+// Adapters that can have a sixteen of tokens to themselves: places for the parts of an F16 factor.
+static uint64_t parts_slots(const lmz_projection *p) { return std::min<uint64_t>(p->index ? p->adapters : 1, (p->tokens + 15) / 16); }
+
 // What a projection's kernels read in place of tensors that do not lie on boundaries, and between each other.
 struct ProjectLayout {
-    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, hidden, scattered, in_order, thin, end = 0;
+    uint64_t x, w, a, b, dy, g, keys[2], pos[2], start, hidden, scattered, in_order, thin, parts, slot, halves[2], scale[2], end = 0;
     bool pack_x, pack_w, pack_a, pack_b, pack_dy;
     bool sorts;                                // the projection takes scattered tokens by adapter
     ProjectLayout(const lmz_projection *p, bool grad)
@@ -289,7 +292,11 @@ struct ProjectLayout {
         hidden = take(!grad && !p->hidden, p->tokens * 4 * up8(p->rank));
         scattered = take(may_sort, 4);
         in_order = take(may_sort, p->tokens * up8(grad ? p->out : p->in) * 2);
-        thin = take(may_sort && (grad || p->hidden), p->tokens * 4 * up8(p->rank));
+        const bool f16 = p->dtype == LMZ_GPU_F16;
+        thin = take((may_sort || f16) && (grad || p->hidden), p->tokens * 4 * up8(p->rank));
+        parts = take(f16, 4 * parts_slots(p) * (grad ? p->rank * up8(p->in) : p->out * up8(p->rank)));
+        slot = take(f16, p->adapters * 4ull);
+        for (int i = 0; i < 2; i++) halves[i] = take(grad && f16, p->tokens * 4 * up8(p->rank)), scale[i] = take(grad && f16, p->adapters * 4ull);
     }
 };
 
@@ -331,14 +338,32 @@ struct InOrder {
     const T *x = nullptr;                        // rows of up8(k) elements
 };
 
+// An F16 factor's parts, behind the thin product and beside it.
+static int launch_parts(const lmz_projection *p, const SortedTokens &sorted, const __half *factor, uint64_t each, Thin *parts, uint32_t *slot, cudaStream_t cs)
+{
+    const uint64_t slots = parts_slots(p);
+    PartsArgs a{};
+    a.in = factor, a.out = parts, a.slot = slot, a.index = token_index(p), a.sorted = sorted;
+    a.each = each, a.tokens = p->tokens, a.sixteens = (p->tokens + 15) / 16;
+    const uint64_t blocks = (each + PARTS_VALUES - 1) / PARTS_VALUES;          // (below 2^21 * 256 / 2^13)
+    return launch("launch k_parts", k_parts, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(slots)), PARTS_THREADS, 0, cs, a);
+}
+
 // y[t][f] = sum of x[t][k] W(f, k) + sum of h[t][j] F_i(f, j) (MN: W and F with their f next to each other).
 template <class T, bool MN>
 static int launch_project(const lmz_projection *p, const InOrder<T> &o, const T *x, uint64_t x_stride, uint64_t k, const T *w, uint64_t w_stride, uint64_t feats, const T *factor,
-                          uint64_t factor_rows, uint64_t factor_row, const T *hidden, T *y, cudaStream_t cs)
+                          uint64_t factor_rows, uint64_t factor_row, const Thin *hidden, const ProjectLayout &l, T *y, cudaStream_t cs)
 {
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     ProjectArgs<T> a{};
+    Thin *parts = reinterpret_cast<Thin *>(static_cast<uint8_t *>(p->work) + l.parts);
+    if constexpr (std::is_same_v<T, __half>) {
+        uint32_t *slot = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->work) + l.slot);
+        a.slot = slot;
+        rc = launch_parts(p, o.sorted, factor, factor_rows * factor_row, parts, slot, cs);
+        if (rc) return rc;
+    }
     a.index = token_index(p), a.sorted = o.sorted, a.hidden = hidden, a.factor = factor, a.factor_each = factor_rows * factor_row, a.factor_row = factor_row;
     a.y = y, a.tokens = p->tokens, a.feats = feats, a.rank = p->rank, a.rp = static_cast<uint32_t>(up8(p->rank));
     a.steps = static_cast<uint32_t>((k + STEP_K - 1) / STEP_K), a.split = 1;
@@ -372,9 +397,11 @@ static int launch_project(const lmz_projection *p, const InOrder<T> &o, const T 
     rc = tensor_map(&a.x, x, bf16, k, p->tokens, x_stride, pair ? a.nt / 2 : a.nt);
     if (!rc && o.x) rc = tensor_map(&a.xs, o.x, bf16, k, p->tokens, up8(k), pair ? a.nt / 2 : a.nt);
     if (!rc) rc = MN ? tensor_map(&a.w, w, bf16, feats, k, w_stride, STEP_K) : tensor_map(&a.w, w, bf16, k, feats, w_stride, P_FEATS);
-    if (!rc) rc = tensor_map(&a.h, hidden, bf16, a.rp, 2, a.rp, 1, p->tokens, pair ? a.nt / 2 : a.nt);
-    if (!rc) rc = MN ? tensor_map(&a.f, factor, bf16, feats, factor_rows, factor_row, STEP_K, p->adapters)
-                     : tensor_map(&a.f, factor, bf16, a.rp, factor_rows, factor_row, P_FEATS, p->adapters);
+    if (!rc) rc = tensor_map(&a.h, hidden, true, a.rp, 2, a.rp, 1, p->tokens, pair ? a.nt / 2 : a.nt);
+    const void *f = factor;
+    if (!bf16) f = parts;
+    const uint64_t planes = bf16 ? p->adapters : 2 * parts_slots(p);
+    if (!rc) rc = MN ? tensor_map(&a.f, f, true, feats, factor_rows, factor_row, STEP_K, planes) : tensor_map(&a.f, f, true, a.rp, factor_rows, factor_row, P_FEATS, planes);
     if (rc) return rc;
     if (pair) return launch_project_as<T, MN, true>(a, static_cast<unsigned>(std::min<uint64_t>(count, sms / 2) * 2), cs);
     return launch_project_as<T, MN, false>(a, static_cast<unsigned>(a.split > 1 ? count * a.split : std::min<uint64_t>(count, sms)), cs);
@@ -382,7 +409,7 @@ static int launch_project(const lmz_projection *p, const InOrder<T> &o, const T 
 
 // h = s x F^T for each token's own adapter; f: [adapter][rank][f_stride], its first k of each row.
 template <class T>
-static int launch_hidden(const lmz_projection *p, const InOrder<T> &o, const T *x, uint64_t x_stride, uint64_t k, const T *f, uint64_t f_stride, T *h, T *kept,
+static int launch_hidden(const lmz_projection *p, const InOrder<T> &o, const T *x, uint64_t x_stride, uint64_t k, const T *f, uint64_t f_stride, Thin *h, void *kept,
                          cudaStream_t cs)
 {
     static bool done[64];
@@ -421,6 +448,7 @@ struct FactorGrad {
     const T *thin;
     T *out;
     uint64_t wide, place;
+    const float *scale;                          // F16 (k_thin)
 };
 
 template <class T>
@@ -440,7 +468,7 @@ static int launch_factor_grad(const lmz_projection *p, const FactorGrad<T> *jobs
     for (uint32_t i = 0; i < count; i++) {
         const FactorGrad<T> &f = jobs[i];
         FactorGradJob<T> &g = a.job[i];
-        g.out = f.out, g.feats = f.feats, g.each = f.feats * p->rank, g.wide = f.wide, g.place = f.place;
+        g.out = f.out, g.scale = f.scale, g.feats = f.feats, g.each = f.feats * p->rank, g.wide = f.wide, g.place = f.place;
         g.clusters = static_cast<uint32_t>((f.feats + a.blocks * FG_FEATS - 1) / (a.blocks * FG_FEATS));
         clusters += g.clusters;
         rc = tensor_map(&g.z, f.z, bf16, f.feats, p->tokens, f.stride, STEP_K);
@@ -521,18 +549,31 @@ static int project_as(const lmz_projection *p, cudaStream_t cs)
 {
     const ProjectLayout l(p, false);
     const ProjectInputs<T> in(p, l, false, cs);
-    auto work = [&](uint64_t off) { return reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off); };
+    auto work = [&](uint64_t off) -> void * { return static_cast<uint8_t *>(p->work) + off; };
     int rc = in.rc;
     InOrder<T> o;
-    T *h = p->hidden ? static_cast<T *>(p->hidden) : work(l.hidden), *kept = nullptr;
+    constexpr bool f16 = std::is_same_v<T, __half>;
+    Thin *h = static_cast<Thin *>(p->hidden && !l.sorts && !f16 ? p->hidden : work(p->hidden ? l.thin : l.hidden));
+    void *kept = h == p->hidden ? nullptr : p->hidden;
     if (!rc && l.sorts) {
         rc = launch_token_sort(p, l, false, &o.sorted, cs);
         if (!rc) rc = launch_in_order(p, l, in.x, in.x_stride, p->in, &o, cs);
-        if (p->hidden) kept = h, h = work(l.thin);
     }
     if (!rc) rc = launch_hidden(p, o, in.x, in.x_stride, p->in, in.a, in.a_stride, h, kept, cs);
-    if (!rc) rc = launch_project<T, false>(p, o, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, in.b, p->out, up8(p->rank), h, static_cast<T *>(p->y), cs);
+    if (!rc) rc = launch_project<T, false>(p, o, in.x, in.x_stride, p->in, in.w, in.w_stride, p->out, in.b, p->out, up8(p->rank), h, l, static_cast<T *>(p->y), cs);
     return rc;
+}
+
+// The halves of F16's thin products.
+static int launch_thin(const lmz_projection *p, const ThinJob *jobs, uint32_t count, const uint32_t *order, const uint32_t *start, cudaStream_t cs)
+{
+    ThinArgs a{};
+    for (uint32_t i = 0; i < count; i++) a.job[i] = jobs[i];
+    a.order = order, a.start = start, a.tokens = static_cast<uint32_t>(p->tokens), a.rp = static_cast<uint32_t>(up8(p->rank));
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(dim3(THIN_CTAS, p->adapters, count), THIN_THREADS, 0, cs, THIN_CTAS, attrs);
+    CK("launch k_thin", cudaLaunchKernelEx(&c, k_thin, static_cast<const ThinArgs>(a)));
+    return LMZ_GPU_OK;
 }
 
 template <class T>
@@ -546,28 +587,39 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
     }
     const ProjectLayout l(p, true);
     const ProjectInputs<T> in(p, l, true, cs);
-    auto work = [&](uint64_t off) { return reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off); };
+    auto work = [&](uint64_t off) -> void * { return static_cast<uint8_t *>(p->work) + off; };
+    constexpr bool f16 = std::is_same_v<T, __half>;
     int rc = in.rc;
     InOrder<T> o;
     SortedTokens tokens{};
-    T *g = work(l.g), *h = g, *kept = nullptr;
+    void *g = work(l.g);                                         // what da needs of the thin product
+    Thin *h = static_cast<Thin *>(l.sorts || f16 ? work(l.thin) : g);
     const bool factors = p->da || p->db;
     if (!rc && l.sorts) {
         rc = launch_token_sort(p, l, factors, &tokens, cs);
         o.sorted = tokens;
         if (!rc) rc = launch_in_order(p, l, in.dy, in.dy_stride, p->out, &o, cs);
-        h = work(l.thin), kept = p->da ? g : nullptr;
     }
-    if (!rc && (p->dx || p->da)) rc = launch_hidden(p, o, in.dy, in.dy_stride, p->out, in.b, up8(p->out), h, kept, cs);
-    if (!rc && p->dx) rc = launch_project<T, true>(p, o, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, h, static_cast<T *>(p->dx), cs);
+    if (!rc && (p->dx || p->da)) rc = launch_hidden(p, o, in.dy, in.dy_stride, p->out, in.b, up8(p->out), h, p->da && h != g ? g : nullptr, cs);
+    if (!rc && p->dx) rc = launch_project<T, true>(p, o, in.dy, in.dy_stride, p->out, in.w, in.w_stride, p->in, in.a, r, in.a_stride, h, l, static_cast<T *>(p->dx), cs);
     if (rc || !factors) return rc;
     if (p->index && !l.sorts) rc = launch_token_sort(p, l, true, &tokens, cs);
     if (rc) return rc;
-    FactorGrad<T> jobs[2];
+    const uint32_t *start = p->index ? static_cast<const uint32_t *>(work(l.start)) : nullptr;
+    FactorGrad<T> jobs[2]{};
     uint32_t count = 0;
     if (p->db) jobs[count++] = {in.dy, in.dy_stride, p->out, static_cast<const T *>(p->hidden), static_cast<T *>(p->db), r, 1};
-    if (p->da) jobs[count++] = {in.x, in.x_stride, p->in, g, static_cast<T *>(p->da), 1, p->in};
-    return launch_factor_grad<T>(p, jobs, count, tokens.order, p->index ? reinterpret_cast<const uint32_t *>(work(l.start)) : nullptr, cs);
+    if (p->da) jobs[count++] = {in.x, in.x_stride, p->in, static_cast<const T *>(g), static_cast<T *>(p->da), 1, p->in};
+    if constexpr (f16) {
+        ThinJob thin[2]{};
+        for (uint32_t i = 0; i < count; i++) {
+            thin[i] = {reinterpret_cast<const float *>(jobs[i].thin), static_cast<__half *>(work(l.halves[i])), static_cast<float *>(work(l.scale[i]))};
+            jobs[i].thin = thin[i].to, jobs[i].scale = thin[i].scale;
+        }
+        rc = launch_thin(p, thin, count, tokens.order, start, cs);
+        if (rc) return rc;
+    }
+    return launch_factor_grad<T>(p, jobs, count, tokens.order, start, cs);
 }
 
 API int lmz_gpu_ops_gave_up(void)

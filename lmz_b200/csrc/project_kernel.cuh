@@ -37,11 +37,13 @@ template <class T>
 struct ProjectArgs {
     CUtensorMap x, w;
     CUtensorMap xs;                            // x in the order of `sorted`
-    CUtensorMap h, f;                          // hidden as tokens x 2 x rp, and the factors as adapters x their two sides
+    CUtensorMap h, f;                          // hidden as tokens x 2 x rp, and the factors as adapters x their two sides (F16:
+                                               // as slots x 2 x those, in BF16)
     TokenIndex index;
     SortedTokens sorted;
-    const T *hidden;                           // [token][2][rp]: the thin product, its upper and its lower half (in that order if x is)
+    const Thin *hidden;                        // [token][2][rp]: the thin product, its upper and its lower half (in that order if x is)
     const T *factor;                           // of adapter i from i * factor_each; rows of factor_row elements, multiples of 8
+    const uint32_t *slot;                      // F16: where an adapter's parts are (k_parts)
     uint64_t factor_each, factor_row;
     T *y;
     uint64_t tokens, feats;
@@ -130,10 +132,10 @@ __device__ __forceinline__ void mixed_group(const ProjectArgs<T> &a, const int32
         sync_threads(barrier, P_FEED);
         {
             const uint32_t c = id >> 3, j = j0 + (id & 7) * 8;
-            Vec<T, 16> upper, lower;
+            Vec<Thin, 16> upper, lower;
             upper.raw = lower.raw = {};
             if (adapter[c] >= 0 && j < a.rp) {
-                const T *h = a.hidden + (t0 + c) * 2 * a.rp + j;
+                const Thin *h = a.hidden + (t0 + c) * 2 * a.rp + j;
                 upper.raw = *reinterpret_cast<const uint4 *>(h), lower.raw = *reinterpret_cast<const uint4 *>(h + a.rp);
             }
             float v[8];
@@ -274,7 +276,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
         const uint32_t w = a.token_tiles - 8 * b < 8 ? a.token_tiles - 8 * b : 8;
         ft = in / w, tt = 8 * b + in % w;
     };
-    const uint32_t places = (a.rp + STEP_K - 1) / STEP_K;        // steps of a run, for each half of h
+    constexpr uint32_t PARTS = __is_same(T, __half) ? 2 : 1;     // of a factor
+    const uint32_t places = (a.rp + STEP_K - 1) / STEP_K;        // steps of a run, for each half of h and each part of the factor
     auto mine = [&](uint32_t run) { return run % a.split == rank; };
     auto mixed = [&](const TileInfo &info, uint32_t g) { return (info.mixed >> g & 1) && (a.split == 1 || g % a.split == rank); };
     auto features = [&](uint32_t ft) { return (ft * CTAS + side) * P_FEATS; };      // where this CTA's begin
@@ -325,25 +328,33 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
             for (uint32_t r = 0; r < info.runs && ok; r++) {
                 if (!mine(r)) continue;
                 const uint32_t token = tt * a.nt + info.run[r].column + side * (info.run[r].tokens / CTAS), adapter = info.run[r].adapter;
-                for (uint32_t j = 0; j < 2 * places; j++, at.next(a.stages)) {
-                    const uint32_t st = at.stage, half = j >= places, j0 = (half ? j - places : j) * STEP_K;
-                    ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
-                    if (!ok) break;
-                    if (elected()) {
-                        const uint32_t dst = ring + st * a.stage_bytes, bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
-                        if (side) peer_expect(bar, a.stage_bytes);
-                        else bar_expect(&s.full[st], a.stage_bytes);
-                        if constexpr (MN) {
-                            tma_load_3d<PAIR>(&a.f, bar, dst, f, j0, adapter);
-                            tma_load_3d<PAIR>(&a.f, bar, dst + STEP_K * ROW_BYTES, f + 64, j0, adapter);
-                        } else {
-                            tma_load_3d<PAIR>(&a.f, bar, dst, j0, f, adapter);
-                        }
-                    }
-                    __syncwarp();
+                uint32_t plane = adapter;
+                if constexpr (PARTS > 1) {
                     if (!h_here) wait_for_previous(), h_here = true;
-                    if (elected()) tma_load_3d<PAIR>(&a.h, PAIR ? full + st * 8 : smem_addr(&s.full[st]), ring + st * a.stage_bytes + P_FEATS * ROW_BYTES, j0, half, token);
-                    __syncwarp();
+                    plane = __ldcg(a.slot + adapter) * PARTS;
+                }
+                for (uint32_t q = 0; q < 2 * PARTS && ok; q++) {          // the factor's parts with the upper half, then with the lower
+                    const uint32_t half = q / PARTS;
+                    for (uint32_t j0 = 0; j0 < places * STEP_K; j0 += STEP_K, at.next(a.stages)) {
+                        const uint32_t st = at.stage;
+                        ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
+                        if (!ok) break;
+                        if (elected()) {
+                            const uint32_t dst = ring + st * a.stage_bytes, bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
+                            if (side) peer_expect(bar, a.stage_bytes);
+                            else bar_expect(&s.full[st], a.stage_bytes);
+                            if constexpr (MN) {
+                                tma_load_3d<PAIR>(&a.f, bar, dst, f, j0, plane + q % PARTS);
+                                tma_load_3d<PAIR>(&a.f, bar, dst + STEP_K * ROW_BYTES, f + 64, j0, plane + q % PARTS);
+                            } else {
+                                tma_load_3d<PAIR>(&a.f, bar, dst, j0, f, plane + q % PARTS);
+                            }
+                        }
+                        __syncwarp();
+                        if (!h_here) wait_for_previous(), h_here = true;
+                        if (elected()) tma_load_3d<PAIR>(&a.h, PAIR ? full + st * 8 : smem_addr(&s.full[st]), ring + st * a.stage_bytes + P_FEATS * ROW_BYTES, j0, half, token);
+                        __syncwarp();
+                    }
                 }
             }
             if (!ok) break;
@@ -387,18 +398,19 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_project(const __grid_constant_
                 const TileInfo &info = s.info[n % P_INFOS];
                 for (uint32_t r = 0; r < info.runs && ok; r++) {
                     if (!mine(r)) continue;
-                    const uint32_t column = info.run[r].column, rdesc = mma_desc(bf16, MN, false, CTAS * P_FEATS, info.run[r].tokens);
-                    for (uint32_t j = 0; j < 2 * places; j++, at.next(a.stages)) {
-                        const uint32_t st = at.stage, off = st * a.stage_bytes >> 4, j0 = (j >= places ? j - places : j) * STEP_K;
-                        ok = warp_wait(&s.full[st], at.turn & 1, over);
-                        if (!ok) break;
-                        if (elected()) {
-                            for (uint32_t c = 0; c < STEP_K / 16 && j0 + c * 16 < a.rp; c++)
-                                mma16<PAIR>(sums + column, a_lo + off + (c * a_step >> 4), b_lo + off + c * 2, rdesc, true);
-                            mma_commit<PAIR>(&s.empty[st]);
+                    const uint32_t column = info.run[r].column, rdesc = mma_desc(true, MN, false, CTAS * P_FEATS, info.run[r].tokens);
+                    for (uint32_t q = 0; q < 2 * PARTS && ok; q++)
+                        for (uint32_t j0 = 0; j0 < places * STEP_K; j0 += STEP_K, at.next(a.stages)) {
+                            const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+                            ok = warp_wait(&s.full[st], at.turn & 1, over);
+                            if (!ok) break;
+                            if (elected()) {
+                                for (uint32_t c = 0; c < STEP_K / 16 && j0 + c * 16 < a.rp; c++)
+                                    mma16<PAIR>(sums + column, a_lo + off + (c * a_step >> 4), b_lo + off + c * 2, rdesc, true);
+                                mma_commit<PAIR>(&s.empty[st]);
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
-                    }
                 }
                 if (!ok) break;
                 __syncwarp();

@@ -37,3 +37,16 @@ def test_project_and_its_gradients_of_every_layout(dtype, tokens, inp, out, n, k
     leaves = [t.requires_grad_(True) for t in (x, a, b)]
     y = adapters.project(x, w, a, b, index, scale=scales)
     _check_project(x, w, a, b, scales, index, y.detach(), dy, torch.autograd.grad(y, leaves, dy))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, inp, out, rank, n, kind", [(1, 72, 136, 8, 40, "runs"), (17, 264, 392, 5, 2, "runs"), (200, 136, 264, 16, 70, "runs"), (200, 136, 264, 16, 13, "short"),
+                                                             (600, 264, 1032, 24, 38, "short"), (900, 72, 328, 40, 500, "runs"), (5000, 72, 136, 8, 300, "short"),
+                                                             (5000, 72, 136, 8, 312, "short"), (5000, 72, 136, 8, 313, "short")])
+def test_more_and_fewer_adapters_than_sixteens(dtype, tokens, inp, out, rank, n, kind):
+    from lmz_b200 import adapters
+    x, w, a, b, scales = _inputs(tokens, inp, out, rank, n, dtype)
+    index, dy = _index(kind, tokens, n), _randn(40, (tokens, out), dtype)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = adapters.project(x, w, a, b, index, scale=scales)
+    _check_project(x, w, a, b, scales, index, y.detach(), dy, torch.autograd.grad(y, leaves, dy))

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops import DTYPES, _index
+from test_gpu_ops import DTYPES, _check, _index, _randn, _rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,46 @@ def _product(p, q):
     down = f(p == math.inf) @ f(q < 0) + f(p == -math.inf) @ f(q > 0) + f(p > 0) @ f(q == -math.inf) + f(p < 0) @ f(q == math.inf)
     out = torch.where(up > 0, math.inf, torch.where(down > 0, -math.inf, clean))
     return torch.where((nan > 0) | ((up > 0) & (down > 0)), math.nan, out)
+
+
+# F16 whose thin products leave its range, while the results do not: standard deviations of x, W, A, B and dy.
+RANGES = {"large h, tiny g": (3000.0, 1e-3, 4.0, 1e-4, 1e-3), "large g, tiny h": (1e-3, 1e-3, 1e-4, 4.0, 3000.0), "tiny dy": (30.0, 0.05, 0.1, 1.0, 1e-6),
+          "tiny x": (1e-6, 0.05, 0.1, 1.0, 30.0), "b of zeros": (3000.0, 1e-3, 4.0, 0.0, 1e-3)}
+
+
+@pytest.mark.parametrize("tokens, inp, out, rank, n, kind", LAYOUTS)
+@pytest.mark.parametrize("stds", RANGES.values(), ids=RANGES)
+def test_f16_over_its_range(tokens, inp, out, rank, n, kind, stds):
+    """The bounds of test_gpu_ops, less their allowance for thin products kept in F16: 2^-16 of their magnitude, wherever that is."""
+    from lmz_b200 import adapters
+    dtype = torch.float16
+    x, w, a, b, dy = (_randn(70 + i, s, dtype, std) for i, (s, std) in enumerate(zip(((tokens, inp), (out, inp), (n, rank, inp), (n, out, rank), (tokens, out)), stds)))
+    scales = 0.5 + torch.arange(n, device="cuda").float() / 2
+    index = _index(kind, tokens, n)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    y = adapters.project(x, w, a, b, index, scale=scales)
+    got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    xd, wd, ad, bd, dyd = (t.detach().double() for t in (x, w, a, b, dy))
+    want = [xd @ wd.t(), dyd @ wd, torch.zeros_like(ad), torch.zeros_like(bd)]
+    size = [xd.abs() @ wd.abs().t(), dyd.abs() @ wd.abs(), torch.zeros_like(ad), torch.zeros_like(bd)]
+    carried = [torch.zeros_like(t) for t in want]
+    largest = 0.0
+    for i in range(n):
+        at, s = _rows_of(index, tokens, i), float(scales[i])
+        if not at.numel():
+            continue
+        h, hs = s * (xd[at] @ ad[i].t()), s * (xd[at].abs() @ ad[i].abs().t())
+        g, gs = s * (dyd[at] @ bd[i]), s * (dyd[at].abs() @ bd[i].abs())
+        largest = max(largest, float(h.abs().max()), float(g.abs().max()))
+        for k, (rows, p, ps, q) in enumerate(((at, h, hs, bd[i].t()), (at, g, gs, ad[i]), (i, g.t(), gs.t(), xd[at]), (i, dyd[at].t(), dyd[at].abs().t(), h))):
+            want[k][rows] += p @ q
+            size[k][rows] += ps @ (hs if k == 3 else q.abs())
+            carried[k][rows] += 2 ** -16 * (p.abs() @ q.abs())
+    assert largest > 65504 or "tiny" in [k for k, v in RANGES.items() if v == stds][0] or tokens == 1
+    for v, w_, s_, c, terms, what in zip(got, want, size, carried, (inp + rank + 8, out + rank + 8, tokens + out + 8, tokens + inp + 8), ("y", "dx", "da", "db")):
+        # (F16 ends at 65504, and what is nearer to 65536 is infinite: from 65520 on, give or take what the sums may be off by)
+        slack = (1 + 2 ** -11) * (terms * 2 ** -23 * s_ + c)
+        inside, beyond = w_.abs() + slack < 65520, w_.abs() - slack >= 65520
+        assert (v[beyond].double() == w_[beyond].sign() * math.inf).all(), what
+        assert inside.double().mean() > 0.9
+        _check(torch.where(inside, v, torch.zeros_like(v)), torch.where(inside, w_, 0.0), s_, c, terms, what)
