@@ -405,6 +405,9 @@ int lmz_gpu_ops_gave_up(void);
  * may be the weight itself where that is. */
 int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a,
                       const void *d_b, unsigned rank, float scale, int dtype, void *d_out, void *cuda_stream);
+/* The same with factors in F32, for a weight of any of the three types. */
+int lmz_gpu_merge_wide_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const float *d_a,
+                           const float *d_b, unsigned rank, float scale, int dtype, void *d_out, void *cuda_stream);
 
 #ifdef __cplusplus
 }

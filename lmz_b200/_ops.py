@@ -29,7 +29,8 @@ def bind(lib) -> None:
             ("lmz_gpu_project_dev", _int, [proj, _v]),
             ("lmz_gpu_project_grad_dev", _int, [proj, _v]),
             ("lmz_gpu_ops_gave_up", _int, []),
-            ("lmz_gpu_merge_dev", _int, [_v, _u64, _u64, _u64, _v, _v, ctypes.c_uint, ctypes.c_float, _int, _v, _v])):
+            ("lmz_gpu_merge_dev", _int, [_v, _u64, _u64, _u64, _v, _v, ctypes.c_uint, ctypes.c_float, _int, _v, _v]),
+            ("lmz_gpu_merge_wide_dev", _int, [_v, _u64, _u64, _u64, _v, _v, ctypes.c_uint, ctypes.c_float, _int, _v, _v])):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
 

@@ -149,13 +149,14 @@ _made = None
 def merge(weight, a, b, scale: float = 1.0, out=None):
     """`weight + scale * b @ a`, summed in 32 bits and rounded once: the weight of the fine-tune that an adapter is.
 
-    `weight`: [out, in], `a`: [rank, in], `b`: [out, rank], all bfloat16 or all float16.  `out`: a contiguous tensor like
-    the weight to write to, the weight itself among them; without it a new one.  Not differentiable."""
+    `weight`: [out, in], `a`: [rank, in], `b`: [out, rank], all bfloat16 or all float16, or both factors float32 and the weight any
+    of the three.  `out`: a contiguous tensor like the weight to write to, the weight itself among them; without it a new one.  Not differentiable."""
     import torch
     index = _ops.on_cuda("weight a b out", weight, a, b, out)
-    code = _ops.type_code(weight, "weight", half_only=True)
-    if a.dtype != weight.dtype or b.dtype != weight.dtype:
-        raise TypeError(f"a is {a.dtype} and b {b.dtype}, the weight {weight.dtype}")
+    code = _ops.type_code(weight, "weight")
+    wide = a.dtype == torch.float32
+    if a.dtype != b.dtype or not (wide or (a.dtype == weight.dtype)):
+        raise TypeError(f"a is {a.dtype} and b {b.dtype}, the weight {weight.dtype}: the factors must be of its type, or float32")
     if weight.dim() != 2 or a.dim() != 2 or b.dim() != 2 or a.shape[1] != weight.shape[1] or b.shape[0] != weight.shape[0] or \
             a.shape[0] != b.shape[1]:
         raise ValueError(f"weight {list(weight.shape)}, a {list(a.shape)} and b {list(b.shape)} do not fit [out, in], [rank, in] and [out, rank]")
@@ -175,7 +176,7 @@ def merge(weight, a, b, scale: float = 1.0, out=None):
         raise ValueError("out may be the weight itself, but not overlap a, b or a part of the weight")
     if out.numel():
         a, b = _packed(a), _packed(b)
-        _ops.launch(index, "lmz_gpu_merge_dev", weight.data_ptr(), weight.shape[0], weight.shape[1], weight.stride(0), a.data_ptr(), b.data_ptr(),
+        _ops.launch(index, "lmz_gpu_merge_wide_dev" if wide else "lmz_gpu_merge_dev", weight.data_ptr(), weight.shape[0], weight.shape[1], weight.stride(0), a.data_ptr(), b.data_ptr(),
                     a.shape[0], scale, code, out.data_ptr())
         if given:                                          # (autograd notices where what was there is still needed)
             torch.autograd.graph.increment_version(out)

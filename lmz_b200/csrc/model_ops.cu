@@ -10,6 +10,7 @@
 #include "factor_grad_kernel.cuh"
 #include "hidden_kernel.cuh"
 #include "merge_kernel.cuh"
+#include "merge_wide_kernel.cuh"
 #include "project_kernel.cuh"
 #include "rows_kernels.cuh"
 #include "sort_kernel.cuh"
@@ -670,6 +671,31 @@ static int merge_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, c
         const uint64_t tiles = ((in + M_COLS - 1) / M_COLS) * ((out + M_ROWS - 1) / M_ROWS), room = (uint64_t)sms * (merge_smem(m.places) <= 113u << 10 ? 2 : 1);
         return launch("launch k_merge", k_merge<T, VB>, dim3(static_cast<unsigned>(std::min(tiles, room))), M_THREADS, merge_smem(m.places), cs, m);
     });
+}
+
+template <class T>
+static int merge_wide_as(const void *w, uint64_t out, uint64_t in, uint64_t stride, const float *a, const float *b, unsigned rank, float scale, void *to,
+                         cudaStream_t cs)
+{
+    const MergeWideArgs<T> m{static_cast<const T *>(w), a, b, static_cast<T *>(to), out, in, stride, rank, scale};
+    const uint64_t tiles = ((in + MW_TILE - 1) / MW_TILE) * ((out + MW_TILE - 1) / MW_TILE);       // (below 2^28)
+    const bool four = in % 4 == 0 && stride % 4 == 0 && (address(w) | address(to)) % (4 * sizeof(T)) == 0;
+    return launch("launch k_merge_wide", four ? k_merge_wide<T, true> : k_merge_wide<T, false>, dim3(static_cast<unsigned>(tiles)), MW_THREADS, 0, cs, m);
+}
+
+API int lmz_gpu_merge_wide_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const float *d_a, const float *d_b, unsigned rank,
+                               float scale, int dtype, void *d_out, void *cuda_stream)
+{
+    lmz_projection p{};
+    p.dtype = dtype == LMZ_GPU_F32 ? LMZ_GPU_BF16 : dtype, p.rank = rank, p.adapters = 1, p.in = in, p.out = out;
+    int rc = check_projection(&p);
+    if (rc) return rc;
+    rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    if (dtype == LMZ_GPU_F32) return merge_wide_as<float>(d_weight, out, in, weight_stride, d_a, d_b, rank, scale, d_out, cs);
+    return dtype == LMZ_GPU_BF16 ? merge_wide_as<__nv_bfloat16>(d_weight, out, in, weight_stride, d_a, d_b, rank, scale, d_out, cs)
+                                 : merge_wide_as<__half>(d_weight, out, in, weight_stride, d_a, d_b, rank, scale, d_out, cs);
 }
 
 API int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const void *d_a, const void *d_b, unsigned rank,

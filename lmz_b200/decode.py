@@ -596,7 +596,8 @@ def decode_tensors(ar, names, device=None, checksum: bool = True, adapter=None, 
 
     `adapter`: an archive (or path, or bytes) that holds a fine-tune of this one as low-rank factors (`adapters.load` says
     how they are named).  The named tensors that it has factors for come out as the fine-tune's own, merged with
-    `scale` (alpha / rank); the others as they are."""
+    `scale` (alpha / rank); the others as they are.  Weights of BF16, F16 or F32, and factors of any of these types: they are
+    merged as they are stored, and only the result is rounded to the weight's type."""
     ar = ar if isinstance(ar, fmt.Archive) else fmt.Archive(ar)
     index = ar.tensor_index()
     keys = _resolve(index, names)
@@ -626,13 +627,16 @@ def _torch_type(name):
 
 def _merge_adapter(tensors, adapter, scale):
     """Put merged weights in the place of the tensors that an adapter archive has factors for."""
+    import torch
     from . import adapters
     adapter = adapter if isinstance(adapter, fmt.Archive) else fmt.Archive(adapter)
     merged = None
     for key, weight in tensors.items():
         pair = adapters._factors(adapter, key[1], weight.device)
         if pair is not None:
-            a, b = (t.to(weight.dtype) for t in pair)
+            a, b = pair
+            if not a.dtype == b.dtype == weight.dtype:     # (to more bits, never to fewer)
+                a, b = (t.float() if t.dtype in (torch.bfloat16, torch.float16) else t for t in pair)
             tensors[key] = merged = adapters.merge(weight, a, b, scale=scale)
     if merged is not None:
         adapters.check(merged.device)                      # (as the decoded tensors have been)

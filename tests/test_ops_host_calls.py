@@ -1,8 +1,19 @@
 """Calls that the operators refuse, as far as it can be said without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
-from lmz_b200 import _ops, adapters, embed
+from lmz_b200 import _ops, adapters, build, embed
+
+
+@pytest.fixture(scope="module")
+def lib():
+    path = build.build()
+    assert path, build.last_error
+    lib = ctypes.CDLL(path)
+    _ops.bind(lib)
+    return lib
 
 
 def test_tangents_are_refused():
@@ -20,3 +31,8 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(ValueError, match="CUDA"):      # (others are taken, or refused for what they lack)
             adapters.merge(t, t, t)
+
+
+@pytest.mark.parametrize("out, inp, rank, dtype", [(8, 8, 0, 0), (8, 8, 257, 2), (8, 8, 4, 3), (0, 8, 4, 2), (8, 1 << 21, 4, 2)])
+def test_wide_merges_the_library_refuses(lib, out, inp, rank, dtype):
+    assert lib.lmz_gpu_merge_wide_dev(None, out, inp, inp, None, None, rank, 1.0, dtype, None, None) == -2
