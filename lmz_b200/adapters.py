@@ -250,7 +250,7 @@ def _factors(ar, name: str, device=None):
     if len(found) == 1:
         raise KeyError(f"the adapter has only one factor for {name!r}: {found[0][1]!r}")
     got = decode.decode_tensors(ar, found, device=device)
-    a, b = (got[k] for k in found)
+    a, b = (decode._typed(got[k], ar.tensor_index()[k]) for k in found)
     if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1]:
         raise ValueError(f"the factors for {name!r} are {list(a.shape)} and {list(b.shape)}, not [rank, in] and [out, rank]")
     return a, b

@@ -616,7 +616,7 @@ def decode_tensors(ar, names, device=None, checksum: bool = True, adapter=None, 
                 pass
         out[k] = raw
     if adapter is not None:
-        _merge_adapter(out, adapter, scale)
+        _merge_adapter(out, index, adapter, scale)
     return out
 
 
@@ -625,7 +625,13 @@ def _torch_type(name):
     return getattr(torch, name)
 
 
-def _merge_adapter(tensors, adapter, scale):
+def _typed(t, entry):
+    """A decoded tensor as what it is: one that does not lie on a boundary of its elements came as bytes, and is copied."""
+    name, shape = _TORCH_DTYPES.get(entry[0]), entry[1]
+    return t if name is None or t.dtype == _torch_type(name) else t.clone().view(_torch_type(name)).reshape(shape)
+
+
+def _merge_adapter(tensors, index, adapter, scale):
     """Put merged weights in the place of the tensors that an adapter archive has factors for."""
     import torch
     from . import adapters
@@ -635,6 +641,7 @@ def _merge_adapter(tensors, adapter, scale):
         pair = adapters._factors(adapter, key[1], weight.device)
         if pair is not None:
             a, b = pair
+            weight = _typed(weight, index[key])
             if not a.dtype == b.dtype == weight.dtype:     # (to more bits, never to fewer)
                 a, b = (t.float() if t.dtype in (torch.bfloat16, torch.float16) else t for t in pair)
             tensors[key] = merged = adapters.merge(weight, a, b, scale=scale)

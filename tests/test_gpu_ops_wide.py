@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops import ALL, _archive, _randn
+from test_gpu_ops import ALL, _archive, _randn, _safetensors
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,32 @@ def test_factors_of_two_types():
     ar, mixed = archive.Archive(_archive({"p.weight": w})), archive.Archive(_archive({"p.lora_A.weight": a, "p.lora_B.weight": b}))
     (got,) = decode.decode_tensors(ar, ["p.weight"], adapter=mixed).values()
     _check_merge(got, w, a, b.float(), 1.0)
+
+
+@pytest.mark.parametrize("weight, pad", [(torch.bfloat16, 1), (torch.float32, 2), (torch.float32, 1), (torch.float16, 2)])
+def test_a_weight_off_the_boundary_of_its_elements(weight, pad):
+    """A safetensors header of any length puts a tensor at any byte: it comes as bytes then, and merged as what it is; so with
+    an adapter's factors."""
+    import struct
+
+    import numpy as np
+
+    from lmz_b200 import adapters, archive, decode
+    from oracle import archive as oa
+
+    def shifted(tensors):
+        whole = _safetensors(tensors).tobytes()
+        n = struct.unpack("<Q", whole[:8])[0]
+        head = whole[8:8 + n].rstrip()
+        head += b" " * ((pad - len(head)) % 8)
+        member = struct.pack("<Q", len(head)) + head + whole[8 + n:]
+        return archive.Archive(oa.write_archive([("m.safetensors", np.frombuffer(member, dtype=np.uint8))]))
+
+    w, a, b = _randn(60, (64, 40), weight), _randn(61, (8, 40), weight, 0.2), _randn(62, (64, 8), weight)
+    ar, tuned = shifted({"p.weight": w}), shifted({"p.lora_A.weight": a, "p.lora_B.weight": b})
+    (plain,) = decode.decode_tensors(ar, ["p.weight"]).values()
+    assert torch.equal(plain.clone().view(weight).view(64, 40), w)
+    (got,) = decode.decode_tensors(ar, ["p.weight"], adapter=tuned, scale=0.5).values()
+    assert torch.equal(got, adapters.merge(w, a, b, scale=0.5))
+    p, q = adapters.load([tuned], "p.weight")
+    assert torch.equal(p[0], a) and torch.equal(q[0], b)
