@@ -409,6 +409,71 @@ int lmz_gpu_merge_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t 
 int lmz_gpu_merge_wide_dev(const void *d_weight, uint64_t out, uint64_t in, uint64_t weight_stride, const float *d_a,
                            const float *d_b, unsigned rank, float scale, int dtype, void *d_out, void *cuda_stream);
 
+/* Root-mean-square norms, with the addition of a residual in front.  s[t] = x[t] + residual[t], rounded to the tensors' type
+ * (x[t] without a residual);  y[t] = s[t] / sqrt(mean(s[t]^2) + eps) * weight.  In 8 bits (E4M3): q[t] = y[t] / scale[t] with
+ * scale[t] = max |y[t]| / 448, but no less than 2^-126, from y in 32 bits. */
+typedef struct lmz_norm {
+    const void *x, *residual;   /* tokens x dim, rows x_stride and residual_stride elements apart; residual: or NULL */
+    const void *weight;         /* dim, of the tensors' type or F32; NULL (in 8 bits alone): no norm, y is s */
+    void *y;                    /* tokens x dim; NULL in 8 bits */
+    void *q;                    /* tokens x dim bytes; NULL otherwise */
+    float *scale;               /* tokens, with q */
+    void *stream;               /* s, tokens x dim; NULL without a residual */
+    float *rstd;                /* tokens: what the gradients need of the forward pass; NULL where there will be none */
+    const void *dy, *dstream;   /* gradients of y and of s (NULL: none), tokens x dim */
+    void *dx;                   /* tokens x dim: the gradient of x, and of the residual; NULL: not wanted */
+    void *dweight;              /* dim, of the weight's type; NULL: not wanted */
+    void *work;                 /* lmz_gpu_norm_grad_work_bytes(), 256-byte aligned */
+    uint64_t tokens, dim, x_stride, residual_stride;
+    uint32_t dtype, weight_dtype;
+    float eps;
+} lmz_norm;
+int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream);
+/* x: what was normed (s where there was a residual, rows x_stride apart). */
+size_t lmz_gpu_norm_grad_work_bytes(const lmz_norm *p);
+int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream);
+
+/* Products with what stands behind them:  z[t] = x[t] W_e^T + bias_e,  y[t] = act(z[t]) * times[t] + residual[t]
+ * where e is the expert whose rows t is one of: offsets[e] <= t < offsets[e + 1].  Offsets that do not ascend, or leave the rows there are, are
+ * taken as the nearest that do not.  Rows of no expert are zeros, in y and in every gradient.  Without offsets there is one weight, for all
+ * rows.  BF16 or F16; or x and the weight in 8 bits (E4M3), z[t][o] = x_scale[t] weight_scale[o] (x[t] W^T)[o] + bias[o], the other tensors
+ * BF16 or F16.  y, z, dy and all gradients are contiguous. */
+#define LMZ_GPU_E4M3 3
+#define LMZ_GPU_MAX_EXPERTS 1024
+#define LMZ_GPU_ACT_NONE 0
+#define LMZ_GPU_ACT_RELU 1
+#define LMZ_GPU_ACT_SILU 2
+#define LMZ_GPU_ACT_GELU 3
+#define LMZ_GPU_ACT_GELU_TANH 4
+typedef struct lmz_product {
+    const void *x;              /* rows x in, x_stride elements apart */
+    const void *weight;         /* experts x out x in, rows weight_stride elements apart, experts weight_plane */
+    const void *bias;           /* experts x out, or NULL */
+    const void *times;          /* rows x out, times_stride elements apart, or NULL */
+    const void *residual;       /* rows x out, residual_stride elements apart, or NULL */
+    const void *offsets;        /* experts + 1 int32 or int64 (offset_bytes 4 or 8), or NULL: one expert, all rows */
+    const float *x_scale, *weight_scale;   /* rows, and out: in 8 bits; NULL otherwise */
+    void *y;                    /* rows x out */
+    float *z;                   /* rows x out: what the gradients need of the forward pass where there is an activation or `times`; or NULL */
+    const void *dy;             /* rows x out */
+    void *dx, *dweight, *dbias, *dtimes;   /* contiguous, like x, weight, bias and times; NULL: not wanted */
+    void *work;                 /* lmz_gpu_product_work_bytes(), 256-byte aligned */
+    uint64_t rows, in, out, x_stride, weight_stride, weight_plane, times_stride, residual_stride;
+    uint32_t experts, dtype, result_dtype, activation, offset_bytes;   /* dtype: of x and weight; result_dtype: of the others */
+} lmz_product;
+/* Reads the sizes, strides and types alone, the addresses' last bits and which tensors there are; `grad`: for the gradients' call. */
+size_t lmz_gpu_product_work_bytes(const lmz_product *p, int grad);
+int lmz_gpu_product_dev(const lmz_product *p, void *cuda_stream);
+/* dz[t] = dy[t] times[t] act'(z[t]), rounded to the tensors' type;  dx[t] = dz[t] W_e, dW_e = the sum of dz[t]^T x[t], dbias_e = the sum of dz[t] over
+ * the rows of expert e (zeros for one without any), dtimes[t] = dy[t] act(z[t]).  The residual's gradient is dy. */
+int lmz_gpu_product_grad_dev(const lmz_product *p, void *cuda_stream);
+
+/* Whole numbers of n places sorted, stably: order[i] is the place of the i-th smallest (ids outside [0, experts) come last), and
+ * offsets[e] how many are below e, for e up to `experts`.  d_work: lmz_gpu_order_work_bytes(n), 256-byte aligned. */
+size_t lmz_gpu_order_work_bytes(uint64_t n);
+int lmz_gpu_order_dev(const void *d_ids, int id_bytes, uint64_t n, uint64_t experts, uint32_t *d_order, uint32_t *d_offsets, void *d_work,
+                      void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

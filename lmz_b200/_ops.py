@@ -8,7 +8,7 @@ import math
 from . import gpu
 
 _v, _u64, _u32, _int = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int
-BF16, F16, F32 = 0, 1, 2
+BF16, F16, F32, E4M3 = 0, 1, 2, 3
 
 
 class Projection(ctypes.Structure):
@@ -18,8 +18,21 @@ class Projection(ctypes.Structure):
         [(n, _u32) for n in ("adapters", "rank", "dtype", "index_bytes")] + [("scale", ctypes.c_float)]
 
 
+class Norm(ctypes.Structure):
+    """Mirror of `lmz_norm`."""
+    _fields_ = [(n, _v) for n in ("x", "residual", "weight", "y", "q", "scale", "stream", "rstd", "dy", "dstream", "dx", "dweight", "work")] + \
+        [(n, _u64) for n in ("tokens", "dim", "x_stride", "residual_stride")] + [("dtype", _u32), ("weight_dtype", _u32), ("eps", ctypes.c_float)]
+
+
+class Product(ctypes.Structure):
+    """Mirror of `lmz_product`."""
+    _fields_ = [(n, _v) for n in ("x", "weight", "bias", "times", "residual", "offsets", "x_scale", "weight_scale", "y", "z", "dy", "dx", "dweight", "dbias", "dtimes", "work")] + \
+        [(n, _u64) for n in ("rows", "in_", "out", "x_stride", "weight_stride", "weight_plane", "times_stride", "residual_stride")] + \
+        [(n, _u32) for n in ("experts", "dtype", "result_dtype", "activation", "offset_bytes")]
+
+
 def bind(lib) -> None:
-    proj = ctypes.POINTER(Projection)
+    proj, norm, product = ctypes.POINTER(Projection), ctypes.POINTER(Norm), ctypes.POINTER(Product)
     for name, res, args in (
             ("lmz_gpu_rows_dev", _int, [_v, _u64, _u64, _u64, _int, _v, _int, _u64, ctypes.c_float, _v, _v]),
             ("lmz_gpu_rows_grad_work_bytes", ctypes.c_size_t, [_u64] * 3),
@@ -28,6 +41,14 @@ def bind(lib) -> None:
             ("lmz_gpu_project_work_bytes", ctypes.c_size_t, [proj, _int]),
             ("lmz_gpu_project_dev", _int, [proj, _v]),
             ("lmz_gpu_project_grad_dev", _int, [proj, _v]),
+            ("lmz_gpu_norm_dev", _int, [norm, _v]),
+            ("lmz_gpu_norm_grad_work_bytes", ctypes.c_size_t, [norm]),
+            ("lmz_gpu_norm_grad_dev", _int, [norm, _v]),
+            ("lmz_gpu_product_work_bytes", ctypes.c_size_t, [product, _int]),
+            ("lmz_gpu_product_dev", _int, [product, _v]),
+            ("lmz_gpu_product_grad_dev", _int, [product, _v]),
+            ("lmz_gpu_order_work_bytes", ctypes.c_size_t, [_u64]),
+            ("lmz_gpu_order_dev", _int, [_v, _int, _u64, _u64, _v, _v, _v, _v]),
             ("lmz_gpu_ops_gave_up", _int, []),
             ("lmz_gpu_merge_dev", _int, [_v, _u64, _u64, _u64, _v, _v, ctypes.c_uint, ctypes.c_float, _int, _v, _v]),
             ("lmz_gpu_merge_wide_dev", _int, [_v, _u64, _u64, _u64, _v, _v, ctypes.c_uint, ctypes.c_float, _int, _v, _v])):
@@ -110,6 +131,19 @@ def whole_numbers(t, what: str) -> int:
     if t.dtype is not torch.int32 and t.dtype is not torch.int64:
         raise TypeError(f"{what} must be int32 or int64, not {t.dtype}")
     return 4 if t.dtype is torch.int32 else 8
+
+
+def rows_of(t):
+    """A tensor as [rows, columns] with the elements of a row next to each other, without a copy where it can be."""
+    if t is None:
+        return None
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def finite(scale, what: str = "scale") -> float:

@@ -1,0 +1,202 @@
+// What stands behind a product's sums, forwards and backwards:  z = sums + bias,  y = act(z) times + residual.
+#pragma once
+#include "tcgen.cuh"
+#include "vectors.cuh"
+
+namespace lmz {
+
+enum Activation : uint32_t { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_COUNT };
+
+constexpr float ROOT_HALF = 0.70710678f, ROOT_2_PI = 0.79788456f, ROOT_1_2PI = 0.39894228f, TANH_CUBE = 0.044715f;
+
+__device__ __forceinline__ float act(uint32_t kind, float z)
+{
+    switch (kind) {
+    case ACT_RELU: return z < 0 ? 0.0f : z;                      // (a NaN stays)
+    case ACT_SILU: return z / (1 + expf(-z));
+    case ACT_GELU: return 0.5f * z * (1 + erff(z * ROOT_HALF));
+    case ACT_GELU_TANH: return 0.5f * z * (1 + tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z)));
+    default: return z;
+    }
+}
+
+// The activation and its derivative.
+__device__ __forceinline__ void act_and_slope(uint32_t kind, float z, float &y, float &slope)
+{
+    switch (kind) {
+    case ACT_RELU: y = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f; return;
+    case ACT_SILU: {
+        const float e = 1 / (1 + expf(-z));
+        y = z * e, slope = e * (1 + z * (1 - e));
+        return;
+    }
+    case ACT_GELU: {
+        const float below = 0.5f * (1 + erff(z * ROOT_HALF));
+        y = z * below, slope = below + z * ROOT_1_2PI * expf(-0.5f * z * z);
+        return;
+    }
+    case ACT_GELU_TANH: {
+        const float t = tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z));
+        y = 0.5f * z * (1 + t), slope = 0.5f * (1 + t) + 0.5f * z * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * z * z);
+        return;
+    }
+    default: y = z, slope = 1;
+    }
+}
+
+// Which rows an expert has: offsets that ascend, 32 or 64 bits each, kept within the rows there are.
+struct Groups {
+    const void *offsets;                         // NULL: one, of all rows
+    uint32_t count;
+    bool wide;
+    uint64_t rows;
+    __device__ __forceinline__ uint64_t at(uint32_t i) const
+    {
+        if (!offsets) return i ? rows : 0;
+        const int64_t v = wide ? static_cast<const int64_t *>(offsets)[i] : static_cast<const int32_t *>(offsets)[i];
+        return v < 0 ? 0 : static_cast<uint64_t>(v) < rows ? static_cast<uint64_t>(v) : rows;
+    }
+};
+
+// Where each group's rows begin, count + 1 of them in shared memory: the offsets, none below one before it (so that no row has two groups
+// whatever they are).  By the block's first warp; the caller's barrier follows.
+__device__ __forceinline__ void group_starts(const Groups &g, uint32_t *starts)
+{
+    if (threadIdx.x >= 32) return;
+    uint32_t most = 0;
+    for (uint32_t i0 = 0; i0 <= g.count; i0 += 32) {
+        const uint32_t i = i0 + threadIdx.x;
+        uint32_t v = i <= g.count ? static_cast<uint32_t>(g.at(i)) : 0;
+#pragma unroll
+        for (uint32_t o = 1; o < 32; o <<= 1) {
+            const uint32_t below = __shfl_up_sync(~0u, v, o);
+            if (threadIdx.x >= o) v = max(v, below);
+        }
+        v = max(v, most);
+        if (i <= g.count) starts[i] = v;
+        most = __shfl_sync(~0u, v, 31);
+    }
+}
+
+// Of count + 1 ascending starts the last group whose start is not above `row` (empty groups before it are passed over).
+__device__ __forceinline__ uint32_t group_of(const uint32_t *starts, uint32_t count, uint32_t row)
+{
+    uint32_t lo = 0, hi = count;                                 // starts[lo] <= row < starts[hi], or an end
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (starts[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+constexpr uint32_t MAX_EXPERTS = 1024;
+constexpr uint32_t EG_THREADS = 128, EG_ROWS = 32;
+
+struct EpilogueGradArgs {
+    const void *dy, *times;                      // times: or NULL, rows times_stride apart
+    const float *z;                              // NULL without an activation and `times`
+    void *dz, *dtimes;                           // or NULL
+    float *partial;                              // [chunk of rows + group][out]: sums of dz, or NULL
+    Groups groups;
+    uint64_t rows, out, times_stride, dz_stride;
+    uint32_t vectors, activation;
+};
+
+template <int N>
+__device__ __forceinline__ void load_floats(const float *from, float *to)
+{
+    constexpr int B = N * 4 < 16 ? N * 4 : 16;
+#pragma unroll
+    for (int i = 0; i < N * 4 / B; i++) reinterpret_cast<typename Raw<B>::type *>(to)[i] = reinterpret_cast<const typename Raw<B>::type *>(from)[i];
+}
+
+// dz = dy times act'(z), dtimes = dy act(z), and what each chunk of rows adds to the gradient of its groups' bias: a chunk and a group that
+// meet have the place chunk + group, which no other two have.  Rows of no group get zeros.
+//
+// z comes in 32 bits: in 16 its rounding would be worse in dtimes than the result's own (one and a half times the error of a z that is not rounded).
+// Bound by HBM.  A thread has a vector of columns and goes down a chunk's rows.
+template <class T, int VB>
+__global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGradArgs a)
+{
+    using V = Vec<T, VB>;
+    using R = typename Raw<VB>::type;
+    __shared__ uint32_t starts[MAX_EXPERTS + 1];
+    wait_for_previous();
+    let_next_start();
+    group_starts(a.groups, starts);
+    __syncthreads();
+    const uint64_t v = blockIdx.y * static_cast<uint64_t>(EG_THREADS) + threadIdx.x;
+    const uint32_t chunk = blockIdx.x, begin = chunk * EG_ROWS, end = begin + EG_ROWS < a.rows ? begin + EG_ROWS : static_cast<uint32_t>(a.rows);
+    if (v >= a.vectors) return;
+    const uint32_t first = starts[0], last = starts[a.groups.count];
+    uint32_t group = group_of(starts, a.groups.count, begin < first ? first : begin);
+    float sum[V::N];
+#pragma unroll
+    for (int e = 0; e < V::N; e++) sum[e] = 0;
+    bool any = false;
+    auto flush = [&] {
+        if (a.partial && any) {
+            float *to = a.partial + (static_cast<uint64_t>(chunk) + group) * a.out + v * V::N;
+#pragma unroll
+            for (int e = 0; e < V::N; e++) to[e] = sum[e];
+        }
+#pragma unroll
+        for (int e = 0; e < V::N; e++) sum[e] = 0;
+        any = false;
+    };
+    for (uint32_t t = begin; t < end; t++) {
+        const bool on = t >= first && t < last;
+        if (on && t >= starts[group + 1]) {
+            flush();
+            group = group_of(starts, a.groups.count, t);
+        }
+        V d, m, dz, dm;
+        alignas(16) float z[V::N] = {};
+        d.raw = m.raw = dz.raw = dm.raw = {};
+        if (on) {
+            d.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + t * a.out)[v];
+            if (a.z) load_floats<V::N>(a.z + t * a.out + v * V::N, z);
+            if (a.times) m.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.times) + t * a.times_stride)[v];
+#pragma unroll
+            for (int e = 0; e < V::N; e++) {
+                float y, slope;
+                act_and_slope(a.activation, z[e], y, slope);
+                const float g = widen(d.e[e]);
+                dm.e[e] = narrow<T>(g * y);
+                float u = g * slope;
+                if (a.times) u *= widen(m.e[e]);
+                sum[e] += u;
+                dz.e[e] = narrow<T>(u);
+            }
+            any = true;
+        }
+        if (a.dz) reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = dz.raw;
+        if (a.dtimes) reinterpret_cast<R *>(static_cast<T *>(a.dtimes) + t * a.out)[v] = dm.raw;
+    }
+    flush();
+}
+
+// A group's bias gradient: what the chunks that its rows lie in have for it, in their order.
+template <class T>
+__global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups groups, uint64_t out, T *dbias)
+{
+    __shared__ uint32_t starts[MAX_EXPERTS + 1];
+    __shared__ float sums[8][32];
+    wait_for_previous();
+    let_next_start();
+    group_starts(groups, starts);
+    __syncthreads();
+    const uint32_t g = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t d = blockIdx.x * 32ull + lane;
+    float sum = 0;
+    if (starts[g + 1] > starts[g] && d < out)
+        for (uint32_t c = starts[g] / EG_ROWS + warp; c <= (starts[g + 1] - 1) / EG_ROWS; c += 8) sum += partial[(static_cast<uint64_t>(c) + g) * out + d];
+    sums[warp][lane] = sum;
+    __syncthreads();
+    if (warp || d >= out) return;
+    for (uint32_t w = 1; w < 8; w++) sum += sums[w][lane];
+    dbias[g * out + d] = narrow<T>(sum);
+}
+
+}  // namespace lmz

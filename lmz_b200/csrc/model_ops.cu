@@ -2,7 +2,6 @@
 // adapters, merges.  Declarations and the per-function contract live in include/lmz_b200.h.
 #include <algorithm>
 #include <cstdint>
-#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/lmz_b200.h"
@@ -24,65 +23,7 @@ static_assert(M_MAX_PLACES == LMZ_GPU_MAX_RANK);
 #include "host_error.inl"
 #include "host_device.inl"
 #include "host_gave_up.inl"
-
-static uint32_t element_bytes(int dtype) { return dtype == LMZ_GPU_F32 ? 4 : dtype == LMZ_GPU_BF16 || dtype == LMZ_GPU_F16 ? 2 : 0; }
-
-// The widest vector, of at most 16 bytes, that rows of `row_bytes` at the given addresses and strides are made of.
-static uint32_t vector_bytes(uint64_t row_bytes, std::initializer_list<uint64_t> at)
-{
-    uint64_t bits = row_bytes | 16;
-    for (uint64_t v : at) bits |= v;
-    return static_cast<uint32_t>(bits & (~bits + 1));
-}
-
-static uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
-
-// f(type tag, vector width tag) for a type and width; EUNSUPPORTED for a width below the type's.
-template <class T, class F>
-static int by_width(uint32_t vb, F f)
-{
-    switch (vb) {
-    case 16: return f(Vec<T, 16>{});
-    case 8: return f(Vec<T, 8>{});
-    case 4: return f(Vec<T, 4>{});
-    case 2:
-        if constexpr (sizeof(T) == 2) return f(Vec<T, 2>{});
-        break;
-    }
-    return fail_msg(LMZ_GPU_EUNSUPPORTED, "a tensor does not start on a boundary of its elements");
-}
-
-template <class F>
-static int by_type(int dtype, uint32_t vb, F f)
-{
-    if (dtype == LMZ_GPU_BF16) return by_width<__nv_bfloat16>(vb, [&](auto v) { return f(__nv_bfloat16{}, v); });
-    if (dtype == LMZ_GPU_F16) return by_width<__half>(vb, [&](auto v) { return f(__half{}, v); });
-    if (dtype == LMZ_GPU_F32) return by_width<float>(vb, [&](auto v) { return f(float{}, v); });
-    return fail_msg(LMZ_GPU_EUNSUPPORTED, "an element type other than BF16, F16 and F32");
-}
-
-// A launch in clusters along x whose blocks may start before the kernel in front of it has ended: each of these kernels waits
-// for that itself, before it reads or writes what another may have to do with.
-static cudaLaunchConfig_t clustered(dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, unsigned cluster, cudaLaunchAttribute (&attrs)[2])
-{
-    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[0].val.programmaticStreamSerializationAllowed = 1;
-    attrs[1].id = cudaLaunchAttributeClusterDimension;
-    attrs[1].val.clusterDim.x = cluster, attrs[1].val.clusterDim.y = 1, attrs[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = cs, c.attrs = attrs, c.numAttrs = cluster > 1 ? 2 : 1;
-    return c;
-}
-
-// The same without clusters.
-template <class K, class... A>
-static int launch(const char *what, K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t cs, A... args)
-{
-    cudaLaunchAttribute attrs[2]{};
-    const cudaLaunchConfig_t c = clustered(grid, threads, smem, cs, 1, attrs);
-    CK(what, cudaLaunchKernelEx(&c, kernel, args...));
-    return LMZ_GPU_OK;
-}
+#include "host_launch.inl"
 
 static uint32_t lanes_log(uint32_t vectors)
 {
@@ -204,6 +145,30 @@ API int lmz_gpu_rows_grad_dev(const void *d_dy, uint64_t n, uint64_t dim, int dt
     });
 }
 
+API size_t lmz_gpu_order_work_bytes(uint64_t n) { return 3 * up256(n * 4); }
+
+API int lmz_gpu_order_dev(const void *d_ids, int id_bytes, uint64_t n, uint64_t experts, uint32_t *d_order, uint32_t *d_offsets, void *d_work, void *cuda_stream)
+{
+    if (id_bytes != 4 && id_bytes != 8) return fail_msg(LMZ_GPU_EUNSUPPORTED, "ids are int32 or int64");
+    if (experts == 0 || experts > LMZ_GPU_MAX_EXPERTS || n >= 1ull << 31) return report(LMZ_GPU_EUNSUPPORTED, "between 1 and %d experts, below 2^31 ids", LMZ_GPU_MAX_EXPERTS);
+    const int rc = device_ready();
+    if (rc) return rc;
+    const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
+    if (n == 0) {
+        CK("cudaMemsetAsync", cudaMemsetAsync(d_offsets, 0, (experts + 1) * 4, cs));
+        return LMZ_GPU_OK;
+    }
+    uint8_t *work = static_cast<uint8_t *>(d_work);
+    auto words = [&](int i) { return reinterpret_cast<uint32_t *>(work + i * up256(n * 4)); };
+    const int last = experts >> SORT_DIGIT ? 1 : 0;              // the side that the last pass writes
+    SortArgs s{};
+    s.ids = d_ids, s.n = n, s.nkeys = experts, s.wide = id_bytes == 8, s.start = d_offsets;
+    s.keys[0] = words(0), s.keys[1] = words(1), s.pos[last] = d_order, s.pos[1 - last] = words(2);
+    int side = 0;
+    const int failed = launch_sort(s, cs, &side);
+    return failed ? failed : side == last ? LMZ_GPU_OK : fail_msg(LMZ_GPU_EUNSUPPORTED, "a sort of other passes than it was laid out for");
+}
+
 // ------------------------------------------------------------------ adapters
 
 static int check_projection(const lmz_projection *p)
@@ -221,34 +186,6 @@ static int check_projection(const lmz_projection *p)
 static TokenIndex token_index(const lmz_projection *p)
 {
     return {p->index, static_cast<const float *>(p->scales), p->scale, p->adapters, p->index_bytes == 8};
-}
-
-static uint64_t up8(uint64_t n) { return (n + 7) & ~7ull; }
-static uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
-
-// Rows of 16-bit elements that TMA and 16-byte copies take as they lie.
-static bool on_boundary(const void *p, uint64_t cols, uint64_t stride) { return address(p) % 16 == 0 && stride % 8 == 0 && stride >= cols; }
-
-// A tensor map of planes x rows x cols 16-bit elements, a plane's rows behind those of the plane before: tiles of 64 columns
-// with the 128-byte swizzle.
-static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0,
-                      uint32_t tile_planes = 1)
-{
-    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Encode encode = [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
-        return reinterpret_cast<Encode>(f);
-    }();
-    if (!encode) return fail_msg(LMZ_GPU_EUNSUPPORTED, "the driver makes no tensor maps");
-    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {stride * 2, stride * rows * 2};
-    const cuuint32_t box[3] = {STEP_K, tile_rows, tile_planes}, steps[3] = {1, 1, 1};
-    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes ? 3 : 2, const_cast<void *>(p), dims,
-                              strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? LMZ_GPU_OK : report(LMZ_GPU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
 
 // Whether a projection that finds more than a quarter of its sixteens of tokens with several adapters takes the tokens in the
@@ -307,13 +244,6 @@ API size_t lmz_gpu_project_work_bytes(const lmz_projection *p, int grad) { retur
 constexpr uint32_t OPS_SMEM = 201u << 10;      // dynamic shared memory that the kernels below are laid out within
 constexpr uint32_t PROJECT_SMEM = 222u << 10;
 static_assert(PROJECT_SMEM + sizeof(ProjectShared) <= 227u << 10);
-
-static uint32_t tmem_columns(uint32_t n)
-{
-    uint32_t c = 32;
-    while (c < n) c *= 2;
-    return c;
-}
 
 template <class T, bool MN, bool PAIR>
 static int launch_project_as(ProjectArgs<T> &a, unsigned grid, cudaStream_t cs)

@@ -11,6 +11,7 @@ template <> struct Raw<16> { using type = uint4; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
+template <> struct Raw<1> { using type = uint8_t; };
 
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }

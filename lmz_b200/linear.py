@@ -1,0 +1,174 @@
+"""Products of activations with a checkpoint's weights, and what stands behind them in a layer: bias, activation, an
+elementwise factor (the other half of a gated block) and the residual, in the product's own kernel.
+
+`adapters.project` is the same for a frozen weight with adapters of many requests beside it, `experts.project` for rows that
+have different weights.
+"""
+from __future__ import annotations
+
+from . import _ops, gpu
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def project(x, weight, bias=None, activation=None, times=None, residual=None):
+    """`act(x @ weight.T + bias) * times + residual`.
+
+    `x`: [..., in], `weight`: [out, in], `bias`: [out], `times` and `residual`: [..., out], all bfloat16 or all float16; what is not given is left
+    out.  `activation`: None, "relu", "silu", "gelu" (with the error function) or "gelu_tanh" (its approximation by tanh).
+
+    Returns a contiguous [..., out], worked out in 32 bits and rounded once.  Differentiable once, in all five tensors; with an
+    activation or a factor the sums are kept for that in 32 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type.
+    Gradients are the same in every run."""
+    import torch
+    index = _ops.on_cuda("x weight bias times residual", x, weight, bias, times, residual)
+    code = _ops.type_code(x, "x", half_only=True)
+    for name, t in (("weight", weight), ("bias", bias), ("times", times), ("residual", residual)):
+        if t is not None and t.dtype is not x.dtype:
+            raise TypeError(f"{name} is {t.dtype}, but x {x.dtype}")
+    kind = _activation(activation)
+    _check_shapes(x, weight, bias, times, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, times, residual)):
+        return _function().apply(x, weight, bias, times, residual, None, kind)
+    return _forward(index, code, code, kind, x, weight, bias, times, residual, None, None, None, False)[0]
+
+
+def project_8bit(x, x_scale, weight, weight_scale, bias=None, activation=None, times=None, residual=None, dtype=None):
+    """The same for rows and a weight in 8 bits: `act(x_scale * weight_scale * (x @ weight.T) + bias) * times + residual`.
+
+    `x`: [..., in] and `weight`: [out, in], float8_e4m3fn; `x_scale`: x's leading shape, one per row, and `weight_scale`: [out], float32
+    (what `norms.rms_norm_8bit` and `norms.to_8bit` return).  `dtype`: the result's, bfloat16 (the default) or float16; bias, times and residual
+    are of it.  Products of 8 bits are exact and summed in 32 bits.  Not differentiable."""
+    import torch
+    index = _ops.on_cuda("x x_scale weight weight_scale bias times residual", x, x_scale, weight, weight_scale, bias, times, residual)
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError(f"dtype must be bfloat16 or float16, not {dtype}")
+    for name, t in (("x", x), ("weight", weight)):
+        if t.dtype is not torch.float8_e4m3fn:
+            raise TypeError(f"{name} must be float8_e4m3fn, not {t.dtype}")
+    for name, t in (("bias", bias), ("times", times), ("residual", residual)):
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"{name} is {t.dtype}, but the result {dtype}")
+    kind = _activation(activation)
+    _check_shapes(x, weight, bias, times, residual)
+    for name, t, shape in (("x_scale", x_scale, x.shape[:-1]), ("weight_scale", weight_scale, weight.shape[:1])):
+        if t.dtype is not torch.float32 or t.shape != shape:
+            raise ValueError(f"{name} must be float32 {list(shape)}, not {t.dtype} {list(t.shape)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, x_scale, weight, weight_scale, bias, times, residual)):
+        raise ValueError("project_8bit has no gradient: call it under torch.no_grad()")
+    return _forward(index, _ops.E4M3, _ops.BF16 if dtype is torch.bfloat16 else _ops.F16, kind, x, weight, bias, times, residual, None, x_scale, weight_scale, False)[0]
+
+
+def _activation(name) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {', '.join(map(repr, ACTIVATIONS))}, not {name!r}") from None
+
+
+def _check_shapes(x, weight, bias, times, residual):
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} do not fit [..., in] and [out, in]")
+    out, inp = weight.shape
+    if not out or not inp:
+        raise ValueError("an empty weight")
+    if weight.stride(1) != 1 and inp > 1:
+        raise ValueError("the elements of a row of the weight must be next to each other")
+    if bias is not None and bias.shape != (out,):
+        raise ValueError(f"bias must be [{out}], not {list(bias.shape)}")
+    for name, t in (("times", times), ("residual", residual)):
+        if t is not None and t.shape != (*x.shape[:-1], out):
+            raise ValueError(f"{name} must be {[*x.shape[:-1], out]}, not {list(t.shape)}")
+
+
+def _call(code, rcode, kind, x, weight, bias, times, residual, offsets):
+    """(`lmz_product`, what it points to) for x as [rows, in]."""
+    at = lambda t: None if t is None else t.data_ptr()     # noqa: E731
+    x, times, residual, bias, offsets = _ops.rows_of(x), _ops.rows_of(times), _ops.rows_of(residual), _ops.packed(bias), _ops.packed(offsets)
+    p = _ops.Product(x.data_ptr(), weight.data_ptr(), at(bias), at(times), at(residual), at(offsets))
+    p.rows, p.in_ = x.shape
+    p.out, p.x_stride, p.weight_stride = weight.shape[-2], x.stride(0), weight.stride(-2)
+    p.experts, p.weight_plane = (1, 0) if weight.dim() == 2 else (weight.shape[0], weight.stride(0))
+    if times is not None:
+        p.times_stride = times.stride(0)
+    if residual is not None:
+        p.residual_stride = residual.stride(0)
+    p.dtype, p.result_dtype, p.activation = code, rcode, kind
+    if offsets is not None:
+        p.offset_bytes = offsets.element_size()
+    return p, (x, times, residual, bias, offsets)
+
+
+def _work(p, grad: int, like):
+    import torch
+    size = gpu.library().lmz_gpu_product_work_bytes(p, grad)
+    if not size:
+        return None
+    work = like.new_empty(size, dtype=torch.uint8)
+    p.work = work.data_ptr()
+    return work
+
+
+def _forward(index, code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, keep):
+    """(y, what the gradients need of the sums if `keep`)."""
+    import torch
+    dtype = torch.bfloat16 if rcode == _ops.BF16 else torch.float16
+    y, z = x.new_empty((*x.shape[:-1], weight.shape[-2]), dtype=dtype), None
+    p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets)
+    x_scale, weight_scale = _ops.packed(x_scale), _ops.packed(weight_scale)
+    p.y = y.data_ptr()
+    if x_scale is not None:
+        p.x_scale, p.weight_scale = x_scale.data_ptr(), weight_scale.data_ptr()
+    if keep and (kind or times is not None):
+        z = y.new_empty(y.shape, dtype=torch.float32)
+        p.z = z.data_ptr()
+    held = held, _work(p, 0, x)                            # (copies and workspace live until the launch)
+    _ops.launch(index, "lmz_gpu_product_dev", p)
+    return y, z
+
+
+def _backward(kind, dy, x, weight, bias, times, offsets, z, wanted):
+    """The gradients of x, weight, bias and times, where `wanted`."""
+    _ops.no_tangents("dy", dy)
+    code = _ops.type_code(x, "x", half_only=True)
+    grads = [t.new_empty(t.shape) if w else None for t, w in zip((x, weight, bias, times), wanted)]
+    dy = _ops.packed(dy)
+    p, held = _call(code, code, kind, x, weight, bias, times, None, offsets)
+    p.dy = dy.data_ptr()
+    if z is not None:
+        p.z = z.data_ptr()
+    p.dx, p.dweight, p.dbias, p.dtimes = (None if t is None else t.data_ptr() for t in grads)
+    held = held, _work(p, 1, x)
+    _ops.launch(x.get_device(), "lmz_gpu_product_grad_dev", p)
+    return grads
+
+
+def _function():
+    """The autograd function (made on first use: importing this package does not import torch)."""
+    global _made
+    if _made is None:
+        import torch
+
+        class Product(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x, weight, bias, times, residual, offsets, kind):
+                code = _ops.type_code(x, "x", half_only=True)
+                y, z = _forward(x.get_device(), code, code, kind, x, weight, bias, times, residual, offsets, None, None, True)
+                ctx.save_for_backward(x, weight, bias, times, offsets, z)
+                ctx.kind = kind
+                return y
+
+            @staticmethod
+            @_ops.once
+            def backward(ctx, dy):
+                x, weight, bias, times, offsets, z = ctx.saved_tensors
+                wanted = ctx.needs_input_grad[:4]
+                grads = _backward(ctx.kind, dy, x, weight, bias, times, offsets, z, wanted) if any(wanted) else [None] * 4
+                return *grads, dy if ctx.needs_input_grad[4] else None, None, None
+
+        _made = Product
+    return _made
+
+
+_made = None
