@@ -1,5 +1,7 @@
 // What stands behind a product's sums, forwards and backwards:  z = sums + bias,  y = act(z) times + residual.
 #pragma once
+#include <type_traits>
+
 #include "tcgen.cuh"
 #include "vectors.cuh"
 
@@ -17,6 +19,22 @@ __device__ __forceinline__ float act(uint32_t kind, float z)
     case ACT_GELU: return 0.5f * z * (1 + erff(z * ROOT_HALF));
     case ACT_GELU_TANH: return 0.5f * z * (1 + tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z)));
     default: return z;
+    }
+}
+
+// N of them: the kind is asked for once.
+template <int N>
+__device__ __forceinline__ void act_all(uint32_t kind, float *v)
+{
+    auto each = [&](auto k) {
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = act(decltype(k)::value, v[e]);
+    };
+    switch (kind) {
+    case ACT_RELU: return each(std::integral_constant<uint32_t, ACT_RELU>{});
+    case ACT_SILU: return each(std::integral_constant<uint32_t, ACT_SILU>{});
+    case ACT_GELU: return each(std::integral_constant<uint32_t, ACT_GELU>{});
+    case ACT_GELU_TANH: return each(std::integral_constant<uint32_t, ACT_GELU_TANH>{});
     }
 }
 

@@ -70,10 +70,9 @@ static uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
 // Rows of 16-bit elements that TMA and 16-byte copies take as they lie.
 static bool on_boundary(const void *p, uint64_t cols, uint64_t stride) { return address(p) % 16 == 0 && stride % 8 == 0 && stride >= cols; }
 
-// A tensor map of planes x rows x cols 16-bit elements, a plane's rows behind those of the plane before: tiles of 64 columns
-// with the 128-byte swizzle.
-static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0,
-                      uint32_t tile_planes = 1)
+// A tensor map of planes x rows x cols elements (planes 0: of rows x cols): tiles of 128 bytes of a row with the 128-byte swizzle.
+static int tile_map(CUtensorMap *map, const void *p, CUtensorMapDataType type, uint32_t bytes, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows,
+                    uint64_t planes, uint64_t plane_stride, uint32_t tile_planes = 1)
 {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -84,12 +83,27 @@ static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols,
         return reinterpret_cast<Encode>(f);
     }();
     if (!encode) return fail_msg(LMZ_GPU_EUNSUPPORTED, "the driver makes no tensor maps");
-    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {stride * 2, stride * rows * 2};
-    const cuuint32_t box[3] = {STEP_K, tile_rows, tile_planes}, steps[3] = {1, 1, 1};
-    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes ? 3 : 2, const_cast<void *>(p), dims,
-                              strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {stride * bytes, plane_stride * bytes};
+    const cuuint32_t box[3] = {ROW_BYTES / bytes, tile_rows, tile_planes}, steps[3] = {1, 1, 1};
+    auto make = [&] {
+        return encode(map, type, planes ? 3 : 2, const_cast<void *>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = make();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {                       // a thread that has launched nothing yet (autograd's): the driver asks for its context
+        int dev = 0;
+        CK("cudaGetDevice", cudaGetDevice(&dev));
+        CK("cudaSetDevice", cudaSetDevice(dev));
+        r = make();
+    }
     return r == CUDA_SUCCESS ? LMZ_GPU_OK : report(LMZ_GPU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+// The same of 16-bit elements, a plane's rows behind those of the plane before.
+static int tensor_map(CUtensorMap *map, const void *p, bool bf16, uint64_t cols, uint64_t rows, uint64_t stride, uint32_t tile_rows, uint64_t planes = 0,
+                      uint32_t tile_planes = 1)
+{
+    return tile_map(map, p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols, rows, stride, tile_rows, planes, stride * rows, tile_planes);
 }
 
 static uint32_t tmem_columns(uint32_t n)

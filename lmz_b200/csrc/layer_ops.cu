@@ -19,6 +19,13 @@ static_assert(MAX_EXPERTS == LMZ_GPU_MAX_EXPERTS && ACT_SILU == LMZ_GPU_ACT_SILU
 #include "host_device.inl"
 #include "host_launch.inl"
 
+// Where this source's kernels say that one has given up waiting (lmz_gpu_ops_gave_up).
+__attribute__((visibility("hidden"))) int layer_gave_up_word(void **word)
+{
+    CK("cudaGetSymbolAddress", cudaGetSymbolAddress(word, g_gave_up));
+    return LMZ_GPU_OK;
+}
+
 // ------------------------------------------------------------------ norms
 
 static int check_norm(const lmz_norm *p)
@@ -159,10 +166,18 @@ static int check_product(const lmz_product *p)
 
 static Groups groups_of(const lmz_product *p) { return {p->offsets, p->experts, p->offset_bytes == 8, p->rows}; }
 
-// What a product's kernels leave each other.
+// Rows that TMA takes as they lie: they start on 16 bytes.  (A single row has no next one.)
+static bool in_place(const void *p, uint64_t bytes, uint64_t cols, uint64_t rows, uint64_t stride)
+{
+    return address(p) % 16 == 0 && (rows <= 1 ? cols * bytes % 16 == 0 : stride * bytes % 16 == 0 && stride >= cols);
+}
+
+static uint64_t up16(uint64_t n) { return (n + 15) & ~15ull; }
+
+// What a product's kernels read in place of tensors that do not lie on boundaries, and leave each other.
 struct ProductLayout {
-    uint64_t dz, partial, end = 0;
-    bool epilogue;                               // dz is not dy
+    uint64_t x, w, dz, partial, end = 0;
+    bool pack_x, pack_w, own_dz;                 // own_dz: dz is not dy, or does not lie where TMA takes it
     ProductLayout(const lmz_product *p, bool grad)
     {
         auto take = [&](bool on, uint64_t bytes) {
@@ -170,36 +185,132 @@ struct ProductLayout {
             if (on) end += up256(bytes);
             return r;
         };
-        epilogue = p->activation != ACT_NONE || p->times;
-        dz = take(grad && epilogue, p->rows * p->out * 2);
+        const uint64_t e = p->dtype == LMZ_GPU_E4M3 ? 1 : 2;
+        pack_x = !in_place(p->x, e, p->in, p->rows, p->x_stride);
+        pack_w = !in_place(p->weight, e, p->in, p->out, p->weight_stride) || (p->experts > 1 && (p->weight_plane * e % 16 || p->weight_plane < p->out * (p->out <= 1 ? p->in : p->weight_stride)));
+        own_dz = p->activation != ACT_NONE || p->times || !in_place(p->dy, 2, p->out, 2, p->out);
+        x = take(pack_x && (!grad || p->dweight), p->rows * up16(p->in) * e);
+        w = take(pack_w && (!grad || p->dx), p->experts * p->out * up16(p->in) * e);
+        dz = take(grad && own_dz, p->rows * up8(p->out) * 2);
         partial = take(grad && p->dbias, ((p->rows + EG_ROWS - 1) / EG_ROWS + p->experts) * p->out * 4);
     }
 };
 
 API size_t lmz_gpu_product_work_bytes(const lmz_product *p, int grad) { return ProductLayout(p, grad).end; }
 
-template <class T, class O>
-static int launch_product(const ProductArgs<T> &a, cudaStream_t cs)
+// x and the weight as the kernels take them: where they lie, or in the workspace (in one launch).
+template <class T>
+struct ProductInputs {
+    const T *x, *w;
+    uint64_t x_stride, w_stride, w_plane;
+    int rc = LMZ_GPU_OK;
+    ProductInputs(const lmz_product *p, const ProductLayout &l, bool want_x, bool want_w, cudaStream_t cs)
+        : x(static_cast<const T *>(p->x)), w(static_cast<const T *>(p->weight)), x_stride(p->rows <= 1 ? p->in : p->x_stride),
+          w_stride(p->out <= 1 ? p->in : p->weight_stride), w_plane(p->experts <= 1 ? p->out * w_stride : p->weight_plane)
+    {
+        using E = std::conditional_t<sizeof(T) == 1, uint8_t, uint16_t>;
+        AlignArgs args{};
+        uint32_t jobs = 0;
+        uint64_t most = 0;
+        const uint64_t pitch = up16(p->in);
+        auto job = [&](const T *&t, uint64_t plane_stride, uint64_t stride, uint64_t rows, uint64_t planes, uint64_t off) {
+            T *to = reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + off);
+            args.job[jobs++] = {t, to, plane_stride, stride, rows, p->in, pitch, rows * planes};
+            most = std::max(most, rows * planes * pitch * sizeof(T) / 16);
+            t = to;
+        };
+        if (want_x && l.pack_x) job(x, 0, p->x_stride, p->rows, 1, l.x), x_stride = pitch;
+        if (want_w && l.pack_w) job(w, p->weight_plane, p->weight_stride, p->out, p->experts, l.w), w_stride = pitch, w_plane = p->out * pitch;
+        if (jobs) rc = launch("launch k_align", k_align<E>, dim3(static_cast<unsigned>(std::min<uint64_t>((most + ALIGN_THREADS - 1) / ALIGN_THREADS, 1u << 20)), jobs), ALIGN_THREADS, 0, cs, args);
+    }
+};
+
+constexpr uint32_t PRODUCT_SMEM = 217u << 10;
+static_assert(PRODUCT_SMEM + sizeof(ProductShared) <= 227u << 10);
+
+template <class T, class O, int P, bool PAIR>
+static int launch_product_as(ProductArgs &a, unsigned grid, cudaStream_t cs)
 {
-    const dim3 grid(static_cast<unsigned>((a.feats + S_TILE - 1) / S_TILE), static_cast<unsigned>(std::min<uint64_t>(1024, (a.cols + S_TILE - 1) / S_TILE)),
-                    std::min(64u, a.groups.count));
-    return launch("launch k_product", k_product<T, O>, grid, S_THREADS, 0, cs, a);
+    static bool done[64];
+    const int rc = opt_in_smem(k_product<T, O, P, PAIR>, PRODUCT_SMEM, done);
+    if (rc) return rc;
+    a.stage_bytes = product_stage_bytes(a.nt, PAIR);
+    const uint32_t rest = ATOM_BYTES + G_EPILOGUE / 32 * G_TURN_BYTES;
+    a.stages = std::min<uint32_t>(G_MAX_STAGES, (PRODUCT_SMEM - rest) / a.stage_bytes);
+    cudaLaunchAttribute attrs[2]{};
+    const cudaLaunchConfig_t c = clustered(dim3(grid), G_THREADS, a.stages * a.stage_bytes + rest, cs, PAIR ? 2 : a.split, attrs);
+    CK("launch k_product", cudaLaunchKernelEx(&c, k_product<T, O, P, PAIR>, a));
+    return LMZ_GPU_OK;
+}
+
+// One of the three products: A, B and their strides; `a` has the rest.  `depth`: k, of all groups where it has them.
+template <class T, class O, int P>
+static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64_t a_plane, const T *bt, uint64_t b_stride, uint64_t depth, cudaStream_t cs)
+{
+    constexpr bool by_k = P == WEIGHT_GRAD;
+    constexpr uint32_t step_elements = ROW_BYTES / sizeof(T);
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    const uint64_t groups = a.groups.count, used = by_k ? groups : std::min<uint64_t>(groups, std::max<uint64_t>(a.cols, 1));
+    // (tiles of columns: an estimate, and no fewer than there can be)
+    auto col_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : used * ((a.cols / used + nt - 1) / nt + (a.cols / used % nt == 0 && groups > 1 ? 1 : 0)); };
+    auto most_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : groups == 1 ? (a.cols + nt - 1) / nt : a.cols / nt + used; };
+    const uint64_t rows_each = std::max<uint64_t>(1, a.cols / used);
+    const uint64_t all_steps = by_k ? std::max<uint64_t>(1, (depth / groups + STEP_K - 1) / STEP_K) : (depth + step_elements - 1) / step_elements;
+    // Tiles of 256 by 256 by pairs of CTAs, or of 128 features by 16 to 128 columns by one, or by a cluster that shares k: by what they are reckoned to
+    // take (in 10 ns).
+    uint64_t best = ~0ull;
+    bool pair = false;
+    a.split = 1;
+    auto consider = [&](bool p2, uint32_t nt, uint32_t split) {
+        const uint64_t feats = (a.feats + (p2 ? 2 : 1) * G_FEATS - 1) / ((p2 ? 2 : 1) * G_FEATS), places = p2 ? sms / 2 : sms;
+        const uint64_t n = feats * col_tiles(nt) * split;
+        if (split > 1 && feats * most_tiles(nt) * split > places) return;
+        const uint64_t waves = (n + places - 1) / places, steps = (all_steps + split - 1) / split;
+        const uint64_t step = p2 ? 30 : std::max<uint64_t>(19, std::min(n, places) * (G_FEATS + nt) / 940);
+        const uint64_t meeting = split == 1 ? 0 : split == 2 ? 150 + 5 * nt / 2 : 180 * split;
+        const uint64_t cost = waves * (step * steps + (p2 ? 600 : 4 * nt + meeting)) + 600;
+        if (cost < best) best = cost, pair = p2, a.nt = nt, a.split = split;
+    };
+    const uint64_t wide = by_k ? a.cols : rows_each;
+    for (uint32_t nt = by_k ? 64 : G_GROUP; nt < G_COLS; nt *= 2)
+        for (uint32_t split = 1; split <= 8 && 2 * split <= std::max<uint64_t>(2, all_steps); split *= 2)
+            if (nt == (by_k ? 64 : G_GROUP) || nt < 2 * wide) consider(false, nt, split);
+    if (wide > G_COLS / 2) consider(true, G_COLS, 1);
+    const uint64_t per = (pair ? 2 : 1) * G_FEATS, feat_tiles = (a.feats + per - 1) / per, most = feat_tiles * most_tiles(a.nt);
+    if (most >= 1u << 28) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many rows for a weight of this size");
+    a.feat_tiles = static_cast<uint32_t>(feat_tiles), a.col_tiles = static_cast<uint32_t>((a.cols + a.nt - 1) / a.nt);
+    a.steps = static_cast<uint32_t>((depth + step_elements - 1) / step_elements);
+    a.tmem_columns = tmem_columns(a.split > 1 ? a.nt : 2 * a.nt);
+    const CUtensorMapDataType type = sizeof(T) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const uint32_t cols_each = pair ? a.nt / 2 : a.nt;
+    if (P == FORWARD) rc = tile_map(&a.a, at, type, sizeof(T), depth, a.feats, a_stride, G_FEATS, groups, a_plane);
+    else if (P == ROWS_GRAD) rc = tile_map(&a.a, at, type, sizeof(T), a.feats, depth, a_stride, STEP_K, groups, a_plane);
+    else rc = tile_map(&a.a, at, type, sizeof(T), a.feats, depth, a_stride, STEP_K, 0, 0);
+    if (!rc && by_k) rc = tile_map(&a.b, bt, type, sizeof(T), a.cols, depth, b_stride, STEP_K, 0, 0);
+    else if (!rc) rc = tile_map(&a.b, bt, type, sizeof(T), depth, a.cols, b_stride, cols_each, 0, 0);
+    if (rc) return rc;
+    if (pair) return launch_product_as<T, O, P, true>(a, static_cast<unsigned>(std::min<uint64_t>(most, sms / 2) * 2), cs);
+    return launch_product_as<T, O, P, false>(a, static_cast<unsigned>(a.split > 1 ? most * a.split : std::min<uint64_t>(most, sms)), cs);
 }
 
 template <class T, class O>
 static int product_as(const lmz_product *p, cudaStream_t cs)
 {
-    ProductArgs<T> a{};
-    a.a = static_cast<const T *>(p->weight), a.b = static_cast<const T *>(p->x), a.out = p->y, a.z = p->z;
-    a.bias = p->bias, a.times = p->times, a.residual = p->residual, a.a_scale = p->weight_scale, a.b_scale = p->x_scale;
-    a.groups = groups_of(p), a.feats = p->out, a.cols = p->rows, a.depth = p->in;
-    a.a_f = p->weight_stride, a.a_k = 1, a.b_c = p->x_stride, a.b_k = 1, a.a_plane = p->weight_plane;
+    const ProductLayout l(p, false);
+    const ProductInputs<T> in(p, l, true, true, cs);
+    if (in.rc) return in.rc;
+    ProductArgs a{};
+    a.out = p->y, a.z = p->z, a.bias = p->bias, a.times = p->times, a.residual = p->residual, a.a_scale = p->weight_scale, a.b_scale = p->x_scale;
+    a.groups = groups_of(p), a.feats = p->out, a.cols = p->rows;
     a.times_stride = p->times_stride, a.residual_stride = p->residual_stride, a.activation = p->activation;
-    return launch_product<T, O>(a, cs);
+    a.vectors = vector_bytes(p->out * 2, {address(p->y), address(p->z), address(p->bias), address(p->times), p->times ? p->times_stride * 2 : 0, address(p->residual),
+                                          p->residual ? p->residual_stride * 2 : 0}) == 16;
+    return launch_product<T, O, FORWARD>(a, in.w, in.w_stride, in.w_plane, in.x, in.x_stride, p->in, cs);
 }
 
 template <class T>
-static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, void *dz, cudaStream_t cs)
+static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T *dz, cudaStream_t cs)
 {
     const uint64_t chunks = (p->rows + EG_ROWS - 1) / EG_ROWS;
     float *partial = p->dbias ? reinterpret_cast<float *>(static_cast<uint8_t *>(p->work) + l.partial) : nullptr;
@@ -207,7 +318,7 @@ static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, vo
         constexpr int VB = sizeof(vec.raw);
         EpilogueGradArgs a{};
         a.dy = p->dy, a.z = p->z, a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
-        a.rows = p->rows, a.out = a.dz_stride = p->out, a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation;
+        a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation;
         return launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, dim3(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS), EG_THREADS, 0, cs, a);
     });
     if (!rc && p->dbias)
@@ -225,26 +336,30 @@ static int product_grad_as(const lmz_product *p, cudaStream_t cs)
         return LMZ_GPU_OK;
     }
     const ProductLayout l(p, true);
-    T *own = l.epilogue ? reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + l.dz) : nullptr;
-    if (l.epilogue || p->dbias) {
-        const int rc = launch_epilogue_grad<T>(p, l, own, cs);
-        if (rc) return rc;
-    }
-    const T *dz = own ? own : static_cast<const T *>(p->dy), *w = static_cast<const T *>(p->weight), *x = static_cast<const T *>(p->x);
-    ProductArgs<T> a{};
-    a.groups = groups_of(p), a.feats = p->in;
+    const bool products = p->dx || p->dweight;
+    T *own = l.own_dz && products ? reinterpret_cast<T *>(static_cast<uint8_t *>(p->work) + l.dz) : nullptr;
+    int rc = LMZ_GPU_OK;
+    if (own || p->dbias || p->dtimes) rc = launch_epilogue_grad<T>(p, l, own, cs);
+    if (rc || !products) return rc;
+    const ProductInputs<T> in(p, l, p->dweight != nullptr, p->dx != nullptr, cs);
+    if (in.rc) return in.rc;
+    const T *dz = own ? own : static_cast<const T *>(p->dy);
+    const uint64_t dz_stride = own ? up8(p->out) : p->out;
+    auto args = [&](void *out, uint64_t cols) {
+        ProductArgs a{};
+        a.out = out, a.groups = groups_of(p), a.feats = p->in, a.cols = cols;
+        a.vectors = vector_bytes(p->in * 2, {address(out)}) == 16;
+        return a;
+    };
     if (p->dx) {
-        a.a = w, a.b = dz, a.out = p->dx, a.cols = p->rows, a.depth = p->out;
-        a.a_f = 1, a.a_k = p->weight_stride, a.b_c = p->out, a.b_k = 1, a.a_plane = p->weight_plane;
-        const int rc = launch_product<T, T>(a, cs);
-        if (rc) return rc;
+        ProductArgs a = args(p->dx, p->rows);
+        rc = launch_product<T, T, ROWS_GRAD>(a, in.w, in.w_stride, in.w_plane, dz, dz_stride, p->out, cs);
     }
-    if (p->dweight) {
-        a.a = x, a.b = dz, a.out = p->dweight, a.cols = p->out, a.depth = p->rows, a.by_k = true;
-        a.a_f = 1, a.a_k = p->x_stride, a.b_c = 1, a.b_k = p->out, a.a_plane = 0;
-        return launch_product<T, T>(a, cs);
+    if (!rc && p->dweight) {
+        ProductArgs a = args(p->dweight, p->out);
+        rc = launch_product<T, T, WEIGHT_GRAD>(a, in.x, in.x_stride, 0, dz, dz_stride, p->rows, cs);
     }
-    return LMZ_GPU_OK;
+    return rc;
 }
 
 API int lmz_gpu_product_dev(const lmz_product *p, void *cuda_stream)

@@ -553,13 +553,18 @@ static int project_grad_as(const lmz_projection *p, cudaStream_t cs)
     return launch_factor_grad<T>(p, jobs, count, tokens.order, start, cs);
 }
 
+int layer_gave_up_word(void **word);           // layer_ops.cu
+
 API int lmz_gpu_ops_gave_up(void)
 {
     const int rc = device_ready();
     if (rc) return rc;
-    void *word = nullptr;
+    void *word = nullptr, *layers = nullptr;
     CK("cudaGetSymbolAddress", cudaGetSymbolAddress(&word, g_gave_up));
-    return taken_word(word);
+    const int failed = layer_gave_up_word(&layers);
+    if (failed) return failed;
+    const int mine = taken_word(word), theirs = taken_word(layers);              // (both are taken, whatever the first says)
+    return mine < 0 ? mine : theirs < 0 ? theirs : mine | theirs;
 }
 
 API int lmz_gpu_project_dev(const lmz_projection *p, void *cuda_stream)

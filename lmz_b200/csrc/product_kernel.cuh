@@ -1,4 +1,4 @@
-// Products of rows with a weight, or with their experts' weights, their epilogue, and both gradients.
+// Products of rows with a weight, or with their experts' weights, their epilogue, and both gradients, on the tensor cores.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -7,82 +7,418 @@
 
 namespace lmz {
 
-__device__ __forceinline__ float widen(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
-
-// out[c][f] = sum over k of A(f, k) B(c, k), the three that a layer has:
-//   forwards         f: the output's features, c: rows,                  k: the input's; A is the weight, B is x
-//   rows' gradient   f: the input's features,  c: rows,                  k: the output's; A is the weight (k by k), B is dz
-//   weight's         f: the input's features,  c: the output's features, k: rows; A is x, B is dz (both k by k)
+// out[c][f] = sum over k of A(f, k) B(c, k), the three products that a layer has:
+//   FORWARD      f: the output's features, c: rows,                  k: the input's features;  A is the weight, B is x, both with their k side by side
+//   ROWS_GRAD    f: the input's features,  c: rows,                  k: the output's features; A is the weight with its f side by side, B is dz
+//   WEIGHT_GRAD  f: the input's features,  c: the output's features, k: rows;                  A is x, B is dz, with their f and c side by side
 // A group is an expert: in the first two its rows are some of c, in the last they are its k.
-template <class T>
-struct ProductArgs {
-    const T *a, *b;
-    void *out;
-    float *z;
-    const void *bias, *times, *residual;
-    const float *a_scale, *b_scale;              // of 8-bit features and rows, or NULL
-    Groups groups;
-    uint64_t feats, cols, depth;                 // of f, c and k (those of c, or of k, in all groups)
-    uint64_t a_f, a_k, b_c, b_k, a_plane, times_stride, residual_stride;
-    uint32_t activation;
-    bool by_k;                                   // groups are of k
+enum Product : int { FORWARD, ROWS_GRAD, WEIGHT_GRAD };
+
+constexpr uint32_t G_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
+constexpr uint32_t G_COLS = 256;               // most columns of a tile: its N, a TMEM column each
+constexpr uint32_t G_GROUP = 16;               // columns of a TMEM load
+constexpr uint32_t G_MAX_STAGES = 10, G_EPILOGUE = 256, G_THREADS = G_EPILOGUE + 96;
+constexpr uint32_t G_PITCH = 36;               // words from one column to the next where a warp turns 32 lanes' features round
+constexpr uint32_t G_TURN_BYTES = G_GROUP * G_PITCH * 4;      // a warp's
+constexpr uint32_t G_BLOCK = STEP_K * ROW_BYTES;              // 64 k of 64 f or c side by side
+
+struct ProductShared {
+    uint64_t full[G_MAX_STAGES], empty[G_MAX_STAGES], ready[G_MAX_STAGES];
+    uint64_t sums_full[2], sums_empty[2];
+    uint32_t tmem, over;
+    uint32_t starts[MAX_EXPERTS + 1], tiles[MAX_EXPERTS + 1];  // where a group's rows, and its tiles of columns, begin
 };
 
-constexpr uint32_t S_TILE = 64, S_K = 16, S_THREADS = 256;
+struct ProductArgs {
+    CUtensorMap a, b;
+    void *out;                                   // [c][f], a group's behind the one before where k has the groups
+    float *z;                                    // the sums and the bias, or NULL
+    const void *bias, *times, *residual;         // [group][f], [c][f], [c][f], or NULL
+    const float *a_scale, *b_scale;              // per f and per c: of 8-bit operands
+    Groups groups;
+    uint64_t feats, cols;                        // of f and c (those of c in all groups)
+    uint64_t times_stride, residual_stride;
+    uint32_t activation;
+    uint32_t steps;                              // of 128 bytes along k (not where k has the groups)
+    uint32_t nt;                                 // columns of a tile
+    uint32_t split;                              // CTAs of a cluster that share k
+    uint32_t feat_tiles, col_tiles;              // of G_FEATS (a pair: twice that) and, where k has the groups, of nt
+    uint32_t stages, stage_bytes, tmem_columns;
+    bool vectors;                                // rows of all tensors that the epilogue has to do with start on 16 bytes
+};
 
-template <class T, class O>
-__global__ void __launch_bounds__(S_THREADS) k_product(const ProductArgs<T> a)
+// Tiles of a stage: A's 128 f, and the columns' (of a pair's 256 each CTA has half).
+__host__ __device__ constexpr uint32_t product_stage_bytes(uint32_t nt, bool pair) { return (G_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
+
+// A tile's place.
+struct TilePlace {
+    uint32_t group, ft;
+    uint32_t c, c_end;                           // its first column, and its group's end
+    uint32_t k, k_rows;                          // WEIGHT_GRAD: the group's rows
+};
+
+// N neighbours of f of a column, from sums to result: z = sums + bias, y = act(z) times + residual.
+template <class O, int N>
+__device__ __forceinline__ void finish(const ProductArgs &a, uint64_t c, uint64_t f, uint64_t at, float *v, const float *bias, const float *a_scale, const O *times, const O *residual)
 {
-    __shared__ float as[S_K][S_TILE + 1], bs[S_K][S_TILE + 1];
-    __shared__ uint32_t starts[MAX_EXPERTS + 1];
-    wait_for_previous();
-    group_starts(a.groups, starts);
-    __syncthreads();
-    const uint32_t tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    const uint64_t f0 = static_cast<uint64_t>(blockIdx.x) * S_TILE;
-    for (uint32_t g = blockIdx.z; g < a.groups.count; g += gridDim.z) {
-        const uint64_t c_lo = a.by_k ? 0 : starts[g], c_hi = a.by_k ? a.cols : starts[g + 1];
-        const uint64_t k_lo = a.by_k ? starts[g] : 0, k_hi = a.by_k ? starts[g + 1] : a.depth;
-        for (uint64_t c0 = c_lo + static_cast<uint64_t>(blockIdx.y) * S_TILE; c0 < c_hi; c0 += static_cast<uint64_t>(gridDim.y) * S_TILE) {
-            float sum[4][4] = {};
-            for (uint64_t k0 = k_lo; k0 < k_hi; k0 += S_K) {
-                __syncthreads();
-                for (uint32_t i = tid; i < S_K * S_TILE; i += S_THREADS) {
-                    const uint32_t r = a.a_k == 1 ? i / S_K : i % S_TILE, k = a.a_k == 1 ? i % S_K : i / S_TILE;
-                    as[k][r] = f0 + r < a.feats && k0 + k < k_hi ? widen(a.a[(a.by_k ? 0 : g * a.a_plane) + (f0 + r) * a.a_f + (k0 + k) * a.a_k]) : 0;
-                    const uint32_t c = a.b_k == 1 ? i / S_K : i % S_TILE, j = a.b_k == 1 ? i % S_K : i / S_TILE;
-                    bs[j][c] = c0 + c < c_hi && k0 + j < k_hi ? widen(a.b[(c0 + c) * a.b_c + (k0 + j) * a.b_k]) : 0;
-                }
-                __syncthreads();
+    if (a.a_scale) {
+        const float s = a.b_scale[c];
 #pragma unroll
-                for (uint32_t k = 0; k < S_K; k++)
+        for (int e = 0; e < N; e++) v[e] *= a_scale[e] * s;
+    }
+    if (a.bias) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++)
+        for (int e = 0; e < N; e++) v[e] += bias[e];
+    }
+    if (a.z) {
+        if constexpr (N % 4 == 0) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; j++) sum[i][j] += bs[k][ty + i * 16] * as[k][tx + j * 16];
-            }
-            for (uint32_t i = 0; i < 4; i++)
-                for (uint32_t j = 0; j < 4; j++) {
-                    const uint64_t c = c0 + ty + i * 16, f = f0 + tx + j * 16, at = ((a.by_k ? g * a.cols : 0) + c) * a.feats + f;
-                    if (c >= c_hi || f >= a.feats) continue;
-                    float z = sum[i][j];
-                    if (a.a_scale) z *= a.a_scale[f] * a.b_scale[c];
-                    if (a.bias) z += widen(static_cast<const O *>(a.bias)[g * a.feats + f]);
-                    if (a.z) a.z[at] = z;
-                    float y = act(a.activation, z);
-                    if (a.times) y *= widen(static_cast<const O *>(a.times)[c * a.times_stride + f]);
-                    if (a.residual) y += widen(static_cast<const O *>(a.residual)[c * a.residual_stride + f]);
-                    static_cast<O *>(a.out)[at] = narrow<O>(y);
-                }
+            for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(a.z + at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        } else {
+            for (int e = 0; e < N; e++) a.z[at + e] = v[e];
         }
     }
-    if (a.by_k) return;
-    const uint64_t first = starts[0], last = starts[a.groups.count], idle = first + (a.cols - last);          // rows of no group
-    const uint64_t block = (static_cast<uint64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-    const uint64_t blocks = static_cast<uint64_t>(gridDim.x) * gridDim.y * gridDim.z;
-    for (uint64_t i = block * S_THREADS + tid; i < idle * a.feats; i += blocks * S_THREADS) {
-        const uint64_t r = i / a.feats, c = r < first ? r : last + (r - first);
-        static_cast<O *>(a.out)[c * a.feats + i % a.feats] = narrow<O>(0.0f);
+    act_all<N>(a.activation, v);
+    if (a.times) {
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] *= widen(times[e]);
+    }
+    if (a.residual) {
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] += widen(residual[e]);
+    }
+}
+
+// Features are the tensor core's M and columns its N, whatever their number: a single row streams the weight past 16 columns, a batch past 256.
+//
+// Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; eight warps take the
+// sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.  They turn 32 features and 16 columns round
+// in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.
+// Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile's columns behind its group's last are another group's
+// rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
+// last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.
+// Few tiles: the CTAs of a cluster share k, and their sums meet in distributed shared memory.
+// Many (PAIR): two CTAs multiply 256 features by 256 columns together, each loading half of both.
+template <class T, class O, int P, bool PAIR>
+__global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant__ ProductArgs a)
+{
+    constexpr uint32_t CTAS = PAIR ? 2 : 1, STEP = ROW_BYTES / sizeof(T);
+    constexpr bool A_MN = P != FORWARD, B_MN = P == WEIGHT_GRAD, BY_K = P == WEIGHT_GRAD;
+    static_assert(sizeof(T) == 2 || P == FORWARD);
+    extern __shared__ uint8_t g_smem[];
+    __shared__ ProductShared s;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t side = PAIR ? cluster_rank() : 0, rank = !PAIR && a.split > 1 ? cluster_rank() : 0;
+    const uint32_t team = PAIR ? 2 : a.split;
+    const uint32_t first = blockIdx.x / team, stride = gridDim.x / team;
+    const uint32_t ring = (smem_addr(g_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
+    uint8_t *const local = g_smem + (ring - smem_addr(g_smem));
+    volatile uint32_t *over = &s.over;
+
+    if (tid == 0) {
+        s.over = 0;
+        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], BY_K ? 1 : CTAS), bar_init(&s.empty[i], 1), bar_init(&s.ready[i], CTAS);
+        for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], CTAS * G_EPILOGUE / 32);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if constexpr (PAIR) {
+        __syncthreads();
+        cluster_barrier();
+    }
+    if (warp == 9) tmem_alloc<PAIR>(&s.tmem, a.tmem_columns);
+    wait_for_previous();
+    group_starts(a.groups, s.starts);
+    if (warp == 0 && !BY_K) {
+        __syncwarp();
+        uint32_t sum = 0;
+        for (uint32_t i0 = 0; i0 <= a.groups.count; i0 += 32) {
+            const uint32_t i = i0 + lane, mine = i < a.groups.count ? (s.starts[i + 1] - s.starts[i] + a.nt - 1) / a.nt : 0;
+            uint32_t v = mine;
+#pragma unroll
+            for (uint32_t o = 1; o < 32; o <<= 1) {
+                const uint32_t below = __shfl_up_sync(~0u, v, o);
+                if (lane >= o) v += below;
+            }
+            if (i <= a.groups.count) s.tiles[i] = sum + v - mine;
+            sum += __shfl_sync(~0u, v, 31);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = s.tmem, groups = a.groups.count;
+    const uint32_t col_tiles = BY_K ? a.col_tiles : s.tiles[groups], tiles = a.feat_tiles * col_tiles * (BY_K ? groups : 1);
+
+    // Eight column tiles side by side, features outside: what a wave reads of A and B stays in L2.
+    auto place = [&](uint32_t tile) {
+        TilePlace p;
+        uint32_t in_group = tile;
+        p.group = 0;
+        if (BY_K) p.group = tile / (a.feat_tiles * col_tiles), in_group = tile - p.group * (a.feat_tiles * col_tiles);
+        const uint32_t band = 8 * a.feat_tiles, b = in_group / band, in = in_group - b * band;
+        const uint32_t w = col_tiles - 8 * b < 8 ? col_tiles - 8 * b : 8;
+        const uint32_t ct = 8 * b + in % w;
+        p.ft = in / w;
+        if (BY_K) {
+            p.c = ct * a.nt, p.c_end = static_cast<uint32_t>(a.cols), p.k = s.starts[p.group], p.k_rows = s.starts[p.group + 1] - p.k;
+        } else {
+            if (groups > 1) p.group = group_of(s.tiles, groups, ct);
+            p.c = s.starts[p.group] + (ct - s.tiles[p.group]) * a.nt, p.c_end = s.starts[p.group + 1], p.k = p.k_rows = 0;
+        }
+        return p;
+    };
+    auto all_steps = [&](const TilePlace &p) { return BY_K ? (p.k_rows + STEP_K - 1) / STEP_K : a.steps; };
+    auto step_from = [&](uint32_t steps, uint32_t r) { return static_cast<uint32_t>(static_cast<uint64_t>(steps) * r / a.split); };
+    auto features = [&](const TilePlace &p) { return (p.ft * CTAS + side) * G_FEATS; };      // where this CTA's begin
+
+    if (warp == 8) {
+        RingPlace at;
+        const uint32_t full = peer_addr(s.full, BY_K ? side : 0);
+        for (uint32_t tile = first; tile < tiles; tile += stride) {
+            const TilePlace p = place(tile);
+            const uint32_t f = features(p), c = p.c + (PAIR ? side * (a.nt / 2) : 0), steps = all_steps(p), k1 = step_from(steps, rank + 1);
+            bool ok = true;
+            for (uint32_t k = step_from(steps, rank); k < k1; k++, at.next(a.stages)) {
+                const uint32_t st = at.stage;
+                ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
+                if (!ok) break;
+                if (elected()) {
+                    const uint32_t dst = ring + st * a.stage_bytes, to_b = dst + G_FEATS * ROW_BYTES;
+                    const uint32_t bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
+                    if (side && !BY_K) peer_expect(bar, a.stage_bytes);
+                    else bar_expect(&s.full[st], a.stage_bytes);
+                    if constexpr (P == FORWARD) {
+                        tma_load_3d<PAIR>(&a.a, bar, dst, k * STEP, f, p.group);
+                    } else if constexpr (P == ROWS_GRAD) {
+                        tma_load_3d<PAIR>(&a.a, bar, dst, f, k * STEP, p.group);
+                        tma_load_3d<PAIR>(&a.a, bar, dst + G_BLOCK, f + 64, k * STEP, p.group);
+                    } else {
+                        tma_load_2d<PAIR>(&a.a, bar, dst, f, p.k + k * STEP);
+                        tma_load_2d<PAIR>(&a.a, bar, dst + G_BLOCK, f + 64, p.k + k * STEP);
+                    }
+                    if constexpr (B_MN) {
+                        for (uint32_t b = 0; b < a.nt / CTAS; b += 64) tma_load_2d<PAIR>(&a.b, bar, to_b + b * ROW_BYTES, c + b, p.k + k * STEP);
+                    } else {
+                        tma_load_2d<PAIR>(&a.b, bar, to_b, k * STEP, c);
+                    }
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+        }
+        // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both).
+        if (*over && (BY_K || !side))
+            for (uint32_t i = 0; i < a.stages; i++) {
+                const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
+                if (used != ~0u) bar_drain(&s.full[i], used & 1);
+            }
+    } else if (warp == 9) {
+        if (!side) {
+            const uint32_t a_step = A_MN ? 16 * ROW_BYTES : 32, b_step = B_MN ? 16 * ROW_BYTES : 32;
+            RingPlace at;
+            uint32_t n = 0, desc;
+            if constexpr (sizeof(T) == 1) desc = mma_desc_e4m3(CTAS * G_FEATS, a.nt);
+            else desc = mma_desc(__is_same(T, __nv_bfloat16), A_MN, B_MN, CTAS * G_FEATS, a.nt);
+            const uint32_t a_lo = desc_lo(ring, A_MN ? G_BLOCK : 16), b_lo = desc_lo(ring + G_FEATS * ROW_BYTES, B_MN ? G_BLOCK : 16);
+            bool ok = true;
+            for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
+                const TilePlace p = place(tile);
+                const uint32_t steps = all_steps(p), k0 = step_from(steps, rank), k1 = step_from(steps, rank + 1);
+                const uint32_t buf = n & 1, sums = tmem + buf * a.nt;
+                ok = n < 2 || warp_wait(&s.sums_empty[buf], (n / 2 - 1) & 1, over);
+                if (!ok) break;
+                tc_after();
+                for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
+                    const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
+                    ok = warp_wait(BY_K ? &s.ready[st] : &s.full[st], at.turn & 1, over);
+                    if (!ok) break;
+                    if (BY_K) tc_after();
+                    if (elected()) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 4; q++) {
+                            if constexpr (sizeof(T) == 1) mma32_e4m3<PAIR>(sums, a_lo + off + (q * a_step >> 4), b_lo + off + (q * b_step >> 4), desc, k != k0 || q);
+                            else mma16<PAIR>(sums, a_lo + off + (q * a_step >> 4), b_lo + off + (q * b_step >> 4), desc, k != k0 || q);
+                        }
+                        mma_commit<PAIR>(&s.empty[st]);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (elected()) mma_commit<PAIR>(&s.sums_full[buf]);
+                __syncwarp();
+            }
+            if (!ok) {                                           // the products under way end before their memory goes
+                if (elected()) mma_commit<PAIR>(&s.sums_full[n & 1]);
+                __syncwarp();
+                bar_drain(&s.sums_full[n & 1], (n / 2) & 1);
+            }
+        }
+    } else if (warp == 10) {
+        if constexpr (BY_K) {                                    // rows that are not the group's become zeros
+            RingPlace at;
+            const uint32_t blocks = a.stage_bytes / G_BLOCK;
+            bool ok = true;
+            for (uint32_t tile = first; ok && tile < tiles; tile += stride) {
+                const TilePlace p = place(tile);
+                const uint32_t steps = all_steps(p), k1 = step_from(steps, rank + 1);
+                for (uint32_t k = step_from(steps, rank); k < k1; k++, at.next(a.stages)) {
+                    const uint32_t st = at.stage, left = p.k_rows - k * STEP_K;
+                    ok = warp_wait(&s.full[st], at.turn & 1, over);
+                    if (!ok) break;
+                    if (left < STEP_K) {
+                        const uint32_t each = (STEP_K - left) * 8;               // 16-byte parts of a block's rows
+                        for (uint32_t i = lane; i < blocks * each; i += 32)
+                            *reinterpret_cast<uint4 *>(local + st * a.stage_bytes + i / each * G_BLOCK + left * ROW_BYTES + i % each * 16) = make_uint4(0, 0, 0, 0);
+                        publish_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (side) peer_arrive(peer_addr(&s.ready[st], 0));
+                        else bar_arrive(&s.ready[st]);
+                    }
+                }
+            }
+        }
+    } else {
+        O *const out = static_cast<O *>(a.out);
+        const O *const times = static_cast<const O *>(a.times), *const residual = static_cast<const O *>(a.residual);
+        const uint32_t quarter = warp & 3, half = warp >> 2;
+        float *const turn = reinterpret_cast<float *>(local + a.stages * a.stage_bytes + warp * G_TURN_BYTES);
+        if (!BY_K && a.groups.offsets) {                         // rows of no group
+            const uint64_t lead = s.starts[0], idle = (lead + (a.cols - s.starts[groups])) * a.feats;
+            for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * G_EPILOGUE + tid; i < idle; i += static_cast<uint64_t>(gridDim.x) * G_EPILOGUE)
+                out[i < lead * a.feats ? i : i + (s.starts[groups] - lead) * a.feats] = narrow<O>(0.0f);
+        }
+        uint32_t n = 0;
+        for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
+            const TilePlace p = place(tile);
+            const uint32_t buf = n & 1, steps = all_steps(p);
+            const bool any = step_from(steps, rank + 1) > step_from(steps, rank), vectors = a.vectors && a.split == 1;
+            const uint64_t plane = BY_K ? p.group * a.cols : 0;
+            const uint64_t f = features(p) + quarter * 32 + (vectors ? (lane & 3) * 8 : lane);     // this lane's, eight of them or one
+            const uint64_t last = a.feats - 1, in = f < a.feats ? f : last;
+            float bias[8], a_scale[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                const uint64_t i = vectors && in + e < a.feats ? in + e : in;
+                bias[e] = a.bias ? widen(static_cast<const O *>(a.bias)[p.group * a.feats + i]) : 0.0f;
+                a_scale[e] = a.a_scale ? a.a_scale[i] : 0.0f;
+            }
+            if (!warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
+            tc_after();
+            for (uint32_t g = half; g * G_GROUP < a.nt; g += 2) {
+                const uint32_t c0 = p.c + g * G_GROUP;
+                if (c0 >= p.c_end) break;
+                float v[G_GROUP];
+                if (vectors) {
+                    const uint32_t c[2] = {c0 + (lane >> 2), c0 + (lane >> 2) + 8};
+                    Vec<O, 16> m[2], r[2];
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; j++) {
+                        m[j].raw = r[j].raw = make_uint4(0, 0, 0, 0);
+                        if (c[j] < p.c_end && f < a.feats) {
+                            if (times) m[j].raw = *reinterpret_cast<const uint4 *>(times + c[j] * a.times_stride + f);
+                            if (residual) r[j].raw = *reinterpret_cast<const uint4 *>(residual + c[j] * a.residual_stride + f);
+                        }
+                    }
+                    __syncwarp();
+                    tmem_load16(tmem + (quarter << 21) + buf * a.nt + g * G_GROUP, v);
+#pragma unroll
+                    for (uint32_t q = 0; q < G_GROUP; q++) turn[q * G_PITCH + lane] = any ? v[q] : 0.0f;
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; j++) {
+                        const float4 *from = reinterpret_cast<const float4 *>(turn + ((lane >> 2) + j * 8) * G_PITCH + (lane & 3) * 8);
+                        *reinterpret_cast<float4 *>(v) = from[0], *reinterpret_cast<float4 *>(v + 4) = from[1];
+                        if (c[j] >= p.c_end || f >= a.feats) continue;
+                        const uint64_t at = (plane + c[j]) * a.feats + f;
+                        finish<O, 8>(a, c[j], f, at, v, bias, a_scale, m[j].e, r[j].e);
+                        Vec<O, 16> y;
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; e++) y.e[e] = narrow<O>(v[e]);
+                        *reinterpret_cast<uint4 *>(out + at) = y.raw;
+                    }
+                } else {
+                    __syncwarp();
+                    tmem_load16(tmem + (quarter << 21) + buf * a.nt + g * G_GROUP, v);
+#pragma unroll
+                    for (uint32_t q = 0; q < G_GROUP; q++) {
+                        if (!any) v[q] = 0;
+                        if (!PAIR && a.split > 1) {              // (the stages are free: all products have ended)
+                            reinterpret_cast<float *>(local)[(g * G_GROUP + q) * G_FEATS + quarter * 32 + lane] = v[q];
+                        } else if (c0 + q < p.c_end && f < a.feats) {
+                            const uint64_t c = c0 + q, at = (plane + c) * a.feats + f;
+                            finish<O, 1>(a, c, f, at, v + q, bias, a_scale, times + c * a.times_stride + f, residual + c * a.residual_stride + f);
+                            out[at] = narrow<O>(v[q]);
+                        }
+                    }
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (side) peer_arrive(peer_addr(&s.sums_empty[buf], 0));
+                else bar_arrive(&s.sums_empty[buf]);
+            }
+        }
+    }
+    __syncwarp();
+    if (!PAIR && a.split > 1) {                                  // one tile per cluster: every CTA adds up its share of the columns
+        cluster_barrier();
+        if (warp < 8 && first < tiles && !*over) {
+            const TilePlace p = place(first);
+            const uint64_t plane = BY_K ? p.group * a.cols : 0;
+            O *const out = static_cast<O *>(a.out);
+            const O *const times = static_cast<const O *>(a.times), *const residual = static_cast<const O *>(a.residual);
+            const uint32_t share = a.nt / a.split, feat = tid & (G_FEATS - 1);
+            const uint64_t f = features(p) + feat;
+            const Peers peers(ring, a.split);
+            if (f < a.feats) {
+                const float bias = a.bias ? widen(static_cast<const O *>(a.bias)[p.group * a.feats + f]) : 0.0f, a_scale = a.a_scale ? a.a_scale[f] : 0.0f;
+#pragma unroll 2
+                for (uint32_t q = rank * share + tid / G_FEATS; q < (rank + 1) * share && p.c + q < p.c_end; q += 2) {
+                    const uint64_t c = p.c + q, at = (plane + c) * a.feats + f;
+                    float v = peers.sum((q * G_FEATS + feat) * 4);
+                    finish<O, 1>(a, c, f, at, &v, &bias, &a_scale, times + c * a.times_stride + f, residual + c * a.residual_stride + f);
+                    out[at] = narrow<O>(v);
+                }
+            }
+        }
+        cluster_barrier();
+    }
+    if constexpr (PAIR) cluster_barrier();                       // nobody's barriers or tiles go while the other may use them
+    tc_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_after();
+        tmem_free<PAIR>(tmem, a.tmem_columns);
+    }
+}
+
+// Rows that start on 16 bytes: out[plane][r][c] = in[plane][r][c], and zeros behind a row's last element.  16 bytes of the result a thread.
+struct AlignJob {
+    const void *in;
+    void *out;
+    uint64_t plane_stride, row_stride, rows, cols, pitch, total;   // in elements; total: rows of all planes
+};
+struct AlignArgs {
+    AlignJob job[2];
+};
+constexpr uint32_t ALIGN_THREADS = 256;
+template <class E>
+__global__ void __launch_bounds__(ALIGN_THREADS) k_align(const __grid_constant__ AlignArgs a)
+{
+    constexpr uint32_t N = 16 / sizeof(E);
+    const AlignJob &j = a.job[blockIdx.y];
+    const uint64_t each = j.pitch / N, all = j.total * each;
+    wait_for_previous();
+    for (uint64_t u = static_cast<uint64_t>(blockIdx.x) * ALIGN_THREADS + threadIdx.x; u < all; u += static_cast<uint64_t>(gridDim.x) * ALIGN_THREADS) {
+        const uint64_t row = u / each, plane = row / j.rows, c = (u - row * each) * N;
+        const E *in = static_cast<const E *>(j.in) + plane * j.plane_stride + (row - plane * j.rows) * j.row_stride + c;
+        union { E e[N]; uint4 raw; } v;
+#pragma unroll
+        for (uint32_t e = 0; e < N; e++) v.e[e] = c + e < j.cols ? in[e] : E(0);
+        reinterpret_cast<uint4 *>(j.out)[u] = v.raw;
     }
 }
 

@@ -202,6 +202,21 @@ __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, ui
 {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (m >> 4) << 24;
 }
+// 8-bit operands (E4M3), sums in 32 bits.
+__device__ __forceinline__ uint32_t mma_desc_e4m3(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
+// D (+)= A B^T over 32 K elements of 8 bits.
+template <bool PAIR = false>
+__device__ __forceinline__ void mma32_e4m3(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add)
+{
+    if constexpr (PAIR)
+        asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], x, y, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(DESC_HI) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], x, y, %3, p;\n}\n"
+                     ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "r"(DESC_HI) : "memory");
+}
 // D (+)= A B^T over 16 K elements; the tiles by their descriptors' lower words.
 template <bool PAIR = false>
 __device__ __forceinline__ void mma16(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add)

@@ -39,7 +39,9 @@ def _check(got, want):
 # rows, in, out: one of each, a tile of the tensor core and its neighbours, sizes that no vector fits, few rows and wide weights, many rows
 SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (1, 64, 128), (2, 72, 136), (16, 64, 128), (17, 65, 129), (31, 200, 96), (64, 128, 256), (100, 250, 331), (127, 512, 127),
           (128, 256, 128), (129, 264, 384), (255, 129, 513), (256, 320, 256), (257, 1000, 264), (333, 777, 1001), (1, 4096, 1024), (1, 1001, 4097), (8, 2048, 512), (600, 64, 64),
-          (1000, 96, 2050), (2049, 512, 300), (40, 3000, 40), (5000, 33, 17)]
+          (1000, 96, 2050), (2049, 512, 300), (40, 3000, 40), (5000, 33, 17),
+          # (pairs of CTAs: forwards, for the rows' gradient, for the weight's)
+          (2304, 512, 2304), (2301, 520, 2311), (2304, 2304, 512), (2305, 2312, 505), (512, 2304, 2304), (501, 2312, 2307)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -137,7 +139,9 @@ def _starts(seed, rows, experts, how):
 @pytest.mark.parametrize("rows, experts, inp, out, how", [(1, 1, 8, 8, "one"), (1, 4, 64, 128, "any"), (7, 3, 33, 19, "any"), (64, 64, 128, 72, "any"), (50, 8, 96, 130, "one"),
                                                           (128, 16, 512, 264, "any"), (300, 4, 200, 100, "inside"), (300, 3, 64, 256, "even"), (900, 5, 136, 520, "any"),
                                                           (2000, 6, 256, 384, "any"), (40, 1024, 40, 24, "any"), (1500, 2, 77, 333, "inside"), (0, 5, 16, 16, "even"),
-                                                          (777, 7, 1024, 512, "any")])
+                                                          (777, 7, 1024, 512, "any"),
+                                                          # (pairs of CTAs)
+                                                          (5000, 3, 512, 2304, "any"), (4000, 4, 2304, 520, "any"), (1500, 6, 1536, 1544, "any"), (5000, 3, 515, 2307, "inside")])
 def test_experts(dtype, rows, experts, inp, out, how):
     from lmz_b200 import experts as ex
     starts = _starts(1, rows, experts, how)
