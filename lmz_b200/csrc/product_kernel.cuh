@@ -17,13 +17,13 @@ enum Product : int { FORWARD, ROWS_GRAD, WEIGHT_GRAD };
 constexpr uint32_t G_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
 constexpr uint32_t G_COLS = 256;               // most columns of a tile: its N, a TMEM column each
 constexpr uint32_t G_GROUP = 16;               // columns of a TMEM load
-constexpr uint32_t G_MAX_STAGES = 10, G_EPILOGUE = 256, G_THREADS = G_EPILOGUE + 96;
+constexpr uint32_t G_MAX_STAGES = 10, G_EPILOGUE = 512, G_THREADS = G_EPILOGUE + 96, G_TMA_WARP = G_EPILOGUE / 32;
 constexpr uint32_t G_PITCH = 36;               // words from one column to the next where a warp turns 32 lanes' features round
-constexpr uint32_t G_TURN_BYTES = G_GROUP * G_PITCH * 4;      // a warp's
+constexpr uint32_t G_TURN_BYTES = G_GROUP / 2 * G_PITCH * 4;  // a warp's
 constexpr uint32_t G_BLOCK = STEP_K * ROW_BYTES;              // 64 k of 64 f or c side by side
 
 struct ProductShared {
-    uint64_t full[G_MAX_STAGES], empty[G_MAX_STAGES], ready[G_MAX_STAGES];
+    uint64_t full[G_MAX_STAGES], empty[G_MAX_STAGES], tail[G_MAX_STAGES];
     uint64_t sums_full[2], sums_empty[2];
     uint32_t tmem, over;
     uint32_t starts[MAX_EXPERTS + 1], tiles[MAX_EXPERTS + 1];  // where a group's rows, and its tiles of columns, begin
@@ -57,53 +57,78 @@ struct TilePlace {
     uint32_t k, k_rows;                          // WEIGHT_GRAD: the group's rows
 };
 
-// N neighbours of f of a column, from sums to result: z = sums + bias, y = act(z) times + residual.
-template <class O, int N>
-__device__ __forceinline__ void finish(const ProductArgs &a, uint64_t c, uint64_t f, uint64_t at, float *v, const float *bias, const float *a_scale, const O *times, const O *residual)
+// N neighbours of f of each of J columns, from sums to result: z = sums + bias, y = act(z) times + residual.  `on`: whether there is such a column.
+template <class O, bool SCALED, int J, int N>
+__device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at, const bool *on, float (*v)[N], const O *bias, const float *a_scale, const float *b_scale,
+                                       const O *const *times, const O *const *residual)
 {
-    if (a.a_scale) {
-        const float s = a.b_scale[c];
+    if constexpr (SCALED) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] *= a_scale[e] * s;
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[j][e] *= a_scale[e] * b_scale[j];
     }
     if (a.bias) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] += bias[e];
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[j][e] += widen(bias[e]);
     }
     if (a.z) {
-        if constexpr (N % 4 == 0) {
 #pragma unroll
-            for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(a.z + at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        } else {
-            for (int e = 0; e < N; e++) a.z[at + e] = v[e];
+        for (int j = 0; j < J; j++) {
+            if (!on[j]) continue;
+            if constexpr (N % 4 == 0) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(a.z + at[j] + e) = make_float4(v[j][e], v[j][e + 1], v[j][e + 2], v[j][e + 3]);
+            } else {
+                for (int e = 0; e < N; e++) a.z[at[j] + e] = v[j][e];
+            }
         }
     }
-    act_all<N>(a.activation, v);
+    act_all<J * N>(a.activation, v[0]);
     if (a.times) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] *= widen(times[e]);
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[j][e] *= widen(times[j][e]);
     }
     if (a.residual) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[e] += widen(residual[e]);
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[j][e] += widen(residual[j][e]);
     }
+}
+
+// One of them.
+template <class O, bool SCALED>
+__device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group, uint32_t c, uint64_t f, uint64_t at, float sum)
+{
+    const O *const times = static_cast<const O *>(a.times) + c * a.times_stride + f, *const residual = static_cast<const O *>(a.residual) + c * a.residual_stride + f;
+    const bool on = true;
+    float v[1][1] = {{sum}};
+    finish<O, SCALED, 1, 1>(a, &at, &on, v, static_cast<const O *>(a.bias) + group * a.feats + f, SCALED ? a.a_scale + f : nullptr, SCALED ? a.b_scale + c : nullptr, &times,
+                           &residual);
+    static_cast<O *>(a.out)[at] = narrow<O>(v[0][0]);
 }
 
 // Features are the tensor core's M and columns its N, whatever their number: a single row streams the weight past 16 columns, a batch past 256.
 //
-// Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; eight warps take the
+// Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; sixteen warps take the
 // sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.  They turn 32 features and 16 columns round
 // in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.
 // Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile's columns behind its group's last are another group's
 // rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
-// last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.
+// last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.  Only such
+// steps go by that warp (all of them did at first: handing a step on to another CTA takes 1 us, and 8192 rows 4096x14336 took 2070 us and not 634).
 // Few tiles: the CTAs of a cluster share k, and their sums meet in distributed shared memory.
 // Many (PAIR): two CTAs multiply 256 features by 256 columns together, each loading half of both.
 template <class T, class O, int P, bool PAIR>
 __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant__ ProductArgs a)
 {
     constexpr uint32_t CTAS = PAIR ? 2 : 1, STEP = ROW_BYTES / sizeof(T);
-    constexpr bool A_MN = P != FORWARD, B_MN = P == WEIGHT_GRAD, BY_K = P == WEIGHT_GRAD;
+    constexpr bool A_MN = P != FORWARD, B_MN = P == WEIGHT_GRAD, BY_K = P == WEIGHT_GRAD, SCALED = sizeof(T) == 1;
     static_assert(sizeof(T) == 2 || P == FORWARD);
     extern __shared__ uint8_t g_smem[];
     __shared__ ProductShared s;
@@ -114,10 +139,11 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     const uint32_t ring = (smem_addr(g_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
     uint8_t *const local = g_smem + (ring - smem_addr(g_smem));
     volatile uint32_t *over = &s.over;
+    const bool tails = BY_K && a.groups.offsets;                 // (without groups what is behind the last row reads as zeros)
 
     if (tid == 0) {
         s.over = 0;
-        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], BY_K ? 1 : CTAS), bar_init(&s.empty[i], 1), bar_init(&s.ready[i], CTAS);
+        for (uint32_t i = 0; i < a.stages; i++) bar_init(&s.full[i], CTAS), bar_init(&s.empty[i], 1), bar_init(&s.tail[i], 1);
         for (uint32_t i = 0; i < 2; i++) bar_init(&s.sums_full[i], 1), bar_init(&s.sums_empty[i], CTAS * G_EPILOGUE / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -125,7 +151,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         __syncthreads();
         cluster_barrier();
     }
-    if (warp == 9) tmem_alloc<PAIR>(&s.tmem, a.tmem_columns);
+    if (warp == G_TMA_WARP + 1) tmem_alloc<PAIR>(&s.tmem, a.tmem_columns);
     wait_for_previous();
     group_starts(a.groups, s.starts);
     if (warp == 0 && !BY_K) {
@@ -171,9 +197,10 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     auto step_from = [&](uint32_t steps, uint32_t r) { return static_cast<uint32_t>(static_cast<uint64_t>(steps) * r / a.split); };
     auto features = [&](const TilePlace &p) { return (p.ft * CTAS + side) * G_FEATS; };      // where this CTA's begin
 
-    if (warp == 8) {
+    if (warp == G_TMA_WARP) {
         RingPlace at;
-        const uint32_t full = peer_addr(s.full, BY_K ? side : 0);
+        const uint32_t full = peer_addr(s.full, 0), own_tail = peer_addr(s.tail, side);
+        uint32_t last_tail = 0, tail_turn = 0;                   // bits per stage: its last use was a tail; how many of its tails there were
         for (uint32_t tile = first; tile < tiles; tile += stride) {
             const TilePlace p = place(tile);
             const uint32_t f = features(p), c = p.c + (PAIR ? side * (a.nt / 2) : 0), steps = all_steps(p), k1 = step_from(steps, rank + 1);
@@ -182,11 +209,19 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 const uint32_t st = at.stage;
                 ok = !at.turn || warp_wait(&s.empty[st], (at.turn - 1) & 1, over);
                 if (!ok) break;
+                const bool tail = tails && (k + 1) * STEP_K > p.k_rows;
+                last_tail = (last_tail & ~(1u << st)) | static_cast<uint32_t>(tail) << st, tail_turn ^= static_cast<uint32_t>(tail) << st;
                 if (elected()) {
                     const uint32_t dst = ring + st * a.stage_bytes, to_b = dst + G_FEATS * ROW_BYTES;
-                    const uint32_t bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
-                    if (side && !BY_K) peer_expect(bar, a.stage_bytes);
-                    else bar_expect(&s.full[st], a.stage_bytes);
+                    uint32_t bar = PAIR ? full + st * 8 : smem_addr(&s.full[st]);
+                    if (tail) {
+                        bar = PAIR ? own_tail + st * 8 : smem_addr(&s.tail[st]);
+                        bar_expect(&s.tail[st], a.stage_bytes);
+                    } else if (side) {
+                        peer_expect(bar, a.stage_bytes);
+                    } else {
+                        bar_expect(&s.full[st], a.stage_bytes);
+                    }
                     if constexpr (P == FORWARD) {
                         tma_load_3d<PAIR>(&a.a, bar, dst, k * STEP, f, p.group);
                     } else if constexpr (P == ROWS_GRAD) {
@@ -206,13 +241,16 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             }
             if (!ok) break;
         }
-        // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both).
-        if (*over && (BY_K || !side))
+        // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both; those of tails are each
+        // CTA's own).
+        if (*over)
             for (uint32_t i = 0; i < a.stages; i++) {
                 const uint32_t used = at.turn - (i >= at.stage);                 // the last turn that filled this stage
-                if (used != ~0u) bar_drain(&s.full[i], used & 1);
+                if (used == ~0u) continue;
+                if (last_tail >> i & 1) bar_drain(&s.tail[i], ~(tail_turn >> i) & 1);
+                else if (!side) bar_drain(&s.full[i], used & 1);
             }
-    } else if (warp == 9) {
+    } else if (warp == G_TMA_WARP + 1) {
         if (!side) {
             const uint32_t a_step = A_MN ? 16 * ROW_BYTES : 32, b_step = B_MN ? 16 * ROW_BYTES : 32;
             RingPlace at;
@@ -230,9 +268,8 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 tc_after();
                 for (uint32_t k = k0; k < k1; k++, at.next(a.stages)) {
                     const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
-                    ok = warp_wait(BY_K ? &s.ready[st] : &s.full[st], at.turn & 1, over);
+                    ok = warp_wait(&s.full[st], at.turn & 1, over);
                     if (!ok) break;
-                    if (BY_K) tc_after();
                     if (elected()) {
 #pragma unroll
                         for (uint32_t q = 0; q < 4; q++) {
@@ -253,36 +290,39 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 bar_drain(&s.sums_full[n & 1], (n / 2) & 1);
             }
         }
-    } else if (warp == 10) {
-        if constexpr (BY_K) {                                    // rows that are not the group's become zeros
+    } else if (warp == G_TMA_WARP + 2) {
+        if (tails) {                                             // rows that are not the group's become zeros
             RingPlace at;
+            uint32_t turns = 0;                                  // bit per stage: the phase that its next tail is
             const uint32_t blocks = a.stage_bytes / G_BLOCK;
-            bool ok = true;
-            for (uint32_t tile = first; ok && tile < tiles; tile += stride) {
+            for (uint32_t tile = first; tile < tiles; tile += stride) {
                 const TilePlace p = place(tile);
-                const uint32_t steps = all_steps(p), k1 = step_from(steps, rank + 1);
-                for (uint32_t k = step_from(steps, rank); k < k1; k++, at.next(a.stages)) {
-                    const uint32_t st = at.stage, left = p.k_rows - k * STEP_K;
-                    ok = warp_wait(&s.full[st], at.turn & 1, over);
-                    if (!ok) break;
-                    if (left < STEP_K) {
-                        const uint32_t each = (STEP_K - left) * 8;               // 16-byte parts of a block's rows
-                        for (uint32_t i = lane; i < blocks * each; i += 32)
-                            *reinterpret_cast<uint4 *>(local + st * a.stage_bytes + i / each * G_BLOCK + left * ROW_BYTES + i % each * 16) = make_uint4(0, 0, 0, 0);
-                        publish_smem();
-                    }
+                const uint32_t steps = all_steps(p), n = step_from(steps, rank + 1) - step_from(steps, rank), left = p.k_rows % STEP_K;
+                if (n && left && step_from(steps, rank + 1) == steps) {
+                    at.skip(n - 1, a.stages);
+                    const uint32_t st = at.stage;
+                    if (!warp_wait(&s.tail[st], turns >> st & 1, over)) break;
+                    turns ^= 1u << st;
+                    const uint32_t each = (STEP_K - left) * 8;                   // 16-byte parts of a block's rows
+                    for (uint32_t i = lane; i < blocks * each; i += 32)
+                        *reinterpret_cast<uint4 *>(local + st * a.stage_bytes + i / each * G_BLOCK + left * ROW_BYTES + i % each * 16) = make_uint4(0, 0, 0, 0);
+                    publish_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        if (side) peer_arrive(peer_addr(&s.ready[st], 0));
-                        else bar_arrive(&s.ready[st]);
+                        if (side) peer_arrive(peer_addr(&s.full[st], 0));
+                        else bar_arrive(&s.full[st]);
                     }
+                    at.next(a.stages);
+                } else {
+                    at.skip(n, a.stages);
                 }
             }
         }
     } else {
         O *const out = static_cast<O *>(a.out);
         const O *const times = static_cast<const O *>(a.times), *const residual = static_cast<const O *>(a.residual);
-        const uint32_t quarter = warp & 3, half = warp >> 2;
+        const uint32_t quarter = warp & 3, share = warp >> 2;     // of the lanes, and of the groups of columns
+        constexpr uint32_t SHARES = G_EPILOGUE / 128;
         float *const turn = reinterpret_cast<float *>(local + a.stages * a.stage_bytes + warp * G_TURN_BYTES);
         if (!BY_K && a.groups.offsets) {                         // rows of no group
             const uint64_t lead = s.starts[0], idle = (lead + (a.cols - s.starts[groups])) * a.feats;
@@ -296,61 +336,91 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             const bool any = step_from(steps, rank + 1) > step_from(steps, rank), vectors = a.vectors && a.split == 1;
             const uint64_t plane = BY_K ? p.group * a.cols : 0;
             const uint64_t f = features(p) + quarter * 32 + (vectors ? (lane & 3) * 8 : lane);     // this lane's, eight of them or one
-            const uint64_t last = a.feats - 1, in = f < a.feats ? f : last;
-            float bias[8], a_scale[8];
+            const uint64_t in = f < a.feats ? f : a.feats - 1;
+            auto live = [&](uint32_t g) { return g * G_GROUP < a.nt && p.c + g * G_GROUP < p.c_end; };
+            Vec<O, 16> bias, m[2], r[2];
+            float a_scale[SCALED ? 8 : 1], b_scale[2];
+            auto ask = [&](uint32_t g) {                         // what sixteen columns meet in the epilogue
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) {
-                const uint64_t i = vectors && in + e < a.feats ? in + e : in;
-                bias[e] = a.bias ? widen(static_cast<const O *>(a.bias)[p.group * a.feats + i]) : 0.0f;
-                a_scale[e] = a.a_scale ? a.a_scale[i] : 0.0f;
+                for (uint32_t j = 0; j < 2; j++) {
+                    const uint32_t c = p.c + g * G_GROUP + j * 8 + (lane >> 2);
+                    m[j].raw = r[j].raw = make_uint4(0, 0, 0, 0);
+                    if (SCALED) b_scale[j] = c < p.c_end ? a.b_scale[c] : 0.0f;
+                    if (c < p.c_end && f < a.feats) {
+                        if (times) m[j].raw = *reinterpret_cast<const uint4 *>(times + c * a.times_stride + f);
+                        if (residual) r[j].raw = *reinterpret_cast<const uint4 *>(residual + c * a.residual_stride + f);
+                    }
+                }
+            };
+            if (vectors) {
+                bias.raw = make_uint4(0, 0, 0, 0);
+                if (a.bias) bias.raw = *reinterpret_cast<const uint4 *>(static_cast<const O *>(a.bias) + p.group * a.feats + (f < a.feats ? f : 0));
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) a_scale[e] = a.a_scale[in + e < a.feats ? in + e : in];
+                }
+                if (live(share)) ask(share);
+                if (times || residual)                           // (the others' come to L2 under the products)
+                    for (uint32_t g = share + SHARES; live(g); g += SHARES) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 2; j++) {
+                            const uint32_t c = p.c + g * G_GROUP + j * 8 + (lane >> 2);
+                            if (c < p.c_end && f < a.feats) {
+                                if (times) asm volatile("prefetch.global.L2 [%0];" ::"l"(times + c * a.times_stride + f));
+                                if (residual) asm volatile("prefetch.global.L2 [%0];" ::"l"(residual + c * a.residual_stride + f));
+                            }
+                        }
+                    }
             }
             if (!warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
             tc_after();
-            for (uint32_t g = half; g * G_GROUP < a.nt; g += 2) {
-                const uint32_t c0 = p.c + g * G_GROUP;
-                if (c0 >= p.c_end) break;
-                float v[G_GROUP];
+            const uint32_t sums = tmem + (quarter << 21) + buf * a.nt;
+            for (uint32_t g = share; live(g); g += SHARES) {
+                uint32_t v[G_GROUP];
+                __syncwarp();
+                tmem_ask16(sums + g * G_GROUP, v);
+                tmem_wait16(v);
                 if (vectors) {
-                    const uint32_t c[2] = {c0 + (lane >> 2), c0 + (lane >> 2) + 8};
-                    Vec<O, 16> m[2], r[2];
+                    float u[2][8];
 #pragma unroll
                     for (uint32_t j = 0; j < 2; j++) {
-                        m[j].raw = r[j].raw = make_uint4(0, 0, 0, 0);
-                        if (c[j] < p.c_end && f < a.feats) {
-                            if (times) m[j].raw = *reinterpret_cast<const uint4 *>(times + c[j] * a.times_stride + f);
-                            if (residual) r[j].raw = *reinterpret_cast<const uint4 *>(residual + c[j] * a.residual_stride + f);
-                        }
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; q++) turn[q * G_PITCH + lane] = __uint_as_float(v[j * 8 + q]);
+                        __syncwarp();
+                        const float4 *from = reinterpret_cast<const float4 *>(turn + (lane >> 2) * G_PITCH + (lane & 3) * 8);
+                        *reinterpret_cast<float4 *>(u[j]) = from[0], *reinterpret_cast<float4 *>(u[j] + 4) = from[1];
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    tmem_load16(tmem + (quarter << 21) + buf * a.nt + g * G_GROUP, v);
+                    if (BY_K && !any) {
 #pragma unroll
-                    for (uint32_t q = 0; q < G_GROUP; q++) turn[q * G_PITCH + lane] = any ? v[q] : 0.0f;
-                    __syncwarp();
+                        for (uint32_t e = 0; e < 16; e++) u[e / 8][e % 8] = 0;
+                    }
+                    uint64_t at[2];
+                    bool on[2];
 #pragma unroll
                     for (uint32_t j = 0; j < 2; j++) {
-                        const float4 *from = reinterpret_cast<const float4 *>(turn + ((lane >> 2) + j * 8) * G_PITCH + (lane & 3) * 8);
-                        *reinterpret_cast<float4 *>(v) = from[0], *reinterpret_cast<float4 *>(v + 4) = from[1];
-                        if (c[j] >= p.c_end || f >= a.feats) continue;
-                        const uint64_t at = (plane + c[j]) * a.feats + f;
-                        finish<O, 8>(a, c[j], f, at, v, bias, a_scale, m[j].e, r[j].e);
+                        const uint32_t c = p.c + g * G_GROUP + j * 8 + (lane >> 2);
+                        at[j] = (plane + c) * a.feats + f, on[j] = c < p.c_end && f < a.feats;
+                    }
+                    const O *const ms[2] = {m[0].e, m[1].e}, *const rs[2] = {r[0].e, r[1].e};
+                    finish<O, SCALED, 2, 8>(a, at, on, u, bias.e, a_scale, b_scale, ms, rs);
+                    if (live(g + SHARES)) ask(g + SHARES);
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; j++) {
                         Vec<O, 16> y;
 #pragma unroll
-                        for (uint32_t e = 0; e < 8; e++) y.e[e] = narrow<O>(v[e]);
-                        *reinterpret_cast<uint4 *>(out + at) = y.raw;
+                        for (uint32_t e = 0; e < 8; e++) y.e[e] = narrow<O>(u[j][e]);
+                        if (on[j]) *reinterpret_cast<uint4 *>(out + at[j]) = y.raw;
                     }
                 } else {
-                    __syncwarp();
-                    tmem_load16(tmem + (quarter << 21) + buf * a.nt + g * G_GROUP, v);
 #pragma unroll
                     for (uint32_t q = 0; q < G_GROUP; q++) {
-                        if (!any) v[q] = 0;
-                        if (!PAIR && a.split > 1) {              // (the stages are free: all products have ended)
-                            reinterpret_cast<float *>(local)[(g * G_GROUP + q) * G_FEATS + quarter * 32 + lane] = v[q];
-                        } else if (c0 + q < p.c_end && f < a.feats) {
-                            const uint64_t c = c0 + q, at = (plane + c) * a.feats + f;
-                            finish<O, 1>(a, c, f, at, v + q, bias, a_scale, times + c * a.times_stride + f, residual + c * a.residual_stride + f);
-                            out[at] = narrow<O>(v[q]);
-                        }
+                        const float sum = any ? __uint_as_float(v[q]) : 0.0f;
+                        const uint32_t c = p.c + g * G_GROUP + q;
+                        if (!PAIR && a.split > 1)                // (the stages are free: all products have ended)
+                            reinterpret_cast<float *>(local)[(g * G_GROUP + q) * G_FEATS + quarter * 32 + lane] = sum;
+                        else if (c < p.c_end && f < a.feats)
+                            finish_one<O, SCALED>(a, p.group, c, f, (plane + c) * a.feats + f, sum);
                     }
                 }
             }
@@ -365,23 +435,16 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     __syncwarp();
     if (!PAIR && a.split > 1) {                                  // one tile per cluster: every CTA adds up its share of the columns
         cluster_barrier();
-        if (warp < 8 && first < tiles && !*over) {
+        if (warp < G_TMA_WARP && first < tiles && !*over) {
             const TilePlace p = place(first);
             const uint64_t plane = BY_K ? p.group * a.cols : 0;
-            O *const out = static_cast<O *>(a.out);
-            const O *const times = static_cast<const O *>(a.times), *const residual = static_cast<const O *>(a.residual);
             const uint32_t share = a.nt / a.split, feat = tid & (G_FEATS - 1);
             const uint64_t f = features(p) + feat;
             const Peers peers(ring, a.split);
             if (f < a.feats) {
-                const float bias = a.bias ? widen(static_cast<const O *>(a.bias)[p.group * a.feats + f]) : 0.0f, a_scale = a.a_scale ? a.a_scale[f] : 0.0f;
 #pragma unroll 2
-                for (uint32_t q = rank * share + tid / G_FEATS; q < (rank + 1) * share && p.c + q < p.c_end; q += 2) {
-                    const uint64_t c = p.c + q, at = (plane + c) * a.feats + f;
-                    float v = peers.sum((q * G_FEATS + feat) * 4);
-                    finish<O, 1>(a, c, f, at, &v, &bias, &a_scale, times + c * a.times_stride + f, residual + c * a.residual_stride + f);
-                    out[at] = narrow<O>(v);
-                }
+                for (uint32_t q = rank * share + tid / G_FEATS; q < (rank + 1) * share && p.c + q < p.c_end; q += G_EPILOGUE / G_FEATS)
+                    finish_one<O, SCALED>(a, p.group, p.c + q, f, (plane + p.c + q) * a.feats + f, peers.sum((q * G_FEATS + feat) * 4));
             }
         }
         cluster_barrier();
@@ -389,7 +452,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     if constexpr (PAIR) cluster_barrier();                       // nobody's barriers or tiles go while the other may use them
     tc_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == G_TMA_WARP + 1) {
         tc_after();
         tmem_free<PAIR>(tmem, a.tmem_columns);
     }
