@@ -40,27 +40,32 @@ __device__ __forceinline__ void act_all(uint32_t kind, float *v)
     }
 }
 
-// The activation and its derivative.
-__device__ __forceinline__ void act_and_slope(uint32_t kind, float z, float &y, float &slope)
+// N activations and their derivatives.
+template <int N>
+__device__ __forceinline__ void act_and_slope(uint32_t kind, const float *z, float *y, float *slope)
 {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < N; e++) f(z[e], y[e], slope[e]);
+    };
     switch (kind) {
-    case ACT_RELU: y = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f; return;
-    case ACT_SILU: {
-        const float e = __fdividef(1, 1 + __expf(-z));
-        y = z * e, slope = e * (1 + z * (1 - e));
-        return;
-    }
-    case ACT_GELU: {
-        const float below = 0.5f * (1 + erff(z * ROOT_HALF));
-        y = z * below, slope = below + z * ROOT_1_2PI * __expf(-0.5f * z * z);
-        return;
-    }
-    case ACT_GELU_TANH: {
-        const float t = tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z));
-        y = 0.5f * z * (1 + t), slope = 0.5f * (1 + t) + 0.5f * z * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * z * z);
-        return;
-    }
-    default: y = z, slope = 1;
+    case ACT_RELU: return each([](float z, float &y, float &slope) { y = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f; });
+    case ACT_SILU:
+        return each([](float z, float &y, float &slope) {
+            const float e = __fdividef(1, 1 + __expf(-z));
+            y = z * e, slope = e * (1 + z * (1 - e));
+        });
+    case ACT_GELU:
+        return each([](float z, float &y, float &slope) {
+            const float below = 0.5f * (1 + erff(z * ROOT_HALF));
+            y = z * below, slope = below + z * ROOT_1_2PI * __expf(-0.5f * z * z);
+        });
+    case ACT_GELU_TANH:
+        return each([](float z, float &y, float &slope) {
+            const float t = tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z));
+            y = 0.5f * z * (1 + t), slope = 0.5f * (1 + t) + 0.5f * z * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * z * z);
+        });
+    default: return each([](float z, float &y, float &slope) { y = z, slope = 1; });
     }
 }
 
@@ -111,7 +116,7 @@ __device__ __forceinline__ uint32_t group_of(const uint32_t *starts, uint32_t co
 }
 
 constexpr uint32_t MAX_EXPERTS = 1024;
-constexpr uint32_t EG_THREADS = 128, EG_ROWS = 32;
+constexpr uint32_t EG_THREADS = 128, EG_MOST_ROWS = 32, EG_LEAST_ROWS = 4, EG_STEP = 2;     // rows of a chunk, and of those under way together
 
 struct EpilogueGradArgs {
     const void *dy, *times;                      // times: or NULL, rows times_stride apart
@@ -120,7 +125,7 @@ struct EpilogueGradArgs {
     float *partial;                              // [chunk of rows + group][out]: sums of dz, or NULL
     Groups groups;
     uint64_t rows, out, times_stride, dz_stride;
-    uint32_t vectors, activation;
+    uint32_t vectors, activation, chunk;         // chunk: rows
 };
 
 template <int N>
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
     group_starts(a.groups, starts);
     __syncthreads();
     const uint64_t v = blockIdx.y * static_cast<uint64_t>(EG_THREADS) + threadIdx.x;
-    const uint32_t chunk = blockIdx.x, begin = chunk * EG_ROWS, end = begin + EG_ROWS < a.rows ? begin + EG_ROWS : static_cast<uint32_t>(a.rows);
+    const uint32_t chunk = blockIdx.x, begin = chunk * a.chunk, end = begin + a.chunk < a.rows ? begin + a.chunk : static_cast<uint32_t>(a.rows);
     if (v >= a.vectors) return;
     const uint32_t first = starts[0], last = starts[a.groups.count];
     uint32_t group = group_of(starts, a.groups.count, begin < first ? first : begin);
@@ -165,41 +170,56 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
         for (int e = 0; e < V::N; e++) sum[e] = 0;
         any = false;
     };
-    for (uint32_t t = begin; t < end; t++) {
-        const bool on = t >= first && t < last;
-        if (on && t >= starts[group + 1]) {
-            flush();
-            group = group_of(starts, a.groups.count, t);
-        }
-        V d, m, dz, dm;
-        alignas(16) float z[V::N] = {};
-        d.raw = m.raw = dz.raw = dm.raw = {};
-        if (on) {
-            d.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + t * a.out)[v];
-            if (a.z) load_floats<V::N>(a.z + t * a.out + v * V::N, z);
-            if (a.times) m.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.times) + t * a.times_stride)[v];
+    for (uint32_t t0 = begin; t0 < end; t0 += EG_STEP) {
+        V d[EG_STEP], m[EG_STEP];
+        alignas(16) float z[EG_STEP][V::N];
 #pragma unroll
-            for (int e = 0; e < V::N; e++) {
-                float y, slope;
-                act_and_slope(a.activation, z[e], y, slope);
-                const float g = widen(d.e[e]);
-                dm.e[e] = narrow<T>(g * y);
-                float u = g * slope;
-                if (a.times) u *= widen(m.e[e]);
-                sum[e] += u;
-                dz.e[e] = narrow<T>(u);
-            }
-            any = true;
+        for (uint32_t i = 0; i < EG_STEP; i++) {
+            const uint32_t t = t0 + i;
+            d[i].raw = m[i].raw = {};
+#pragma unroll
+            for (int e = 0; e < V::N; e++) z[i][e] = 0;
+            if (t >= end || t < first || t >= last) continue;
+            d[i].raw = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + t * a.out)[v];
+            if (a.z) load_floats<V::N>(a.z + t * a.out + v * V::N, z[i]);
+            if (a.times) m[i].raw = reinterpret_cast<const R *>(static_cast<const T *>(a.times) + t * a.times_stride)[v];
         }
-        if (a.dz) reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = dz.raw;
-        if (a.dtimes) reinterpret_cast<R *>(static_cast<T *>(a.dtimes) + t * a.out)[v] = dm.raw;
+#pragma unroll
+        for (uint32_t i = 0; i < EG_STEP; i++) {
+            const uint32_t t = t0 + i;
+            if (t >= end) break;
+            V dz, dm;
+            dz.raw = dm.raw = {};
+            if (t >= first && t < last) {
+                if (t >= starts[group + 1]) {
+                    flush();
+                    group = group_of(starts, a.groups.count, t);
+                }
+                float y[V::N], u[V::N];
+                act_and_slope<V::N>(a.activation, z[i], y, u);
+#pragma unroll
+                for (int e = 0; e < V::N; e++) {
+                    const float g = widen(d[i].e[e]);
+                    dm.e[e] = narrow<T>(g * y[e]), u[e] *= g;
+                }
+                if (a.times) {
+#pragma unroll
+                    for (int e = 0; e < V::N; e++) u[e] *= widen(m[i].e[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < V::N; e++) sum[e] += u[e], dz.e[e] = narrow<T>(u[e]);
+                any = true;
+            }
+            if (a.dz) reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = dz.raw;
+            if (a.dtimes) reinterpret_cast<R *>(static_cast<T *>(a.dtimes) + t * a.out)[v] = dm.raw;
+        }
     }
     flush();
 }
 
 // A group's bias gradient: what the chunks that its rows lie in have for it, in their order.
 template <class T>
-__global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups groups, uint64_t out, T *dbias)
+__global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups groups, uint64_t out, uint32_t chunk, T *dbias)
 {
     __shared__ uint32_t starts[MAX_EXPERTS + 1];
     __shared__ float sums[8][32];
@@ -211,7 +231,7 @@ __global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups 
     const uint64_t d = blockIdx.x * 32ull + lane;
     float sum = 0;
     if (starts[g + 1] > starts[g] && d < out)
-        for (uint32_t c = starts[g] / EG_ROWS + warp; c <= (starts[g + 1] - 1) / EG_ROWS; c += 8) sum += partial[(static_cast<uint64_t>(c) + g) * out + d];
+        for (uint32_t c = starts[g] / chunk + warp; c <= (starts[g + 1] - 1) / chunk; c += 8) sum += partial[(static_cast<uint64_t>(c) + g) * out + d];
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp || d >= out) return;

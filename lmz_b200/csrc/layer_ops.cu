@@ -178,6 +178,13 @@ static uint64_t up16(uint64_t n) { return (n + 15) & ~15ull; }
 struct ProductLayout {
     uint64_t x, w, dz, partial, end = 0;
     bool pack_x, pack_w, own_dz;                 // own_dz: dz is not dy, or does not lie where TMA takes it
+    // Rows of a chunk of the epilogue's gradients: as few as give every multiprocessor blocks enough.
+    static uint32_t chunk(const lmz_product *p)
+    {
+        uint32_t rows = EG_MOST_ROWS;
+        while (rows > EG_LEAST_ROWS && p->rows * p->out < 1024ull * EG_THREADS * 8 * rows) rows /= 2;
+        return rows;
+    }
     ProductLayout(const lmz_product *p, bool grad)
     {
         auto take = [&](bool on, uint64_t bytes) {
@@ -192,7 +199,7 @@ struct ProductLayout {
         x = take(pack_x && (!grad || p->dweight), p->rows * up16(p->in) * e);
         w = take(pack_w && (!grad || p->dx), p->experts * p->out * up16(p->in) * e);
         dz = take(grad && own_dz, p->rows * up8(p->out) * 2);
-        partial = take(grad && p->dbias, ((p->rows + EG_ROWS - 1) / EG_ROWS + p->experts) * p->out * 4);
+        partial = take(grad && p->dbias, ((p->rows + chunk(p) - 1) / chunk(p) + p->experts) * p->out * 4);
     }
 };
 
@@ -234,7 +241,7 @@ static int launch_product_as(ProductArgs &a, unsigned grid, cudaStream_t cs)
     static bool done[64];
     const int rc = opt_in_smem(k_product<T, O, P, PAIR>, PRODUCT_SMEM, done);
     if (rc) return rc;
-    a.stage_bytes = product_stage_bytes(a.nt, PAIR);
+    a.stage_bytes = product_stage_bytes(a.nt, PAIR, P == WEIGHT_GRAD);
     const uint32_t rest = ATOM_BYTES + G_EPILOGUE / 32 * G_TURN_BYTES;
     a.stages = std::min<uint32_t>(G_MAX_STAGES, (PRODUCT_SMEM - rest) / a.stage_bytes);
     cudaLaunchAttribute attrs[2]{};
@@ -257,8 +264,12 @@ static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64
     auto most_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : groups == 1 ? (a.cols + nt - 1) / nt : a.cols / nt + used; };
     const uint64_t rows_each = std::max<uint64_t>(1, a.cols / used);
     const uint64_t all_steps = by_k ? std::max<uint64_t>(1, (depth / groups + STEP_K - 1) / STEP_K) : (depth + step_elements - 1) / step_elements;
-    // Tiles of 256 by 256 by pairs of CTAs, or of 128 features by 16 to 128 columns by one, or by a cluster that shares k: by what they are reckoned to
-    // take (in 10 ns).
+    // Tiles of 256 features by 160 to 256 columns by pairs of CTAs, or of 128 by 16 to 128 by one, or by a cluster that shares k: by what they are
+    // reckoned to take (in 10 ns).  A step of a pair takes 0.3 us at 256 columns, of a CTA 0.19 whatever they are; what a tile takes beside its steps is a
+    // pair's 2.6 us and more, a CTA's 0.04 a column; a cluster's meeting 1.4 us and more; the launch and the first tiles 6.  One B200, us, rows x in x
+    // out, reckoned and measured: 4096x4096x4096 pairs of 256 93 (92), of 192 94 (95), 128 a CTA 74 for half the rows (75); 512x4096x4096 pairs of 160 22
+    // (22), of 256 28 (28), 128 a CTA 23 (24); 1x4096x4096 by four CTAs 11 (13), by two 14 (14), by one 19 (19); the weight's gradient of
+    // 5000x256x256 by eight 13 (10), by two 18 (19).
     uint64_t best = ~0ull;
     bool pair = false;
     a.split = 1;
@@ -267,16 +278,17 @@ static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64
         const uint64_t n = feats * col_tiles(nt) * split;
         if (split > 1 && feats * most_tiles(nt) * split > places) return;
         const uint64_t waves = (n + places - 1) / places, steps = (all_steps + split - 1) / split;
-        const uint64_t step = p2 ? 30 : std::max<uint64_t>(19, std::min(n, places) * (G_FEATS + nt) / 940);
-        const uint64_t meeting = split == 1 ? 0 : split == 2 ? 150 + 5 * nt / 2 : 180 * split;
-        const uint64_t cost = waves * (step * steps + (p2 ? 600 : 4 * nt + meeting)) + 600;
+        const uint64_t tile = p2 ? 30 * nt * steps / 256 + 516 - nt : 19 * steps + 4 * nt + (split == 1 ? 0 : 100 + 20 * split);
+        const uint64_t cost = waves * tile + 600;
         if (cost < best) best = cost, pair = p2, a.nt = nt, a.split = split;
     };
+    // (columns side by side come in blocks of 64, so that pairs of fewer than 256 of them load as much)
     const uint64_t wide = by_k ? a.cols : rows_each;
-    for (uint32_t nt = by_k ? 64 : G_GROUP; nt < G_COLS; nt *= 2)
+    for (uint32_t nt = by_k ? 64 : G_GROUP; nt <= 128; nt *= 2)
         for (uint32_t split = 1; split <= 8 && 2 * split <= std::max<uint64_t>(2, all_steps); split *= 2)
             if (nt == (by_k ? 64 : G_GROUP) || nt < 2 * wide) consider(false, nt, split);
-    if (wide > G_COLS / 2) consider(true, G_COLS, 1);
+    for (uint32_t nt = 256; nt >= (by_k ? 256 : 160); nt -= 32)
+        if (wide > nt / 2) consider(true, nt, 1);
     const uint64_t per = (pair ? 2 : 1) * G_FEATS, feat_tiles = (a.feats + per - 1) / per, most = feat_tiles * most_tiles(a.nt);
     if (most >= 1u << 28) return fail_msg(LMZ_GPU_EUNSUPPORTED, "too many rows for a weight of this size");
     a.feat_tiles = static_cast<uint32_t>(feat_tiles), a.col_tiles = static_cast<uint32_t>((a.cols + a.nt - 1) / a.nt);
@@ -312,18 +324,19 @@ static int product_as(const lmz_product *p, cudaStream_t cs)
 template <class T>
 static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T *dz, cudaStream_t cs)
 {
-    const uint64_t chunks = (p->rows + EG_ROWS - 1) / EG_ROWS;
+    const uint32_t chunk = ProductLayout::chunk(p);
+    const uint64_t chunks = (p->rows + chunk - 1) / chunk;
     float *partial = p->dbias ? reinterpret_cast<float *>(static_cast<uint8_t *>(p->work) + l.partial) : nullptr;
     int rc = by_width<T>(vector_bytes(p->out * 2, {address(p->dy), address(p->z) / 2, address(p->times), p->times ? p->times_stride * 2 : 0, address(p->dtimes)}), [&](auto vec) {
         constexpr int VB = sizeof(vec.raw);
         EpilogueGradArgs a{};
         a.dy = p->dy, a.z = p->z, a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
-        a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation;
+        a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation, a.chunk = chunk;
         return launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, dim3(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS), EG_THREADS, 0, cs, a);
     });
     if (!rc && p->dbias)
         rc = launch("launch k_bias_join", k_bias_join<T>, dim3(static_cast<unsigned>((p->out + 31) / 32), p->experts), 256, 0, cs, static_cast<const float *>(partial),
-                    groups_of(p), p->out, static_cast<T *>(p->dbias));
+                    groups_of(p), p->out, chunk, static_cast<T *>(p->dbias));
     return rc;
 }
 

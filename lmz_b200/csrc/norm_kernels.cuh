@@ -35,8 +35,8 @@ __device__ __forceinline__ float row_join(float v, uint32_t log, float *room, F 
     __syncthreads();
     if ((threadIdx.x & 31) == 0) room[warp] = v;
     __syncthreads();
-    v = room[first];
-    for (uint32_t w = 1; w < warps; w++) v = both(v, room[first + w]);
+    v = room[first + (threadIdx.x & (warps - 1))];
+    for (uint32_t o = 1; o < warps; o <<= 1) v = both(v, __shfl_xor_sync(~0u, v, o));
     return v;
 }
 __device__ __forceinline__ float row_sum(float v, uint32_t log, float *room)
@@ -71,6 +71,14 @@ __device__ __forceinline__ float scale_of_most(float most)
 {
     const float s = most / 448.0f;
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;            // (a NaN stays)
+}
+
+// u / v rounded once, by v's reciprocal: the quotient's remainder, which one multiply-add has exactly, corrects it (Markstein's theorem: a
+// correctly rounded reciprocal and this step give the correctly rounded quotient).  A third of a division's instructions.
+__device__ __forceinline__ float divided(float u, float v, float reciprocal)
+{
+    const float q = u * reciprocal;
+    return fmaf(fmaf(-q, v, u), reciprocal, q);
 }
 
 // N numbers of 8 bits, as one store.
@@ -179,12 +187,13 @@ __global__ void __launch_bounds__(NORM_MOST) k_norm(const NormArgs a)
 #pragma unroll
             for (int e = 0; e < V::N; e++) most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(u[e]) & 0x7FFFFFFF));
         });
-        const float scale = scale_of_most(row_most(most, a.lane_log, room[1]));
+        const float scale = scale_of_most(row_most(most, a.lane_log, room[1])), inverse = 1.0f / scale;
         if (on && lane == 0) a.scale[t] = scale;
+        const bool quick = scale > 1e-30f && scale < 1e30f;      // (neither NaN nor infinite, and no remainder below the smallest number)
         each([&](uint32_t v, const float *u) {
             float d[V::N];
 #pragma unroll
-            for (int e = 0; e < V::N; e++) d[e] = u[e] / scale;
+            for (int e = 0; e < V::N; e++) d[e] = quick ? divided(u[e], scale, inverse) : u[e] / scale;
             store_8bit<V::N>(a.q + t * a.dim + static_cast<uint64_t>(v) * V::N, d);
         });
     } else {

@@ -15,7 +15,6 @@ namespace lmz {
 enum Product : int { FORWARD, ROWS_GRAD, WEIGHT_GRAD };
 
 constexpr uint32_t G_FEATS = 128;              // features of a tile: the tensor core's M, a TMEM lane each
-constexpr uint32_t G_COLS = 256;               // most columns of a tile: its N, a TMEM column each
 constexpr uint32_t G_GROUP = 16;               // columns of a TMEM load
 constexpr uint32_t G_MAX_STAGES = 10, G_EPILOGUE = 512, G_THREADS = G_EPILOGUE + 96, G_TMA_WARP = G_EPILOGUE / 32;
 constexpr uint32_t G_PITCH = 36;               // words from one column to the next where a warp turns 32 lanes' features round
@@ -47,13 +46,18 @@ struct ProductArgs {
     bool vectors;                                // rows of all tensors that the epilogue has to do with start on 16 bytes
 };
 
-// Tiles of a stage: A's 128 f, and the columns' (of a pair's 256 each CTA has half).
-__host__ __device__ constexpr uint32_t product_stage_bytes(uint32_t nt, bool pair) { return (G_FEATS + (pair ? nt / 2 : nt)) * ROW_BYTES; }
+// Tiles of a stage: A's 128 f, and the columns' (of a pair's each CTA has half); of columns side by side in blocks of 64.
+__host__ __device__ constexpr uint32_t product_stage_bytes(uint32_t nt, bool pair, bool side_by_side)
+{
+    const uint32_t cols = pair ? nt / 2 : nt;
+    return (G_FEATS + (side_by_side ? (cols + 63) / 64 * 64 : cols)) * ROW_BYTES;
+}
 
 // A tile's place.
 struct TilePlace {
     uint32_t group, ft;
     uint32_t c, c_end;                           // its first column, and its group's end
+    uint32_t n;                                  // its columns as the products have them: a multiple of 16 (a pair's: 32), nt at most
     uint32_t k, k_rows;                          // WEIGHT_GRAD: the group's rows
 };
 
@@ -118,8 +122,8 @@ __device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group,
 // Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; sixteen warps take the
 // sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.  They turn 32 features and 16 columns round
 // in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.
-// Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile's columns behind its group's last are another group's
-// rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
+// Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile ends with its group,
+// to a multiple of 16 columns; what is behind its group's last column is another group's rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
 // last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.  Only such
 // steps go by that warp (all of them did at first: handing a step on to another CTA takes 1 us, and 8192 rows 4096x14336 took 2070 us and not 634).
 // Few tiles: the CTAs of a cluster share k, and their sums meet in distributed shared memory.
@@ -191,6 +195,8 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             if (groups > 1) p.group = group_of(s.tiles, groups, ct);
             p.c = s.starts[p.group] + (ct - s.tiles[p.group]) * a.nt, p.c_end = s.starts[p.group + 1], p.k = p.k_rows = 0;
         }
+        const uint32_t left = (p.c_end - p.c + 16 * CTAS - 1) / (16 * CTAS) * (16 * CTAS);
+        p.n = left < a.nt ? left : a.nt;
         return p;
     };
     auto all_steps = [&](const TilePlace &p) { return BY_K ? (p.k_rows + STEP_K - 1) / STEP_K : a.steps; };
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         uint32_t last_tail = 0, tail_turn = 0;                   // bits per stage: its last use was a tail; how many of its tails there were
         for (uint32_t tile = first; tile < tiles; tile += stride) {
             const TilePlace p = place(tile);
-            const uint32_t f = features(p), c = p.c + (PAIR ? side * (a.nt / 2) : 0), steps = all_steps(p), k1 = step_from(steps, rank + 1);
+            const uint32_t f = features(p), c = p.c + (PAIR ? side * (p.n / 2) : 0), steps = all_steps(p), k1 = step_from(steps, rank + 1);
             bool ok = true;
             for (uint32_t k = step_from(steps, rank); k < k1; k++, at.next(a.stages)) {
                 const uint32_t st = at.stage;
@@ -254,15 +260,14 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         if (!side) {
             const uint32_t a_step = A_MN ? 16 * ROW_BYTES : 32, b_step = B_MN ? 16 * ROW_BYTES : 32;
             RingPlace at;
-            uint32_t n = 0, desc;
-            if constexpr (sizeof(T) == 1) desc = mma_desc_e4m3(CTAS * G_FEATS, a.nt);
-            else desc = mma_desc(__is_same(T, __nv_bfloat16), A_MN, B_MN, CTAS * G_FEATS, a.nt);
+            uint32_t n = 0;
             const uint32_t a_lo = desc_lo(ring, A_MN ? G_BLOCK : 16), b_lo = desc_lo(ring + G_FEATS * ROW_BYTES, B_MN ? G_BLOCK : 16);
             bool ok = true;
             for (uint32_t tile = first; tile < tiles; tile += stride, n++) {
                 const TilePlace p = place(tile);
                 const uint32_t steps = all_steps(p), k0 = step_from(steps, rank), k1 = step_from(steps, rank + 1);
                 const uint32_t buf = n & 1, sums = tmem + buf * a.nt;
+                const uint32_t desc = sizeof(T) == 1 ? mma_desc_e4m3(CTAS * G_FEATS, p.n) : mma_desc(__is_same(T, __nv_bfloat16), A_MN, B_MN, CTAS * G_FEATS, p.n);
                 ok = n < 2 || warp_wait(&s.sums_empty[buf], (n / 2 - 1) & 1, over);
                 if (!ok) break;
                 tc_after();
