@@ -197,17 +197,19 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
                 }
                 float y[V::N], u[V::N];
                 act_and_slope<V::N>(a.activation, z[i], y, u);
+                float g[V::N];
+                widen_all(d[i], g);
 #pragma unroll
-                for (int e = 0; e < V::N; e++) {
-                    const float g = widen(d[i].e[e]);
-                    dm.e[e] = narrow<T>(g * y[e]), u[e] *= g;
-                }
+                for (int e = 0; e < V::N; e++) y[e] *= g[e], u[e] *= g[e];
+                narrow_all<V::N>(y, dm.e);
                 if (a.times) {
+                    widen_all(m[i], g);
 #pragma unroll
-                    for (int e = 0; e < V::N; e++) u[e] *= widen(m[i].e[e]);
+                    for (int e = 0; e < V::N; e++) u[e] *= g[e];
                 }
 #pragma unroll
-                for (int e = 0; e < V::N; e++) sum[e] += u[e], dz.e[e] = narrow<T>(u[e]);
+                for (int e = 0; e < V::N; e++) sum[e] += u[e];
+                narrow_all<V::N>(u, dz.e);
                 any = true;
             }
             if (a.dz) reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = dz.raw;

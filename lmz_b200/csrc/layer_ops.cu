@@ -59,9 +59,9 @@ static int by_norm_types(const lmz_norm *p, std::initializer_list<uint64_t> at, 
 struct NormShape {
     uint32_t lane_log = 0, threads;
     bool is_long;
-    NormShape(uint32_t vectors, uint32_t elements)
+    NormShape(uint32_t vectors, uint32_t elements, uint32_t vector_bytes)
     {
-        const uint32_t each = NORM_EACH / elements;
+        const uint32_t each = norm_each(vector_bytes) / elements;
         while ((1u << lane_log) < NORM_MOST && (each << lane_log) < vectors) lane_log++;
         is_long = (each << lane_log) < vectors;
         threads = std::max(NORM_THREADS, 1u << lane_log);
@@ -85,7 +85,7 @@ API int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream)
         a.x = p->x, a.residual = p->residual, a.weight = p->weight, a.y = p->y, a.stream = p->stream, a.q = static_cast<uint8_t *>(p->q);
         a.scale = p->scale, a.rstd = p->rstd, a.tokens = p->tokens, a.dim = p->dim, a.x_stride = p->x_stride, a.residual_stride = p->residual_stride;
         a.vectors = static_cast<uint32_t>(p->dim / N), a.eps = p->eps;
-        const NormShape shape(a.vectors, N);
+        const NormShape shape(a.vectors, N, VB);
         a.lane_log = shape.lane_log;
         const uint32_t per = shape.threads >> shape.lane_log;
         const dim3 grid(static_cast<unsigned>((p->tokens + per - 1) / per));
@@ -95,22 +95,22 @@ API int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream)
     });
 }
 
-// Blocks of the gradients' kernel: the shares of the weight's gradient are read again, so no more of them than keep the multiprocessors busy.
-constexpr uint32_t NORM_GRAD_BLOCKS = 4 * 148;
-static uint64_t norm_grad_shares(const lmz_norm *p, const NormShape &shape)
+// Blocks of the gradients' kernel: a share of the weight's gradient each, which are read again.  As many as there is room for (four of 256
+// threads to a multiprocessor), and where there are few tokens, no more than have two turns each.
+static uint64_t norm_grad_blocks(uint64_t tokens, uint32_t per)
 {
-    const uint32_t per = shape.threads >> shape.lane_log;
-    return std::min<uint64_t>((p->tokens + per - 1) / per, NORM_GRAD_BLOCKS) * per;
+    const uint64_t rows = (tokens + per - 1) / per;
+    return std::min<uint64_t>(rows, std::max<uint64_t>(148, std::min<uint64_t>(4 * 148, (rows + 1) / 2)));
 }
 
 API size_t lmz_gpu_norm_grad_work_bytes(const lmz_norm *p)
 {
-    // (whatever the vectors' width, a thread has NORM_EACH elements or fewer, and a block NORM_THREADS threads or one row's)
-    const uint64_t row = std::min<uint64_t>(NORM_MOST, (p->dim + NORM_EACH - 1) / NORM_EACH);
-    uint64_t lanes = 1;
-    while (lanes < row) lanes *= 2;
-    const uint64_t per = std::max<uint64_t>(1, NORM_THREADS / lanes);
-    return std::min<uint64_t>((p->tokens + per - 1) / per, NORM_GRAD_BLOCKS) * per * p->dim * sizeof(float);
+    uint64_t most = 0;                           // (of wide and of narrow vectors: how many threads share a row goes by its elements alone)
+    for (uint32_t vb : {16u, 8u}) {
+        const NormShape shape(static_cast<uint32_t>(p->dim), 1, vb);
+        most = std::max(most, norm_grad_blocks(p->tokens, shape.threads >> shape.lane_log));
+    }
+    return most * p->dim * sizeof(float);
 }
 
 API int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream)
@@ -134,11 +134,12 @@ API int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream)
         a.s = p->x, a.weight = p->weight, a.dy = p->dy, a.ds = p->dstream, a.rstd = p->rstd, a.dx = p->dx;
         a.partial = p->dweight ? static_cast<float *>(p->work) : nullptr;
         a.tokens = p->tokens, a.dim = p->dim, a.s_stride = p->x_stride, a.vectors = static_cast<uint32_t>(p->dim / N);
-        const NormShape shape(a.vectors, N);
+        const NormShape shape(a.vectors, N, VB);
         a.lane_log = shape.lane_log;
-        const uint64_t shares = norm_grad_shares(p, shape);
-        const dim3 grid(static_cast<unsigned>(shares / (shape.threads >> shape.lane_log)));
-        int failed = launch("launch k_norm_grad", shape.is_long ? k_norm_grad<T, W, VB, true> : k_norm_grad<T, W, VB, false>, grid, shape.threads, 0, cs, a);
+        const uint64_t shares = norm_grad_blocks(p->tokens, shape.threads >> shape.lane_log);
+        int failed = launch("launch k_norm_grad", shape.is_long ? k_norm_grad<T, W, VB, true, NORM_MOST> : shape.threads > NORM_THREADS ? k_norm_grad<T, W, VB, false, NORM_MOST>
+                                                                                                         : k_norm_grad<T, W, VB, false, NORM_THREADS>,
+                            dim3(static_cast<unsigned>(shares)), shape.threads, 0, cs, a);
         if (!failed && p->dweight)
             failed = launch("launch k_join", k_join<W>, dim3(static_cast<unsigned>((p->dim + 31) / 32)), 32 * JOIN_WARPS, 0, cs, static_cast<const float *>(a.partial),
                             shares, p->dim, static_cast<W *>(p->dweight));

@@ -11,7 +11,10 @@
 
 namespace lmz {
 
-constexpr uint32_t NORM_THREADS = 256, NORM_MOST = 1024, NORM_EACH = 16;     // elements that a thread has of a row in registers
+constexpr uint32_t NORM_THREADS = 256, NORM_MOST = 1024;
+// Elements that a thread has of a row in registers.  Where vectors are narrow, half as many: a thread has more loads to wait for then (one B200, gradients
+// of 3001x997 FP32, rows that start on 4 bytes: 31 us by sixteen, 9 by eight).
+__host__ __device__ constexpr uint32_t norm_each(uint32_t vector_bytes) { return vector_bytes == 16 ? 16 : 8; }
 
 struct NormArgs {
     const void *x, *residual, *weight;           // residual: or NULL; weight: NULL for rows that only go to 8 bits
@@ -43,10 +46,16 @@ __device__ __forceinline__ float row_sum(float v, uint32_t log, float *room)
 {
     return row_join(v, log, room, [](float a, float b) { return a + b; });
 }
-// (By their bits: those of a NaN are above those of infinity, so that it stays.)
+// (A NaN stays.)
+__device__ __forceinline__ float larger(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 __device__ __forceinline__ float row_most(float v, uint32_t log, float *room)
 {
-    return row_join(v, log, room, [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); });
+    return row_join(v, log, room, larger);
 }
 
 template <class W, int N>
@@ -58,8 +67,7 @@ __device__ __forceinline__ void load_weights(const W *from, float *to)
     for (int i = 0; i < N / V::N; i++) {
         V v;
         v.raw = reinterpret_cast<const typename Raw<B>::type *>(from)[i];
-#pragma unroll
-        for (int e = 0; e < V::N; e++) to[i * V::N + e] = widen(v.e[e]);
+        widen_all(v, to + i * V::N);
     }
 }
 
@@ -100,11 +108,11 @@ __device__ __forceinline__ void store_8bit(uint8_t *to, const float *v)
 //
 // Bound by HBM: x and the residual read, the stream and y written.
 template <class T, class W, int VB, bool BITS8, bool LONG>
-__global__ void __launch_bounds__(NORM_MOST) k_norm(const NormArgs a)
+__global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
 {
     using V = Vec<T, VB>;
     using R = typename Raw<VB>::type;
-    constexpr int NV = LONG ? 1 : NORM_EACH / V::N;
+    constexpr int NV = LONG ? 1 : norm_each(VB) / V::N;
     __shared__ float room[2][32];
     const uint32_t lanes = 1u << a.lane_log, lane = threadIdx.x & (lanes - 1);
     const uint64_t t = static_cast<uint64_t>(blockIdx.x) * (blockDim.x >> a.lane_log) + (threadIdx.x >> a.lane_log);
@@ -122,12 +130,14 @@ __global__ void __launch_bounds__(NORM_MOST) k_norm(const NormArgs a)
         if (a.residual) {
             V q;
             q.raw = res[v];
+            float both[V::N], other[V::N];
+            widen_all(p, both), widen_all(q, other);
 #pragma unroll
-            for (int e = 0; e < V::N; e++) p.e[e] = narrow<T>(widen(p.e[e]) + widen(q.e[e]));
+            for (int e = 0; e < V::N; e++) both[e] += other[e];
+            narrow_all<V::N>(both, p.e);
             if (write && a.stream) stream[v] = p.raw;
         }
-#pragma unroll
-        for (int e = 0; e < V::N; e++) to[e] = widen(p.e[e]);
+        widen_all(p, to);
     };
     float s[NV][V::N];
     float squares = 0;
@@ -185,22 +195,25 @@ __global__ void __launch_bounds__(NORM_MOST) k_norm(const NormArgs a)
         float most = 0;
         each([&](uint32_t, const float *u) {
 #pragma unroll
-            for (int e = 0; e < V::N; e++) most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(u[e]) & 0x7FFFFFFF));
+            for (int e = 0; e < V::N; e++) most = larger(most, fabsf(u[e]));
         });
         const float scale = scale_of_most(row_most(most, a.lane_log, room[1])), inverse = 1.0f / scale;
         if (on && lane == 0) a.scale[t] = scale;
         const bool quick = scale > 1e-30f && scale < 1e30f;      // (neither NaN nor infinite, and no remainder below the smallest number)
-        each([&](uint32_t v, const float *u) {
-            float d[V::N];
+        auto write = [&](auto quotient) {
+            each([&](uint32_t v, const float *u) {
+                float d[V::N];
 #pragma unroll
-            for (int e = 0; e < V::N; e++) d[e] = quick ? divided(u[e], scale, inverse) : u[e] / scale;
-            store_8bit<V::N>(a.q + t * a.dim + static_cast<uint64_t>(v) * V::N, d);
-        });
+                for (int e = 0; e < V::N; e++) d[e] = quotient(u[e]);
+                store_8bit<V::N>(a.q + t * a.dim + static_cast<uint64_t>(v) * V::N, d);
+            });
+        };
+        if (quick) write([&](float u) { return divided(u, scale, inverse); });
+        else write([&](float u) { return u / scale; });
     } else {
         each([&](uint32_t v, const float *u) {
             V p;
-#pragma unroll
-            for (int e = 0; e < V::N; e++) p.e[e] = narrow<T>(u[e]);
+            narrow_all<V::N>(u, p.e);
             reinterpret_cast<R *>(static_cast<T *>(a.y) + t * a.dim)[v] = p.raw;
         });
     }
@@ -210,26 +223,28 @@ struct NormGradArgs {
     const void *s, *weight, *dy, *ds;            // s: what was normed (rows s_stride apart); ds: the stream's own gradient, or NULL
     const float *rstd;
     void *dx;                                    // or NULL
-    float *partial;                              // [row of threads][dim]: each one's sum of dy n; or NULL
+    float *partial;                              // [block][dim]: its sum of dy n; or NULL
     uint64_t tokens, dim, s_stride;
     uint32_t vectors, lane_log;
 };
 
-// The gradient of s, and each row of threads' share of the weight's: a row of threads takes every (rows of threads)-th token, so that
-// its sums have one order.  LONG: the shares lie in global memory, where a thread finds its own columns again.
+// The gradient of s, and each block's share of the weight's: a row of threads takes every (rows of threads)-th token, and a block's rows of
+// threads add up in their order, so that sums have one order.  LONG: the shares lie in global memory, where a thread finds its own columns again.
 //
-// Bound by HBM: dy, s and ds read, dx written.
-template <class T, class W, int VB, bool LONG>
-__global__ void __launch_bounds__(NORM_MOST) k_norm_grad(const NormGradArgs a)
+// Bound by HBM: dy, s and ds read, dx written.  MOST: threads of a block.
+template <class T, class W, int VB, bool LONG, uint32_t MOST>
+__global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const NormGradArgs a)
 {
     using V = Vec<T, VB>;
     using R = typename Raw<VB>::type;
-    constexpr int NV = LONG ? 1 : NORM_EACH / V::N;
+    constexpr int NV = LONG ? 1 : norm_each(VB) / V::N;
+    constexpr bool SEVERAL = MOST == NORM_THREADS;               // rows of threads in a block, at times
     __shared__ float room[2][32];
-    const uint32_t lanes = 1u << a.lane_log, lane = threadIdx.x & (lanes - 1), per = blockDim.x >> a.lane_log;
-    const uint64_t me = static_cast<uint64_t>(blockIdx.x) * per + (threadIdx.x >> a.lane_log), step = static_cast<uint64_t>(gridDim.x) * per;
+    __shared__ float shares[SEVERAL ? NORM_THREADS * norm_each(VB) / 2 : 1];
+    const uint32_t lanes = 1u << a.lane_log, lane = threadIdx.x & (lanes - 1), per = blockDim.x >> a.lane_log, sub = threadIdx.x >> a.lane_log;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * per;
     const W *weight = static_cast<const W *>(a.weight);
-    float *share = a.partial + me * a.dim;
+    float *share = a.partial + blockIdx.x * a.dim;
     wait_for_previous();
     let_next_start();
     float sum[NV][V::N];
@@ -240,58 +255,69 @@ __global__ void __launch_bounds__(NORM_MOST) k_norm_grad(const NormGradArgs a)
     uint32_t turn = 0;
     // (a block's rows of threads make as many turns as its first one, whose tokens are the lowest: they meet at barriers)
     for (uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * per; t0 < a.tokens; t0 += step, turn++) {
-        const uint64_t t = t0 + (threadIdx.x >> a.lane_log);
+        const uint64_t t = t0 + sub;
         const bool on = t < a.tokens;
         const R *s = reinterpret_cast<const R *>(static_cast<const T *>(a.s) + (on ? t : 0) * a.s_stride);
         const R *dy = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + (on ? t : 0) * a.dim);
+        const R *ds = reinterpret_cast<const R *>(static_cast<const T *>(a.ds) + (on ? t : 0) * a.dim);
+        R *dx = reinterpret_cast<R *>(static_cast<T *>(a.dx) + t * a.dim);
         const float rstd = on ? a.rstd[t] : 0;
-        V n[NV], g[NV];
-        float along = 0;
-        auto load = [&](uint32_t v, V &p, V &q) { p.raw = s[v], q.raw = dy[v]; };
-        auto add = [&](uint32_t v, const V &p, const V &q) {
-            float w[V::N];
-            load_weights<W, V::N>(weight + v * V::N, w);
-#pragma unroll
-            for (int e = 0; e < V::N; e++) along += widen(q.e[e]) * w[e] * (widen(p.e[e]) * rstd);
+        V n[NV], g[NV], d[NV];
+        float along = 0;                                         // the sum of dy w s
+        auto load = [&](uint32_t v, V &p, V &q, V &r) {
+            p.raw = s[v], q.raw = dy[v];
+            if (a.ds) r.raw = ds[v];
         };
-        auto finish = [&](uint32_t v, const V &p, const V &q, float mean, float *sums) {
-            float w[V::N];
-            V d;
+        auto add = [&](uint32_t v, const V &p, const V &q) {
+            float w[V::N], x[V::N], y[V::N];
             load_weights<W, V::N>(weight + v * V::N, w);
-            d.raw = {};
-            if (a.ds) d.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.ds) + t * a.dim)[v];
+            widen_all(p, x), widen_all(q, y);
+#pragma unroll
+            for (int e = 0; e < V::N; e++) along += y[e] * w[e] * x[e];
+        };
+        auto finish = [&](uint32_t v, const V &p, const V &q, V r, float toward, float *sums) {
+            float w[V::N], x[V::N], y[V::N], u[V::N];
+            load_weights<W, V::N>(weight + v * V::N, w);
+            widen_all(p, x), widen_all(q, y);
 #pragma unroll
             for (int e = 0; e < V::N; e++) {
-                const float ne = widen(p.e[e]) * rstd, ge = widen(q.e[e]);
-                sums[e] += ge * ne;
-                const float u = rstd * (ge * w[e] - ne * mean);
-                d.e[e] = narrow<T>(a.ds ? u + widen(d.e[e]) : u);
+                y[e] *= rstd;
+                sums[e] += y[e] * x[e];
+                u[e] = y[e] * w[e] - x[e] * toward;
             }
-            if (a.dx) reinterpret_cast<R *>(static_cast<T *>(a.dx) + t * a.dim)[v] = d.raw;
+            if (!a.dx) return;
+            if (a.ds) {
+                widen_all(r, w);
+#pragma unroll
+                for (int e = 0; e < V::N; e++) u[e] += w[e];
+            }
+            narrow_all<V::N>(u, r.e);
+            dx[v] = r.raw;
         };
         if constexpr (LONG) {
             if (on)
                 for (uint32_t v = lane; v < a.vectors; v += lanes) {
-                    load(v, n[0], g[0]);
+                    load(v, n[0], g[0], d[0]);
                     add(v, n[0], g[0]);
                 }
         } else {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (on && lane + i * lanes < a.vectors) load(lane + i * lanes, n[i], g[i]);
+                if (on && lane + i * lanes < a.vectors) load(lane + i * lanes, n[i], g[i], d[i]);
 #pragma unroll
             for (int i = 0; i < NV; i++)
                 if (on && lane + i * lanes < a.vectors) add(lane + i * lanes, n[i], g[i]);
         }
-        const float mean = row_sum(along, a.lane_log, room[turn & 1]) / static_cast<float>(a.dim);
+        // rstd n mean(dy w n) = s rstd^3 mean(dy w s)
+        const float toward = row_sum(along, a.lane_log, room[turn & 1]) / static_cast<float>(a.dim) * rstd * rstd * rstd;
         if (!on) continue;
         if constexpr (LONG) {
             for (uint32_t v = lane; v < a.vectors; v += lanes) {
                 float *mine = share + static_cast<uint64_t>(v) * V::N;
-                load(v, n[0], g[0]);
+                load(v, n[0], g[0], d[0]);
 #pragma unroll
                 for (int e = 0; e < V::N; e++) sum[0][e] = turn && a.partial ? mine[e] : 0;
-                finish(v, n[0], g[0], mean, sum[0]);
+                finish(v, n[0], g[0], d[0], toward, sum[0]);
 #pragma unroll
                 for (int e = 0; e < V::N; e++)
                     if (a.partial) mine[e] = sum[0][e];
@@ -299,19 +325,30 @@ __global__ void __launch_bounds__(NORM_MOST) k_norm_grad(const NormGradArgs a)
         } else {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (lane + i * lanes < a.vectors) finish(lane + i * lanes, n[i], g[i], mean, sum[i]);
+                if (lane + i * lanes < a.vectors) finish(lane + i * lanes, n[i], g[i], d[i], toward, sum[i]);
         }
     }
     if (LONG || !a.partial) return;
+    auto each = [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-        if (lane + i * lanes < a.vectors)
+        for (int i = 0; i < NV; i++)
+            if (lane + i * lanes < a.vectors)
 #pragma unroll
-            for (int e = 0; e < V::N; e++) share[(lane + i * lanes) * V::N + e] = sum[i][e];
+                for (int e = 0; e < V::N; e++) f((lane + i * lanes) * V::N + e, sum[i][e]);
+    };
+    if constexpr (SEVERAL) {                                     // (of at most half of the columns that NORM_THREADS have)
+        for (uint32_t k = 0; k + 1 < per; k++) {
+            if (sub == k) each([&](uint32_t c, float v) { shares[c] = k ? shares[c] + v : v; });
+            __syncthreads();
+        }
+        if (sub + 1 != per) return;
+        if (per > 1) each([&](uint32_t c, float &v) { v += shares[c]; });
+    }
+    each([&](uint32_t c, float v) { share[c] = v; });
 }
 
 // out[d] = the sum of `rows` shares.  A block has 32 columns; its warps take the shares in turn, and their sums meet in their order.
-constexpr uint32_t JOIN_WARPS = 16;
+constexpr uint32_t JOIN_WARPS = 16, JOIN_AHEAD = 8;
 template <class W>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) k_join(const float *partial, uint64_t rows, uint64_t dim, W *out)
 {
@@ -322,7 +359,13 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_join(const float *partial, 
     let_next_start();
     float sum = 0;
     if (d < dim)
-        for (uint64_t r = warp; r < rows; r += JOIN_WARPS) sum += partial[r * dim + d];
+        for (uint64_t r = warp; r < rows; r += JOIN_WARPS * JOIN_AHEAD) {
+            float v[JOIN_AHEAD];
+#pragma unroll
+            for (uint32_t i = 0; i < JOIN_AHEAD; i++) v[i] = r + i * JOIN_WARPS < rows ? partial[(r + i * JOIN_WARPS) * dim + d] : 0;
+#pragma unroll
+            for (uint32_t i = 0; i < JOIN_AHEAD; i++) sum += v[i];
+        }
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp || d >= dim) return;

@@ -61,6 +61,20 @@ struct TilePlace {
     uint32_t k, k_rows;                          // WEIGHT_GRAD: the group's rows
 };
 
+template <class O, int N>
+__device__ __forceinline__ void widen_some(const O *from, float *to)
+{
+    if constexpr (N * sizeof(O) == 16) {
+        Vec<O, 16> v;
+#pragma unroll
+        for (int e = 0; e < N; e++) v.e[e] = from[e];
+        widen_all(v, to);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) to[e] = widen(from[e]);
+    }
+}
+
 // N neighbours of f of each of J columns, from sums to result: z = sums + bias, y = act(z) times + residual.  `on`: whether there is such a column.
 template <class O, bool SCALED, int J, int N>
 __device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at, const bool *on, float (*v)[N], const O *bias, const float *a_scale, const float *b_scale,
@@ -73,10 +87,12 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at,
             for (int e = 0; e < N; e++) v[j][e] *= a_scale[e] * b_scale[j];
     }
     if (a.bias) {
+        float w[N];
+        widen_some<O, N>(bias, w);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int e = 0; e < N; e++) v[j][e] += widen(bias[e]);
+            for (int e = 0; e < N; e++) v[j][e] += w[e];
     }
     if (a.z) {
 #pragma unroll
@@ -93,15 +109,21 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at,
     act_all<J * N>(a.activation, v[0]);
     if (a.times) {
 #pragma unroll
-        for (int j = 0; j < J; j++)
+        for (int j = 0; j < J; j++) {
+            float w[N];
+            widen_some<O, N>(times[j], w);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[j][e] *= widen(times[j][e]);
+            for (int e = 0; e < N; e++) v[j][e] *= w[e];
+        }
     }
     if (a.residual) {
 #pragma unroll
-        for (int j = 0; j < J; j++)
+        for (int j = 0; j < J; j++) {
+            float w[N];
+            widen_some<O, N>(residual[j], w);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[j][e] += widen(residual[j][e]);
+            for (int e = 0; e < N; e++) v[j][e] += w[e];
+        }
     }
 }
 
@@ -413,8 +435,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
 #pragma unroll
                     for (uint32_t j = 0; j < 2; j++) {
                         Vec<O, 16> y;
-#pragma unroll
-                        for (uint32_t e = 0; e < 8; e++) y.e[e] = narrow<O>(u[j][e]);
+                        narrow_all<8>(u[j], y.e);
                         if (on[j]) *reinterpret_cast<uint4 *>(out + at[j]) = y.raw;
                     }
                 } else {

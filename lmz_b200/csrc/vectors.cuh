@@ -21,6 +21,24 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
+// N of them, two to an instruction where there are two.
+template <int N, class T>
+__device__ __forceinline__ void narrow_all(const float *v, T *to)
+{
+    if constexpr (N % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            union { uint32_t raw; T e[2]; } both;
+            if constexpr (__is_same(T, __half)) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(both.raw) : "f"(v[e + 1]), "f"(v[e]));
+            else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(both.raw) : "f"(v[e + 1]), "f"(v[e]));
+            to[e] = both.e[0], to[e + 1] = both.e[1];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) to[e] = narrow<T>(v[e]);
+    }
+}
+
 // VB bytes of T as a memory instruction moves them.
 template <class T, int VB>
 struct Vec {
@@ -31,5 +49,20 @@ struct Vec {
     };
     __device__ __forceinline__ Vec() {}
 };
+
+// A vector's elements in 32 bits: of two BF16 in a word each is one instruction away.
+template <class T, int VB>
+__device__ __forceinline__ void widen_all(const Vec<T, VB> &v, float *to)
+{
+    if constexpr (__is_same(T, __nv_bfloat16) && VB >= 4) {
+        union { typename Raw<VB>::type raw; uint32_t word[VB / 4]; } w;
+        w.raw = v.raw;
+#pragma unroll
+        for (int e = 0; e < VB / 4; e++) to[2 * e] = __uint_as_float(w.word[e] << 16), to[2 * e + 1] = __uint_as_float(w.word[e] & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int e = 0; e < Vec<T, VB>::N; e++) to[e] = widen(v.e[e]);
+    }
+}
 
 }  // namespace lmz
