@@ -178,6 +178,27 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         cluster_barrier();
     }
     if (warp == G_TMA_WARP + 1) tmem_alloc<PAIR>(&s.tmem, a.tmem_columns);
+    if (warp == G_TMA_WARP) {
+        if (elected()) map_prefetch(&a.a), map_prefetch(&a.b);
+        __syncwarp();
+        // The weight's first tiles come to L2 while the kernel before still runs (whose tiles is known without it where there are no groups).
+        if (!BY_K && !a.groups.offsets) {
+            const uint32_t ct = static_cast<uint32_t>((a.cols + a.nt - 1) / a.nt), wide = ct < 8 ? ct : 8;
+            const uint32_t f = ((first < a.feat_tiles * wide ? first / wide : first % (8 * a.feat_tiles) / wide) * CTAS + side) * G_FEATS;
+            const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split), k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
+            for (uint32_t k = k0; k < k1 && k - k0 < a.stages; k++) {
+                if (elected()) {
+                    if constexpr (P == FORWARD) {
+                        tma_prefetch_3d(&a.a, k * STEP, f, 0);
+                    } else if constexpr (P == ROWS_GRAD) {
+                        tma_prefetch_3d(&a.a, f, k * STEP, 0);
+                        tma_prefetch_3d(&a.a, f + 64, k * STEP, 0);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
     wait_for_previous();
     group_starts(a.groups, s.starts);
     if (warp == 0 && !BY_K) {
@@ -269,6 +290,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             }
             if (!ok) break;
         }
+        let_next_start();                                        // (all tensor memory that this kernel wants is its own by now)
         // Nothing may still be on its way into this block's memory (a pair's barriers are the first CTA's, and stand for both; those of tails are each
         // CTA's own).
         if (*over)
