@@ -142,6 +142,24 @@ def rows_of(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def address(t):
+    return None if t is None else t.data_ptr()
+
+
+def trained(*tensors) -> bool:
+    """Whether one of the tensors (None for one that is not given) wants a gradient."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def empty_like(t, dtype=None):
+    """A contiguous tensor of the same shape."""
+    import torch
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def packed(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -177,16 +195,22 @@ def stream_of(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_entries = {}
+
+
 def launch(index: int, name: str, *args) -> None:
     """Call an entry point on the device's current stream (its last argument)."""
     import torch
-    fn = getattr(gpu.library(), name)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, stream_of(index))
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(gpu.library(), name)
+    c = torch._C
+    if c._cuda_getDevice() == index:
+        rc = fn(*args, c._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, stream_of(index))
-    if rc == gpu.OK:
+            rc = fn(*args, c._cuda_getCurrentRawStream(index))
+    if rc == 0:
         return
     if rc == gpu.EUNSUPPORTED:
         raise ValueError(gpu.last_error())

@@ -60,6 +60,6 @@ def project(x, weight, offsets, bias=None, activation=None, times=None):
         raise ValueError(f"bias must be {[experts, out]}, not {list(bias.shape)}")
     if times is not None and times.shape != (x.shape[0], out):
         raise ValueError(f"times must be {[x.shape[0], out]}, not {list(times.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, times)):
+    if torch.is_grad_enabled() and _ops.trained(x, weight, bias, times):
         return linear._function().apply(x, weight, bias, times, None, offsets, kind)
     return linear._forward(index, code, code, kind, x, weight, bias, times, None, offsets, None, None, False)[0]

@@ -28,7 +28,7 @@ def project(x, weight, bias=None, activation=None, times=None, residual=None):
             raise TypeError(f"{name} is {t.dtype}, but x {x.dtype}")
     kind = _activation(activation)
     _check_shapes(x, weight, bias, times, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, times, residual)):
+    if torch.is_grad_enabled() and _ops.trained(x, weight, bias, times, residual):
         return _function().apply(x, weight, bias, times, residual, None, kind)
     return _forward(index, code, code, kind, x, weight, bias, times, residual, None, None, None, False)[0]
 
@@ -55,7 +55,7 @@ def project_8bit(x, x_scale, weight, weight_scale, bias=None, activation=None, t
     for name, t, shape in (("x_scale", x_scale, x.shape[:-1]), ("weight_scale", weight_scale, weight.shape[:1])):
         if t.dtype is not torch.float32 or t.shape != shape:
             raise ValueError(f"{name} must be float32 {list(shape)}, not {t.dtype} {list(t.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, x_scale, weight, weight_scale, bias, times, residual)):
+    if torch.is_grad_enabled() and _ops.trained(x, x_scale, weight, weight_scale, bias, times, residual):
         raise ValueError("project_8bit has no gradient: call it under torch.no_grad()")
     return _forward(index, _ops.E4M3, _ops.BF16 if dtype is torch.bfloat16 else _ops.F16, kind, x, weight, bias, times, residual, None, x_scale, weight_scale, False)[0]
 
@@ -82,29 +82,23 @@ def _check_shapes(x, weight, bias, times, residual):
             raise ValueError(f"{name} must be {[*x.shape[:-1], out]}, not {list(t.shape)}")
 
 
-def _call(code, rcode, kind, x, weight, bias, times, residual, offsets):
-    """(`lmz_product`, what it points to) for x as [rows, in]."""
-    at = lambda t: None if t is None else t.data_ptr()     # noqa: E731
-    x, times, residual, bias, offsets = _ops.rows_of(x), _ops.rows_of(times), _ops.rows_of(residual), _ops.packed(bias), _ops.packed(offsets)
-    p = _ops.Product(x.data_ptr(), weight.data_ptr(), at(bias), at(times), at(residual), at(offsets))
-    p.rows, p.in_ = x.shape
-    p.out, p.x_stride, p.weight_stride = weight.shape[-2], x.stride(0), weight.stride(-2)
-    p.experts, p.weight_plane = (1, 0) if weight.dim() == 2 else (weight.shape[0], weight.stride(0))
-    if times is not None:
-        p.times_stride = times.stride(0)
-    if residual is not None:
-        p.residual_stride = residual.stride(0)
-    p.dtype, p.result_dtype, p.activation = code, rcode, kind
-    if offsets is not None:
-        p.offset_bytes = offsets.element_size()
-    return p, (x, times, residual, bias, offsets)
+def _call(code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale=None, weight_scale=None, y=None, z=None):
+    """(`lmz_product`, copies that live as long as it) for x as [rows, in]."""
+    at, rows_of = _ops.address, _ops.rows_of
+    x, times, residual, bias, offsets = rows_of(x), rows_of(times), rows_of(residual), _ops.packed(bias), _ops.packed(offsets)
+    x_scale, weight_scale = _ops.packed(x_scale), _ops.packed(weight_scale)
+    (rows, inp), (experts, plane) = x.shape, (1, 0) if weight.dim() == 2 else (weight.shape[0], weight.stride(0))
+    p = _ops.Product(x.data_ptr(), weight.data_ptr(), at(bias), at(times), at(residual), at(offsets), at(x_scale), at(weight_scale), at(y), at(z), None, None, None, None,
+                     None, None, rows, inp, weight.shape[-2], x.stride(0), weight.stride(-2), plane, 0 if times is None else times.stride(0),
+                     0 if residual is None else residual.stride(0), experts, code, rcode, kind, 0 if offsets is None else offsets.element_size())
+    return p, (x, times, residual, bias, offsets, x_scale, weight_scale)
 
 
 def _work(p, grad: int, like):
-    import torch
     size = gpu.library().lmz_gpu_product_work_bytes(p, grad)
     if not size:
         return None
+    import torch
     work = like.new_empty(size, dtype=torch.uint8)
     p.work = work.data_ptr()
     return work
@@ -113,16 +107,10 @@ def _work(p, grad: int, like):
 def _forward(index, code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, keep):
     """(y, what the gradients need of the sums if `keep`)."""
     import torch
-    dtype = torch.bfloat16 if rcode == _ops.BF16 else torch.float16
-    y, z = x.new_empty((*x.shape[:-1], weight.shape[-2]), dtype=dtype), None
-    p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets)
-    x_scale, weight_scale = _ops.packed(x_scale), _ops.packed(weight_scale)
-    p.y = y.data_ptr()
-    if x_scale is not None:
-        p.x_scale, p.weight_scale = x_scale.data_ptr(), weight_scale.data_ptr()
-    if keep and (kind or times is not None):
-        z = y.new_empty(y.shape, dtype=torch.float32)
-        p.z = z.data_ptr()
+    like = times if times is not None else residual        # (of the result's shape and type)
+    y = _ops.empty_like(like) if like is not None else x.new_empty((*x.shape[:-1], weight.shape[-2]), dtype=torch.bfloat16 if rcode == _ops.BF16 else torch.float16)
+    z = _ops.empty_like(y, torch.float32) if keep and (kind or times is not None) else None
+    p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, y, z)
     held = held, _work(p, 0, x)                            # (copies and workspace live until the launch)
     _ops.launch(index, "lmz_gpu_product_dev", p)
     return y, z
@@ -132,13 +120,11 @@ def _backward(kind, dy, x, weight, bias, times, offsets, z, wanted):
     """The gradients of x, weight, bias and times, where `wanted`."""
     _ops.no_tangents("dy", dy)
     code = _ops.type_code(x, "x", half_only=True)
-    grads = [t.new_empty(t.shape) if w else None for t, w in zip((x, weight, bias, times), wanted)]
-    dy = _ops.packed(dy)
-    p, held = _call(code, code, kind, x, weight, bias, times, None, offsets)
+    grads = [_ops.empty_like(t) if w else None for t, w in zip((x, weight, bias, times), wanted)]
+    dy, at = _ops.packed(dy), _ops.address
+    p, held = _call(code, code, kind, x, weight, bias, times, None, offsets, z=z)
     p.dy = dy.data_ptr()
-    if z is not None:
-        p.z = z.data_ptr()
-    p.dx, p.dweight, p.dbias, p.dtimes = (None if t is None else t.data_ptr() for t in grads)
+    p.dx, p.dweight, p.dbias, p.dtimes = at(grads[0]), at(grads[1]), at(grads[2]), at(grads[3])
     held = held, _work(p, 1, x)
     _ops.launch(x.get_device(), "lmz_gpu_product_grad_dev", p)
     return grads

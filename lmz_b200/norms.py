@@ -52,7 +52,7 @@ def _checked(x, weight, residual, eps):
         raise TypeError(f"weight must be {x.dtype}, as x is, or float32, not {weight.dtype}")
     if x.dim() < 1 or not x.shape[-1] or weight.shape != x.shape[-1:]:
         raise ValueError(f"x must be [..., dim] and weight [dim], not {list(x.shape)} and {list(weight.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype is not x.dtype):
+    if residual is not None and (residual.dtype is not x.dtype or residual.shape != x.shape):
         raise ValueError(f"residual must be like x, {x.dtype} {list(x.shape)}, not {residual.dtype} {list(residual.shape)}")
     eps = _ops.finite(eps, "eps")
     if eps < 0:
@@ -62,44 +62,34 @@ def _checked(x, weight, residual, eps):
 
 def _no_gradient(name, *tensors):
     import torch
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and _ops.trained(*tensors):
         raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
-def _call(code, wcode, x, weight, residual, eps):
+def _call(code, wcode, x, weight, residual, eps, y=None, q=None, scale=None, stream=None, rstd=None):
     tokens, dim = x.shape
-    p = _ops.Norm(x.data_ptr(), None if residual is None else residual.data_ptr(), None if weight is None else weight.data_ptr())
-    p.tokens, p.dim, p.x_stride, p.residual_stride = tokens, dim, x.stride(0), 0 if residual is None else residual.stride(0)
-    p.dtype, p.weight_dtype, p.eps = code, wcode, eps
-    return p
+    at = _ops.address
+    return _ops.Norm(x.data_ptr(), at(residual), at(weight), at(y), at(q), at(scale), at(stream), at(rstd), None, None, None, None, None, tokens, dim, x.stride(0),
+                     0 if residual is None else residual.stride(0), code, wcode, eps)
 
 
 def _forward(index, code, wcode, x, weight, residual, eps, keep):
     """(y, s, rstd): s is None without a residual, rstd unless `keep`."""
-    import torch
-    y, stream, rstd = x.new_empty(x.shape), None if residual is None else x.new_empty(x.shape), None
-    flat, weight, residual = _ops.rows_of(x), _ops.packed(weight), _ops.rows_of(residual)
-    p = _call(code, wcode, flat, weight, residual, eps)
-    p.y = y.data_ptr()
-    if stream is not None:
-        p.stream = stream.data_ptr()
+    y, stream, rstd = _ops.empty_like(x), None if residual is None else _ops.empty_like(x), None
+    x, weight, residual = _ops.rows_of(x), _ops.packed(weight), _ops.rows_of(residual)
     if keep:
-        rstd = flat.new_empty(flat.shape[0], dtype=torch.float32)
-        p.rstd = rstd.data_ptr()
-    _ops.launch(index, "lmz_gpu_norm_dev", p)
+        import torch
+        rstd = x.new_empty(x.shape[0], dtype=torch.float32)
+    _ops.launch(index, "lmz_gpu_norm_dev", _call(code, wcode, x, weight, residual, eps, y, None, None, stream, rstd))
     return y, stream, rstd
 
 
 def _eight_bits(index, code, wcode, x, weight, residual, eps):
     import torch
-    q, scale = x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
-    stream = None if residual is None else x.new_empty(x.shape)
+    q, stream = _ops.empty_like(x, torch.float8_e4m3fn), None if residual is None else _ops.empty_like(x)
+    scale = x.new_empty(x.shape[0] if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
     x, weight, residual = _ops.rows_of(x), _ops.packed(weight), _ops.rows_of(residual)
-    p = _call(code, wcode, x, weight, residual, eps)
-    p.q, p.scale = q.data_ptr(), scale.data_ptr()
-    if stream is not None:
-        p.stream = stream.data_ptr()
-    _ops.launch(index, "lmz_gpu_norm_dev", p)
+    _ops.launch(index, "lmz_gpu_norm_dev", _call(code, wcode, x, weight, residual, eps, None, q, scale, stream))
     return q, scale, stream
 
 
@@ -109,11 +99,10 @@ def _backward(s, weight, rstd, dy, ds, eps, want_dx, want_dw):
     _ops.no_tangents("dy ds", dy, ds)
     if dy is None:                                         # (only the stream was used)
         return (ds if want_dx else None), (torch.zeros_like(weight) if want_dw else None)
-    dx, dw = s.new_empty(s.shape) if want_dx else None, weight.new_empty(weight.shape) if want_dw else None
+    dx, dw = _ops.empty_like(s) if want_dx else None, _ops.empty_like(weight) if want_dw else None
     flat, weight, dy, ds = _ops.rows_of(s), _ops.packed(weight), _ops.packed(dy), _ops.packed(ds)
-    p = _call(_ops.type_code(s, "x"), _ops.type_code(weight, "weight"), flat, weight, None, eps)
-    p.rstd, p.dy = rstd.data_ptr(), dy.data_ptr()
-    p.dstream, p.dx, p.dweight = (None if t is None else t.data_ptr() for t in (ds, dx, dw))
+    p = _call(_ops.type_code(s, "x"), _ops.type_code(weight, "weight"), flat, weight, None, eps, rstd=rstd)
+    p.dy, p.dstream, p.dx, p.dweight = dy.data_ptr(), _ops.address(ds), _ops.address(dx), _ops.address(dw)
     if want_dw:
         work = s.new_empty(gpu.library().lmz_gpu_norm_grad_work_bytes(p), dtype=torch.uint8)
         p.work = work.data_ptr()
