@@ -319,6 +319,7 @@ static int product_as(const lmz_product *p, cudaStream_t cs)
     a.times_stride = p->times_stride, a.residual_stride = p->residual_stride, a.activation = p->activation;
     a.vectors = vector_bytes(p->out * 2, {address(p->y), address(p->z), address(p->bias), address(p->times), p->times ? p->times_stride * 2 : 0, address(p->residual),
                                           p->residual ? p->residual_stride * 2 : 0}) == 16;
+    a.plain = !p->z && !p->times && !p->residual && address(p->x_scale) % 16 == 0;
     return launch_product<T, O, FORWARD>(a, in.w, in.w_stride, in.w_plane, in.x, in.x_stride, p->in, cs);
 }
 
@@ -362,7 +363,7 @@ static int product_grad_as(const lmz_product *p, cudaStream_t cs)
     auto args = [&](void *out, uint64_t cols) {
         ProductArgs a{};
         a.out = out, a.groups = groups_of(p), a.feats = p->in, a.cols = cols;
-        a.vectors = vector_bytes(p->in * 2, {address(out)}) == 16;
+        a.vectors = vector_bytes(p->in * 2, {address(out)}) == 16, a.plain = true;
         return a;
     };
     if (p->dx) {

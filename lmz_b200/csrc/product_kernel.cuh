@@ -44,6 +44,7 @@ struct ProductArgs {
     uint32_t feat_tiles, col_tiles;              // of G_FEATS (a pair: twice that) and, where k has the groups, of nt
     uint32_t stages, stage_bytes, tmem_columns;
     bool vectors;                                // rows of all tensors that the epilogue has to do with start on 16 bytes
+    bool plain;                                  // and they are the result's alone: what else there is goes by feature or by column
 };
 
 // Tiles of a stage: A's 128 f, and the columns' (of a pair's each CTA has half); of columns side by side in blocks of 64.
@@ -143,7 +144,9 @@ __device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group,
 //
 // Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; sixteen warps take the
 // sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.  They turn 32 features and 16 columns round
-// in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.
+// in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.  Where nothing of the rows' own
+// stands in it the results are turned round and not the sums, in half the bytes: the products want shared memory's whole bandwidth, and every byte of
+// the epilogue's is time of theirs (8192 rows 16384x1024x4096 100 to 95 us).
 // Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile ends with its group,
 // to a multiple of 16 columns; what is behind its group's last column is another group's rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
 // last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.  Only such
@@ -401,7 +404,14 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                     }
                 }
             };
-            if (vectors) {
+            float f_bias = 0, f_scale = 0;                       // of the lane's own feature
+            if (vectors && a.plain) {
+                const uint64_t own = features(p) + quarter * 32 + lane;
+                if (own < a.feats) {
+                    if (a.bias) f_bias = widen(static_cast<const O *>(a.bias)[p.group * a.feats + own]);
+                    if constexpr (SCALED) f_scale = a.a_scale[own];
+                }
+            } else if (vectors) {
                 bias.raw = make_uint4(0, 0, 0, 0);
                 if (a.bias) bias.raw = *reinterpret_cast<const uint4 *>(static_cast<const O *>(a.bias) + p.group * a.feats + (f < a.feats ? f : 0));
                 if constexpr (SCALED) {
@@ -429,7 +439,43 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 __syncwarp();
                 tmem_ask16(sums + g * G_GROUP, v);
                 tmem_wait16(v);
-                if (vectors) {
+                if (vectors && a.plain) {
+                    float u[G_GROUP];
+#pragma unroll
+                    for (uint32_t q = 0; q < G_GROUP; q++) u[q] = !BY_K || any ? __uint_as_float(v[q]) : 0.0f;
+                    if constexpr (SCALED) {
+                        const uint32_t c = p.c + g * G_GROUP;
+#pragma unroll
+                        for (uint32_t q = 0; q < G_GROUP; q += 4) {
+                            float4 s4;
+                            if (c + q + 3 < a.cols) s4 = *reinterpret_cast<const float4 *>(a.b_scale + c + q);
+                            else s4 = make_float4(c + q < a.cols ? a.b_scale[c + q] : 0, c + q + 1 < a.cols ? a.b_scale[c + q + 1] : 0, c + q + 2 < a.cols ? a.b_scale[c + q + 2] : 0, 0);
+                            u[q] *= s4.x * f_scale, u[q + 1] *= s4.y * f_scale, u[q + 2] *= s4.z * f_scale, u[q + 3] *= s4.w * f_scale;
+                        }
+                    }
+                    if (a.bias) {
+#pragma unroll
+                        for (uint32_t q = 0; q < G_GROUP; q++) u[q] += f_bias;
+                    }
+                    act_all<G_GROUP>(a.activation, u);
+                    // two columns to a word on their way round
+                    uint32_t *words = reinterpret_cast<uint32_t *>(turn);
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; q++) words[q * G_PITCH + lane] = narrow_two<O>(u[2 * q], u[2 * q + 1]);
+                    __syncwarp();
+                    uint32_t w[8];
+                    const uint4 *from = reinterpret_cast<const uint4 *>(words + (lane >> 2) * G_PITCH + (lane & 3) * 8);
+                    *reinterpret_cast<uint4 *>(w) = from[0], *reinterpret_cast<uint4 *>(w + 4) = from[1];
+                    __syncwarp();
+                    const uint32_t c = p.c + g * G_GROUP + (lane >> 2) * 2;
+                    O *to = out + (plane + c) * a.feats + f;
+                    if (f < a.feats) {
+                        if (c < p.c_end)
+                            *reinterpret_cast<uint4 *>(to) = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[4], w[5], 0x5410), __byte_perm(w[6], w[7], 0x5410));
+                        if (c + 1 < p.c_end)
+                            *reinterpret_cast<uint4 *>(to + a.feats) = make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632), __byte_perm(w[4], w[5], 0x7632), __byte_perm(w[6], w[7], 0x7632));
+                    }
+                } else if (vectors) {
                     float u[2][8];
 #pragma unroll
                     for (uint32_t j = 0; j < 2; j++) {

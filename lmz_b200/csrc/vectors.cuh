@@ -21,6 +21,16 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
+// Two in a word, the first in its lower half.
+template <class T>
+__device__ __forceinline__ uint32_t narrow_two(float lo, float hi)
+{
+    uint32_t word;
+    if constexpr (__is_same(T, __half)) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(word) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(word) : "f"(hi), "f"(lo));
+    return word;
+}
+
 // N of them, two to an instruction where there are two.
 template <int N, class T>
 __device__ __forceinline__ void narrow_all(const float *v, T *to)
@@ -29,8 +39,7 @@ __device__ __forceinline__ void narrow_all(const float *v, T *to)
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
             union { uint32_t raw; T e[2]; } both;
-            if constexpr (__is_same(T, __half)) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(both.raw) : "f"(v[e + 1]), "f"(v[e]));
-            else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(both.raw) : "f"(v[e + 1]), "f"(v[e]));
+            both.raw = narrow_two<T>(v[e], v[e + 1]);
             to[e] = both.e[0], to[e + 1] = both.e[1];
         }
     } else {
