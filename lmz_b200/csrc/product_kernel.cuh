@@ -225,22 +225,24 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     const uint32_t tmem = s.tmem, groups = a.groups.count;
     const uint32_t col_tiles = BY_K ? a.col_tiles : s.tiles[groups], tiles = a.feat_tiles * col_tiles * (BY_K ? groups : 1);
 
-    // Eight column tiles side by side, features outside: what a wave reads of A and B stays in L2.
+    // Group by group, in a group eight column tiles side by side, features outside: what a wave reads of A and B stays in L2.
     auto place = [&](uint32_t tile) {
         TilePlace p;
-        uint32_t in_group = tile;
         p.group = 0;
-        if (BY_K) p.group = tile / (a.feat_tiles * col_tiles), in_group = tile - p.group * (a.feat_tiles * col_tiles);
+        uint32_t cols = col_tiles, before = 0;                   // column tiles of the group, and of those in front of it
+        if (BY_K) {
+            p.group = tile / (a.feat_tiles * col_tiles), before = p.group * col_tiles;
+        } else if (groups > 1) {
+            p.group = group_of(s.tiles, groups, tile / a.feat_tiles);
+            before = s.tiles[p.group], cols = s.tiles[p.group + 1] - before;
+        }
+        const uint32_t in_group = tile - before * a.feat_tiles;
         const uint32_t band = 8 * a.feat_tiles, b = in_group / band, in = in_group - b * band;
-        const uint32_t w = col_tiles - 8 * b < 8 ? col_tiles - 8 * b : 8;
+        const uint32_t w = cols - 8 * b < 8 ? cols - 8 * b : 8;
         const uint32_t ct = 8 * b + in % w;
         p.ft = in / w;
-        if (BY_K) {
-            p.c = ct * a.nt, p.c_end = static_cast<uint32_t>(a.cols), p.k = s.starts[p.group], p.k_rows = s.starts[p.group + 1] - p.k;
-        } else {
-            if (groups > 1) p.group = group_of(s.tiles, groups, ct);
-            p.c = s.starts[p.group] + (ct - s.tiles[p.group]) * a.nt, p.c_end = s.starts[p.group + 1], p.k = p.k_rows = 0;
-        }
+        if (BY_K) p.c = ct * a.nt, p.c_end = static_cast<uint32_t>(a.cols), p.k = s.starts[p.group], p.k_rows = s.starts[p.group + 1] - p.k;
+        else p.c = s.starts[p.group] + ct * a.nt, p.c_end = s.starts[p.group + 1], p.k = p.k_rows = 0;
         const uint32_t left = (p.c_end - p.c + 16 * CTAS - 1) / (16 * CTAS) * (16 * CTAS);
         p.n = left < a.nt ? left : a.nt;
         return p;
