@@ -63,7 +63,9 @@ __device__ __forceinline__ void act_and_slope(uint32_t kind, const float *z, flo
     case ACT_GELU_TANH:
         return each([](float z, float &y, float &slope) {
             const float t = tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z));
-            y = 0.5f * z * (1 + t), slope = 0.5f * (1 + t) + 0.5f * z * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * z * z);
+            y = 0.5f * z * (1 + t);
+            const float near = fminf(fmaxf(z, -16.0f), 16.0f);   // (beyond, 1 - t * t is zero, and the square may be infinite)
+            slope = 0.5f * (1 + t) + 0.5f * near * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * near * near);
         });
     default: return each([](float z, float &y, float &slope) { y = z, slope = 1; });
     }
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
                 widen_all(d[i], g);
 #pragma unroll
                 for (int e = 0; e < V::N; e++) y[e] *= g[e], u[e] *= g[e];
-                narrow_all<V::N>(y, dm.e);
+                narrow_all(y, dm);
                 if (a.times) {
                     widen_all(m[i], g);
 #pragma unroll
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
                 }
 #pragma unroll
                 for (int e = 0; e < V::N; e++) sum[e] += u[e];
-                narrow_all<V::N>(u, dz.e);
+                narrow_all(u, dz);
                 any = true;
             }
             if (a.dz) reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = dz.raw;

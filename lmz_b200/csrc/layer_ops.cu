@@ -72,9 +72,10 @@ API int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream)
 {
     int rc = check_norm(p);
     if (rc || p->tokens == 0) return rc;
+    if (!p->weight && !p->q) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm has a weight");
+    if (p->q ? p->y || !p->scale : !p->y) return fail_msg(LMZ_GPU_EUNSUPPORTED, "either y, or q and scale");
     rc = device_ready();
     if (rc) return rc;
-    if (!p->weight && !p->q) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm has a weight");
     const uint64_t e = element_bytes(p->dtype);
     return by_norm_types(p, {address(p->x), address(p->residual), address(p->y), address(p->stream), p->x_stride * e, p->residual ? p->residual_stride * e : 0, p->q ? address(p->q) * e : 0},
                          [&](auto type, auto weight_type, auto vec) {
@@ -116,6 +117,7 @@ API size_t lmz_gpu_norm_grad_work_bytes(const lmz_norm *p)
 API int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream)
 {
     int rc = check_norm(p);
+    if (!rc && p->tokens && (!p->weight || !p->rstd || !p->dy)) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm's gradients go by its weight, rstd and dy");
     if (rc) return rc;
     rc = device_ready();
     if (rc) return rc;
@@ -393,6 +395,8 @@ API int lmz_gpu_product_grad_dev(const lmz_product *p, void *cuda_stream)
 {
     int rc = check_product(p);
     if (!rc && p->dtype == LMZ_GPU_E4M3) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "products in 8 bits have no gradients");
+    if (!rc && p->rows && (!p->dy || ((p->activation != ACT_NONE || p->dtimes) && !p->z)))
+        rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a product's gradients go by dy, and z where there is an activation or `times`");
     if (rc) return rc;
     rc = device_ready();
     if (rc) return rc;

@@ -27,35 +27,34 @@ struct NormArgs {
     float eps;
 };
 
-// Sums and largest values over the 2^log threads that share a row; `room`: a word per warp of the block.  All threads of a block call it
-// together, and once per pass over rows with a room of its own.
-template <class F>
-__device__ __forceinline__ float row_join(float v, uint32_t log, float *room, F both)
+// A row's sum over the 2^log threads that share it; `room`: a word per warp of the block.  All threads of a block call it together.
+__device__ __forceinline__ float row_sum(float v, uint32_t log, float *room)
 {
-    for (uint32_t o = 1; o < 32 && o >> log == 0; o <<= 1) v = both(v, __shfl_xor_sync(~0u, v, o));
+    for (uint32_t o = 1; o < 32 && o >> log == 0; o <<= 1) v += __shfl_xor_sync(~0u, v, o);
     if (log <= 5) return v;
     const uint32_t warps = 1u << (log - 5), warp = threadIdx.x >> 5, first = warp & ~(warps - 1);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) room[warp] = v;
     __syncthreads();
     v = room[first + (threadIdx.x & (warps - 1))];
-    for (uint32_t o = 1; o < warps; o <<= 1) v = both(v, __shfl_xor_sync(~0u, v, o));
+    for (uint32_t o = 1; o < warps; o <<= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
-__device__ __forceinline__ float row_sum(float v, uint32_t log, float *room)
+
+// And its largest magnitude, by its bits: those of a NaN are above those of infinity, so that it stays.
+__device__ __forceinline__ float row_most(uint32_t v, uint32_t log, float *room)
 {
-    return row_join(v, log, room, [](float a, float b) { return a + b; });
-}
-// (A NaN stays.)
-__device__ __forceinline__ float larger(float a, float b)
-{
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
-}
-__device__ __forceinline__ float row_most(float v, uint32_t log, float *room)
-{
-    return row_join(v, log, room, larger);
+    if (log < 5) {
+        for (uint32_t o = 1; o >> log == 0; o <<= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
+        return __uint_as_float(v);
+    }
+    v = __reduce_max_sync(~0u, v);
+    if (log == 5) return __uint_as_float(v);
+    const uint32_t warps = 1u << (log - 5), warp = threadIdx.x >> 5, first = warp & ~(warps - 1);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) room[warp] = __uint_as_float(v);
+    __syncthreads();
+    return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(room[first + (threadIdx.x & (warps - 1))])));
 }
 
 template <class W, int N>
@@ -96,10 +95,15 @@ __device__ __forceinline__ void store_8bit(uint8_t *to, const float *v)
     if constexpr (N == 1) {
         *to = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
     } else {
-        union { uint16_t part[N / 2]; typename Raw<N>::type raw; } all;
+        auto two = [&](int e) -> uint32_t { return __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3); };
+        if constexpr (N == 2) {
+            *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(two(0));
+        } else {
+            union { uint32_t word[N / 4]; typename Raw<N>::type raw; } all;
 #pragma unroll
-        for (int e = 0; e < N; e += 2) all.part[e / 2] = __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3);
-        *reinterpret_cast<typename Raw<N>::type *>(to) = all.raw;
+            for (int e = 0; e < N; e += 4) all.word[e / 4] = two(e) | two(e + 2) << 16;
+            *reinterpret_cast<typename Raw<N>::type *>(to) = all.raw;
+        }
     }
 }
 
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
             widen_all(p, both), widen_all(q, other);
 #pragma unroll
             for (int e = 0; e < V::N; e++) both[e] += other[e];
-            narrow_all<V::N>(both, p.e);
+            narrow_all(both, p);
             if (write && a.stream) stream[v] = p.raw;
         }
         widen_all(p, to);
@@ -192,10 +196,10 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
             if (on && lane + i * lanes < a.vectors) normed(lane + i * lanes, s[i]);
     }
     if constexpr (BITS8) {
-        float most = 0;
+        uint32_t most = 0;
         each([&](uint32_t, const float *u) {
 #pragma unroll
-            for (int e = 0; e < V::N; e++) most = larger(most, fabsf(u[e]));
+            for (int e = 0; e < V::N; e++) most = max(most, __float_as_uint(u[e]) & 0x7FFFFFFF);
         });
         const float scale = scale_of_most(row_most(most, a.lane_log, room[1])), inverse = 1.0f / scale;
         if (on && lane == 0) a.scale[t] = scale;
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
     } else {
         each([&](uint32_t v, const float *u) {
             V p;
-            narrow_all<V::N>(u, p.e);
+            narrow_all(u, p);
             reinterpret_cast<R *>(static_cast<T *>(a.y) + t * a.dim)[v] = p.raw;
         });
     }
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
 #pragma unroll
                 for (int e = 0; e < V::N; e++) u[e] += w[e];
             }
-            narrow_all<V::N>(u, r.e);
+            narrow_all(u, r);
             dx[v] = r.raw;
         };
         if constexpr (LONG) {

@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
 #pragma unroll
                     for (uint32_t j = 0; j < 2; j++) {
                         Vec<O, 16> y;
-                        narrow_all<8>(u[j], y.e);
+                        narrow_all(u[j], y);
                         if (on[j]) *reinterpret_cast<uint4 *>(out + at[j]) = y.raw;
                     }
                 } else {

@@ -31,23 +31,6 @@ __device__ __forceinline__ uint32_t narrow_two(float lo, float hi)
     return word;
 }
 
-// N of them, two to an instruction where there are two.
-template <int N, class T>
-__device__ __forceinline__ void narrow_all(const float *v, T *to)
-{
-    if constexpr (N % 2 == 0 && sizeof(T) == 2) {
-#pragma unroll
-        for (int e = 0; e < N; e += 2) {
-            union { uint32_t raw; T e[2]; } both;
-            both.raw = narrow_two<T>(v[e], v[e + 1]);
-            to[e] = both.e[0], to[e + 1] = both.e[1];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; e++) to[e] = narrow<T>(v[e]);
-    }
-}
-
 // VB bytes of T as a memory instruction moves them.
 template <class T, int VB>
 struct Vec {
@@ -71,6 +54,21 @@ __device__ __forceinline__ void widen_all(const Vec<T, VB> &v, float *to)
     } else {
 #pragma unroll
         for (int e = 0; e < Vec<T, VB>::N; e++) to[e] = widen(v.e[e]);
+    }
+}
+
+// And back, each rounded once: two to an instruction where there are two to a word.
+template <class T, int VB>
+__device__ __forceinline__ void narrow_all(const float *from, Vec<T, VB> &v)
+{
+    if constexpr (sizeof(T) == 2 && VB >= 4) {
+        union { typename Raw<VB>::type raw; uint32_t word[VB / 4]; } w;
+#pragma unroll
+        for (int e = 0; e < VB / 4; e++) w.word[e] = narrow_two<T>(from[2 * e], from[2 * e + 1]);
+        v.raw = w.raw;
+    } else {
+#pragma unroll
+        for (int e = 0; e < Vec<T, VB>::N; e++) v.e[e] = narrow<T>(from[e]);
     }
 }
 

@@ -42,7 +42,7 @@ def test_numbers_of_the_header():
 
 def _norm(**kw):
     p = _ops.Norm()
-    p.weight, p.tokens, p.dim, p.x_stride, p.eps = 64, 4, 64, 64, 1e-6
+    p.weight, p.tokens, p.dim, p.x_stride, p.eps = 64, 4, 64, 64, 1e-6    # (nothing is read at these addresses)
     for k, v in kw.items():
         setattr(p, k, v)
     return p
@@ -53,6 +53,16 @@ def _norm(**kw):
 def test_norms_the_library_refuses(lib, bad):
     assert lib.lmz_gpu_norm_dev(_norm(**bad), None) == -2 and lib.lmz_gpu_last_error()
     assert lib.lmz_gpu_norm_grad_dev(_norm(**bad), None) == -2
+
+
+@pytest.mark.parametrize("without", [dict(), dict(y=64, q=64, scale=64), dict(q=64), dict(weight=None, y=64)])
+def test_norms_without_what_they_write_to(lib, without):
+    assert lib.lmz_gpu_norm_dev(_norm(**without), None) == -2 and lib.lmz_gpu_last_error()
+
+
+@pytest.mark.parametrize("without", [dict(), dict(rstd=64), dict(dy=64), dict(rstd=64, dy=64, weight=None)])
+def test_norms_gradients_without_what_they_go_by(lib, without):
+    assert lib.lmz_gpu_norm_grad_dev(_norm(dx=64, **without), None) == -2 and lib.lmz_gpu_last_error()
 
 
 def _product(**kw):
@@ -74,6 +84,11 @@ def test_products_the_library_refuses(lib, bad):
 
 def test_products_in_8_bits_have_no_gradients_in_the_library(lib):
     assert lib.lmz_gpu_product_grad_dev(_product(dtype=3, x_scale=64, weight_scale=64), None) == -2
+
+
+@pytest.mark.parametrize("without", [dict(dx=64), dict(dx=64, dy=64, activation=2), dict(dtimes=64, dy=64, times=64)])
+def test_products_gradients_without_what_they_go_by(lib, without):
+    assert lib.lmz_gpu_product_grad_dev(_product(**without), None) == -2 and lib.lmz_gpu_last_error()
 
 
 @pytest.mark.parametrize("id_bytes, n, count", [(2, 1, 4), (4, 1, 0), (4, 1, 1025), (8, 1 << 31, 4)])
