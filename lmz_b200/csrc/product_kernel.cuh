@@ -324,9 +324,12 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                     const uint32_t st = at.stage, off = st * a.stage_bytes >> 4;
                     ok = warp_wait(&s.full[st], at.turn & 1, over);
                     if (!ok) break;
+                    // (a group's last rows: as many sixteens as they take)
+                    const uint32_t parts = tails && (k + 1) * STEP_K > p.k_rows ? (p.k_rows - k * STEP_K + 15) / 16 : 4;
                     if (elected()) {
 #pragma unroll
                         for (uint32_t q = 0; q < 4; q++) {
+                            if (BY_K && q >= parts) break;
                             if constexpr (sizeof(T) == 1) mma32_e4m3<PAIR>(sums, a_lo + off + (q * a_step >> 4), b_lo + off + (q * b_step >> 4), desc, k != k0 || q);
                             else mma16<PAIR>(sums, a_lo + off + (q * a_step >> 4), b_lo + off + (q * b_step >> 4), desc, k != k0 || q);
                         }
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                     const uint32_t st = at.stage;
                     if (!warp_wait(&s.tail[st], turns >> st & 1, over)) break;
                     turns ^= 1u << st;
-                    const uint32_t each = (STEP_K - left) * 8;                   // 16-byte parts of a block's rows
+                    const uint32_t each = (-left & 15) * 8;                      // 16-byte parts of a block's rows up to the next sixteen
                     for (uint32_t i = lane; i < blocks * each; i += 32)
                         *reinterpret_cast<uint4 *>(local + st * a.stage_bytes + i / each * G_BLOCK + left * ROW_BYTES + i % each * 16) = make_uint4(0, 0, 0, 0);
                     publish_smem();
