@@ -154,6 +154,13 @@ def trained(*tensors) -> bool:
     return False
 
 
+def same_type(dtype, whose: str, **tensors) -> None:
+    """A TypeError for the first of the tensors (None for one that is not given) of another type."""
+    for name, t in tensors.items():
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"{name} is {t.dtype}, but {whose} {dtype}")
+
+
 def empty_like(t, dtype=None):
     """A contiguous tensor of the same shape."""
     import torch

@@ -42,9 +42,7 @@ def project(x, weight, offsets, bias=None, activation=None, times=None):
     import torch
     index = _ops.on_cuda("x weight offsets bias times", x, weight, offsets, bias, times)
     code = _ops.type_code(x, "x", half_only=True)
-    for name, t in (("weight", weight), ("bias", bias), ("times", times)):
-        if t is not None and t.dtype is not x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, but x {x.dtype}")
+    _ops.same_type(x.dtype, "x", weight=weight, bias=bias, times=times)
     _ops.whole_numbers(offsets, "offsets")
     kind = linear._activation(activation)
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:

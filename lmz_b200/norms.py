@@ -67,10 +67,22 @@ def _no_gradient(name, *tensors):
 
 
 def _call(code, wcode, x, weight, residual, eps, y=None, q=None, scale=None, stream=None, rstd=None):
-    tokens, dim = x.shape
-    at = _ops.address
-    return _ops.Norm(x.data_ptr(), at(residual), at(weight), at(y), at(q), at(scale), at(stream), at(rstd), None, None, None, None, None, tokens, dim, x.stride(0),
-                     0 if residual is None else residual.stride(0), code, wcode, eps)
+    p = _ops.Norm(x.data_ptr())                            # (set one by one, and only what there is: a third of the time of all at once)
+    p.tokens, p.dim = x.shape
+    p.x_stride, p.dtype, p.weight_dtype, p.eps = x.stride(0), code, wcode, eps
+    if weight is not None:
+        p.weight = weight.data_ptr()
+    if residual is not None:
+        p.residual, p.residual_stride = residual.data_ptr(), residual.stride(0)
+    if y is not None:
+        p.y = y.data_ptr()
+    if q is not None:
+        p.q, p.scale = q.data_ptr(), scale.data_ptr()
+    if stream is not None:
+        p.stream = stream.data_ptr()
+    if rstd is not None:
+        p.rstd = rstd.data_ptr()
+    return p
 
 
 def _forward(index, code, wcode, x, weight, residual, eps, keep):
