@@ -91,8 +91,15 @@ API int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream)
         const uint32_t per = shape.threads >> shape.lane_log;
         const dim3 grid(static_cast<unsigned>((p->tokens + per - 1) / per));
         const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
-        if (p->q) return launch("launch k_norm", shape.is_long ? k_norm<T, W, VB, true, true> : k_norm<T, W, VB, true, false>, grid, shape.threads, 0, cs, a);
-        return launch("launch k_norm", shape.is_long ? k_norm<T, W, VB, false, true> : k_norm<T, W, VB, false, false>, grid, shape.threads, 0, cs, a);
+        auto run = [&](auto bits8) {
+            constexpr bool B = decltype(bits8)::value;
+            if (shape.is_long) return launch("launch k_norm", k_norm<T, W, VB, B, true, false>, grid, shape.threads, 0, cs, a);
+            if constexpr (VB == 16)
+                if (p->dim == norm_each(VB) << shape.lane_log && p->tokens % per == 0)
+                    return launch("launch k_norm", k_norm<T, W, VB, B, false, true>, grid, shape.threads, 0, cs, a);
+            return launch("launch k_norm", k_norm<T, W, VB, B, false, false>, grid, shape.threads, 0, cs, a);
+        };
+        return p->q ? run(std::true_type{}) : run(std::false_type{});
     });
 }
 

@@ -110,8 +110,9 @@ __device__ __forceinline__ void store_8bit(uint8_t *to, const float *v)
 // A row's 2^lane_log threads take its vectors of VB bytes in turn.  What a thread has of a row stays in registers, so that a row is read once;
 // LONG: rows of more elements than NORM_MOST threads hold are read again for each pass, out of L2.  Sums in 32 bits.
 //
+// WHOLE: every thread has a whole share of a row, and nothing is asked for each vector.
 // Bound by HBM: x and the residual read, the stream and y written.
-template <class T, class W, int VB, bool BITS8, bool LONG>
+template <class T, class W, int VB, bool BITS8, bool LONG, bool WHOLE>
 __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
 {
     using V = Vec<T, VB>;
@@ -120,7 +121,8 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
     __shared__ float room[2][32];
     const uint32_t lanes = 1u << a.lane_log, lane = threadIdx.x & (lanes - 1);
     const uint64_t t = static_cast<uint64_t>(blockIdx.x) * (blockDim.x >> a.lane_log) + (threadIdx.x >> a.lane_log);
-    const bool on = t < a.tokens;
+    const bool on = WHOLE || t < a.tokens;
+    auto has = [&](int i) { return WHOLE || (on && lane + i * lanes < a.vectors); };
     const R *x = reinterpret_cast<const R *>(static_cast<const T *>(a.x) + (on ? t : 0) * a.x_stride);
     const R *res = reinterpret_cast<const R *>(static_cast<const T *>(a.residual) + (on ? t : 0) * a.residual_stride);
     R *stream = reinterpret_cast<R *>(static_cast<T *>(a.stream) + t * a.dim);
@@ -128,12 +130,8 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
     wait_for_previous();
     let_next_start();
 
-    auto load = [&](uint32_t v, float *to, bool write) {         // s
-        V p;
-        p.raw = x[v];
+    auto take = [&](uint32_t v, V p, V q, float *to, bool write) {               // s
         if (a.residual) {
-            V q;
-            q.raw = res[v];
             float both[V::N], other[V::N];
             widen_all(p, both), widen_all(q, other);
 #pragma unroll
@@ -142,6 +140,12 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
             if (write && a.stream) stream[v] = p.raw;
         }
         widen_all(p, to);
+    };
+    auto load = [&](uint32_t v, float *to, bool write) {
+        V p, q;
+        p.raw = x[v];
+        if (a.residual) q.raw = res[v];
+        take(v, p, q, to, write);
     };
     float s[NV][V::N];
     float squares = 0;
@@ -153,16 +157,22 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
                 for (int e = 0; e < V::N; e++) squares += s[0][e] * s[0][e];
             }
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-#pragma unroll
-            for (int e = 0; e < V::N; e++) s[i][e] = 0;
-            if (on && lane + i * lanes < a.vectors) load(lane + i * lanes, s[i], true);
-        }
+        V p[NV], q[NV];                                          // (all on their way before the first is waited for)
 #pragma unroll
         for (int i = 0; i < NV; i++)
+            if (has(i)) p[i].raw = x[lane + i * lanes];
+        if (a.residual) {
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+                if (has(i)) q[i].raw = res[lane + i * lanes];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (!has(i)) continue;
+            take(lane + i * lanes, p[i], q[i], s[i], true);
 #pragma unroll
             for (int e = 0; e < V::N; e++) squares += s[i][e] * s[i][e];
+        }
     }
     float rstd = 1;
     if (weight) {
@@ -187,13 +197,13 @@ __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
         } else {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (lane + i * lanes < a.vectors) f(lane + i * lanes, s[i]);
+                if (has(i)) f(lane + i * lanes, s[i]);
         }
     };
     if constexpr (!LONG) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
-            if (on && lane + i * lanes < a.vectors) normed(lane + i * lanes, s[i]);
+            if (has(i)) normed(lane + i * lanes, s[i]);
     }
     if constexpr (BITS8) {
         uint32_t most = 0;
