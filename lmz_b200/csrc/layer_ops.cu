@@ -146,9 +146,12 @@ API int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream)
         const NormShape shape(a.vectors, N, VB);
         a.lane_log = shape.lane_log;
         const uint64_t shares = norm_grad_blocks(p->tokens, shape.threads >> shape.lane_log);
-        int failed = launch("launch k_norm_grad", shape.is_long ? k_norm_grad<T, W, VB, true, NORM_MOST> : shape.threads > NORM_THREADS ? k_norm_grad<T, W, VB, false, NORM_MOST>
-                                                                                                         : k_norm_grad<T, W, VB, false, NORM_THREADS>,
-                            dim3(static_cast<unsigned>(shares)), shape.threads, 0, cs, a);
+        auto run = [&](auto kernel) { return launch("launch k_norm_grad", kernel, dim3(static_cast<unsigned>(shares)), shape.threads, 0, cs, a); };
+        int failed;
+        if (shape.is_long) failed = run(k_norm_grad<T, W, VB, true, NORM_MOST, false>);
+        else if (shape.threads > NORM_THREADS) failed = run(k_norm_grad<T, W, VB, false, NORM_MOST, false>);
+        else if (VB == 16 && p->dim == norm_each(VB) << shape.lane_log) failed = run(k_norm_grad<T, W, VB, false, NORM_THREADS, VB == 16>);
+        else failed = run(k_norm_grad<T, W, VB, false, NORM_THREADS, false>);
         if (!failed && p->dweight)
             failed = launch("launch k_join", k_join<W>, dim3(static_cast<unsigned>((p->dim + 31) / 32)), 32 * JOIN_WARPS, 0, cs, static_cast<const float *>(a.partial),
                             shares, p->dim, static_cast<W *>(p->dweight));

@@ -245,8 +245,8 @@ struct NormGradArgs {
 // The gradient of s, and each block's share of the weight's: a row of threads takes every (rows of threads)-th token, and a block's rows of
 // threads add up in their order, so that sums have one order.  LONG: the shares lie in global memory, where a thread finds its own columns again.
 //
-// Bound by HBM: dy, s and ds read, dx written.  MOST: threads of a block.
-template <class T, class W, int VB, bool LONG, uint32_t MOST>
+// Bound by HBM: dy, s and ds read, dx written.  MOST: threads of a block.  WHOLE: every thread has a whole share of a row.
+template <class T, class W, int VB, bool LONG, uint32_t MOST, bool WHOLE>
 __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const NormGradArgs a)
 {
     using V = Vec<T, VB>;
@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
     for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int e = 0; e < V::N; e++) sum[i][e] = 0;
+    auto has = [&](int i) { return WHOLE || lane + i * lanes < a.vectors; };
     uint32_t turn = 0;
     // (a block's rows of threads make as many turns as its first one, whose tokens are the lowest: they meet at barriers)
     for (uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * per; t0 < a.tokens; t0 += step, turn++) {
@@ -317,10 +318,10 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
         } else {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (on && lane + i * lanes < a.vectors) load(lane + i * lanes, n[i], g[i], d[i]);
+                if (on && has(i)) load(lane + i * lanes, n[i], g[i], d[i]);
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (on && lane + i * lanes < a.vectors) add(lane + i * lanes, n[i], g[i]);
+                if (on && has(i)) add(lane + i * lanes, n[i], g[i]);
         }
         // rstd n mean(dy w n) = s rstd^3 mean(dy w s)
         const float toward = row_sum(along, a.lane_log, room[turn & 1]) / static_cast<float>(a.dim) * rstd * rstd * rstd;
@@ -339,14 +340,14 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
         } else {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (lane + i * lanes < a.vectors) finish(lane + i * lanes, n[i], g[i], d[i], toward, sum[i]);
+                if (has(i)) finish(lane + i * lanes, n[i], g[i], d[i], toward, sum[i]);
         }
     }
     if (LONG || !a.partial) return;
     auto each = [&](auto f) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
-            if (lane + i * lanes < a.vectors)
+            if (has(i))
 #pragma unroll
                 for (int e = 0; e < V::N; e++) f((lane + i * lanes) * V::N + e, sum[i][e]);
     };
