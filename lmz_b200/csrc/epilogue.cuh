@@ -221,12 +221,13 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
     flush();
 }
 
-// A group's bias gradient: what the chunks that its rows lie in have for it, in their order.
+// A group's bias gradient: what the chunks that its rows lie in have for it; a block's warps take them in turn, and their sums meet in their order.
+constexpr uint32_t BJ_WARPS = 16, BJ_AHEAD = 8;
 template <class T>
-__global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups groups, uint64_t out, uint32_t chunk, T *dbias)
+__global__ void __launch_bounds__(32 * BJ_WARPS) k_bias_join(const float *partial, Groups groups, uint64_t out, uint32_t chunk, T *dbias)
 {
     __shared__ uint32_t starts[MAX_EXPERTS + 1];
-    __shared__ float sums[8][32];
+    __shared__ float sums[BJ_WARPS][32];
     wait_for_previous();
     let_next_start();
     group_starts(groups, starts);
@@ -234,12 +235,20 @@ __global__ void __launch_bounds__(256) k_bias_join(const float *partial, Groups 
     const uint32_t g = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint64_t d = blockIdx.x * 32ull + lane;
     float sum = 0;
-    if (starts[g + 1] > starts[g] && d < out)
-        for (uint32_t c = starts[g] / chunk + warp; c <= (starts[g + 1] - 1) / chunk; c += 8) sum += partial[(static_cast<uint64_t>(c) + g) * out + d];
+    if (starts[g + 1] > starts[g] && d < out) {
+        const uint32_t end = (starts[g + 1] - 1) / chunk + 1;
+        for (uint32_t c = starts[g] / chunk + warp; c < end; c += BJ_WARPS * BJ_AHEAD) {
+            float v[BJ_AHEAD];
+#pragma unroll
+            for (uint32_t i = 0; i < BJ_AHEAD; i++) v[i] = c + i * BJ_WARPS < end ? partial[(static_cast<uint64_t>(c) + i * BJ_WARPS + g) * out + d] : 0;
+#pragma unroll
+            for (uint32_t i = 0; i < BJ_AHEAD; i++) sum += v[i];
+        }
+    }
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp || d >= out) return;
-    for (uint32_t w = 1; w < 8; w++) sum += sums[w][lane];
+    for (uint32_t w = 1; w < BJ_WARPS; w++) sum += sums[w][lane];
     dbias[g * out + d] = narrow<T>(sum);
 }
 

@@ -349,7 +349,7 @@ static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T 
         return launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, dim3(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS), EG_THREADS, 0, cs, a);
     });
     if (!rc && p->dbias)
-        rc = launch("launch k_bias_join", k_bias_join<T>, dim3(static_cast<unsigned>((p->out + 31) / 32), p->experts), 256, 0, cs, static_cast<const float *>(partial),
+        rc = launch("launch k_bias_join", k_bias_join<T>, dim3(static_cast<unsigned>((p->out + 31) / 32), p->experts), 32 * BJ_WARPS, 0, cs, static_cast<const float *>(partial),
                     groups_of(p), p->out, chunk, static_cast<T *>(p->dbias));
     return rc;
 }

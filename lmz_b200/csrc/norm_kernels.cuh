@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
 }
 
 // out[d] = the sum of `rows` shares.  A block has 32 columns; its warps take the shares in turn, and their sums meet in their order.
-constexpr uint32_t JOIN_WARPS = 16, JOIN_AHEAD = 8;
+constexpr uint32_t JOIN_WARPS = 32, JOIN_AHEAD = 10;
 template <class W>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) k_join(const float *partial, uint64_t rows, uint64_t dim, W *out)
 {
