@@ -11,8 +11,8 @@ enum Activation : uint32_t { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TA
 
 constexpr float ROOT_HALF = 0.70710678f, ROOT_2_PI = 0.79788456f, ROOT_1_2PI = 0.39894228f, TANH_CUBE = 0.044715f;
 
-// (The exponential and the quotient are the fast ones: 2^-21 and less off where the result is not far below the 2^-24 of a factor of one, and a third of the
-// instructions.  Behind the products of a tile of 256 by 256 with 4096 k they have 19 us.)
+// The exponential and the quotient are the fast ones, whose errors are some 2^-21 of their result: far below the rounding to 16 bits that follows, and
+// a third of the instructions, which the products of the next tile would wait for.
 __device__ __forceinline__ float act(uint32_t kind, float z)
 {
     switch (kind) {
@@ -142,7 +142,8 @@ __device__ __forceinline__ void load_floats(const float *from, float *to)
 // meet have the place chunk + group, which no other two have.  Rows of no group get zeros.
 //
 // z comes in 32 bits: in 16 its rounding would be worse in dtimes than the result's own (one and a half times the error of a z that is not rounded).
-// Bound by HBM.  A thread has a vector of columns and goes down a chunk's rows.
+// Bound by HBM.  A thread has a vector of columns and goes down a chunk's rows, two under way at a time (four cost the threads that an SM has: 380 us and
+// not 228).  One B200, 8192x14336 BF16, silu and a factor: 228 us (6.2 TB/s).
 template <class T, int VB>
 __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGradArgs a)
 {

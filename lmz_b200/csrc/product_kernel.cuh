@@ -62,6 +62,7 @@ struct TilePlace {
     uint32_t k, k_rows;                          // WEIGHT_GRAD: the group's rows
 };
 
+// N elements in 32 bits.
 template <class O, int N>
 __device__ __forceinline__ void widen_some(const O *from, float *to)
 {
@@ -143,16 +144,25 @@ __device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group,
 // Features are the tensor core's M and columns its N, whatever their number: a single row streams the weight past 16 columns, a batch past 256.
 //
 // Roles: a TMA warp loads tiles of A and B (128 bytes along k, or 64 k) into a ring of stages; a warp issues the MMAs; sixteen warps take the
-// sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products.  They turn 32 features and 16 columns round
-// in shared memory, so that a lane has eight neighbours of a row, and what stands in the epilogue comes and goes by 16 bytes.  Where nothing of the rows' own
-// stands in it the results are turned round and not the sums, in half the bytes: the products want shared memory's whole bandwidth, and every byte of
-// the epilogue's is time of theirs (8192 rows 16384x1024x4096 100 to 95 us).
-// Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile ends with its group,
-// to a multiple of 16 columns; what is behind its group's last column is another group's rows, whose sums are left where they are (a column's sums are its own).  Where k has the groups (WEIGHT_GRAD) the rows behind the group's
-// last are made zeros in both operands' tiles by a warp between the copies and the products: of either alone the other's infinities would make NaN.  Only such
-// steps go by that warp (all of them did at first: handing a step on to another CTA takes 1 us, and 8192 rows 4096x14336 took 2070 us and not 634).
+// sums out of TMEM, which holds two tiles' sums, so that a tile's way out runs under the next tile's products (eight warps took 9 to 11 us
+// a tile, more than 1024 k's products; these take 5).  They turn 32 features and 16 columns round in shared memory, so that a lane has eight neighbours
+// of a row, and what stands in the epilogue comes and goes by 16 bytes, on its way since the sixteen columns before.  Where nothing of the rows' own
+// stands in it the results are turned round and not the sums, in half the bytes: the products want shared memory's bandwidth, and the epilogue's
+// bytes are time of theirs (16384 rows 1024x4096 100 to 95 us).
+//
+// Tiles are those of all groups: where the groups' rows begin is found on the device.  A tile ends with its group, to a multiple of 16 columns;
+// what is behind the group's last column is another group's rows, whose sums are left where they are (a column's sums are its own).  Where k has
+// the groups (WEIGHT_GRAD) the rows behind the group's last are made zeros in both operands' tiles by a warp between the copies and the
+// products: of either alone the other's infinities would make NaN.  Only such steps go by that warp (all of them did at first: handing a step on to
+// another CTA takes 1 us, and the weight's gradient of 8192 rows 4096x14336 took 2070 us and not 634).
+//
 // Few tiles: the CTAs of a cluster share k, and their sums meet in distributed shared memory.
-// Many (PAIR): two CTAs multiply 256 features by 256 columns together, each loading half of both.
+// Many (PAIR): two CTAs multiply 256 features by up to 256 columns together, each loading half of both.
+//
+// Bound by the tensor pipe, whose clock is bound by power, where there are many rows; by reading the weight where there are few.  One B200, us for the
+// kernel alone (and its share of the tensor pipe's cycles, at the 1.45 to 1.5 GHz that 1000 W leave): 4096 rows 4096x14336 314 (95 %), with z and
+// a factor 365 (82 %), rows' gradient 329 (92 %), weight's 329 (90 %), in 8 bits 168 (90 %); 16384 rows of 16 experts 2048x4096 200, 200 and 250
+// (their weights come from HBM once a few tiles); in a graph one row 4096x14336 22.6 (5.2 TB/s), 4096x4096 11.8.
 template <class T, class O, int P, bool PAIR>
 __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant__ ProductArgs a)
 {
