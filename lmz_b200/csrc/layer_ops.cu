@@ -72,7 +72,7 @@ API int lmz_gpu_norm_dev(const lmz_norm *p, void *cuda_stream)
 {
     int rc = check_norm(p);
     if (rc || p->tokens == 0) return rc;
-    if (!p->weight && !p->q) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm has a weight");
+    if (!p->x || (!p->weight && !p->q)) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm has x and a weight");
     if (p->q ? p->y || !p->scale : !p->y) return fail_msg(LMZ_GPU_EUNSUPPORTED, "either y, or q and scale");
     rc = device_ready();
     if (rc) return rc;
@@ -124,7 +124,8 @@ API size_t lmz_gpu_norm_grad_work_bytes(const lmz_norm *p)
 API int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream)
 {
     int rc = check_norm(p);
-    if (!rc && p->tokens && (!p->weight || !p->rstd || !p->dy)) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm's gradients go by its weight, rstd and dy");
+    if (!rc && p->tokens && (!p->x || !p->weight || !p->rstd || !p->dy || (p->dweight && !p->work)))
+        rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a norm's gradients go by x, its weight, rstd and dy, the weight's by a workspace, too");
     if (rc) return rc;
     rc = device_ready();
     if (rc) return rc;
@@ -393,6 +394,7 @@ API int lmz_gpu_product_dev(const lmz_product *p, void *cuda_stream)
 {
     int rc = check_product(p);
     if (rc || p->rows == 0) return rc;
+    if (!p->x || !p->weight || !p->y || (!p->work && ProductLayout(p, false).end)) return fail_msg(LMZ_GPU_EUNSUPPORTED, "a product goes by x, a weight, y, and the workspace that it asks for");
     rc = device_ready();
     if (rc) return rc;
     const cudaStream_t cs = static_cast<cudaStream_t>(cuda_stream);
@@ -405,8 +407,9 @@ API int lmz_gpu_product_grad_dev(const lmz_product *p, void *cuda_stream)
 {
     int rc = check_product(p);
     if (!rc && p->dtype == LMZ_GPU_E4M3) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "products in 8 bits have no gradients");
-    if (!rc && p->rows && (!p->dy || ((p->activation != ACT_NONE || p->dtimes) && !p->z)))
-        rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a product's gradients go by dy, and z where there is an activation or `times`");
+    if (!rc && p->rows && !p->work && ProductLayout(p, true).end) rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a product's gradients go by the workspace that they ask for");
+    if (!rc && p->rows && (!p->dy || (p->dx && !p->weight) || (p->dweight && !p->x) || ((p->activation != ACT_NONE || p->dtimes) && !p->z)))
+        rc = fail_msg(LMZ_GPU_EUNSUPPORTED, "a product's gradients go by dy, x and the weight, and z where there is an activation or `times`");
     if (rc) return rc;
     rc = device_ready();
     if (rc) return rc;

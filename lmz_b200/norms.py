@@ -12,7 +12,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6):
 
     `x`, `residual`: [..., dim], bfloat16, float16 or float32, the elements of a row next to each other.  `weight`: [dim], of their
     type or float32.  `s` is rounded to the tensors' type, and what is normed is the rounded one.  Squares are summed and
-    the result is worked out in 32 bits and rounded once.  Results are contiguous.
+    the result is worked out in 32 bits and rounded once (so that a row's squares have to stay within float32's range).  Results are contiguous.
 
     Differentiable once, in x, residual and weight (and through s); the weight's gradient is summed in 32 bits in one order, and is the
     same in every run."""

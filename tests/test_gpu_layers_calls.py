@@ -264,3 +264,34 @@ def test_activations_at_the_ends_of_their_range():
             want = want_products(x[small], w, kind=kind, dy=dy[small])
             close(y[small], want["y"]), close(dx[small], want["dx"])
             assert torch.equal(y[~small][:, 0], z[~small].clamp_min(0)) and torch.equal(dx[~small][:, 0], (z[~small] > 0).to(BF16))
+
+
+def test_experts_weights_in_other_orders():
+    """Side by side instead of behind each other, one for all of them, in reverse, every other one."""
+    from lmz_b200 import experts
+    x, dy, offsets, starts = _randn(1, (90, 64)), _randn(2, (90, 48)), torch.tensor([0, 30, 41, 90], device="cuda"), [0, 30, 41, 90]
+    block = _randn(3, (48, 3, 64), std=0.2)
+    for w in (block.transpose(0, 1), block[:, :1].transpose(0, 1).expand(3, 48, 64), _randn(4, (6, 48, 64), std=0.2)[::2], _randn(5, (3, 96, 64), std=0.2)[:, ::2], _randn(6, (3, 48, 80), std=0.2)[:, :, 8:72]):
+        leaf = w.detach().requires_grad_(True)
+        v = x.clone().requires_grad_(True)
+        y = experts.project(v, leaf, offsets)
+        dx, dw = torch.autograd.grad(y, (v, leaf), dy)
+        with torch.no_grad():
+            want = want_products(x, w, dy=dy, starts=starts)
+            close(y, want["y"]), close(dx, want["dx"]), close(dw, want["dweight"])
+
+
+def test_a_padded_batch():
+    """Rows behind the last sequence: zeros out, none of theirs in any gradient, whatever they hold."""
+    from lmz_b200 import experts
+    x, w, dy, m = _randn(1, (200, 40)), _randn(2, (4, 24, 40), std=0.2), _randn(3, (200, 24)), _randn(4, (200, 24))
+    offsets = torch.tensor([0, 50, 50, 120, 137], dtype=torch.int32, device="cuda")
+    x[137:], dy[137:], m[137:] = float("nan"), float("inf"), float("nan")
+    leaves = [t.requires_grad_(True) for t in (x, w, m)]
+    y = experts.project(x, w, offsets, activation="gelu", times=m)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert (y[137:] == 0).all() and (grads[0][137:] == 0).all() and (grads[2][137:] == 0).all() and all(g.isfinite().all() for g in grads)
+    short = [t.detach()[:137].clone().requires_grad_(True) if t.dim() == 2 else t for t in leaves]
+    again = experts.project(short[0], short[1], offsets, activation="gelu", times=short[2])
+    for a, b in zip((y, *grads), (again, *torch.autograd.grad(again, short, dy[:137]))):
+        assert torch.equal(a[:137], b) if a.dim() == 2 else torch.equal(a, b)

@@ -55,12 +55,12 @@ def test_norms_the_library_refuses(lib, bad):
     assert lib.lmz_gpu_norm_grad_dev(_norm(**bad), None) == -2
 
 
-@pytest.mark.parametrize("without", [dict(), dict(y=64, q=64, scale=64), dict(q=64), dict(weight=None, y=64)])
+@pytest.mark.parametrize("without", [dict(), dict(x=64), dict(y=64), dict(x=64, y=64, q=64, scale=64), dict(x=64, q=64), dict(x=64, weight=None, y=64)])
 def test_norms_without_what_they_write_to(lib, without):
     assert lib.lmz_gpu_norm_dev(_norm(**without), None) == -2 and lib.lmz_gpu_last_error()
 
 
-@pytest.mark.parametrize("without", [dict(), dict(rstd=64), dict(dy=64), dict(rstd=64, dy=64, weight=None)])
+@pytest.mark.parametrize("without", [dict(), dict(x=64, rstd=64), dict(x=64, dy=64), dict(x=64, rstd=64, dy=64, weight=None), dict(x=64, rstd=64, dy=64, dweight=64), dict(rstd=64, dy=64)])
 def test_norms_gradients_without_what_they_go_by(lib, without):
     assert lib.lmz_gpu_norm_grad_dev(_norm(dx=64, **without), None) == -2 and lib.lmz_gpu_last_error()
 
@@ -86,7 +86,13 @@ def test_products_in_8_bits_have_no_gradients_in_the_library(lib):
     assert lib.lmz_gpu_product_grad_dev(_product(dtype=3, x_scale=64, weight_scale=64), None) == -2
 
 
-@pytest.mark.parametrize("without", [dict(dx=64), dict(dx=64, dy=64, activation=2), dict(dtimes=64, dy=64, times=64)])
+@pytest.mark.parametrize("without", [dict(), dict(x=64, y=64), dict(weight=64, y=64), dict(x=64, weight=64), dict(x=2, weight=64, y=64)])
+def test_products_without_what_they_go_by(lib, without):
+    assert lib.lmz_gpu_product_dev(_product(**without), None) == -2 and lib.lmz_gpu_last_error()
+
+
+@pytest.mark.parametrize("without", [dict(dx=64), dict(dx=64, dy=64), dict(dweight=64, dy=64), dict(dx=64, dy=64, weight=64, activation=2, work=256), dict(dx=64, dy=64, z=64, activation=2, weight=64),
+                                     dict(dtimes=64, dy=64, times=64, work=256)])
 def test_products_gradients_without_what_they_go_by(lib, without):
     assert lib.lmz_gpu_product_grad_dev(_product(**without), None) == -2 and lib.lmz_gpu_last_error()
 
