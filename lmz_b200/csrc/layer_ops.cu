@@ -273,8 +273,8 @@ static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64
     int sms = 0, rc = sm_count(&sms);
     if (rc) return rc;
     const uint64_t groups = a.groups.count, used = by_k ? groups : std::min<uint64_t>(groups, std::max<uint64_t>(a.cols, 1));
-    // (tiles of columns: an estimate, and no fewer than there can be)
-    auto col_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : used * ((a.cols / used + nt - 1) / nt + (a.cols / used % nt == 0 && groups > 1 ? 1 : 0)); };
+    // (tiles of columns: as many as groups that end anywhere have on average, half a tile more each, and no fewer than there can be)
+    auto col_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : groups == 1 ? (a.cols + nt - 1) / nt : std::max(used, a.cols / nt + used / 2); };
     auto most_tiles = [&](uint64_t nt) { return by_k ? (a.cols + nt - 1) / nt * groups : groups == 1 ? (a.cols + nt - 1) / nt : a.cols / nt + used; };
     const uint64_t rows_each = std::max<uint64_t>(1, a.cols / used);
     const uint64_t all_steps = by_k ? std::max<uint64_t>(1, (depth / groups + STEP_K - 1) / STEP_K) : (depth + step_elements - 1) / step_elements;
