@@ -308,6 +308,7 @@ static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64
     a.feat_tiles = static_cast<uint32_t>(feat_tiles), a.col_tiles = static_cast<uint32_t>((a.cols + a.nt - 1) / a.nt);
     a.steps = static_cast<uint32_t>((depth + step_elements - 1) / step_elements);
     a.tmem_columns = tmem_columns(a.split > 1 ? a.nt : 2 * a.nt);
+    for (a.split_log = 0; 1u << a.split_log < a.split;) a.split_log++;
     const CUtensorMapDataType type = sizeof(T) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const uint32_t cols_each = pair ? a.nt / 2 : a.nt;
     if (P == FORWARD) rc = tile_map(&a.a, at, type, sizeof(T), depth, a.feats, a_stride, G_FEATS, groups, a_plane);

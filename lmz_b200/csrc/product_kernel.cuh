@@ -40,8 +40,8 @@ struct ProductArgs {
     uint32_t activation;
     uint32_t steps;                              // of 128 bytes along k (not where k has the groups)
     uint32_t nt;                                 // columns of a tile
-    uint32_t split;                              // CTAs of a cluster that share k
-    uint32_t feat_tiles, col_tiles;              // of G_FEATS (a pair: twice that) and, where k has the groups, of nt
+    uint32_t split, split_log;                   // CTAs of a cluster that share k: a power of two
+    uint32_t feat_tiles, col_tiles;              // of G_FEATS (a pair: twice that) and, where c has no groups, of nt
     uint32_t stages, stage_bytes, tmem_columns;
     bool vectors;                                // rows of all tensors that the epilogue has to do with start on 16 bytes
     bool plain;                                  // and they are the result's alone: what else there is goes by feature or by column
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     __shared__ ProductShared s;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t side = PAIR ? cluster_rank() : 0, rank = !PAIR && a.split > 1 ? cluster_rank() : 0;
-    const uint32_t team = PAIR ? 2 : a.split;
-    const uint32_t first = blockIdx.x / team, stride = gridDim.x / team;
+    const uint32_t team_log = PAIR ? 1 : a.split_log;
+    const uint32_t first = blockIdx.x >> team_log, stride = gridDim.x >> team_log;
     const uint32_t ring = (smem_addr(g_smem) + ATOM_BYTES - 1) & ~(ATOM_BYTES - 1);
     uint8_t *const local = g_smem + (ring - smem_addr(g_smem));
     volatile uint32_t *over = &s.over;
@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         __syncwarp();
         // The weight's first tiles come to L2 while the kernel before still runs (whose tiles is known without it where there are no groups).
         if (!BY_K && !a.groups.offsets) {
-            const uint32_t ct = static_cast<uint32_t>((a.cols + a.nt - 1) / a.nt), wide = ct < 8 ? ct : 8;
+            const uint32_t wide = a.col_tiles < 8 ? a.col_tiles : 8;
             const uint32_t f = ((first < a.feat_tiles * wide ? first / wide : first % (8 * a.feat_tiles) / wide) * CTAS + side) * G_FEATS;
-            const uint32_t k0 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * rank / a.split), k1 = static_cast<uint32_t>(static_cast<uint64_t>(a.steps) * (rank + 1) / a.split);
+            const uint32_t k0 = a.steps * rank >> a.split_log, k1 = a.steps * (rank + 1) >> a.split_log;
             for (uint32_t k = k0; k < k1 && k - k0 < a.stages; k++) {
                 if (elected()) {
                     if constexpr (P == FORWARD) {
@@ -213,8 +213,12 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         }
     }
     wait_for_previous();
-    group_starts(a.groups, s.starts);
-    if (warp == 0 && !BY_K) {
+    if (!a.groups.offsets) {
+        if (tid == 0) s.starts[0] = s.tiles[0] = 0, s.starts[1] = static_cast<uint32_t>(a.groups.rows), s.tiles[1] = a.col_tiles;
+    } else {
+        group_starts(a.groups, s.starts);
+    }
+    if (warp == 0 && !BY_K && a.groups.offsets) {
         __syncwarp();
         uint32_t sum = 0;
         for (uint32_t i0 = 0; i0 <= a.groups.count; i0 += 32) {
@@ -246,11 +250,12 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             p.group = group_of(s.tiles, groups, tile / a.feat_tiles);
             before = s.tiles[p.group], cols = s.tiles[p.group + 1] - before;
         }
+        // (a division takes a hundred cycles, which a kernel of few tiles waits for)
         const uint32_t in_group = tile - before * a.feat_tiles;
-        const uint32_t band = 8 * a.feat_tiles, b = in_group / band, in = in_group - b * band;
+        const uint32_t band = 8 * a.feat_tiles, b = cols <= 8 ? 0 : in_group / band, in = in_group - b * band;
         const uint32_t w = cols - 8 * b < 8 ? cols - 8 * b : 8;
-        const uint32_t ct = 8 * b + in % w;
-        p.ft = in / w;
+        p.ft = w == 1 ? in : in / w;
+        const uint32_t ct = 8 * b + in - p.ft * w;
         if (BY_K) p.c = ct * a.nt, p.c_end = static_cast<uint32_t>(a.cols), p.k = s.starts[p.group], p.k_rows = s.starts[p.group + 1] - p.k;
         else p.c = s.starts[p.group] + ct * a.nt, p.c_end = s.starts[p.group + 1], p.k = p.k_rows = 0;
         const uint32_t left = (p.c_end - p.c + 16 * CTAS - 1) / (16 * CTAS) * (16 * CTAS);
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         return p;
     };
     auto all_steps = [&](const TilePlace &p) { return BY_K ? (p.k_rows + STEP_K - 1) / STEP_K : a.steps; };
-    auto step_from = [&](uint32_t steps, uint32_t r) { return static_cast<uint32_t>(static_cast<uint64_t>(steps) * r / a.split); };
+    auto step_from = [&](uint32_t steps, uint32_t r) { return steps * r >> a.split_log; };       // (below 2^26 steps, and eight CTAs)
     auto features = [&](const TilePlace &p) { return (p.ft * CTAS + side) * G_FEATS; };      // where this CTA's begin
 
     if (warp == G_TMA_WARP) {
@@ -547,13 +552,54 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
         if (warp < G_TMA_WARP && first < tiles && !*over) {
             const TilePlace p = place(first);
             const uint64_t plane = BY_K ? p.group * a.cols : 0;
-            const uint32_t share = a.nt / a.split, feat = tid & (G_FEATS - 1);
-            const uint64_t f = features(p) + feat;
-            const Peers peers(ring, a.split);
-            if (f < a.feats) {
+            // A warp has a column, a lane four neighbours of f.
+            const uint32_t share = a.nt >> a.split_log;
+            const uint64_t f = features(p) + lane * 4;
+            uint32_t peer[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) peer[i] = peer_addr(local, i < a.split ? i : 0);
 #pragma unroll 2
-                for (uint32_t q = rank * share + tid / G_FEATS; q < (rank + 1) * share && p.c + q < p.c_end; q += G_EPILOGUE / G_FEATS)
-                    finish_one<O, SCALED>(a, p.group, p.c + q, f, (plane + p.c + q) * a.feats + f, peers.sum((q * G_FEATS + feat) * 4));
+            for (uint32_t q = rank * share + warp; q < (rank + 1) * share && p.c + q < p.c_end; q += G_TMA_WARP) {
+                float4 part[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    part[i] = make_float4(0, 0, 0, 0);
+                    if (i < a.split)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(part[i].x), "=f"(part[i].y), "=f"(part[i].z), "=f"(part[i].w)
+                                     : "r"(peer[i] + (q * G_FEATS + lane * 4) * 4) : "memory");
+                }
+                float v[1][4] = {{part[0].x, part[0].y, part[0].z, part[0].w}};
+#pragma unroll
+                for (uint32_t i = 1; i < 8; i++) v[0][0] += part[i].x, v[0][1] += part[i].y, v[0][2] += part[i].z, v[0][3] += part[i].w;
+                const uint32_t c = p.c + q;
+                const uint64_t at = (plane + c) * a.feats + f;
+                if (a.vectors) {
+                    if (f >= a.feats) continue;
+                    O *const out = static_cast<O *>(a.out);
+                    auto four = [&](const void *from, uint64_t i) {
+                        Vec<O, 8> w;
+                        w.raw = make_uint2(0, 0);
+                        if (from) w.raw = *reinterpret_cast<const uint2 *>(static_cast<const O *>(from) + i);
+                        return w;
+                    };
+                    const Vec<O, 8> bias = four(a.bias, p.group * a.feats + f), m = four(a.times, c * a.times_stride + f), r = four(a.residual, c * a.residual_stride + f);
+                    float a_scale[4] = {}, b_scale = 0;
+                    if constexpr (SCALED) {
+                        b_scale = a.b_scale[c];
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; e++) a_scale[e] = a.a_scale[f + e];
+                    }
+                    const bool on = true;
+                    const O *const ms = m.e, *const rs = r.e;
+                    finish<O, SCALED, 1, 4>(a, &at, &on, v, bias.e, a_scale, &b_scale, &ms, &rs);
+                    Vec<O, 8> y;
+                    narrow_all(v[0], y);
+                    *reinterpret_cast<uint2 *>(out + at) = y.raw;
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++)
+                        if (f + e < a.feats) finish_one<O, SCALED>(a, p.group, c, f + e, at + e, v[0][e]);
+                }
             }
         }
         cluster_barrier();
