@@ -437,7 +437,7 @@ int lmz_gpu_norm_grad_dev(const lmz_norm *p, void *cuda_stream);
  * where e is the expert whose rows t is one of: offsets[e] <= t < offsets[e + 1].  Offsets that do not ascend, or leave the rows there are, are
  * taken as the nearest that do not.  Rows of no expert are zeros, in y and in every gradient.  Without offsets there is one weight, for all
  * rows.  BF16 or F16; or x and the weight in 8 bits (E4M3), z[t][o] = x_scale[t] weight_scale[o] (x[t] W^T)[o] + bias[o], the other tensors
- * BF16 or F16.  y, z, dy and all gradients are contiguous. */
+ * BF16 or F16.  y, dy and all gradients are contiguous. */
 #define LMZ_GPU_E4M3 3
 #define LMZ_GPU_MAX_EXPERTS 1024
 #define LMZ_GPU_ACT_NONE 0
@@ -454,7 +454,8 @@ typedef struct lmz_product {
     const void *offsets;        /* experts + 1 int32 or int64 (offset_bytes 4 or 8), or NULL: one expert, all rows */
     const float *x_scale, *weight_scale;   /* rows, and out: in 8 bits; NULL otherwise */
     void *y;                    /* rows x out */
-    float *z;                   /* rows x out: what the gradients need of the forward pass where there is an activation or `times`; or NULL */
+    void *z;                    /* lmz_gpu_product_z_bytes(), 256-byte aligned: what the gradients need of the forward pass where there is an
+                                 * activation or `times` (z in 24 bits); or NULL */
     const void *dy;             /* rows x out */
     void *dx, *dweight, *dbias, *dtimes;   /* contiguous, like x, weight, bias and times; NULL: not wanted */
     void *work;                 /* lmz_gpu_product_work_bytes(), 256-byte aligned */
@@ -463,6 +464,7 @@ typedef struct lmz_product {
 } lmz_product;
 /* Reads the sizes, strides and types alone, the addresses' last bits and which tensors there are; `grad`: for the gradients' call. */
 size_t lmz_gpu_product_work_bytes(const lmz_product *p, int grad);
+size_t lmz_gpu_product_z_bytes(const lmz_product *p);
 int lmz_gpu_product_dev(const lmz_product *p, void *cuda_stream);
 /* dz[t] = dy[t] times[t] act'(z[t]), rounded to the tensors' type;  dx[t] = dz[t] W_e, dW_e = the sum of dz[t]^T x[t], dbias_e = the sum of dz[t] over
  * the rows of expert e (zeros for one without any), dtimes[t] = dy[t] act(z[t]).  The residual's gradient is dy. */

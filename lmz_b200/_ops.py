@@ -45,6 +45,7 @@ def bind(lib) -> None:
             ("lmz_gpu_norm_grad_work_bytes", ctypes.c_size_t, [norm]),
             ("lmz_gpu_norm_grad_dev", _int, [norm, _v]),
             ("lmz_gpu_product_work_bytes", ctypes.c_size_t, [product, _int]),
+            ("lmz_gpu_product_z_bytes", ctypes.c_size_t, [product]),
             ("lmz_gpu_product_dev", _int, [product, _v]),
             ("lmz_gpu_product_grad_dev", _int, [product, _v]),
             ("lmz_gpu_order_work_bytes", ctypes.c_size_t, [_u64]),

@@ -18,7 +18,7 @@ def project(x, weight, bias=None, activation=None, times=None, residual=None):
     out.  `activation`: None, "relu", "silu", "gelu" (with the error function) or "gelu_tanh" (its approximation by tanh).
 
     Returns a contiguous [..., out], worked out in 32 bits and rounded once.  Differentiable once, in all five tensors; with an
-    activation or a factor the sums are kept for that in 32 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type.
+    activation or a factor the sums are kept for that in 24 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type.
     Gradients are the same in every run."""
     import torch
     index = _ops.on_cuda("x weight bias times residual", x, weight, bias, times, residual)
@@ -134,8 +134,11 @@ def _forward(index, code, rcode, kind, x, weight, bias, times, residual, offsets
     import torch
     like = times if times is not None else residual        # (of the result's shape and type)
     y = _ops.empty_like(like) if like is not None else x.new_empty((*x.shape[:-1], weight.shape[-2]), dtype=torch.bfloat16 if rcode == _ops.BF16 else torch.float16)
-    z = _ops.empty_like(y, torch.float32) if keep and (kind or times is not None) else None
-    p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, y, z)
+    p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, y)
+    z = None
+    if keep and (kind or times is not None):
+        z = y.new_empty(gpu.library().lmz_gpu_product_z_bytes(p), dtype=torch.uint8)
+        p.z = z.data_ptr()
     held = held, _work(p, 0, x)                            # (copies and workspace live until the launch)
     _ops.launch(index, "lmz_gpu_product_dev", p)
     return y, z

@@ -73,9 +73,10 @@ def products(x, weight, bias=None, kind=None, times=None, residual=None, dy=None
         if dy is None:
             continue
         d = dy[lo:hi].double()
-        s_off = BEND * off + 8 * STEP * (z.abs() + 1) * (kind is not None)
+        kept = off + (2 ** -15 * z.abs() if kind is not None or times is not None else 0)           # z as the gradients have it: 16 bits of mantissa, cut
+        s_off = BEND * kept + 8 * STEP * (z.abs() + 1) * (kind is not None)
         if kind == "relu":
-            s_off = s_off + (z.abs() <= off)              # (either side of the corner)
+            s_off = s_off + (z.abs() <= kept)              # (either side of the corner)
         if kind is None:
             s_off = 0 * off
         dz, dz_off = d * slope * m, (d * m).abs() * s_off + 3 * STEP * (d * slope * m).abs()
@@ -85,7 +86,7 @@ def products(x, weight, bias=None, kind=None, times=None, residual=None, dy=None
         most = dz.abs() + dz_off
         dx, dx_off = dz @ w, dz_off @ w.abs() + (out + 2) * STEP * (most @ w.abs())
         dw, dw_off = dz.t() @ xs, dz_off.t() @ xs.abs() + (hi - lo + 2) * STEP * (most.t() @ xs.abs())
-        dm, dm_off = d * a, d.abs() * (SLOPE * off + 8 * STEP * (z.abs() + 1)) + 2 * STEP * (d * a).abs()
+        dm, dm_off = d * a, d.abs() * (SLOPE * kept + 8 * STEP * (z.abs() + 1)) + 2 * STEP * (d * a).abs()
         for name, place, v, v_off in (("dx", slice(lo, hi), dx, dx_off), ("dweight", e, dw, dw_off), ("dbias", e, db, db_off), ("dtimes", slice(lo, hi), dm, dm_off)):
             got[name][0][place], got[name][1][place] = v, v_off + u * (v.abs() + v_off) + tiny
     if weight.dim() == 2 and dy is not None:
