@@ -9,17 +9,44 @@ namespace lmz {
 
 enum Activation : uint32_t { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_COUNT };
 
-constexpr float ROOT_HALF = 0.70710678f, ROOT_2_PI = 0.79788456f, ROOT_1_2PI = 0.39894228f, TANH_CUBE = 0.044715f;
+constexpr float ROOT_1_2PI = 0.39894228f, LOG2_E = 1.44269504f, TANH_CUBE = 0.044715f, TANH_TWICE = 1.59576912f;     // (the last: twice the root of 2 / pi)
 
-// The exponential and the quotient are the fast ones, whose errors are some 2^-21 of their result: far below the rounding to 16 bits that follows, and
-// a third of the instructions, which the products of the next tile would wait for.
+// The tensor pipe's neighbours: powers of two and reciprocals as the special function unit has them, some 2^-22 of their result off; what is below 2^-126 is zero.
+__device__ __forceinline__ float power_of_two(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float reciprocal(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+
+// The exponential goes by its root and its square is taken, so that it reaches as far as results of 16 bits do, whose smallest are e^-97: it is off by some 2^-21
+// of itself and 2^-24 for each unit of its argument, under 2^-16 everywhere, where half a step of F16 is 2^-11.
+//
+// 1 / (1 + exp(-v)), good to its own size on both sides (numerator and denominator 2^-64 times what they are: the exponential has room).
+__device__ __forceinline__ float sigmoid(float v)
+{
+    const float h = power_of_two(v * (-0.5f * LOG2_E)) * 0x1p-32f;
+    return reciprocal(fmaf(h, h, 0x1p-64f)) * 0x1p-64f;
+}
+
+// The normal distribution's integral up to v, good to its own size (1 + erf cancels below zero: at -5 it is off by 4 %), and its density's exponential. For v < 0 it
+// is exp(-v^2 / 2) P(-v), where P falls slowly from 1/2 like 0.4 / t: a polynomial in s = 1 / (1 + 0.3 t) without a constant, of the least relative error on
+// [0, 14.6] (2^-22.5; 2^-21 with its roundings; found by reweighted least squares), behind which the exponential is zero.
+__device__ __forceinline__ float normal_below(float v, float &bell)
+{
+    const float t = fabsf(v), s = reciprocal(fmaf(0.3f, t, 1)), h = power_of_two(t * (t * (-0.25f * LOG2_E)));
+    float p = 0.0353742f;
+    p = fmaf(p, s, -0.15595277f), p = fmaf(p, s, 0.20420392f), p = fmaf(p, s, -0.05171105f), p = fmaf(p, s, 0.12752213f);
+    p = fmaf(p, s, 0.100226894f), p = fmaf(p, s, 0.12070406f), p = fmaf(p, s, 0.11963253f);
+    const float tail = h * (p * s) * h;
+    bell = h * h;
+    return v < 0 ? tail : 1 - tail;
+}
+
 __device__ __forceinline__ float act(uint32_t kind, float z)
 {
+    float bell;
     switch (kind) {
     case ACT_RELU: return z < 0 ? 0.0f : z;                      // (a NaN stays)
     case ACT_SILU: return __fdividef(z, 1 + __expf(-z));
-    case ACT_GELU: return 0.5f * z * (1 + erff(z * ROOT_HALF));
-    case ACT_GELU_TANH: return 0.5f * z * (1 + tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z)));
+    case ACT_GELU: return z * normal_below(z, bell);
+    case ACT_GELU_TANH: return z * sigmoid(TANH_TWICE * (z + TANH_CUBE * z * z * z));     // ((1 + tanh u) / 2 is the sigmoid of 2 u)
     default: return z;
     }
 }
@@ -57,15 +84,16 @@ __device__ __forceinline__ void act_and_slope(uint32_t kind, const float *z, flo
         });
     case ACT_GELU:
         return each([](float z, float &y, float &slope) {
-            const float below = 0.5f * (1 + erff(z * ROOT_HALF));
-            y = z * below, slope = below + z * ROOT_1_2PI * __expf(-0.5f * z * z);
+            float bell;
+            const float below = normal_below(z, bell);
+            y = z * below, slope = fmaf(z * ROOT_1_2PI, bell, below);
         });
     case ACT_GELU_TANH:
         return each([](float z, float &y, float &slope) {
-            const float t = tanhf(ROOT_2_PI * (z + TANH_CUBE * z * z * z));
-            y = 0.5f * z * (1 + t);
-            const float near = fminf(fmaxf(z, -16.0f), 16.0f);   // (beyond, 1 - t * t is zero, and the square may be infinite)
-            slope = 0.5f * (1 + t) + 0.5f * near * (1 - t * t) * ROOT_2_PI * (1 + 3 * TANH_CUBE * near * near);
+            const float below = sigmoid(TANH_TWICE * (z + TANH_CUBE * z * z * z));
+            y = z * below;
+            const float near = fminf(fmaxf(z, -16.0f), 16.0f);   // (beyond, below or 1 - below is zero, and the square may be infinite)
+            slope = fmaf(y * (1 - below), TANH_TWICE * (1 + 3 * TANH_CUBE * near * near), below);
         });
     default: return each([](float z, float &y, float &slope) { y = z, slope = 1; });
     }
