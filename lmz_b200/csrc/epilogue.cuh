@@ -44,7 +44,7 @@ __device__ __forceinline__ float act(uint32_t kind, float z)
     float bell;
     switch (kind) {
     case ACT_RELU: return z < 0 ? 0.0f : z;                      // (a NaN stays)
-    case ACT_SILU: return __fdividef(z, 1 + __expf(-z));
+    case ACT_SILU: return z * sigmoid(z);
     case ACT_GELU: return z * normal_below(z, bell);
     case ACT_GELU_TANH: return z * sigmoid(TANH_TWICE * (z + TANH_CUBE * z * z * z));     // ((1 + tanh u) / 2 is the sigmoid of 2 u)
     default: return z;
@@ -79,8 +79,8 @@ __device__ __forceinline__ void act_and_slope(uint32_t kind, const float *z, flo
     case ACT_RELU: return each([](float z, float &y, float &slope) { y = z < 0 ? 0.0f : z, slope = z > 0 ? 1.0f : 0.0f; });
     case ACT_SILU:
         return each([](float z, float &y, float &slope) {
-            const float e = __fdividef(1, 1 + __expf(-z));
-            y = z * e, slope = e * (1 + z * (1 - e));
+            const float below = sigmoid(z);
+            y = z * below, slope = fmaf(y, 1 - below, below);
         });
     case ACT_GELU:
         return each([](float z, float &y, float &slope) {

@@ -25,11 +25,11 @@ def _numbers(dtype, lo, hi):
 
 def _exponent(kind, z):
     """How large the exponential's argument gets that an activation's far side goes by."""
-    return {"gelu": z * z, "gelu_tanh": 1.6 * (z + 0.044715 * z ** 3).abs()}[kind]
+    return {"silu": z.abs(), "gelu": z * z, "gelu_tanh": 1.6 * (z + 0.044715 * z ** 3).abs()}[kind]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh"])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
 def test_far_sides_of_activations(kind, dtype):
     """Relative to the result itself, wherever it can be held: one rounding to the type, and in 32 bits the exponential's error, which grows with its argument
     (an argument of A is off by A 2^-24 a rounding, of which there are up to four, and the function by (2 + 1.2 A) 2^-23), and eight roundings more.  (128 times the
