@@ -77,6 +77,11 @@ __device__ __forceinline__ void widen_some(const O *from, float *to)
     }
 }
 
+// Scales (8 bits) whose product, and its product with any sum of 8-bit products (2^-18 to 2^39), stays within 32 bits.  Rows and weights of ordinary size have such;
+// other sums are multiplied in 64 bits, one scale after the other, and meet scales of 1 in the epilogue.
+__device__ __forceinline__ bool mild(float scale) { return fabsf(scale) >= 0x1p-40f && fabsf(scale) <= 0x1p40f; }
+__device__ __forceinline__ float scaled_in_64(float sum, float a, float b) { return static_cast<float>(static_cast<double>(sum) * a * b); }
+
 // N neighbours of f of each of J columns, from sums to result: z = sums + bias, y = act(z) times + residual.  `on`: whether there is such a column.
 template <class O, bool SCALED, int J, int N>
 __device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at, const bool *on, float (*v)[N], const O *bias, const float *a_scale, const float *b_scale,
@@ -128,9 +133,13 @@ __device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group,
 {
     const O *const times = static_cast<const O *>(a.times) + c * a.times_stride + f, *const residual = static_cast<const O *>(a.residual) + c * a.residual_stride + f;
     const bool on = true;
+    float a_scale = 1, b_scale = 1;
+    if constexpr (SCALED) {
+        a_scale = a.a_scale[f], b_scale = a.b_scale[c];
+        if (!mild(a_scale) || !mild(b_scale)) sum = scaled_in_64(sum, a_scale, b_scale), a_scale = b_scale = 1;
+    }
     float v[1][1] = {{sum}};
-    finish<O, SCALED, 1, 1>(a, &at, &on, v, static_cast<const O *>(a.bias) + group * a.feats + f, SCALED ? a.a_scale + f : nullptr, SCALED ? a.b_scale + c : nullptr, &times,
-                           &residual);
+    finish<O, SCALED, 1, 1>(a, &at, &on, v, static_cast<const O *>(a.bias) + group * a.feats + f, &a_scale, &b_scale, &times, &residual);
     static_cast<O *>(a.out)[at] = narrow<O>(v[0][0]);
 }
 
@@ -405,24 +414,35 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             auto live = [&](uint32_t g) { return g * G_GROUP < a.nt && p.c + g * G_GROUP < p.c_end; };
             Vec<O, 16> bias, m[2], r[2];
             float a_scale[SCALED ? 8 : 1], b_scale[2];
+            // (8 bits) the lane's own feature's scale, and those of two of the warp's columns: are all that its sums meet mild?
+            float own_scale = 1, column_scale[2] = {1, 1};
+            bool quick = true;
+            if (SCALED && vectors) {
+                const uint64_t own = features(p) + quarter * 32 + lane;
+                if (own < a.feats) own_scale = a.a_scale[own];
+#pragma unroll
+                for (uint32_t j = 0; j < 2; j++) {
+                    const uint32_t g = share + SHARES * (2 * j + (lane >> 4)), c = p.c + g * G_GROUP + (lane & 15);
+                    if (live(g) && c < p.c_end) column_scale[j] = a.b_scale[c];
+                }
+            }
             auto ask = [&](uint32_t g) {                         // what sixteen columns meet in the epilogue
 #pragma unroll
                 for (uint32_t j = 0; j < 2; j++) {
                     const uint32_t c = p.c + g * G_GROUP + j * 8 + (lane >> 2);
                     m[j].raw = r[j].raw = make_uint4(0, 0, 0, 0);
-                    if (SCALED) b_scale[j] = c < p.c_end ? a.b_scale[c] : 0.0f;
+                    if (SCALED) b_scale[j] = quick && c < p.c_end ? a.b_scale[c] : 1.0f;
                     if (c < p.c_end && f < a.feats) {
                         if (times) m[j].raw = *reinterpret_cast<const uint4 *>(times + c * a.times_stride + f);
                         if (residual) r[j].raw = *reinterpret_cast<const uint4 *>(residual + c * a.residual_stride + f);
                     }
                 }
             };
-            float f_bias = 0, f_scale = 0;                       // of the lane's own feature
+            float f_bias = 0;                                    // of the lane's own feature
             if (vectors && a.plain) {
                 const uint64_t own = features(p) + quarter * 32 + lane;
                 if (own < a.feats) {
                     if (a.bias) f_bias = widen(static_cast<const O *>(a.bias)[p.group * a.feats + own]);
-                    if constexpr (SCALED) f_scale = a.a_scale[own];
                 }
             } else if (vectors) {
                 bias.raw = make_uint4(0, 0, 0, 0);
@@ -447,11 +467,32 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             if (!warp_wait(&s.sums_full[buf], (n / 2) & 1, over)) break;
             tc_after();
             const uint32_t sums = tmem + (quarter << 21) + buf * a.nt;
+            float f_scale = own_scale;
+            if (SCALED && !__all_sync(~0u, mild(own_scale) && mild(column_scale[0]) && mild(column_scale[1]))) {
+                quick = false, f_scale = b_scale[0] = b_scale[1] = 1;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) a_scale[SCALED ? e : 0] = 1;
+            }
             for (uint32_t g = share; live(g); g += SHARES) {
                 uint32_t v[G_GROUP];
                 __syncwarp();
                 tmem_ask16(sums + g * G_GROUP, v);
                 tmem_wait16(v);
+                if (SCALED && !quick) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; j++) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; q++) turn[q * G_PITCH + lane] = __uint_as_float(v[j * 8 + q]);
+#pragma unroll 1
+                        for (uint32_t q = 0; q < 8; q++) {
+                            const uint32_t c = p.c + g * G_GROUP + j * 8 + q;
+                            turn[q * G_PITCH + lane] = scaled_in_64(turn[q * G_PITCH + lane], own_scale, c < p.c_end ? a.b_scale[c] : 0.0f);
+                        }
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; q++) v[j * 8 + q] = __float_as_uint(turn[q * G_PITCH + lane]);
+                    }
+                    __syncwarp();
+                }
                 if (vectors && a.plain) {
                     float u[G_GROUP];
 #pragma unroll
@@ -461,7 +502,8 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
 #pragma unroll
                         for (uint32_t q = 0; q < G_GROUP; q += 4) {
                             float4 s4;
-                            if (c + q + 3 < a.cols) s4 = *reinterpret_cast<const float4 *>(a.b_scale + c + q);
+                            if (!quick) s4 = make_float4(1, 1, 1, 1);
+                            else if (c + q + 3 < a.cols) s4 = *reinterpret_cast<const float4 *>(a.b_scale + c + q);
                             else s4 = make_float4(c + q < a.cols ? a.b_scale[c + q] : 0, c + q + 1 < a.cols ? a.b_scale[c + q + 1] : 0, c + q + 2 < a.cols ? a.b_scale[c + q + 2] : 0, 0);
                             u[q] *= s4.x * f_scale, u[q + 1] *= s4.y * f_scale, u[q + 2] *= s4.z * f_scale, u[q + 3] *= s4.w * f_scale;
                         }
@@ -581,6 +623,11 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                         b_scale = a.b_scale[c];
 #pragma unroll
                         for (uint32_t e = 0; e < 4; e++) a_scale[e] = a.a_scale[f + e];
+                        if (!mild(b_scale) || !mild(a_scale[0]) || !mild(a_scale[1]) || !mild(a_scale[2]) || !mild(a_scale[3])) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; e++) v[0][e] = scaled_in_64(v[0][e], a_scale[e], b_scale), a_scale[e] = 1;
+                            b_scale = 1;
+                        }
                     }
                     const bool on = true;
                     const O *const ms = m.e, *const rs = r.e;

@@ -3,11 +3,11 @@ their ranges, sums that round one way in 32 bits and another in fewer, against t
 import pytest
 import torch
 
-from layers import STEP, act, close, half_step, least
+from layers import STEP, act, close, half_step, least, products as want_products
 
 pytestmark = pytest.mark.gpu
 
-BF16, F16 = torch.bfloat16, torch.float16
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.fixture(autouse=True)
@@ -15,6 +15,12 @@ def _library(gpu):
     yield gpu
     from lmz_b200 import adapters
     adapters.check()
+
+
+def _randn(seed, shape, dtype=BF16, std=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * std).to(dtype)
 
 
 def _numbers(dtype, lo, hi):
@@ -49,3 +55,24 @@ def test_far_sides_of_activations(kind, dtype):
         size = below + (slope - below).abs()                 # the slope's two terms
         for got, want, o in ((y, a, off * a.abs()), (dm, a, off * a.abs()), (dx, slope, off * size)):
             close(got, (want, o + u * (want.abs() + o) + tiny))
+
+
+@pytest.mark.parametrize("rows, inp, out, residual", [(3, 256, 64, False), (3, 256, 64, True), (2, 256, 33, False), (1, 8192, 64, False), (1, 8192, 64, True), (1, 8192, 33, True), (300, 256, 512, False),
+                                                      (300, 256, 512, True)])
+@pytest.mark.parametrize("x_power, w_power", [(-90, -62), (-126, 126), (126, -126), (100, 40), (-50, -95), (-140, 10), (0, 0)])
+def test_scales_of_8_bits_at_the_ends_of_their_range(rows, inp, out, residual, x_power, w_power):
+    """Neither two small nor two large scales, nor one of each, lose what the result can hold; a sum of zero stays zero."""
+    from lmz_b200 import linear
+    both = x_power + w_power
+    small = -both > 100                                      # (the sums are as large as they get, or as small)
+    x, w = (_randn(k, s, F32, 120.0 if both < 0 else 0.01).clamp(-448, 448).abs().to(torch.float8_e4m3fn) for k, s in ((1, (rows, inp)), (2, (out, inp))))
+    x[-1], w[out // 2] = 0, 0
+    xs, ws = ((1 + 0.9 * torch.rand(n, generator=torch.Generator("cuda").manual_seed(n), device="cuda")) * 2.0 ** p for n, p in ((rows, x_power), (out, w_power)))
+    r = torch.zeros((rows, out), dtype=BF16, device="cuda") if residual else None
+    y = linear.project_8bit(x, xs, w, ws, residual=r)
+    exact, off = want_products(x.float(), w.float(), x_scale=xs, weight_scale=ws, dtype=BF16)["y"]
+    # (32 bits' own smallest numbers, of which a product may pass through one; what is above 16 bits' largest number is infinite)
+    fits = exact.abs() < 2.0 ** 127
+    close(torch.where(fits, y, 0), (torch.where(fits, exact, 0), off.clamp_max(2.0 ** 127) + 2.0 ** -148))
+    assert not y.isnan().any() and (y[-1] == 0).all() and (y[:, out // 2] == 0).all()
+    assert rows == 1 or small or (y[0] != 0).any()
