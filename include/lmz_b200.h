@@ -454,8 +454,8 @@ typedef struct lmz_product {
     const void *offsets;        /* experts + 1 int32 or int64 (offset_bytes 4 or 8), or NULL: one expert, all rows */
     const float *x_scale, *weight_scale;   /* rows, and out: in 8 bits; NULL otherwise */
     void *y;                    /* rows x out */
-    void *z;                    /* lmz_gpu_product_z_bytes(), 256-byte aligned: what the gradients need of the forward pass where there is an
-                                 * activation or `times` (z in 24 bits); or NULL */
+    void *z;                    /* lmz_gpu_product_z_bytes(), 256-byte aligned: z in 32 bits, which the gradients need where there is an
+                                 * activation or `times`; or NULL */
     const void *dy;             /* rows x out */
     void *dx, *dweight, *dbias, *dtimes;   /* contiguous, like x, weight, bias and times; NULL: not wanted */
     void *work;                 /* lmz_gpu_product_work_bytes(), 256-byte aligned */

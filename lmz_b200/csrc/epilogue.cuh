@@ -146,55 +146,11 @@ __device__ __forceinline__ uint32_t group_of(const uint32_t *starts, uint32_t co
 }
 
 constexpr uint32_t MAX_EXPERTS = 1024;
-constexpr uint32_t EG_THREADS = 128, EG_MOST_ROWS = 32, EG_LEAST_ROWS = 4, EG_STEP = 1;     // rows of a chunk, and of those under way together
-
-// What the gradients need of z, in 24 bits: the upper 16 of its bits, and behind all of those the next 8 of each (at `lower`), cut off, so that a NaN stays one.
-// An error of 2^-15 of z: rounded to 16 bits it would make dtimes' error one and a half times what it is (for F16 more), and 32 are a third more to write
-// and read.  A row has `out` elements; N neighbours of one at a time, N at most 8 and a divisor of their place.
-struct KeptSums {
-    uint16_t *upper;
-    uint8_t *lower;
-    __host__ __device__ static uint64_t lower_at(uint64_t elements) { return (elements * 2 + 255) & ~255ull; }
-    template <int N>
-    __device__ __forceinline__ void store(uint64_t at, const float *v) const
-    {
-        if constexpr (N == 1) {
-            upper[at] = static_cast<uint16_t>(__float_as_uint(v[0]) >> 16), lower[at] = static_cast<uint8_t>(__float_as_uint(v[0]) >> 8);
-        } else {
-            static_assert(N == 4 || N == 8);
-            union { uint32_t word[N / 2]; typename Raw<N * 2>::type raw; } hi;
-            union { uint32_t word[N / 4]; typename Raw<N>::type raw; } lo;
-#pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const uint32_t b0 = __float_as_uint(v[e]), b1 = __float_as_uint(v[e + 1]), b2 = __float_as_uint(v[e + 2]), b3 = __float_as_uint(v[e + 3]);
-                hi.word[e / 2] = __byte_perm(b0, b1, 0x7632), hi.word[e / 2 + 1] = __byte_perm(b2, b3, 0x7632);
-                lo.word[e / 4] = __byte_perm(__byte_perm(b0, b1, 0x0051), __byte_perm(b2, b3, 0x0051), 0x5410);
-            }
-            *reinterpret_cast<typename Raw<N * 2>::type *>(upper + at) = hi.raw;
-            *reinterpret_cast<typename Raw<N>::type *>(lower + at) = lo.raw;
-        }
-    }
-    template <int N>
-    __device__ __forceinline__ void load(uint64_t at, float *v) const
-    {
-        if constexpr (N < 4) {
-#pragma unroll
-            for (int e = 0; e < N; e++) v[e] = __uint_as_float(static_cast<uint32_t>(upper[at + e]) << 16 | static_cast<uint32_t>(lower[at + e]) << 8);
-        } else {
-            union { uint32_t word[N / 2]; typename Raw<N * 2>::type raw; } hi;
-            union { uint32_t word[N / 4]; typename Raw<N>::type raw; } lo;
-            hi.raw = *reinterpret_cast<const typename Raw<N * 2>::type *>(upper + at);
-            lo.raw = *reinterpret_cast<const typename Raw<N>::type *>(lower + at);
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                v[e] = __uint_as_float(__byte_perm(hi.word[e / 2], lo.word[e / 4], (e % 2 ? 0x3200 : 0x1000) | (4 + e % 4) * 0x11) & 0xFFFFFF00u);
-        }
-    }
-};
+constexpr uint32_t EG_THREADS = 128, EG_MOST_ROWS = 32, EG_LEAST_ROWS = 4, EG_STEP = 2;     // rows of a chunk, and of those under way together
 
 struct EpilogueGradArgs {
     const void *dy, *times;                      // times: or NULL, rows times_stride apart
-    KeptSums z;                                  // upper: NULL without an activation and `times`
+    const float *z;                              // NULL without an activation and `times`
     void *dz, *dtimes;                           // or NULL
     float *partial;                              // [chunk of rows + group][out]: sums of dz, or NULL
     Groups groups;
@@ -202,11 +158,20 @@ struct EpilogueGradArgs {
     uint32_t vectors, activation, chunk;         // chunk: rows
 };
 
+template <int N>
+__device__ __forceinline__ void load_floats(const float *from, float *to)
+{
+    constexpr int B = N * 4 < 16 ? N * 4 : 16;
+#pragma unroll
+    for (int i = 0; i < N * 4 / B; i++) reinterpret_cast<typename Raw<B>::type *>(to)[i] = reinterpret_cast<const typename Raw<B>::type *>(from)[i];
+}
+
 // dz = dy times act'(z), dtimes = dy act(z), and what each chunk of rows adds to the gradient of its groups' bias: a chunk and a group that
 // meet have the place chunk + group, which no other two have.  Rows of no group get zeros.
 //
-// Bound by HBM.  A thread has a vector of columns and goes down a chunk's rows, EG_STEP under way at a time: more cost the threads that an SM has room for (one
-// B200, 8192x14336 BF16, silu and a factor: two 275 us, one 260; four were 380 when z had 32 bits and two 228 to 260).
+// z comes in 32 bits: a factor's gradient is z or its activation times dy, rounded once.
+// Bound by HBM.  A thread has a vector of columns and goes down a chunk's rows, EG_STEP under way at a time (four cost the threads that an SM has: 380 us and
+// not 228).  One B200, 8192x14336 BF16, silu and a factor: 228 us (6.2 TB/s), the factor's gradient alone 187.
 template <class T, int VB>
 __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGradArgs a)
 {
@@ -247,7 +212,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
             for (int e = 0; e < V::N; e++) z[i][e] = 0;
             if (t >= end || t < first || t >= last) continue;
             d[i].raw = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + t * a.out)[v];
-            if (a.z.upper) a.z.load<V::N>(t * a.out + v * V::N, z[i]);
+            if (a.z) load_floats<V::N>(a.z + t * a.out + v * V::N, z[i]);
             if (a.times) m[i].raw = reinterpret_cast<const R *>(static_cast<const T *>(a.times) + t * a.times_stride)[v];
         }
 #pragma unroll

@@ -217,14 +217,7 @@ struct ProductLayout {
     }
 };
 
-// z as the kernels have it.
-static KeptSums kept_sums(const lmz_product *p)
-{
-    uint8_t *z = static_cast<uint8_t *>(p->z);
-    return {reinterpret_cast<uint16_t *>(z), z ? z + KeptSums::lower_at(p->rows * p->out) : nullptr};
-}
-
-API size_t lmz_gpu_product_z_bytes(const lmz_product *p) { return KeptSums::lower_at(p->rows * p->out) + p->rows * p->out; }
+API size_t lmz_gpu_product_z_bytes(const lmz_product *p) { return p->rows * p->out * sizeof(float); }
 API size_t lmz_gpu_product_work_bytes(const lmz_product *p, int grad) { return ProductLayout(p, grad).end; }
 
 // x and the weight as the kernels take them: where they lie, or in the workspace (in one launch).
@@ -336,7 +329,7 @@ static int product_as(const lmz_product *p, cudaStream_t cs)
     const ProductInputs<T> in(p, l, true, true, cs);
     if (in.rc) return in.rc;
     ProductArgs a{};
-    a.out = p->y, a.z = kept_sums(p), a.bias = p->bias, a.times = p->times, a.residual = p->residual, a.a_scale = p->weight_scale, a.b_scale = p->x_scale;
+    a.out = p->y, a.z = static_cast<float *>(p->z), a.bias = p->bias, a.times = p->times, a.residual = p->residual, a.a_scale = p->weight_scale, a.b_scale = p->x_scale;
     a.groups = groups_of(p), a.feats = p->out, a.cols = p->rows;
     a.times_stride = p->times_stride, a.residual_stride = p->residual_stride, a.activation = p->activation;
     a.vectors = vector_bytes(p->out * 2, {address(p->y), address(p->z), address(p->bias), address(p->times), p->times ? p->times_stride * 2 : 0, address(p->residual),
@@ -351,10 +344,10 @@ static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T 
     const uint32_t chunk = ProductLayout::chunk(p);
     const uint64_t chunks = (p->rows + chunk - 1) / chunk;
     float *partial = p->dbias ? reinterpret_cast<float *>(static_cast<uint8_t *>(p->work) + l.partial) : nullptr;
-    int rc = by_width<T>(vector_bytes(p->out * 2, {address(p->dy), address(p->z), address(p->times), p->times ? p->times_stride * 2 : 0, address(p->dtimes)}), [&](auto vec) {
+    int rc = by_width<T>(vector_bytes(p->out * 2, {address(p->dy), address(p->z) / 2, address(p->times), p->times ? p->times_stride * 2 : 0, address(p->dtimes)}), [&](auto vec) {
         constexpr int VB = sizeof(vec.raw);
         EpilogueGradArgs a{};
-        a.dy = p->dy, a.z = kept_sums(p), a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
+        a.dy = p->dy, a.z = static_cast<const float *>(p->z), a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
         a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation, a.chunk = chunk;
         return launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, dim3(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS), EG_THREADS, 0, cs, a);
     });

@@ -31,7 +31,7 @@ struct ProductShared {
 struct ProductArgs {
     CUtensorMap a, b;
     void *out;                                   // [c][f], a group's behind the one before where k has the groups
-    KeptSums z;                                  // the sums and the bias; upper: or NULL
+    float *z;                                    // the sums and the bias, or NULL
     const void *bias, *times, *residual;         // [group][f], [c][f], [c][f], or NULL
     const float *a_scale, *b_scale;              // per f and per c: of 8-bit operands
     Groups groups;
@@ -101,10 +101,17 @@ __device__ __forceinline__ void finish(const ProductArgs &a, const uint64_t *at,
 #pragma unroll
             for (int e = 0; e < N; e++) v[j][e] += w[e];
     }
-    if (a.z.upper) {
+    if (a.z) {
 #pragma unroll
-        for (int j = 0; j < J; j++)
-            if (on[j]) a.z.store<N>(at[j], v[j]);
+        for (int j = 0; j < J; j++) {
+            if (!on[j]) continue;
+            if constexpr (N % 4 == 0) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(a.z + at[j] + e) = make_float4(v[j][e], v[j][e + 1], v[j][e + 2], v[j][e + 3]);
+            } else {
+                for (int e = 0; e < N; e++) a.z[at[j] + e] = v[j][e];
+            }
+        }
     }
     act_all<J * N>(a.activation, v[0]);
     if (a.times) {

@@ -76,3 +76,17 @@ def test_scales_of_8_bits_at_the_ends_of_their_range(rows, inp, out, residual, x
     close(torch.where(fits, y, 0), (torch.where(fits, exact, 0), off.clamp_max(2.0 ** 127) + 2.0 ** -148))
     assert not y.isnan().any() and (y[-1] == 0).all() and (y[:, out // 2] == 0).all()
     assert rows == 1 or small or (y[0] != 0).any()
+
+
+@pytest.mark.parametrize("dtype, far, near", [(F16, 2.0 ** -11, 2.0 ** -20), (BF16, 2.0 ** -8, 2.0 ** -20)])
+@pytest.mark.parametrize("rows, out", [(1, 1), (3, 8), (300, 264), (2304, 512)])
+def test_a_factors_gradient_is_rounded_once(dtype, far, near, rows, out):
+    """z a little above the middle between two numbers: its last bits decide."""
+    from lmz_b200 import linear
+    x = torch.zeros((rows, 16), dtype=dtype, device="cuda")
+    w = torch.zeros((out, 16), dtype=dtype, device="cuda")
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, far, 2.0 ** -10
+    w[:, 0], w[:, 1], w[:, 2] = 1.0, 1.0, near * 2.0 ** 10
+    m = torch.ones((rows, out), dtype=dtype, device="cuda").requires_grad_(True)
+    (dm,) = torch.autograd.grad(linear.project(x, w, times=m), m, torch.ones_like(m))
+    assert (dm == 1 + 2 * far).all()
