@@ -466,7 +466,7 @@ typedef struct lmz_product {
 size_t lmz_gpu_product_work_bytes(const lmz_product *p, int grad);
 size_t lmz_gpu_product_z_bytes(const lmz_product *p);
 int lmz_gpu_product_dev(const lmz_product *p, void *cuda_stream);
-/* dz[t] = dy[t] times[t] act'(z[t]), rounded to the tensors' type;  dx[t] = dz[t] W_e, dW_e = the sum of dz[t]^T x[t], dbias_e = the sum of dz[t] over
+/* dz[t] = dy[t] times[t] act'(z[t]), rounded to the tensors' type (F16: times a power of two, each expert's own);  dx[t] = dz[t] W_e, dW_e = the sum of dz[t]^T x[t], dbias_e = the sum of dz[t] over
  * the rows of expert e (zeros for one without any), dtimes[t] = dy[t] act(z[t]).  The residual's gradient is dy. */
 int lmz_gpu_product_grad_dev(const lmz_product *p, void *cuda_stream);
 

@@ -148,11 +148,24 @@ __device__ __forceinline__ uint32_t group_of(const uint32_t *starts, uint32_t co
 constexpr uint32_t MAX_EXPERTS = 1024;
 constexpr uint32_t EG_THREADS = 128, EG_MOST_ROWS = 32, EG_LEAST_ROWS = 4, EG_STEP = 2;     // rows of a chunk, and of those under way together
 
+// F16 has few powers of two: dz may leave it where dx and dW do not.  So dz is written times a power of two, its group's own, which the products' sums are divided by.
+// USUAL_POWER is right where the group's largest (finite) element is between 4 and 255, so that an element that is less than half a step of F16 is under 2^-34 of that;
+// other groups are written once more, their largest brought to 2^14 and more.
+constexpr int USUAL_POWER = 8;
+__device__ __forceinline__ int dz_power(uint32_t most)           // `most`: its bits
+{
+    if (most == 0 || (most >= 0x40800000u && most <= 0x437FE000u)) return USUAL_POWER;
+    const int power = 14 - (static_cast<int>(most >> 23) - 127);
+    return power < 100 ? power : 100;
+}
+__device__ __forceinline__ float two_to(int power) { return __int_as_float((127 + power) << 23); }
+
 struct EpilogueGradArgs {
     const void *dy, *times;                      // times: or NULL, rows times_stride apart
     const float *z;                              // NULL without an activation and `times`
     void *dz, *dtimes;                           // or NULL
     float *partial;                              // [chunk of rows + group][out]: sums of dz, or NULL
+    uint32_t *most;                              // [group]: bits of the largest finite dz, zeros before; or NULL: dz is written as it is
     Groups groups;
     uint64_t rows, out, times_stride, dz_stride;
     uint32_t vectors, activation, chunk;         // chunk: rows
@@ -183,6 +196,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
     group_starts(a.groups, starts);
     __syncthreads();
     const uint64_t v = blockIdx.y * static_cast<uint64_t>(EG_THREADS) + threadIdx.x;
+    const uint32_t together = __ballot_sync(~0u, v < a.vectors);
     const uint32_t chunk = blockIdx.x, begin = chunk * a.chunk, end = begin + a.chunk < a.rows ? begin + a.chunk : static_cast<uint32_t>(a.rows);
     if (v >= a.vectors) return;
     const uint32_t first = starts[0], last = starts[a.groups.count];
@@ -191,7 +205,14 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
 #pragma unroll
     for (int e = 0; e < V::N; e++) sum[e] = 0;
     bool any = false;
+    constexpr bool HALF = __is_same(T, __half);
+    uint32_t most = 0;
     auto flush = [&] {
+        if (HALF && a.most) {                                    // (the same groups for all of a warp)
+            most = __reduce_max_sync(together, most);
+            if ((threadIdx.x & 31) == 0 && most > *const_cast<volatile uint32_t *>(a.most + group)) atomicMax(a.most + group, most);
+            most = 0;
+        }
         if (a.partial && any) {
             float *to = a.partial + (static_cast<uint64_t>(chunk) + group) * a.out + v * V::N;
 #pragma unroll
@@ -240,6 +261,14 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
                 }
 #pragma unroll
                 for (int e = 0; e < V::N; e++) sum[e] += u[e];
+                if (HALF && a.most) {
+#pragma unroll
+                    for (int e = 0; e < V::N; e++) {
+                        const uint32_t size = __float_as_uint(u[e]) & 0x7FFFFFFF;
+                        if (size < 0x7F800000) most = max(most, size);
+                        u[e] *= two_to(USUAL_POWER);
+                    }
+                }
                 narrow_all(u, dz);
                 any = true;
             }
@@ -248,6 +277,50 @@ __global__ void __launch_bounds__(EG_THREADS) k_epilogue_grad(const EpilogueGrad
         }
     }
     flush();
+}
+
+// dz again, of the groups whose power is not the usual one.  Bound by HBM as the first time, where there are such; else by the launch.
+template <class T, int VB>
+__global__ void __launch_bounds__(EG_THREADS) k_dz_again(const EpilogueGradArgs a)
+{
+    using V = Vec<T, VB>;
+    using R = typename Raw<VB>::type;
+    __shared__ uint32_t starts[MAX_EXPERTS + 1];
+    wait_for_previous();
+    let_next_start();
+    group_starts(a.groups, starts);
+    __syncthreads();
+    const uint64_t v = blockIdx.y * static_cast<uint64_t>(EG_THREADS) + threadIdx.x;
+    if (v >= a.vectors) return;
+    const uint32_t begin = blockIdx.x * a.chunk, last = starts[a.groups.count];
+    const uint32_t end = begin + a.chunk < last ? begin + a.chunk : last;
+    for (uint32_t t = begin < starts[0] ? starts[0] : begin; t < end;) {
+        const uint32_t group = group_of(starts, a.groups.count, t), stop = starts[group + 1] < end ? starts[group + 1] : end;
+        const int power = dz_power(a.most[group]);
+        for (; power != USUAL_POWER && t < stop; t++) {
+            V d, m;
+            float z[V::N], y[V::N], u[V::N], g[V::N];
+            d.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.dy) + t * a.out)[v];
+            if (a.times) m.raw = reinterpret_cast<const R *>(static_cast<const T *>(a.times) + t * a.times_stride)[v];
+#pragma unroll
+            for (int e = 0; e < V::N; e++) z[e] = 0;
+            if (a.z) load_floats<V::N>(a.z + t * a.out + v * V::N, z);
+            act_and_slope<V::N>(a.activation, z, y, u);
+            widen_all(d, g);
+#pragma unroll
+            for (int e = 0; e < V::N; e++) u[e] *= g[e];
+            if (a.times) {
+                widen_all(m, g);
+#pragma unroll
+                for (int e = 0; e < V::N; e++) u[e] *= g[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V::N; e++) u[e] *= two_to(power);
+            narrow_all(u, d);
+            reinterpret_cast<R *>(static_cast<T *>(a.dz) + t * a.dz_stride)[v] = d.raw;
+        }
+        t = stop;
+    }
 }
 
 // A group's bias gradient: what the chunks that its rows lie in have for it; a block's warps take them in turn, and their sums meet in their order.

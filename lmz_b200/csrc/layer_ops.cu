@@ -190,8 +190,8 @@ static uint64_t up16(uint64_t n) { return (n + 15) & ~15ull; }
 
 // What a product's kernels read in place of tensors that do not lie on boundaries, and leave each other.
 struct ProductLayout {
-    uint64_t x, w, dz, partial, end = 0;
-    bool pack_x, pack_w, own_dz;                 // own_dz: dz is not dy, or does not lie where TMA takes it
+    uint64_t x, w, dz, partial, most, end = 0;
+    bool pack_x, pack_w, own_dz, powers;         // own_dz: dz is not dy, or does not lie where TMA takes it; powers: it is written times powers of two
     // Rows of a chunk of the epilogue's gradients: as few as give every multiprocessor blocks enough.
     static uint32_t chunk(const lmz_product *p)
     {
@@ -214,6 +214,8 @@ struct ProductLayout {
         w = take(pack_w && (!grad || p->dx), p->experts * p->out * up16(p->in) * e);
         dz = take(grad && own_dz, p->rows * up8(p->out) * 2);
         partial = take(grad && p->dbias, ((p->rows + chunk(p) - 1) / chunk(p) + p->experts) * p->out * 4);
+        powers = p->dtype == LMZ_GPU_F16 && (p->activation != ACT_NONE || p->times) && (p->dx || p->dweight);
+        most = take(grad && powers, p->experts * 4ull);
     }
 };
 
@@ -344,12 +346,19 @@ static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T 
     const uint32_t chunk = ProductLayout::chunk(p);
     const uint64_t chunks = (p->rows + chunk - 1) / chunk;
     float *partial = p->dbias ? reinterpret_cast<float *>(static_cast<uint8_t *>(p->work) + l.partial) : nullptr;
+    uint32_t *most = l.powers ? reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->work) + l.most) : nullptr;
+    if (most) CK("cudaMemsetAsync", cudaMemsetAsync(most, 0, p->experts * 4ull, cs));
     int rc = by_width<T>(vector_bytes(p->out * 2, {address(p->dy), address(p->z) / 2, address(p->times), p->times ? p->times_stride * 2 : 0, address(p->dtimes)}), [&](auto vec) {
         constexpr int VB = sizeof(vec.raw);
         EpilogueGradArgs a{};
         a.dy = p->dy, a.z = static_cast<const float *>(p->z), a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
         a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation, a.chunk = chunk;
-        return launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, dim3(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS), EG_THREADS, 0, cs, a);
+        a.most = most;
+        const dim3 grid(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS);
+        const int failed = launch("launch k_epilogue_grad", k_epilogue_grad<T, VB>, grid, EG_THREADS, 0, cs, a);
+        if constexpr (std::is_same_v<T, __half>)
+            if (!failed && most) return launch("launch k_dz_again", k_dz_again<T, VB>, grid, EG_THREADS, 0, cs, a);
+        return failed;
     });
     if (!rc && p->dbias)
         rc = launch("launch k_bias_join", k_bias_join<T>, dim3(static_cast<unsigned>((p->out + 31) / 32), p->experts), 32 * BJ_WARPS, 0, cs, static_cast<const float *>(partial),
@@ -379,6 +388,7 @@ static int product_grad_as(const lmz_product *p, cudaStream_t cs)
         ProductArgs a{};
         a.out = out, a.groups = groups_of(p), a.feats = p->in, a.cols = cols;
         a.vectors = vector_bytes(p->in * 2, {address(out)}) == 16, a.plain = true;
+        a.most = own && l.powers ? reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(p->work) + l.most) : nullptr;
         return a;
     };
     if (p->dx) {

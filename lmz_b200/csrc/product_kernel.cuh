@@ -34,6 +34,7 @@ struct ProductArgs {
     float *z;                                    // the sums and the bias, or NULL
     const void *bias, *times, *residual;         // [group][f], [c][f], [c][f], or NULL
     const float *a_scale, *b_scale;              // per f and per c: of 8-bit operands
+    const uint32_t *most;                        // per group: B is dz times a power of two (dz_power) that goes by these; or NULL
     Groups groups;
     uint64_t feats, cols;                        // of f and c (those of c in all groups)
     uint64_t times_stride, residual_stride;
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
 {
     constexpr uint32_t CTAS = PAIR ? 2 : 1, STEP = ROW_BYTES / sizeof(T);
     constexpr bool A_MN = P != FORWARD, B_MN = P == WEIGHT_GRAD, BY_K = P == WEIGHT_GRAD, SCALED = sizeof(T) == 1;
+    constexpr bool POWERS = P != FORWARD && __is_same(T, __half);
     static_assert(sizeof(T) == 2 || P == FORWARD);
     extern __shared__ uint8_t g_smem[];
     __shared__ ProductShared s;
@@ -273,6 +275,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
     };
     auto all_steps = [&](const TilePlace &p) { return BY_K ? (p.k_rows + STEP_K - 1) / STEP_K : a.steps; };
     auto step_from = [&](uint32_t steps, uint32_t r) { return steps * r >> a.split_log; };       // (below 2^26 steps, and eight CTAs)
+    auto undo = [&](const TilePlace &p) { return POWERS && a.most ? two_to(-dz_power(a.most[p.group])) : 1.0f; };
     auto features = [&](const TilePlace &p) { return (p.ft * CTAS + side) * G_FEATS; };      // where this CTA's begin
 
     if (warp == G_TMA_WARP) {
@@ -446,6 +449,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 }
             };
             float f_bias = 0;                                    // of the lane's own feature
+            const float by_power = undo(p);
             if (vectors && a.plain) {
                 const uint64_t own = features(p) + quarter * 32 + lane;
                 if (own < a.feats) {
@@ -504,6 +508,10 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                     float u[G_GROUP];
 #pragma unroll
                     for (uint32_t q = 0; q < G_GROUP; q++) u[q] = !BY_K || any ? __uint_as_float(v[q]) : 0.0f;
+                    if constexpr (POWERS) {
+#pragma unroll
+                        for (uint32_t q = 0; q < G_GROUP; q++) u[q] *= by_power;
+                    }
                     if constexpr (SCALED) {
                         const uint32_t c = p.c + g * G_GROUP;
 #pragma unroll
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                         if (!PAIR && a.split > 1)                // (the stages are free: all products have ended)
                             reinterpret_cast<float *>(local)[(g * G_GROUP + q) * G_FEATS + quarter * 32 + lane] = sum;
                         else if (c < p.c_end && f < a.feats)
-                            finish_one<O, SCALED>(a, p.group, c, f, (plane + c) * a.feats + f, sum);
+                            finish_one<O, SCALED>(a, p.group, c, f, (plane + c) * a.feats + f, POWERS ? sum * by_power : sum);
                     }
                 }
             }
@@ -596,6 +604,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
             const uint64_t plane = BY_K ? p.group * a.cols : 0;
             // A warp has a column, a lane four neighbours of f.
             const uint32_t share = a.nt >> a.split_log;
+            const float by_power = undo(p);
             const uint64_t f = features(p) + lane * 4;
             uint32_t peer[8];
 #pragma unroll
@@ -613,6 +622,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant_
                 float v[1][4] = {{part[0].x, part[0].y, part[0].z, part[0].w}};
 #pragma unroll
                 for (uint32_t i = 1; i < 8; i++) v[0][0] += part[i].x, v[0][1] += part[i].y, v[0][2] += part[i].z, v[0][3] += part[i].w;
+                if constexpr (POWERS) v[0][0] *= by_power, v[0][1] *= by_power, v[0][2] *= by_power, v[0][3] *= by_power;
                 const uint32_t c = p.c + q;
                 const uint64_t at = (plane + c) * a.feats + f;
                 if (a.vectors) {

@@ -18,8 +18,8 @@ def project(x, weight, bias=None, activation=None, times=None, residual=None):
     out.  `activation`: None, "relu", "silu", "gelu" (with the error function) or "gelu_tanh" (its approximation by tanh).
 
     Returns a contiguous [..., out], worked out in 32 bits and rounded once.  Differentiable once, in all five tensors; with an
-    activation or a factor the sums are kept for that in 32 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type.
-    Gradients are the same in every run."""
+    activation or a factor the sums are kept for that in 32 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type
+    (float16: times a power of two that brings the largest to where that has room, so that its own range is no limit).  Gradients are the same in every run."""
     import torch
     index = _ops.on_cuda("x weight bias times residual", x, weight, bias, times, residual)
     code = _ops.type_code(x, "x", half_only=True)

@@ -90,3 +90,43 @@ def test_a_factors_gradient_is_rounded_once(dtype, far, near, rows, out):
     m = torch.ones((rows, out), dtype=dtype, device="cuda").requires_grad_(True)
     (dm,) = torch.autograd.grad(linear.project(x, w, times=m), m, torch.ones_like(m))
     assert (dm == 1 + 2 * far).all()
+
+
+@pytest.mark.parametrize("rows, inp, out", [(40, 64, 96), (40, 33, 50), (700, 64, 264), (2304, 512, 2304)])
+@pytest.mark.parametrize("kind", [None, "silu"])
+@pytest.mark.parametrize("large", [True, False])
+def test_gradients_of_sums_outside_half_precisions_range(rows, inp, out, kind, large):
+    """dz above F16's largest number, or below its smallest, where what it is made of and what is made of it are inside: an element of dz is as good as F16 holds one of
+    ordinary size, or off by 2^-38 of its group's largest."""
+    from lmz_b200 import experts, linear
+    # dz is dy times the factor, 2^22 or 2^-26 and around; dx and dW some 2^10, or 2^-10 and more
+    far, w_std, x_std = (2.0 ** 11, 2.0 ** -12 / out ** 0.5, 2.0 ** -12 / rows ** 0.5) if large else (2.0 ** -13, 2.0 ** 13, 2.0 ** 13)
+    x, w = _randn(1, (rows, inp), F16, x_std), _randn(2, (3, out, inp), F16, w_std)
+    m, dy = _randn(3, (rows, out), F16, far), _randn(4, (rows, out), F16, far)
+    x[1], w[:, 1] = 0, 0
+    starts = [0, rows // 2, rows - 20, rows - 3]
+    m[starts[2]:] /= far                                     # (an expert with a factor of ordinary size)
+    for dense in (True, False):
+        v, u = x.clone().requires_grad_(True), (w[0] if dense else w).clone().requires_grad_(True)
+        y = linear.project(v, u, activation=kind, times=m) if dense else experts.project(v, u, torch.tensor(starts, device="cuda"), activation=kind, times=m)
+        dx, dw = torch.autograd.grad(y, (v, u), dy)
+        ends, weights = ([0, rows], w[:1]) if dense else (starts, w)
+        for e, (lo, hi) in enumerate(zip(ends, ends[1:])):
+            if lo == hi:
+                assert (dw[e] == 0).all()
+                continue
+            xs, we = x[lo:hi].double(), weights[e].double()
+            z = xs @ we.t()
+            z_off = (inp + 6) * STEP * (xs.abs() @ we.abs().t())
+            _, slope = act(kind, z)
+            d = dy[lo:hi].double() * m[lo:hi].double()
+            dz = d * slope
+            # (no slope bends more than one; beyond 40 SiLU's is zero or one)
+            bent = 0 if kind is None else torch.where(z.abs() < z_off + 40, z_off.clamp_max(1.1), 0) + 20 * STEP
+            off = d.abs() * bent + half_step(F16) * 1.01 * dz.abs() + 2.0 ** -38 * dz.abs().max()
+            most = dz.abs() + off
+            for got, a, b, n in ((dx[lo:hi], (dz, off, most), we, out), ((dw if dense else dw[e]), (dz.t(), off.t(), most.t()), xs, hi - lo)):
+                want = a[0] @ b
+                o = a[1] @ b.abs() + (n + 4) * STEP * (a[2] @ b.abs())
+                close(got, (want, o + half_step(F16) * (want.abs() + o) + least(F16)))
+        assert dx.isfinite().all() and dw.isfinite().all()
