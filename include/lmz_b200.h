@@ -455,7 +455,7 @@ typedef struct lmz_product {
     const float *x_scale, *weight_scale;   /* rows, and out: in 8 bits; NULL otherwise */
     void *y;                    /* rows x out */
     void *z;                    /* lmz_gpu_product_z_bytes(), 256-byte aligned: z in 32 bits, which the gradients need where there is an
-                                 * activation or `times`; or NULL */
+                                 * activation or dtimes is wanted; or NULL */
     const void *dy;             /* rows x out */
     void *dx, *dweight, *dbias, *dtimes;   /* contiguous, like x, weight, bias and times; NULL: not wanted */
     void *work;                 /* lmz_gpu_product_work_bytes(), 256-byte aligned */

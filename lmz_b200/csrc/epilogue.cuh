@@ -162,7 +162,7 @@ __device__ __forceinline__ float two_to(int power) { return __int_as_float((127 
 
 struct EpilogueGradArgs {
     const void *dy, *times;                      // times: or NULL, rows times_stride apart
-    const float *z;                              // NULL without an activation and `times`
+    const float *z;                              // NULL where neither the slope nor dtimes goes by it
     void *dz, *dtimes;                           // or NULL
     float *partial;                              // [chunk of rows + group][out]: sums of dz, or NULL
     uint32_t *most;                              // [group]: bits of the largest finite dz, zeros before; or NULL: dz is written as it is

@@ -351,7 +351,7 @@ static int launch_epilogue_grad(const lmz_product *p, const ProductLayout &l, T 
     int rc = by_width<T>(vector_bytes(p->out * 2, {address(p->dy), address(p->z) / 2, address(p->times), p->times ? p->times_stride * 2 : 0, address(p->dtimes)}), [&](auto vec) {
         constexpr int VB = sizeof(vec.raw);
         EpilogueGradArgs a{};
-        a.dy = p->dy, a.z = static_cast<const float *>(p->z), a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
+        a.dy = p->dy, a.z = p->activation != ACT_NONE || p->dtimes ? static_cast<const float *>(p->z) : nullptr, a.times = p->times, a.dz = dz, a.dtimes = p->dtimes, a.partial = partial, a.groups = groups_of(p);
         a.rows = p->rows, a.out = p->out, a.dz_stride = up8(p->out), a.times_stride = p->times_stride, a.vectors = static_cast<uint32_t>(p->out * 2 / VB), a.activation = p->activation, a.chunk = chunk;
         a.most = most;
         const dim3 grid(static_cast<unsigned>(chunks), (a.vectors + EG_THREADS - 1) / EG_THREADS);

@@ -17,8 +17,8 @@ def project(x, weight, bias=None, activation=None, times=None, residual=None):
     `x`: [..., in], `weight`: [out, in], `bias`: [out], `times` and `residual`: [..., out], all bfloat16 or all float16; what is not given is left
     out.  `activation`: None, "relu", "silu", "gelu" (with the error function) or "gelu_tanh" (its approximation by tanh).
 
-    Returns a contiguous [..., out], worked out in 32 bits and rounded once.  Differentiable once, in all five tensors; with an
-    activation or a factor the sums are kept for that in 32 bits, and their own gradient, which is multiplied once more, is rounded to the tensors' type
+    Returns a contiguous [..., out], worked out in 32 bits and rounded once.  Differentiable once, in all five tensors; where an
+    activation's slope or a factor's gradient is wanted the sums are kept for that in 32 bits; their own gradient, which is multiplied once more, is rounded to the tensors' type
     (float16: times a power of two that brings the largest to where that has room, so that its own range is no limit).  Gradients are the same in every run."""
     import torch
     index = _ops.on_cuda("x weight bias times residual", x, weight, bias, times, residual)
@@ -130,13 +130,13 @@ def _work(p, grad: int, like):
 
 
 def _forward(index, code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, keep):
-    """(y, what the gradients need of the sums if `keep`)."""
+    """(y, the sums in 32 bits if `keep`)."""
     import torch
     like = times if times is not None else residual        # (of the result's shape and type)
     y = _ops.empty_like(like) if like is not None else x.new_empty((*x.shape[:-1], weight.shape[-2]), dtype=torch.bfloat16 if rcode == _ops.BF16 else torch.float16)
     p, held = _call(code, rcode, kind, x, weight, bias, times, residual, offsets, x_scale, weight_scale, y)
     z = None
-    if keep and (kind or times is not None):
+    if keep:
         z = y.new_empty(gpu.library().lmz_gpu_product_z_bytes(p), dtype=torch.uint8)
         p.z = z.data_ptr()
     held = held, _work(p, 0, x)                            # (copies and workspace live until the launch)
@@ -168,7 +168,8 @@ def _function():
             @staticmethod
             def forward(ctx, x, weight, bias, times, residual, offsets, kind):
                 code = _ops.type_code(x, "x", half_only=True)
-                y, z = _forward(x.get_device(), code, code, kind, x, weight, bias, times, residual, offsets, None, None, True)
+                wanted = ctx.needs_input_grad[:4]                # (a slope, or the factor's gradient, goes by the sums)
+                y, z = _forward(x.get_device(), code, code, kind, x, weight, bias, times, residual, offsets, None, None, wanted[3] or (kind and any(wanted)))
                 ctx.save_for_backward(x, weight, bias, times, offsets, z)
                 ctx.kind = kind
                 return y
