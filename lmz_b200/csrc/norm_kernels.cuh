@@ -250,8 +250,8 @@ struct NormGradArgs {
 //
 // MOST: threads of a block.  WHOLE: every thread has a whole share of a row.
 //
-// Bound by HBM: dy, s and ds read, dx written.  One B200, 16384x4096 BF16: 87 us without the weight's gradient (6.2 TB/s), 98 with it and k_join; a
-// third of that was instructions before the mean went by s and not by n, and words were taken apart two elements at a time (130).
+// Bound by HBM: dy, s and ds read, dx written.  One B200, 16384x4096 BF16: 91 us without the weight's gradient (5.9 TB/s), 102 with it and k_join (130 before words
+// were taken apart two elements at a time).  Going by n costs 3 us of that: the same by s times rstd^3 left 32 bits' range on the way.
 template <class T, class W, int VB, bool LONG, uint32_t MOST, bool WHOLE>
 __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const NormGradArgs a)
 {
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
         R *dx = reinterpret_cast<R *>(static_cast<T *>(a.dx) + t * a.dim);
         const float rstd = on ? a.rstd[t] : 0;
         V n[NV], g[NV], d[NV];
-        float along = 0;                                         // the sum of dy w s
+        float along = 0;                                         // the sum of dy w n
         auto load = [&](uint32_t v, V &p, V &q, V &r) {
             p.raw = s[v], q.raw = dy[v];
             if (a.ds) r.raw = ds[v];
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
             load_weights<W, V::N>(weight + v * V::N, w);
             widen_all(p, x), widen_all(q, y);
 #pragma unroll
-            for (int e = 0; e < V::N; e++) along += y[e] * w[e] * x[e];
+            for (int e = 0; e < V::N; e++) along += y[e] * w[e] * (x[e] * rstd);
         };
         auto finish = [&](uint32_t v, const V &p, const V &q, V r, float toward, float *sums) {
             float w[V::N], x[V::N], y[V::N], u[V::N];
@@ -302,9 +302,9 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
             widen_all(p, x), widen_all(q, y);
 #pragma unroll
             for (int e = 0; e < V::N; e++) {
-                y[e] *= rstd;
+                x[e] *= rstd;
                 sums[e] += y[e] * x[e];
-                u[e] = y[e] * w[e] - x[e] * toward;
+                u[e] = (y[e] * w[e] - x[e] * toward) * rstd;
             }
             if (!a.dx) return;
             if (a.ds) {
@@ -329,8 +329,8 @@ __global__ void __launch_bounds__(MOST, NORM_MOST / MOST) k_norm_grad(const Norm
             for (int i = 0; i < NV; i++)
                 if (on && has(i)) add(lane + i * lanes, n[i], g[i]);
         }
-        // rstd n mean(dy w n) = s rstd^3 mean(dy w s)
-        const float toward = row_sum(along, a.lane_log, room[turn & 1]) / static_cast<float>(a.dim) * rstd * rstd * rstd;
+        // (by n, and not by s rstd^3: neither rstd's powers nor products with s stay within 32 bits wherever the squares do)
+        const float toward = row_sum(along, a.lane_log, room[turn & 1]) / static_cast<float>(a.dim);
         if (!on) continue;
         if constexpr (LONG) {
             for (uint32_t v = lane; v < a.vectors; v += lanes) {

@@ -130,3 +130,19 @@ def test_gradients_of_sums_outside_half_precisions_range(rows, inp, out, kind, l
                 o = a[1] @ b.abs() + (n + 4) * STEP * (a[2] @ b.abs())
                 close(got, (want, o + half_step(F16) * (want.abs() + o) + least(F16)))
         assert dx.isfinite().all() and dw.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype, size, slope", [(BF16, 1e-17, 1e7), (BF16, 1e17, 1e-9), (BF16, 1e17, 1e25), (F32, 1e-17, 1e7), (F32, 1e17, 1e-9), (F32, 1e17, 1e25), (BF16, 1.0, 1.0)])
+@pytest.mark.parametrize("rows, dim", [(3, 64), (5, 77), (2, 4096), (2, 17000)])
+def test_norms_of_small_and_large_rows(dtype, size, slope, rows, dim):
+    """Rows whose squares 32 bits hold, and gradients that they hold: neither becomes infinite nor loses bits on the way."""
+    from layers import norms as want_norms
+
+    from lmz_b200 import norms
+    x, w, dy = _randn(1, (rows, dim), dtype, size), _randn(2, dim, dtype), _randn(3, (rows, dim), dtype, slope)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = norms.rms_norm(x, w, eps=0.0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        want = want_norms(x, w, None, 0.0, dy)
+        close(y, want["y"]), close(dx, want["dx"]), close(dw, want["dweight"])
