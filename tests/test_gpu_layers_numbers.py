@@ -146,3 +146,26 @@ def test_norms_of_small_and_large_rows(dtype, size, slope, rows, dim):
     with torch.no_grad():
         want = want_norms(x, w, None, 0.0, dy)
         close(y, want["y"]), close(dx, want["dx"]), close(dw, want["dweight"])
+
+
+@pytest.mark.parametrize("low, high", [(-4, 4), (-61, -59), (59, 61), (-100, -99), (-120, 110)])
+def test_quotients_next_to_the_middle_between_two_numbers_of_8_bits(low, high):
+    """What is divided by its row's scale lies on the middle between two numbers of 8 bits, or up to three steps of 32 bits beside it."""
+    from lmz_b200 import norms
+    g = torch.Generator("cuda")
+    g.manual_seed(1)
+    every = torch.arange(0x7F, device="cuda").to(torch.uint8).view(torch.float8_e4m3fn).double()
+    middles = (every[1:] + every[:-1]) / 2
+    rows, near = 4000, torch.arange(-3, 4, device="cuda")
+    most = (448 * 2.0 ** (torch.rand(rows, 1, generator=g, device="cuda") * (high - low) + low)).float()
+    # (scales of 1 - 2^-24 and around, and of other round numbers)
+    turn = torch.arange(rows // 2, device="cuda").to(torch.int32)
+    power = 2.0 ** (low + turn % max(high - low, 1)).float()
+    most[:rows // 2, 0] = ((torch.tensor(448.0, device="cuda") * (8 + turn // 11 % 9) / 8).view(torch.int32) + turn % 11 - 5).view(F32) * power
+    scale = most / torch.full_like(most, 448)              # (by a number of the host torch would multiply by its reciprocal)
+    u = (middles[None] * scale.double()).float()[:, :, None].repeat(1, 1, 7).view(torch.int32)
+    u = torch.where(u > 8, u + near.to(torch.int32), u).view(F32).flatten(1)
+    x = torch.cat((most, u.clamp_max(most), -u.clamp_max(most)), 1)
+    q, s = norms.to_8bit(x)
+    assert torch.equal(s, scale[:, 0])
+    assert torch.equal(q.view(torch.uint8), (x / scale).to(torch.float8_e4m3fn).view(torch.uint8))
