@@ -169,3 +169,36 @@ def test_quotients_next_to_the_middle_between_two_numbers_of_8_bits(low, high):
     q, s = norms.to_8bit(x)
     assert torch.equal(s, scale[:, 0])
     assert torch.equal(q.view(torch.uint8), (x / scale).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+def test_captured_gradients_in_half_precision_follow_their_sizes():
+    """A graph finds the power that dz is written by anew at each replay: ordinary, far above F16's range, far below, and back."""
+    from lmz_b200 import experts, linear
+    rows, inp, out = 90, 72, 104
+    x, w, ws = _randn(1, (rows, inp), F16, 2.0 ** -12), _randn(2, (out, inp), F16, 2.0 ** -12), _randn(3, (3, out, inp), F16, 2.0 ** -12)
+    m, dy = _randn(4, (rows, out), F16), _randn(5, (rows, out), F16)
+    offsets = torch.tensor([2, 40, 40, 87], device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, ws)]
+
+    def step():
+        y, e = linear.project(x, w, activation="gelu", times=m), experts.project(x, ws, offsets, activation="silu", times=m)
+        return *torch.autograd.grad(y, leaves[:2], dy), *torch.autograd.grad(e, (x, ws), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kept = step()
+    ordinary = [t.detach().clone() for t in (x, w, ws, m, dy)]
+    for far in (1.0, 2.0 ** 11, 2.0 ** -12, 2.0 ** 10, 1.0):
+        with torch.no_grad():
+            for t, o in zip((x, w, ws, m, dy), ordinary):
+                t.copy_(o if far >= 1 or t is m or t is dy else o * 2.0 ** 24)
+            m.mul_(far), dy.mul_(far)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip([t.clone() for t in kept], step()):
+            assert torch.equal(a, b) and a.isfinite().all() and (a != 0).any()
