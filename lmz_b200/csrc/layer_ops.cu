@@ -283,10 +283,11 @@ static int launch_product(ProductArgs &a, const T *at, uint64_t a_stride, uint64
     const uint64_t all_steps = by_k ? std::max<uint64_t>(1, (depth / groups + STEP_K - 1) / STEP_K) : (depth + step_elements - 1) / step_elements;
     // Tiles of 256 features by 160 to 256 columns by pairs of CTAs, or of 128 by 16 to 128 by one, or by a cluster that shares k: by what they are
     // reckoned to take (in 10 ns).  A step of a pair takes 0.3 us at 256 columns, of a CTA 0.19 whatever they are; what a tile takes beside its steps is a
-    // pair's 2.6 us and more, a CTA's 0.04 a column; a cluster's meeting 1.4 us and more; the launch and the first tiles 6.  One B200, us, rows x in x
-    // out, reckoned and measured: 4096x4096x4096 pairs of 256 93 (92), of 192 94 (95), 128 a CTA 74 for half the rows (75); 512x4096x4096 pairs of 160 22
-    // (22), of 256 28 (28), 128 a CTA 23 (24); 1x4096x4096 by four CTAs 11 (13), by two 14 (14), by one 19 (19); the weight's gradient of
-    // 5000x256x256 by eight 13 (10), by two 18 (19).
+    // pair's 2.6 us and more, a CTA's 0.04 a column; a cluster's meeting 1.4 us and more; the launch and the first tiles 6.  The way in and
+    // out and clusters' meetings have become faster than that since, for all tiles alike: the order stands, the sums are two to nine us too many.  One B200, us, rows x in
+    // x out, reckoned and measured: 4096x4096x4096 pairs of 256 93 (94), of 192 94 (94); 2048x4096x4096 pairs of 256 50 (46), 128 a CTA 75 (66); 512x4096x4096 pairs of 160
+    // 22 (19), of 256 28 (24), 128 a CTA 23 (19); 200x4096x4096 128 by two CTAs 19 (17), by one 23 (19); 1x4096x4096 by four CTAs 11 (10), by two 14 (12), by one 19 (17);
+    // the weight's gradient of 5000x256x256 by eight 13 (9), by four 14 (12), by two 18 (17).
     uint64_t best = ~0ull;
     bool pair = false;
     a.split = 1;

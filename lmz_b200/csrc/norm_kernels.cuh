@@ -118,7 +118,8 @@ __device__ __forceinline__ void store_8bit(uint8_t *to, const float *v)
 //
 // Bound by HBM (x and the residual read, the stream and y written), in 8 bits nearly by the instructions, too.  A row is a block's or less: 16 elements
 // a thread (of a row of 8192, by 8 elements 125 us, by 16 95, by 32 103, before loads went ahead).  One B200, BF16 with a residual: 16384x4096 80 us
-// (6.7 TB/s), 8192x8192 to 8 bits 83 (5.7 TB/s), 1x4096 2.4.
+// (6.7 TB/s), 8192x8192 to 8 bits 83 (5.7 TB/s), 1x4096 2.4.  32 registers, so that two blocks of 1024 threads have room: FP32 rows, and odd 16-bit ones, put some of
+// theirs away for that (16384x4096 FP32 197 us, 5.4 TB/s).
 template <class T, class W, int VB, bool BITS8, bool LONG, bool WHOLE>
 __global__ void __launch_bounds__(NORM_MOST, 2) k_norm(const NormArgs a)
 {

@@ -170,9 +170,9 @@ __device__ __forceinline__ void finish_one(const ProductArgs &a, uint32_t group,
 // Many (PAIR): two CTAs multiply 256 features by up to 256 columns together, each loading half of both.
 //
 // Bound by the tensor pipe, whose clock is bound by power, where there are many rows; by reading the weight where there are few.  One B200, us for the
-// kernel alone (and its share of the tensor pipe's cycles, at the 1.45 to 1.5 GHz that 1000 W leave): 4096 rows 4096x14336 314 (95 %), with z and
-// a factor 365 (82 %), rows' gradient 329 (92 %), weight's 329 (90 %), in 8 bits 168 (90 %); 16384 rows of 16 experts 2048x4096 202, 203 and 228
-// (one weight for all: 178; theirs come from HBM for a few tiles each); in a graph one row 4096x14336 21.8 (5.4 TB/s), 4096x4096 10.9.
+// kernel alone (and its share of the tensor pipe's cycles, at the clock that 1000 W leave, 1.45 to 1.6 GHz by the box): 4096 rows 4096x14336 288 (95 %), with z and
+// a factor 344 (80 %), rows' gradient 302 (92 %), weight's 306 (89 %), in 8 bits 148 (90 %); 16384 rows of 16 experts 2048x4096 175, 177 and 216
+// (theirs come from HBM for a few tiles each); in a graph one row 4096x14336 21.5 (5.5 TB/s), 4096x4096 9.7.
 template <class T, class O, int P, bool PAIR>
 __global__ void __launch_bounds__(G_THREADS, 1) k_product(const __grid_constant__ ProductArgs a)
 {
