@@ -92,8 +92,8 @@ __device__ __forceinline__ void act_and_slope(uint32_t kind, const float *z, flo
         return each([](float z, float &y, float &slope) {
             const float below = sigmoid(TANH_TWICE * (z + TANH_CUBE * z * z * z));
             y = z * below;
-            const float near = fminf(fmaxf(z, -16.0f), 16.0f);   // (beyond, below or 1 - below is zero, and the square may be infinite)
-            slope = fmaf(y * (1 - below), TANH_TWICE * (1 + 3 * TANH_CUBE * near * near), below);
+            const float near = fminf(fmaxf(z, -16.0f), 16.0f);   // (beyond, below or 1 - below is zero, and z or its square may be infinite)
+            slope = fmaf(near * below * (1 - below), TANH_TWICE * (1 + 3 * TANH_CUBE * near * near), below);
         });
     default: return each([](float z, float &y, float &slope) { y = z, slope = 1; });
     }

@@ -202,3 +202,15 @@ def test_captured_gradients_in_half_precision_follow_their_sizes():
         torch.cuda.synchronize()
         for a, b in zip([t.clone() for t in kept], step()):
             assert torch.equal(a, b) and a.isfinite().all() and (a != 0).any()
+
+
+def test_slopes_at_infinity():
+    """Where an activation is a straight line in the end its slope is that line's, at infinity, too; what comes from there stays with its own row and feature."""
+    from lmz_b200 import linear
+    inf = float("inf")
+    x = torch.tensor([[inf], [-inf], [2.0]], dtype=BF16, device="cuda").requires_grad_(True)
+    w, dy = torch.ones((1, 1), dtype=BF16, device="cuda"), torch.tensor([[3.0], [5.0], [0.0]], dtype=BF16, device="cuda")
+    for kind in ("relu", "gelu_tanh"):
+        y = linear.project(x, w, activation=kind)
+        (dx,) = torch.autograd.grad(y, x, dy)
+        assert y[0, 0] == inf and dx[:, 0].tolist() == [3.0, 0.0, 0.0]
